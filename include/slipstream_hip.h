@@ -253,6 +253,50 @@ int ss_w4a16_gemm(const void* x, void* out, const int32_t* qweight, const void* 
                   void* workspace, int64_t workspace_bytes, void* stream);
 
 /*
+ * W8A8 linear: out[m, n] = (sum_k x[m, k] w[n, k]) x_scale[m] w_scale[n] (+ bias[n]), int8
+ * operands with a scale for each token and each output channel. No counterpart in the
+ * reference, whose quantized linear is W4A16 (slipstream/kernels/quant_gemm.py:23-42).
+ *   x [m, k] int8, row stride x_stride; w [n, k] int8, row stride w_stride (elements, unit
+ *   column stride); x_scale [m], w_scale [n] fp32; bias [n] of bias_dtype, or NULL;
+ *   out [m, n], row stride o_stride, of out_dtype (SS_DTYPE_BF16/F16/F32).
+ * The sum is exact in int32, so k must be below 131072 (else SS_ERR_UNSUPPORTED); the result
+ * fma(sum * x_scale, w_scale, bias) is rounded in fp32 and once to out_dtype. It is the same
+ * whatever kernel or split computes it.
+ * workspace: ss_w8a8_workspace_size() bytes, 16-byte aligned, any contents; with less (or
+ * NULL, 0) the call succeeds without splitting k over workgroups, more slowly. Calls that
+ * share a workspace must be ordered on one stream.
+ */
+int ss_w8a8_workspace_size(int64_t m, int64_t n, int64_t k, int out_dtype, int64_t* bytes);
+
+int ss_w8a8_gemm(const int8_t* x, const float* x_scale, const int8_t* w, const float* w_scale,
+                 const void* bias, void* out, int64_t m, int64_t n, int64_t k, int64_t x_stride,
+                 int64_t w_stride, int64_t o_stride, int out_dtype, int bias_dtype, void* workspace,
+                 int64_t workspace_bytes, void* stream);
+
+/*
+ * Rows quantized to int8 with one fp32 scale each, the inputs of ss_w8a8_gemm:
+ *   a = max |y|, scale = a / 127, q = rint(y * (127 / a)) (half to even), y ~ q * scale.
+ * A row with a < 127 * 2^-126 is zeros with scale 0; a row that holds a NaN or an infinity is
+ * zeros with scale NaN. q [rows, cols] and scale [rows] are contiguous; x, residual, gate
+ * and up have row strides in elements and unit column strides, at any alignment of their
+ * elements; dtype SS_DTYPE_BF16/F16/F32, arithmetic in fp32. cols < 2^29.
+ *   ss_quantize_int8: y = x.
+ *   ss_rmsnorm_int8: the norm of ss_rmsnorm with an int8 output: s = x + residual rounded to
+ *     dtype and written to sum [rows, cols] (contiguous; residual and sum NULL: s = x),
+ *     y = s * weight / sqrt(mean(s^2) + eps), not rounded before it is quantized.
+ *   ss_swiglu_int8: y = silu(gate) * up, not rounded before it is quantized.
+ */
+int ss_quantize_int8(const void* x, int8_t* q, float* scale, int64_t rows, int64_t cols, int64_t x_stride,
+                     int dtype, void* stream);
+
+int ss_rmsnorm_int8(const void* x, const void* residual, const void* weight, int8_t* q, float* scale, void* sum,
+                    int64_t rows, int64_t cols, int64_t x_stride, int64_t r_stride, float eps, int dtype,
+                    void* stream);
+
+int ss_swiglu_int8(const void* gate, const void* up, int8_t* q, float* scale, int64_t rows, int64_t cols,
+                   int64_t g_stride, int64_t u_stride, int dtype, void* stream);
+
+/*
  * KV page copies: for each pair i, page pairs[2i + 1] of dst <- page pairs[2i] of
  * src, in every plane p in [0, planes) (a plane is one (layer, K/V) of
  * kv_cache[L, 2, NB, ...], so planes = 2L for a contiguous cache). Page b of plane

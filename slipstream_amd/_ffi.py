@@ -79,6 +79,17 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         _i32,
         [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i32, _i64, _i64, _i32, _i32, _vp, _i64, _vp],
     ),
+    "ss_w8a8_workspace_size": (_i32, [_i64, _i64, _i64, _i32, _c_i64p]),
+    "ss_w8a8_gemm": (
+        _i32,
+        [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i32, _i32, _vp, _i64, _vp],
+    ),
+    "ss_quantize_int8": (_i32, [_vp, _vp, _vp, _i64, _i64, _i64, _i32, _vp]),
+    "ss_rmsnorm_int8": (
+        _i32,
+        [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, ctypes.c_float, _i32, _vp],
+    ),
+    "ss_swiglu_int8": (_i32, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i32, _vp]),
     "ss_copy_blocks": (_i32, [_vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _i64, _vp]),
     "ss_build_step_metadata": (_i32, [_vp, _i64, _i32, _vp, _vp, _i32, _i32, _vp, _vp, _vp, _i64, _vp]),
     "ss_rmsnorm": (_i32, [_vp, _vp, _vp, _vp, _i64, _i32, _i64, _i64, _i64, ctypes.c_float, _i32, _vp]),

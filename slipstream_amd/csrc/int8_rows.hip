@@ -1,0 +1,425 @@
+// Rows quantized to int8 with one fp32 scale each, for gfx950: the inputs of the W8A8 product
+// (w8a8.hip). Plain rows, rows behind an RMSNorm with the residual's addition, and rows behind
+// SwiGLU, each in one pass over memory.
+//
+// Mathematics, for a row y of fp32 values:
+//   a = max |y|;  scale = a / 127;  q = rint(y * (127 / a)), half to even;  y ~ q * scale.
+//   A row whose scale would be subnormal (a < 127 * 2^-126) is zeros with scale zero: 127 / a
+//   stays finite, and what is dropped is below 1.5e-36.
+//   A row that holds a NaN or an infinity gets zeros and the scale NaN, so that every product
+//   with it is NaN and none is silently finite. The maximum is taken over the magnitudes' bit
+//   patterns as unsigned integers, in which infinity follows every number and NaN infinity.
+// RMSNorm: s = x + residual, rounded to the inputs' type (it is also returned: the next
+//   residual), r = 1 / sqrt(mean(s^2) + eps), y = s * w * r. Since r scales a whole row, q does
+//   not depend on it: with p = s * w (exact in fp32 for 16-bit types) and a = max |p|,
+//   q = rint(p * (127 / a)) and scale = r * a / 127. So both reductions, the sum of squares and
+//   the maximum, share one exchange between the waves, and q is the same whatever the order
+//   of the sum. Nothing is rounded to 16 bits between the norm and its int8 values.
+// SwiGLU: y = g / (1 + exp(-g)) * u in fp32, not rounded before it is quantized.
+#include "ss_common.h"
+
+namespace {
+
+using ss::u32x2;
+using ss::u32x4;
+
+enum Mode { kRows, kNorm, kNormRes, kSwiglu };
+
+struct RowArgs {
+  const char* x;    // rows; SwiGLU: gate
+  const char* y;    // residual; SwiGLU: up
+  const char* w;    // norm weight
+  int8_t* q;        // [rows, cols], contiguous
+  float* scale;     // [rows]
+  char* s;          // x + residual, contiguous
+  int64_t x_stride, y_stride;  // bytes
+  int cols;
+  float eps;
+};
+
+constexpr float kLevels = 127.f;
+constexpr float kSmallest = 127.f * 1.17549435e-38f;  // 127 * 2^-126
+
+template <typename T>
+__device__ __forceinline__ void unpack(const u32x4& w, float (&f)[16 / sizeof(T)]) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t u = w[e];
+      f[e] = __builtin_bit_cast(float, u);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      f[2 * e] = ss::Elem<T>::lo(w[e]);
+      f[2 * e + 1] = ss::Elem<T>::hi(w[e]);
+    }
+  }
+}
+template <typename T>
+__device__ __forceinline__ u32x4 pack(const float (&f)[16 / sizeof(T)]) {
+  u32x4 w;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    if constexpr (sizeof(T) == 4)
+      w[e] = __builtin_bit_cast(uint32_t, f[e]);
+    else
+      w[e] = ss::Elem<T>::pack2(f[2 * e], f[2 * e + 1]);
+  }
+  return w;
+}
+
+// keeps the compiler from contracting x + r or s * w with what follows
+__device__ __forceinline__ float pin(float x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+
+__device__ __forceinline__ uint32_t magnitude(float x) { return __builtin_bit_cast(uint32_t, x) & 0x7FFFFFFFu; }
+
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp(uint32_t x) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, 0xF, 0xF, true);
+}
+__device__ __forceinline__ uint32_t umax(uint32_t a, uint32_t b) { return a > b ? a : b; }
+__device__ __forceinline__ uint32_t wave_umax(uint32_t x) {
+  const auto s32 = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+  x = umax(s32[0], s32[1]);
+  const auto s16 = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+  x = umax(s16[0], s16[1]);
+  x = umax(x, dpp<0x128>(x));  // row_ror:8
+  x = umax(x, dpp<0x124>(x));  // row_ror:4
+  x = umax(x, dpp<0x4E>(x));   // quad_perm [2, 3, 0, 1]
+  return umax(x, dpp<0xB1>(x));
+}
+template <int CTRL>
+__device__ __forceinline__ float add_dpp(float x) {
+  return x + __builtin_bit_cast(float, dpp<CTRL>(__builtin_bit_cast(uint32_t, x)));
+}
+__device__ __forceinline__ float wave_sum(float x) {
+  x = ss::sum_across_rows(x);
+  x = add_dpp<0x128>(x);
+  x = add_dpp<0x124>(x);
+  x = add_dpp<0x4E>(x);
+  return add_dpp<0xB1>(x);
+}
+
+// g / (1 + exp(-g)) by the hardware's exp2 and reciprocal (one unit in the last place each; the
+// product with log2 e adds |g| 2^-24): a step of int8 is 2^-8 of the row's largest value.
+// exp overflows to infinity below g = -88.7, where the value is under 2^-120 and becomes -0.
+__device__ __forceinline__ float silu(float g) {
+  return g * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-ss::kLog2e * g));
+}
+
+// Four values in [-127, 127] times 1 -> four int8 in a dword. p * inv + 1.5 * 2^23 rounds the
+// exact product to an integer, half to even, whose two's complement is the sum's low bits.
+__device__ __forceinline__ uint32_t quant4(const float* p, float inv) {
+  uint32_t b[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) b[e] = __builtin_bit_cast(uint32_t, fmaf(p[e], inv, 12582912.f));
+  const uint32_t lo = __builtin_amdgcn_perm(b[1], b[0], 0x0C0C0400u), hi = __builtin_amdgcn_perm(b[3], b[2], 0x04000C0Cu);
+  return lo | hi;
+}
+
+// 16 bytes at any alignment (global accesses need none on this target), and the elements of a
+// row's last, partial piece: past the row's end zeros.
+template <typename T>
+__device__ __forceinline__ u32x4 load_piece(const char* row, int i, int cols) {
+  constexpr int EPP = 16 / sizeof(T);
+  u32x4 w = {0u, 0u, 0u, 0u};
+  if (i + EPP <= cols) {
+    __builtin_memcpy(&w, row + (int64_t)i * sizeof(T), 16);
+  } else {
+    T t[EPP];
+#pragma unroll
+    for (int e = 0; e < EPP; ++e) t[e] = i + e < cols ? reinterpret_cast<const T*>(row)[i + e] : (T)0.f;
+    __builtin_memcpy(&w, t, 16);
+  }
+  return w;
+}
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t row_rsrc(const char* p, uint32_t bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(p), 0, (int)bytes, 0x00020000);
+}
+__device__ __forceinline__ u32x4 rsrc_piece(__amdgpu_buffer_rsrc_t r, int at) {
+  return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, at, 0, 0));
+}
+
+// What a piece contributes: its values y (norms: p), their largest magnitude, and for norms
+// the sum of squares of s; with a residual `xw` becomes x + residual in T.
+template <typename T, int MODE>
+__device__ __forceinline__ void fold(u32x4& xw, const u32x4& yw, const u32x4& ww, float (&v)[16 / sizeof(T)],
+                                     uint32_t& top, float& sq) {
+  constexpr int EPP = 16 / sizeof(T);
+  unpack<T>(xw, v);
+  if constexpr (MODE == kNormRes) {
+    float r[EPP];
+    unpack<T>(yw, r);
+#pragma unroll
+    for (int e = 0; e < EPP; ++e) v[e] = pin(v[e] + r[e]);
+    xw = pack<T>(v);
+    unpack<T>(xw, v);
+  }
+  if constexpr (MODE == kNorm || MODE == kNormRes) {
+    float w[EPP];
+    unpack<T>(ww, w);
+#pragma unroll
+    for (int e = 0; e < EPP; ++e) {
+      sq = fmaf(v[e], v[e], sq);
+      v[e] = pin(v[e] * w[e]);
+    }
+  }
+  if constexpr (MODE == kSwiglu) {
+    float u[EPP];
+    unpack<T>(yw, u);
+#pragma unroll
+    for (int e = 0; e < EPP; ++e) v[e] = silu(v[e]) * u[e];
+  }
+#pragma unroll
+  for (int e = 0; e < EPP; ++e) top = umax(top, magnitude(v[e]));
+}
+
+// The row's largest magnitude and sum over the workgroup, then 127 / a, and the scale written.
+template <int MODE, int WAVES>
+__device__ __forceinline__ float finish_row(uint32_t top, float sq, const RowArgs& a, int64_t row) {
+  __shared__ uint32_t s_top[WAVES];
+  __shared__ float s_sq[WAVES];
+  top = wave_umax(top);
+  if constexpr (MODE == kNorm || MODE == kNormRes) sq = wave_sum(sq);
+  if constexpr (WAVES > 1) {
+    if ((threadIdx.x & 63) == 0) {
+      s_top[threadIdx.x >> 6] = top;
+      s_sq[threadIdx.x >> 6] = sq;
+    }
+    __syncthreads();
+    top = s_top[0];
+    sq = s_sq[0];
+#pragma unroll
+    for (int i = 1; i < WAVES; ++i) {
+      top = umax(top, s_top[i]);
+      sq += s_sq[i];
+    }
+  }
+  const float peak = __builtin_bit_cast(float, top);
+  const bool finite = top < 0x7F800000u, live = finite && peak >= kSmallest;
+  const float inv = live ? kLevels / peak : 0.f;
+  if (threadIdx.x == 0) {
+    float scale = live ? peak / kLevels : 0.f;
+    if constexpr (MODE == kNorm || MODE == kNormRes) scale *= 1.f / __builtin_sqrtf(sq / (float)a.cols + a.eps);
+    a.scale[row] = finite ? scale : __builtin_nanf("");
+  }
+  return inv;
+}
+
+template <typename T>
+__device__ __forceinline__ void store_q(int8_t* q, int i, int cols, const float (&v)[16 / sizeof(T)], float inv) {
+  constexpr int EPP = 16 / sizeof(T);
+  uint32_t d[EPP / 4];
+#pragma unroll
+  for (int h = 0; h < EPP / 4; ++h) d[h] = inv != 0.f ? quant4(v + 4 * h, inv) : 0u;
+  if (i + EPP <= cols) {
+    __builtin_memcpy(q + i, d, EPP);
+  } else {
+#pragma unroll
+    for (int e = 0; e < EPP; ++e)
+      if (i + e < cols) q[i + e] = (int8_t)(d[e >> 2] >> (8 * (e & 3)));
+  }
+}
+template <typename T>
+__device__ __forceinline__ void store_s(char* s, int i, int cols, const u32x4& w) {
+  constexpr int EPP = 16 / sizeof(T);
+  if (i + EPP <= cols) {
+    __builtin_memcpy(s + (int64_t)i * sizeof(T), &w, 16);
+  } else {
+    T t[EPP];
+    __builtin_memcpy(t, &w, 16);
+#pragma unroll
+    for (int e = 0; e < EPP; ++e)
+      if (i + e < cols) reinterpret_cast<T*>(s)[i + e] = t[e];
+  }
+}
+
+// One workgroup per row, PPT 16-byte pieces a thread, held in registers between the reduction
+// and the write, so that the row is read once. Bound by memory for many rows and by its
+// latency for few: with ALIGNED rows every piece is requested before the first is used, through
+// descriptors that end with the row (a piece past it reads zeros without an access).
+template <typename T, int MODE, int TPB, int PPT, bool ALIGNED>
+__global__ __launch_bounds__(TPB) void int8_rows_kernel(const RowArgs a) {
+  constexpr int EPP = 16 / sizeof(T);
+  const int64_t row = blockIdx.x;
+  const char* const xr = a.x + row * a.x_stride;
+  const char* const yr = MODE == kNormRes || MODE == kSwiglu ? a.y + row * a.y_stride : xr;
+  u32x4 xw[PPT], yw[PPT], ww[PPT];
+  if constexpr (ALIGNED) {
+    const uint32_t bytes = (uint32_t)a.cols * (uint32_t)sizeof(T);
+    const auto rx = row_rsrc(xr, bytes), ry = row_rsrc(yr, bytes);
+    const auto rw = row_rsrc(MODE == kNorm || MODE == kNormRes ? a.w : xr, bytes);
+    const int at = 16 * threadIdx.x;
+#pragma unroll
+    for (int u = 0; u < PPT; ++u) {
+      xw[u] = rsrc_piece(rx, at + 16 * TPB * u);
+      if constexpr (MODE == kNormRes || MODE == kSwiglu) yw[u] = rsrc_piece(ry, at + 16 * TPB * u);
+    }
+    if constexpr (MODE == kNorm || MODE == kNormRes) {
+#pragma unroll
+      for (int u = 0; u < PPT; ++u) ww[u] = rsrc_piece(rw, at + 16 * TPB * u);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  } else {
+#pragma unroll
+    for (int u = 0; u < PPT; ++u) {
+      const int i = (threadIdx.x + TPB * u) * EPP;
+      xw[u] = load_piece<T>(xr, i, a.cols);
+      if constexpr (MODE == kNormRes || MODE == kSwiglu) yw[u] = load_piece<T>(yr, i, a.cols);
+      if constexpr (MODE == kNorm || MODE == kNormRes) ww[u] = load_piece<T>(a.w, i, a.cols);
+    }
+  }
+  float v[PPT][EPP];
+  uint32_t top = 0;
+  float sq = 0.f;
+#pragma unroll
+  for (int u = 0; u < PPT; ++u) fold<T, MODE>(xw[u], yw[u], ww[u], v[u], top, sq);
+  const float inv = finish_row<MODE, TPB / 64>(top, sq, a, row);
+  int8_t* const q = a.q + row * a.cols;
+  char* const s = a.s + row * a.cols * (int64_t)sizeof(T);
+#pragma unroll
+  for (int u = 0; u < PPT; ++u) {
+    const int i = (threadIdx.x + TPB * u) * EPP;
+    if (i < a.cols) {
+      store_q<T>(q, i, a.cols, v[u], inv);
+      if constexpr (MODE == kNormRes) store_s<T>(s, i, a.cols, xw[u]);
+    }
+  }
+}
+
+// Rows longer than the registers hold: the same pieces in two passes over the row, the second
+// reading it again (from the caches, mostly).
+template <typename T, int MODE>
+__global__ __launch_bounds__(256) void int8_rows_long_kernel(const RowArgs a) {
+  constexpr int EPP = 16 / sizeof(T);
+  const int64_t row = blockIdx.x;
+  const char* const xr = a.x + row * a.x_stride;
+  const char* const yr = MODE == kNormRes || MODE == kSwiglu ? a.y + row * a.y_stride : xr;
+  auto piece = [&](int i, u32x4& xw, float (&v)[EPP], uint32_t& top, float& sq) {
+    u32x4 yw = {}, ww = {};
+    xw = load_piece<T>(xr, i, a.cols);
+    if constexpr (MODE == kNormRes || MODE == kSwiglu) yw = load_piece<T>(yr, i, a.cols);
+    if constexpr (MODE == kNorm || MODE == kNormRes) ww = load_piece<T>(a.w, i, a.cols);
+    fold<T, MODE>(xw, yw, ww, v, top, sq);
+  };
+  uint32_t top = 0;
+  float sq = 0.f;
+  u32x4 xw;
+  float v[EPP];
+  for (int64_t i = (int64_t)threadIdx.x * EPP; i < a.cols; i += 256 * EPP) piece((int)i, xw, v, top, sq);
+  const float inv = finish_row<MODE, 4>(top, sq, a, row);
+  int8_t* const q = a.q + row * a.cols;
+  char* const s = a.s + row * a.cols * (int64_t)sizeof(T);
+  for (int64_t i = (int64_t)threadIdx.x * EPP; i < a.cols; i += 256 * EPP) {
+    piece((int)i, xw, v, top, sq);
+    store_q<T>(q, (int)i, a.cols, v, inv);
+    if constexpr (MODE == kNormRes) store_s<T>(s, (int)i, a.cols, xw);
+  }
+}
+
+bool al16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
+
+template <typename T, int MODE, bool ALIGNED>
+int launch_rows(const RowArgs& a, int64_t rows, hipStream_t stream, const char* who) {
+  const int pieces = (int)(((int64_t)a.cols * sizeof(T) + 15) / 16);
+  const dim3 grid((unsigned)rows);
+  if (pieces <= 64)
+    hipLaunchKernelGGL((int8_rows_kernel<T, MODE, 64, 1, ALIGNED>), grid, dim3(64), 0, stream, a);
+  else if (pieces <= 256)
+    hipLaunchKernelGGL((int8_rows_kernel<T, MODE, 256, 1, ALIGNED>), grid, dim3(256), 0, stream, a);
+  else if (pieces <= 512)
+    hipLaunchKernelGGL((int8_rows_kernel<T, MODE, 256, 2, ALIGNED>), grid, dim3(256), 0, stream, a);
+  else if (pieces <= 1024)
+    hipLaunchKernelGGL((int8_rows_kernel<T, MODE, 256, 4, ALIGNED>), grid, dim3(256), 0, stream, a);
+  else if (pieces <= 2048)
+    hipLaunchKernelGGL((int8_rows_kernel<T, MODE, 256, 8, ALIGNED>), grid, dim3(256), 0, stream, a);
+  else
+    hipLaunchKernelGGL((int8_rows_long_kernel<T, MODE>), grid, dim3(256), 0, stream, a);
+  return ss_host::launch_status(who);
+}
+
+template <int MODE>
+int launch_mode(const RowArgs& a, int64_t rows, int dtype, hipStream_t s, const char* who) {
+  const int es = dtype == SS_DTYPE_F32 ? 4 : 2;
+  const bool aligned = ((int64_t)a.cols * es) % 16 == 0 && al16(a.x) && a.x_stride % 16 == 0 &&
+                       (!a.y || (al16(a.y) && a.y_stride % 16 == 0)) && (!a.w || al16(a.w));
+  if (dtype == SS_DTYPE_BF16)
+    return aligned ? launch_rows<ss::bf16_t, MODE, true>(a, rows, s, who) : launch_rows<ss::bf16_t, MODE, false>(a, rows, s, who);
+  if (dtype == SS_DTYPE_F16)
+    return aligned ? launch_rows<ss::f16_t, MODE, true>(a, rows, s, who) : launch_rows<ss::f16_t, MODE, false>(a, rows, s, who);
+  return aligned ? launch_rows<float, MODE, true>(a, rows, s, who) : launch_rows<float, MODE, false>(a, rows, s, who);
+}
+
+// Extents, pointers and dtype of a call; `go` false: nothing to do, or an error. Element
+// counts of a row stay below 2^29, so that byte offsets in it fit 31 bits.
+int check_rows(const char* who, int64_t rows, int64_t cols, int dtype, bool null, int64_t x_stride, int64_t y_stride,
+               bool& go) {
+  go = false;
+  if (rows < 0 || cols < 0) {
+    ss_host::set_error("%s: negative extent", who);
+    return SS_ERR_INVALID;
+  }
+  if (rows == 0 || cols == 0) return SS_OK;
+  if (null) {
+    ss_host::set_error("%s: null pointer", who);
+    return SS_ERR_INVALID;
+  }
+  if (dtype != SS_DTYPE_BF16 && dtype != SS_DTYPE_F16 && dtype != SS_DTYPE_F32) {
+    ss_host::set_error("%s: dtype code %d not supported", who, dtype);
+    return SS_ERR_UNSUPPORTED;
+  }
+  if (x_stride < 0 || y_stride < 0) {
+    ss_host::set_error("%s: negative row stride", who);
+    return SS_ERR_INVALID;
+  }
+  if (rows > 0x7fffffff || cols >= (1 << 29)) {
+    ss_host::set_error("%s: at most 2^31 - 1 rows of fewer than 2^29 elements", who);
+    return SS_ERR_UNSUPPORTED;
+  }
+  go = true;
+  return SS_OK;
+}
+
+}  // namespace
+
+extern "C" int ss_quantize_int8(const void* x, int8_t* q, float* scale, int64_t rows, int64_t cols, int64_t x_stride,
+                                int dtype, void* stream) {
+  const char* who = "quantize_int8";
+  bool go;
+  const int st = check_rows(who, rows, cols, dtype, !x || !q || !scale, x_stride, 0, go);
+  if (!go) return st;
+  const int es = dtype == SS_DTYPE_F32 ? 4 : 2;
+  const RowArgs a = {(const char*)x, nullptr, nullptr, q, scale, nullptr, x_stride * es, 0, (int)cols, 0.f};
+  return launch_mode<kRows>(a, rows, dtype, (hipStream_t)stream, who);
+}
+
+extern "C" int ss_rmsnorm_int8(const void* x, const void* residual, const void* weight, int8_t* q, float* scale,
+                               void* sum, int64_t rows, int64_t cols, int64_t x_stride, int64_t r_stride, float eps,
+                               int dtype, void* stream) {
+  const char* who = "rmsnorm_int8";
+  bool go;
+  const int st =
+      check_rows(who, rows, cols, dtype, !x || !weight || !q || !scale || (residual && !sum), x_stride, r_stride, go);
+  if (!go) return st;
+  const int es = dtype == SS_DTYPE_F32 ? 4 : 2;
+  const RowArgs a = {(const char*)x,    (const char*)residual, (const char*)weight, q, scale, (char*)sum, x_stride * es,
+                     r_stride * es, (int)cols, eps};
+  if (residual) return launch_mode<kNormRes>(a, rows, dtype, (hipStream_t)stream, who);
+  return launch_mode<kNorm>(a, rows, dtype, (hipStream_t)stream, who);
+}
+
+extern "C" int ss_swiglu_int8(const void* gate, const void* up, int8_t* q, float* scale, int64_t rows, int64_t cols,
+                              int64_t g_stride, int64_t u_stride, int dtype, void* stream) {
+  const char* who = "swiglu_int8";
+  bool go;
+  const int st = check_rows(who, rows, cols, dtype, !gate || !up || !q || !scale, g_stride, u_stride, go);
+  if (!go) return st;
+  const int es = dtype == SS_DTYPE_F32 ? 4 : 2;
+  const RowArgs a = {(const char*)gate, (const char*)up, nullptr, q, scale, nullptr, g_stride * es, u_stride * es,
+                     (int)cols, 0.f};
+  return launch_mode<kSwiglu>(a, rows, dtype, (hipStream_t)stream, who);
+}

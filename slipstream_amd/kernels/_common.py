@@ -2,6 +2,8 @@
 
 from __future__ import annotations
 
+import contextlib
+
 import torch
 
 
@@ -23,6 +25,14 @@ def require_device(who: str, *tensors: torch.Tensor) -> None:
             dev = t.device
         elif t.device != dev:
             raise ValueError(f"{who}: tensors on different devices ({dev} vs {t.device})")
+
+
+_HERE = contextlib.nullcontext()
+
+
+def on_device(device: torch.device):
+    """A context in which ``device`` is the current one, as a launch on its streams needs."""
+    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def unit_last_stride(x: torch.Tensor) -> torch.Tensor:

@@ -1,0 +1,86 @@
+"""W8A8 linear on HIP, gfx950: an int8 product with a scale for each token and each channel.
+
+``w8a8_gemm(q, scale, qweight, w_scale)`` multiplies rows quantized by ``quantize_int8``,
+``fused_rmsnorm_int8`` or ``fused_swiglu_int8`` with a weight quantized per output channel
+(``slipstream_amd.quantized.quantize_weight_int8``). The integer sum is exact (int32), so a
+result does not depend on the batch around it nor on the kernel that ran: it is rounded by
+the scales in fp32 and once to ``out_dtype``. The reference has no counterpart; the
+conventions are those of ``w4a16_gemm``. Device tensors only.
+"""
+
+from __future__ import annotations
+
+import torch
+
+from slipstream_amd import _ffi
+from slipstream_amd.kernels._common import on_device, require_device
+
+# Workspace bytes the library asks for, by shape.
+_WS_NEED: dict[tuple, int] = {}
+
+
+def check_w8a8_args(q: torch.Tensor, scale: torch.Tensor, qweight: torch.Tensor, w_scale: torch.Tensor,
+                    bias: torch.Tensor | None) -> tuple[int, int]:
+    """Shape and dtype checks; returns ``(out, in)``."""
+    if qweight.ndim != 2:
+        raise ValueError(f"qweight must be 2-D [out, in], got {tuple(qweight.shape)}")
+    n, k = qweight.shape
+    if q.dtype != torch.int8 or qweight.dtype != torch.int8:
+        raise ValueError(f"q and qweight must be int8, got {q.dtype} and {qweight.dtype}")
+    if scale.dtype != torch.float32 or w_scale.dtype != torch.float32:
+        raise ValueError(f"scale and w_scale must be float32, got {scale.dtype} and {w_scale.dtype}")
+    if q.ndim == 0 or q.shape[-1] != k:
+        raise ValueError(f"q {tuple(q.shape)} does not end in the weight's {k} input features")
+    if tuple(scale.shape) != tuple(q.shape[:-1]):
+        raise ValueError(f"scale {tuple(scale.shape)} != one for each row of q {tuple(q.shape)}")
+    if tuple(w_scale.shape) != (n,):
+        raise ValueError(f"w_scale {tuple(w_scale.shape)} != [out={n}]")
+    if bias is not None and tuple(bias.shape) != (n,):
+        raise ValueError(f"bias {tuple(bias.shape)} != [out={n}]")
+    return n, k
+
+
+def _workspace_need(m: int, n: int, k: int, dtype: int) -> int:
+    key = (torch.cuda.current_device(), m, n, k, dtype)
+    need = _WS_NEED.get(key)
+    if need is None:
+        out = _ffi.ctypes.c_int64(0)
+        _ffi.check(_ffi.lib().ss_w8a8_workspace_size(m, n, k, dtype, _ffi.ctypes.byref(out)), "w8a8 workspace")
+        if len(_WS_NEED) > 4096:  # many distinct shapes: start over
+            _WS_NEED.clear()
+        need = _WS_NEED[key] = int(out.value)
+    return need
+
+
+def w8a8_gemm(q: torch.Tensor, scale: torch.Tensor, qweight: torch.Tensor, w_scale: torch.Tensor,
+              bias: torch.Tensor | None = None, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """``(q * scale[..., None]) @ (qweight * w_scale[:, None]).T (+ bias)`` in ``out_dtype``:
+    ``q [..., in]`` int8, ``scale [...]`` fp32, ``qweight [out, in]`` int8, ``w_scale [out]``
+    fp32, ``bias [out]`` of any float dtype -> ``[..., out]``."""
+    n, k = check_w8a8_args(q, scale, qweight, w_scale, bias)
+    dtype = _ffi.dtype_code(out_dtype)
+    bias_dtype = _ffi.dtype_code(bias.dtype) if bias is not None else 0
+    out = torch.empty((*q.shape[:-1], n), dtype=out_dtype, device=q.device)
+    if out.numel() == 0:
+        return out
+    require_device("w8a8_gemm", q, scale, qweight, w_scale, *([bias] if bias is not None else []))
+    m = out.numel() // n
+    q2 = q.reshape(m, k)
+    if k and (q2.stride(1) != 1 or (m > 1 and q2.stride(0) < k)):
+        q2 = q2.contiguous()
+    if k and (qweight.stride(1) != 1 or (n > 1 and qweight.stride(0) < k)):
+        qweight = qweight.contiguous()
+    scale = scale.reshape(m).contiguous()
+    w_scale = w_scale.contiguous()
+    bias = bias.contiguous() if bias is not None else None
+    with on_device(q.device):
+        need = _workspace_need(m, n, k, dtype)
+        # of this call alone: nothing is shared between streams, or between captured graphs
+        ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+        status = _ffi.lib().ss_w8a8_gemm(
+            q2.data_ptr(), scale.data_ptr(), qweight.data_ptr(), w_scale.data_ptr(),
+            bias.data_ptr() if bias is not None else None, out.data_ptr(), m, n, k, q2.stride(0),
+            qweight.stride(0), n, dtype, bias_dtype, ws.data_ptr() if ws is not None else None, need,
+            _ffi.stream_ptr(q.device))
+    _ffi.check(status, "w8a8_gemm")
+    return out

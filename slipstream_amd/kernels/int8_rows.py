@@ -1,0 +1,90 @@
+"""Rows quantized to int8 with a scale each (HIP, gfx950): the inputs of ``w8a8_gemm``.
+
+``quantize_int8`` takes rows as they are, ``fused_rmsnorm_int8`` behind the RMS norm with the
+residual's addition, ``fused_swiglu_int8`` behind SwiGLU; the names and arguments follow
+``fused_rmsnorm`` and ``fused_swiglu``. A row ``y`` becomes ``q = rint(y * 127 / max|y|)`` and
+``scale = max|y| / 127``. Everything between the inputs and ``q`` is fp32: unlike the 16-bit
+ops, nothing is rounded to the inputs' type on the way, except the residual sum that is
+returned. A row of zeros (or below 1.5e-36) has scale 0, a row with a NaN or an infinity
+has zeros and scale NaN. Device tensors only.
+"""
+
+from __future__ import annotations
+
+import torch
+
+from slipstream_amd import _ffi
+from slipstream_amd.kernels._common import on_device, require_device
+from slipstream_amd.kernels.norm_act import _rows
+
+
+def _outputs(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    if x.ndim == 0:
+        raise ValueError("rows need at least one dimension")
+    q = torch.empty(x.shape, dtype=torch.int8, device=x.device)
+    make = torch.empty if x.shape[-1] else torch.zeros
+    return q, make(x.shape[:-1], dtype=torch.float32, device=x.device)
+
+
+def quantize_int8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """``x [..., K]`` -> ``(q int8 [..., K], scale fp32 [...])`` with ``x ~ q * scale[..., None]``."""
+    q, scale = _outputs(x)
+    dtype = _ffi.dtype_code(x.dtype)
+    if x.numel() == 0:
+        return q, scale
+    require_device("quantize_int8", x)
+    x2, xs = _rows(x, x.shape[-1])
+    with on_device(x.device):
+        status = _ffi.lib().ss_quantize_int8(x2.data_ptr(), q.data_ptr(), scale.data_ptr(), x2.shape[0], x2.shape[1],
+                                             xs, dtype, _ffi.stream_ptr(x.device))
+    _ffi.check(status, "quantize_int8")
+    return q, scale
+
+
+def fused_rmsnorm_int8(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | None = None,
+                       eps: float = 1e-6) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor | None]:
+    """``rms(x) * w``, or ``rms(x + residual) * w`` when ``residual`` is set, in int8:
+    ``(q, scale, s)``. ``s`` is ``x + residual`` in ``x``'s dtype, the next residual, a new
+    tensor (None without a residual)."""
+    q, scale = _outputs(x)
+    cols = x.shape[-1]
+    if weight.numel() != cols:
+        raise ValueError(f"weight numel {weight.numel()} != hidden {cols}")
+    if residual is not None and residual.shape != x.shape:
+        raise ValueError(f"residual {tuple(residual.shape)} != x {tuple(x.shape)}")
+    dtypes = {x.dtype, weight.dtype} | ({residual.dtype} if residual is not None else set())
+    if len(dtypes) != 1:
+        raise ValueError(f"x, weight and residual must share a dtype, got {sorted(map(str, dtypes))}")
+    dtype = _ffi.dtype_code(x.dtype)
+    s = torch.empty(x.shape, dtype=x.dtype, device=x.device) if residual is not None else None
+    if x.numel() == 0:
+        return q, scale, s
+    require_device("fused_rmsnorm_int8", x, weight, *([residual] if residual is not None else []))
+    x2, xs = _rows(x, cols)
+    r2, rs = _rows(residual, cols) if residual is not None else (None, 0)
+    w = weight.reshape(cols).contiguous()
+    with on_device(x.device):
+        status = _ffi.lib().ss_rmsnorm_int8(x2.data_ptr(), r2.data_ptr() if r2 is not None else None, w.data_ptr(),
+                                            q.data_ptr(), scale.data_ptr(), s.data_ptr() if s is not None else None,
+                                            x2.shape[0], cols, xs, rs, float(eps), dtype, _ffi.stream_ptr(x.device))
+    _ffi.check(status, "fused_rmsnorm_int8")
+    return q, scale, s
+
+
+def fused_swiglu_int8(gate: torch.Tensor, up: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """``silu(gate) * up`` in int8: ``(q, scale)``."""
+    if gate.shape != up.shape or gate.dtype != up.dtype:
+        raise ValueError("gate/up must share shape and dtype")
+    q, scale = _outputs(gate)
+    dtype = _ffi.dtype_code(gate.dtype)
+    if gate.numel() == 0:
+        return q, scale
+    require_device("fused_swiglu_int8", gate, up)
+    cols = gate.shape[-1]
+    g2, gs = _rows(gate, cols)
+    u2, us = _rows(up, cols)
+    with on_device(gate.device):
+        status = _ffi.lib().ss_swiglu_int8(g2.data_ptr(), u2.data_ptr(), q.data_ptr(), scale.data_ptr(), g2.shape[0],
+                                           cols, gs, us, dtype, _ffi.stream_ptr(gate.device))
+    _ffi.check(status, "fused_swiglu_int8")
+    return q, scale

@@ -9,6 +9,10 @@ modules once, at load, with the reference's quantizer (``quant_ref.py:72-100``,
 restated below with torch ops on the weight's device); ``from_awq`` / ``from_gptq`` /
 ``from_state_dict`` re-lay out the tensors of AWQ and GPTQ checkpoints into the reference
 format at load (the quantized-model loading the reference plans, ``MASTERPLAN.md:620-627``).
+``W8A8Linear`` and ``W8A8MLP`` are the same in 8-bit integers: weights in int8 with a scale
+per output channel, activations quantized on the way in with a scale per token
+(``quantize_int8``, ``fused_swiglu_int8``) and multiplied by ``w8a8_gemm``; their
+``forward_int8`` takes rows that are int8 already, as ``fused_rmsnorm_int8`` leaves them.
 The forward passes are the HIP kernels only.
 """
 
@@ -17,6 +21,8 @@ from __future__ import annotations
 import torch
 from torch import nn
 
+from slipstream_amd.kernels.int8_gemm import w8a8_gemm
+from slipstream_amd.kernels.int8_rows import fused_swiglu_int8, quantize_int8
 from slipstream_amd.kernels.norm_act import fused_swiglu
 from slipstream_amd.kernels.quant_gemm import w4a16_gemm
 
@@ -234,3 +240,97 @@ class W4A16MLP(nn.Module):
         gu = self.gate_up_proj(x)
         i = self.intermediate
         return self.down_proj(fused_swiglu(gu[..., :i], gu[..., i:]))
+
+
+def quantize_weight_int8(weight: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """Per output channel (row) of ``weight [N, K]``: ``scale = max|w| / 127``,
+    ``q = round(w * 127 / max|w|)`` (half to even), the rule of ``quantize_int8``. Returns
+    ``(qweight int8 [N, K], scales fp32 [N])``; a channel of zeros (or below 1.5e-36) has
+    scale 0. Torch ops on the weight's device, once at load."""
+    if weight.ndim != 2:
+        raise ValueError(f"weight must be 2-D [out, in], got {tuple(weight.shape)}")
+    w = weight.float()
+    if not torch.isfinite(w).all():
+        raise ValueError("weight has infinities or NaN")
+    top = w.abs().amax(dim=1, keepdim=True) if w.shape[1] else w.new_zeros((w.shape[0], 1))
+    live = top >= 127 * 2.0**-126
+    levels = torch.full((), 127.0, device=w.device)  # a tensor: a true division, as in quantize_weight
+    q = torch.round(w * (levels / torch.where(live, top, 1.0))) * live
+    return q.to(torch.int8), torch.where(live, top / levels, 0.0).squeeze(1)
+
+
+class W8A8Linear(nn.Module):
+    """``y = x @ (qweight * scales[:, None]).T (+ bias)`` with ``x`` quantized per token, through
+    ``w8a8_gemm``."""
+
+    def __init__(self, qweight: torch.Tensor, scales: torch.Tensor, bias: torch.Tensor | None = None) -> None:
+        super().__init__()
+        if qweight.ndim != 2 or qweight.dtype != torch.int8:
+            raise ValueError(f"qweight must be int8 [out, in], got {qweight.dtype} {tuple(qweight.shape)}")
+        self.out_features, self.in_features = qweight.shape
+        if tuple(scales.shape) != (self.out_features,) or scales.dtype != torch.float32:
+            raise ValueError(f"scales must be float32 [out={self.out_features}], got {scales.dtype} {tuple(scales.shape)}")
+        self.register_buffer("qweight", qweight)
+        self.register_buffer("scales", scales)
+        self.register_buffer("bias", bias)
+
+    def _apply(self, fn, recurse: bool = True):
+        scales = self.scales
+        super()._apply(fn, recurse)
+        if self.scales.dtype != torch.float32:  # .half() or .to(dtype) of a model: scales stay fp32
+            self.scales = scales.to(self.scales.device)
+        return self
+
+    @classmethod
+    def from_linear(cls, linear: nn.Linear) -> "W8A8Linear":
+        bias = linear.bias.detach().clone() if linear.bias is not None else None
+        return cls(*quantize_weight_int8(linear.weight.detach()), bias)
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        return self.forward_int8(*quantize_int8(x), x.dtype)
+
+    def forward_int8(self, q: torch.Tensor, scale: torch.Tensor,
+                     out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+        """The product alone, for rows quantized already."""
+        return w8a8_gemm(q, scale, self.qweight, self.scales, self.bias, out_dtype)
+
+    def extra_repr(self) -> str:
+        return f"in={self.in_features}, out={self.out_features}"
+
+
+class W8A8MLP(nn.Module):
+    """SwiGLU MLP (``mlp.py:12-40``) on W8A8 linears, gate and up held as one linear (as in
+    ``W4A16MLP``): its output's halves are read in place by ``fused_swiglu_int8``, whose rows
+    are the down projection's input."""
+
+    def __init__(self, gate_proj: W8A8Linear, up_proj: W8A8Linear, down_proj: W8A8Linear) -> None:
+        super().__init__()
+        if (gate_proj.in_features, gate_proj.out_features) != (up_proj.in_features, up_proj.out_features):
+            raise ValueError("gate_proj and up_proj must share in/out features")
+        if down_proj.in_features != gate_proj.out_features:
+            raise ValueError(f"down_proj reads {down_proj.in_features} features, gate_proj has {gate_proj.out_features}")
+        bias = None
+        if gate_proj.bias is not None or up_proj.bias is not None:
+            like = gate_proj.bias if gate_proj.bias is not None else up_proj.bias
+            bias = torch.cat([lin.bias if lin.bias is not None else torch.zeros_like(like)
+                              for lin in (gate_proj, up_proj)])
+        self.intermediate = gate_proj.out_features
+        self.gate_up_proj = W8A8Linear(torch.cat([gate_proj.qweight, up_proj.qweight]),
+                                       torch.cat([gate_proj.scales, up_proj.scales]), bias)
+        self.down_proj = down_proj
+
+    @classmethod
+    def from_mlp(cls, mlp: nn.Module) -> "W8A8MLP":
+        """Quantize a module with ``gate_proj`` / ``up_proj`` / ``down_proj`` linears (the
+        reference's ``MLP``, HF names)."""
+        return cls(*(W8A8Linear.from_linear(lin) for lin in (mlp.gate_proj, mlp.up_proj, mlp.down_proj)))
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        return self.forward_int8(*quantize_int8(x), x.dtype)
+
+    def forward_int8(self, q: torch.Tensor, scale: torch.Tensor,
+                     out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+        """The MLP for rows quantized already (``fused_rmsnorm_int8``)."""
+        gu = self.gate_up_proj.forward_int8(q, scale, out_dtype)
+        i = self.intermediate
+        return self.down_proj.forward_int8(*fused_swiglu_int8(gu[..., :i], gu[..., i:]), out_dtype)

@@ -1,0 +1,228 @@
+"""Rows quantized to int8 (plain, behind the RMS norm with the residual, behind SwiGLU) against
+the formulas in 64 bits.
+
+Tolerances, in units of u = 2^-24 (a fp32 rounding, relative):
+  q: the value in steps is y * 127 / a; fp32 rounds 127 / a once, the norm s * w once in y and
+     once in a (exact for 16-bit types), so |q - steps| <= 1/2 + 127 * 4 u. SwiGLU: the product
+     g log2 e is rounded (|g| u in exp), exp2 and the reciprocal are within 2 u, 1 + exp, g * r,
+     * u once each: (|g| + 7) u in y and the same in a.
+  scale: a / 127 once (a as above); the norm's sum of squares adds each of a thread's
+     cols / 256 values and 16 partial sums with a rounding each, halved by the root, and the
+     mean, eps, root, reciprocal and two products round once each.
+"""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from slipstream_amd.kernels import fused_rmsnorm, fused_rmsnorm_int8, fused_swiglu_int8, quantize_int8
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0**-24
+SMALLEST = 127 * 2.0**-126
+DTYPES = [torch.bfloat16, torch.float16, torch.float32]
+# one element, one piece and either side of it, odd, each count of pieces a thread, the two-pass rows
+COLS = [1, 7, 8, 9, 64, 513, 896, 1000, 2051, 4096, 4864, 8192, 14336, 16384, 16392, 40001]
+
+
+def _rand(g, shape, dtype, device, spread=True):
+    x = torch.randn(shape, generator=g, device=device)
+    if spread and len(shape) > 1:
+        x = x * torch.exp(torch.randn((*shape[:-1], 1), generator=g, device=device))
+    return x.to(dtype)
+
+
+def _check(q, scale, y, y_err, scale_err, what):
+    """int8 rows against fp64 rows ``y`` known to a relative ``y_err``."""
+    assert q.dtype == torch.int8 and scale.dtype == torch.float32
+    assert q.shape == y.shape and scale.shape == y.shape[:-1]
+    top = y.abs().amax(-1)
+    live = top >= SMALLEST
+    assert not q[~live].any() and not scale[~live].any(), f"{what}: a row of zeros"
+    steps = y * (127 / torch.where(live, top, 1.0))[..., None]
+    off = ((q.double() - steps).abs()[live]).max().item() if live.any() else 0.0
+    assert off <= 0.5 + 127 * (2 * y_err + 2 * U), f"{what}: {off} steps off"
+    rel = ((scale.double() * 127 / top - 1).abs()[live]).max().item() if live.any() else 0.0
+    assert rel <= scale_err, f"{what}: scale {rel / U:.1f} u off"
+    assert (q[live].abs().amax(-1) == 127).all()
+
+
+def _norm64(x, w, r, eps):
+    s = x if r is None else (x.float() + r.float()).to(x.dtype)
+    s64 = s.double()
+    return s64 * w.double() / (s64.square().mean(-1, keepdim=True) + eps).sqrt(), s
+
+
+def _norm_scale_err(cols):
+    return ((cols / 256 + 16 + 16) / 2 + 10) * U
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("cols", COLS)
+def test_rows(device, dtype, cols):
+    g = torch.Generator(device=device).manual_seed(cols)
+    x = _rand(g, (5, cols), dtype, device)
+    x[3] = 0
+    q, scale = quantize_int8(x)
+    _check(q, scale, x.double(), 0.0, 2 * U, f"rows {cols} {dtype}")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("cols", COLS)
+@pytest.mark.parametrize("with_residual", [False, True])
+def test_norm(device, dtype, cols, with_residual):
+    g = torch.Generator(device=device).manual_seed(cols)
+    x = _rand(g, (2, 2, cols), dtype, device)
+    w = (1 + 0.1 * _rand(g, (cols,), torch.float32, device)).to(dtype)
+    r = _rand(g, (2, 2, cols), dtype, device) if with_residual else None
+    x[1, 0] = 0
+    if with_residual:
+        r[1, 0] = 0
+    q, scale, s = fused_rmsnorm_int8(x, w, r, 1e-6)
+    y, want = _norm64(x, w, r, 1e-6)
+    if with_residual:
+        assert s.dtype == dtype and torch.equal(s, want) and s.data_ptr() not in (x.data_ptr(), r.data_ptr())
+    else:
+        assert s is None
+    _check(q, scale, y, U if dtype == torch.float32 else 0.0, _norm_scale_err(cols), f"norm {cols} {dtype}")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("cols", COLS)
+def test_swiglu(device, dtype, cols):
+    g = torch.Generator(device=device).manual_seed(cols)
+    gate, up = 2 * _rand(g, (5, cols), dtype, device), _rand(g, (5, cols), dtype, device)
+    up[2] = 0
+    q, scale = fused_swiglu_int8(gate, up)
+    g64 = gate.double()
+    err = (g64.abs().max().item() + 7) * U
+    _check(q, scale, g64 / (1 + torch.exp(-g64)) * up.double(), err, err + 2 * U, f"swiglu {cols} {dtype}")
+
+
+@pytest.mark.parametrize("rows", [1, 3, 257, 2240])
+def test_row_counts_agree(device, rows):
+    """A row's int8 values and scale do not depend on the rows around it."""
+    g = torch.Generator(device=device).manual_seed(rows)
+    x, r = (_rand(g, (rows, 1024), torch.bfloat16, device) for _ in range(2))
+    w = torch.ones(1024, device=device, dtype=torch.bfloat16)
+    q, scale, s = fused_rmsnorm_int8(x, w, r)
+    at = rows // 2
+    q1, scale1, s1 = fused_rmsnorm_int8(x[at], w, r[at])
+    assert scale1.shape == () and torch.equal(q[at], q1) and torch.equal(scale[at], scale1) and torch.equal(s[at], s1)
+    y, _ = _norm64(x, w, r, 1e-6)
+    _check(q, scale, y, 0.0, _norm_scale_err(1024), f"{rows} rows")
+
+
+def test_norm_in_int8_is_the_norm(device):
+    """The int8 rows stand for what ``fused_rmsnorm`` gives: within half a step and that
+    op's two roundings to bf16 (2^-8 of the value each)."""
+    g = torch.Generator(device=device).manual_seed(5)
+    x, r = (_rand(g, (17, 4096), torch.bfloat16, device) for _ in range(2))
+    w = (1 + 0.1 * torch.randn(4096, generator=g, device=device)).to(torch.bfloat16)
+    q, scale, _ = fused_rmsnorm_int8(x, w, r)
+    y = fused_rmsnorm(x, w, r).double()
+    off = (q.double() * scale.double()[:, None] - y).abs()
+    assert (off <= 0.501 * scale.double()[:, None] + 2 * 2.0**-8 * y.abs() * 1.01).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("cols", [64, 1001, 4096, 40001])
+def test_nan_and_infinity_mark_their_row_only(device, dtype, cols):
+    g = torch.Generator(device=device).manual_seed(cols)
+    x = _rand(g, (6, cols), dtype, device)
+    good = x.clone()
+    for row, v in ((0, float("nan")), (2, float("inf")), (5, float("-inf"))):
+        x[row, (cols * 3) // 4] = v
+    w, one = torch.ones(cols, device=device, dtype=dtype), torch.ones_like(x)
+    zero = torch.zeros_like(x)
+    for what, call in (("rows", lambda t: quantize_int8(t)), ("norm", lambda t: fused_rmsnorm_int8(t, w)[:2]),
+                       ("residual", lambda t: fused_rmsnorm_int8(zero, w, t)[:2]),
+                       ("up", lambda t: fused_swiglu_int8(one, t))):
+        q, scale = call(x)
+        q0, scale0 = call(good)
+        for row in range(6):
+            if row in (0, 2, 5):
+                assert torch.isnan(scale[row]) and not q[row].any(), what
+            else:
+                assert torch.equal(q[row], q0[row]) and torch.equal(scale[row], scale0[row]), what
+    _, scale = fused_swiglu_int8(x, one)
+    assert torch.isnan(scale[[0, 2, 5]]).all() and torch.isfinite(scale[[1, 3, 4]]).all()
+
+
+def test_smallest_and_largest_rows(device):
+    """Either side of the smallest scale, subnormal rows, and rows next to the largest number."""
+    big = torch.finfo(torch.float32).max
+    tops = [1e-45, 1e-38, SMALLEST * 0.999, SMALLEST, SMALLEST * 1.01, 1e-30, 1.0, big / 3, big]
+    base = torch.tensor([1.0, -0.5, 0.25, 0.0, -1.0 / 127, 3.0 / 127], device=device)
+    x = torch.stack([base * t for t in tops])
+    q, scale = quantize_int8(x)
+    assert torch.isfinite(scale).all()
+    _check(q, scale, x.double(), 0.0, 2 * U, "extremes")
+    assert q[-1].tolist()[:2] == [127, -64]  # 63.5 rounds to even
+
+
+def test_ties_round_to_even(device):
+    x = torch.tensor([[127.0, 0.5, 1.5, 2.5, -0.5, -1.5, -2.5, 63.5, 126.5]], device=device)
+    q, scale = quantize_int8(x)
+    assert q.tolist() == [[127, 0, 2, 2, 0, -2, -2, 64, 126]] and scale.item() == 1.0
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_strides_and_alignments(device, dtype):
+    """Rows of wider buffers, at every element offset, transposed and broadcast ones: as the
+    contiguous rows give, and nothing else is read into them."""
+    g = torch.Generator(device=device).manual_seed(3)
+    buf = torch.full((7, 2 * 1000 + 24), 1e4, device=device, dtype=dtype)
+    for off in (0, 1, 3, 8):
+        gate, up = buf[:, off : off + 1000], buf[:, off + 1008 : off + 2008]
+        gate.copy_(torch.randn(gate.shape, generator=g, device=device))
+        up.copy_(torch.randn(up.shape, generator=g, device=device))
+        w = buf[0, off : off + 1000]
+        cg, cu, cw = gate.clone(), up.clone(), w.clone()
+        for got, want in ((quantize_int8(up), quantize_int8(cu)), (fused_swiglu_int8(gate, up), fused_swiglu_int8(cg, cu)),
+                          (fused_rmsnorm_int8(gate, w, up), fused_rmsnorm_int8(cg, cw, cu))):
+            assert all(torch.equal(a, b) for a, b in zip(got, want)), off
+        _check(*quantize_int8(up), cu.double(), 0.0, 2 * U, f"offset {off}")
+        buf.fill_(1e4)
+    t = torch.randn(64, 9, generator=g, device=device).to(dtype).t()
+    assert all(torch.equal(a, b) for a, b in zip(quantize_int8(t), quantize_int8(t.contiguous())))
+    b = t[:1].expand(4, 64)
+    q, scale = quantize_int8(b)
+    assert (q == q[0]).all() and (scale == scale[0]).all()
+
+
+def test_nothing_is_written_past_the_rows(device):
+    """The C entry's outputs in the middle of larger buffers, at an odd width."""
+    from slipstream_amd import _ffi
+
+    rows, cols = 3, 1003
+    x = torch.randn(rows, cols, device=device)
+    for dtype in DTYPES:
+        xt = x.to(dtype)
+        q = torch.full((rows * cols + 64,), 77, dtype=torch.int8, device=device)
+        scale = torch.full((rows + 8,), 77.0, device=device)
+        s = torch.full((rows * cols + 64,), 77.0, dtype=dtype, device=device)
+        w = torch.ones(cols, dtype=dtype, device=device)
+        _ffi.check(_ffi.lib().ss_rmsnorm_int8(xt.data_ptr(), xt.data_ptr(), w.data_ptr(), q[32:].data_ptr(),
+                                              scale[4:].data_ptr(), s[32:].data_ptr(), rows, cols, cols, cols, 1e-6,
+                                              _ffi.dtype_code(dtype), _ffi.stream_ptr(device)), "norm")
+        want = fused_rmsnorm_int8(xt, w, xt)
+        torch.cuda.synchronize()
+        for got, ref, edge in ((q, want[0], 32), (scale, want[1], 4), (s, want[2], 32)):
+            n = ref.numel()
+            assert torch.equal(got[edge : edge + n], ref.reshape(-1))
+            assert (got[:edge] == 77).all() and (got[edge + n :] == 77).all()
+
+
+def test_more_bytes_than_31_bits_hold(device):
+    """Rows whose addresses pass 2^31 and 2^32 bytes: the last ones are as they are alone."""
+    rows, cols = 280_000, 8192  # 4.6 GB in bf16
+    x = torch.zeros((rows, cols), dtype=torch.bfloat16, device=device)
+    tail = torch.randn(3, cols, device=device).to(torch.bfloat16)
+    x[-3:] = tail
+    q, scale = quantize_int8(x)
+    q1, scale1 = quantize_int8(tail)
+    assert torch.equal(q[-3:], q1) and torch.equal(scale[-3:], scale1)
+    assert not scale[:-3].any() and not q[rows // 2].any()
