@@ -21,6 +21,24 @@ struct W8Params {
   int bias_dtype;
 };
 
+// The tile kernel (w8a8_tile.hip): a workgroup's tokens and channels, its grid and K split.
+struct TilePlan {
+  int bm, bn;
+  int ks, per;  // K ranges and 128-key stages per range
+  int n_tiles, m_blocks;
+};
+// The stream kernel (w8a8_stream.hip): a workgroup's 16-row tiles of tokens and channels, its
+// waves and its grid.
+struct StreamPlan {
+  int mt, nt, waves;
+  int n_tiles, m_blocks;
+};
+double plan_w8a8_stream(StreamPlan& pl, int64_t m, int64_t n, int64_t k);  // estimated us
+int launch_w8a8_stream(const W8Params& p, const StreamPlan& pl, int out_dtype, hipStream_t stream);
+
+double plan_w8a8_tile(TilePlan& pl, int64_t m, int64_t n, int64_t k, bool may_split);  // estimated us
+int launch_w8a8_tile(const W8Params& p, const TilePlan& pl, int out_dtype, int* part, hipStream_t stream);
+
 namespace {
 
 // c += a b over 64 keys: lane l's sixteen bytes of a are keys 16 (l / 16) .. + 15 of row l % 16
@@ -40,6 +58,42 @@ __device__ __forceinline__ float load_as_f32(const void* p, int64_t i, int dtype
 // type: three roundings in fp32 (four with a bias).
 __device__ __forceinline__ float scaled(int sum, float xs, float ws, float bias) {
   return fmaf((float)sum * xs, ws, bias);
+}
+
+// N consecutive results, 16-byte aligned
+template <int N>
+__device__ __forceinline__ void store_results(float* o, const float (&y)[N]) {
+#pragma unroll
+  for (int e = 0; e < N; e += 4)
+    store16(o + e, u32x4{__builtin_bit_cast(uint32_t, y[e]), __builtin_bit_cast(uint32_t, y[e + 1]),
+                         __builtin_bit_cast(uint32_t, y[e + 2]), __builtin_bit_cast(uint32_t, y[e + 3])});
+}
+template <int N, typename T>
+__device__ __forceinline__ void store_results(T* o, const float (&y)[N]) {
+#pragma unroll
+  for (int e = 0; e < N; e += 8)
+    store16(o + e, u32x4{Elem<T>::pack2(y[e], y[e + 1]), Elem<T>::pack2(y[e + 2], y[e + 3]),
+                         Elem<T>::pack2(y[e + 4], y[e + 5]), Elem<T>::pack2(y[e + 6], y[e + 7])});
+}
+
+// A raw buffer descriptor over [base, base + bytes) as four scalars: offsets past the end read
+// zeros without a memory access.
+__device__ __forceinline__ i32x4 buffer_words(const void* base, uint32_t bytes) {
+  const uint64_t a = (uint64_t)base;
+  return i32x4{(int)(uint32_t)a, (int)((uint32_t)(a >> 32) & 0xFFFF), (int)bytes, 0x00020000};
+}
+
+// 16 bytes per lane from rs + voff + soff straight into LDS at lds + 16 * lane (M0 holds the
+// LDS destination, written just before: the load may read it one wait state later). Written
+// as asm, with no register to write, so that the compiler's waits do not count it: the
+// kernel waits itself.
+typedef __attribute__((address_space(3))) char* LdsBytes;
+__device__ __forceinline__ void dma_b128(i32x4 rs, LdsBytes lds, int voff, int soff) {
+  const uint32_t m0 = (uint32_t)(uintptr_t)lds;
+  asm volatile("s_nop 1\n\tbuffer_load_dwordx4 %0, %1, %2 offen lds"
+               :
+               : "v"(voff), "s"(rs), "s"(soff), "{m0}"(m0)
+               : "memory");
 }
 
 }  // namespace

@@ -1,0 +1,213 @@
+// W8A8 stream kernel: the int8 product for few tokens, where the weights' bytes set the time.
+//
+// A workgroup of up to eight waves multiplies 16 MT tokens with 16 NT channels; its waves share
+// out the keys, 128 at a time in turn. A wave brings its 128 keys of every row by DMA into a
+// part of the LDS that is its own, two blocks in turn, and reads the matrix
+// instruction's operands from there: no wave waits for another before the end, where the
+// integer sums are added in the LDS, in any order the same result. (Loaded straight into the
+// operands' registers, sixteen lanes in a row touch sixteen cache lines, and the address
+// unit, not the memory, sets the time: 16 x 4096 x 14336 15.0 us.)
+#include "w8a8_common.h"
+
+namespace ss {
+namespace {
+
+constexpr int kFar = 0x40000000;  // a byte offset past any operand tile (host-checked)
+constexpr int kPlane = 68;        // LDS words of the 64 lanes' sums of one accumulator register
+
+// 16-byte chunk c of row r of a 16-row tile lies at chunk c ^ swizzle of its 128 LDS bytes. A
+// 16-byte LDS read takes lanes 0-3, 12-15, 20-27 first, then 4-11, 16-19, 28-31, and the same
+// of the upper half: rows 0-3 and 12-15 of one key group and rows 4-11 of the next, whose
+// chunk differs by 2. Rows 2p and 2p + 1 lie in different halves of the banks; this value
+// keeps the row pairs of a pass apart.
+__device__ __forceinline__ int stream_swizzle(int r) {
+  const int p = r >> 1;
+  return (((p >> 2) ^ (p >> 1)) & 1) << 2 | ((p >> 2) & 1) << 1 | (p & 1);
+}
+
+// a wave's blocks on their way, or in work
+constexpr int D = 2;
+// bytes of a block (128 keys of the weights' and tokens' rows), and of a workgroup's LDS
+constexpr int block_bytes(int mt, int nt) { return (16 * nt + 16 * mt) * 128; }
+constexpr int stream_lds_bytes(int mt, int nt, int waves) {
+  return waves * D * block_bytes(mt, nt) + mt * nt * 4 * kPlane * 4;
+}
+
+// XI: groups of eight tokens that are read (2 MT, or 1 of MT = 1); the rows of the others hold
+// anything, and their sums are not stored.
+template <typename TO, int MT, int NT, int XI>
+__global__ __launch_bounds__(512) void w8a8_stream_kernel(const W8Params p, int n_tiles, int m_blocks) {
+  constexpr int B = block_bytes(MT, NT), ND = 2 * NT + XI;
+  extern __shared__ __attribute__((aligned(16))) char s_dyn[];  // [waves][D][B], then the sums
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+  const int ln = lane & 15, kg = lane >> 4;
+  int* const s_sum = reinterpret_cast<int*>(s_dyn + waves * D * B);
+  // each XCD (workgroups go round robin over the eight) takes a contiguous eighth of the list,
+  // in which the token blocks of a channel tile follow each other: its L2 serves their weights
+  const int total = n_tiles * m_blocks, per_xcd = (total + 7) >> 3;
+  const int item = (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
+  if ((int)(blockIdx.x >> 3) >= per_xcd || item >= total) return;
+  const int64_t n0 = (int64_t)(item / m_blocks) * (16 * NT), m0 = (int64_t)(item % m_blocks) * (16 * MT);
+  const int rows = (int)min((int64_t)(16 * MT), p.m - m0), chans = (int)min((int64_t)(16 * NT), p.n - n0);
+
+  // a DMA instruction brings eight rows of 128 bytes; lane l byte 16 (l % 8) of row l / 8, which
+  // holds chunk (l % 8) ^ swizzle. Rows past the end and, in the last 128 keys, chunks past k
+  // get an offset outside the descriptors: zeros without an access.
+  const i32x4 rx = buffer_words(p.x + m0 * p.x_stride, (uint32_t)((rows - 1) * (int)p.x_stride + p.k));
+  const i32x4 rw = buffer_words(p.w + n0 * p.w_stride, (uint32_t)((chans - 1) * (int)p.w_stride + p.k));
+  const int r8 = lane >> 3;
+  const int chunk[2] = {16 * ((lane & 7) ^ stream_swizzle(r8)), 16 * ((lane & 7) ^ stream_swizzle(8 + r8))};
+  int off[ND];
+#pragma unroll
+  for (int u = 0; u < 2 * NT; ++u) off[u] = 8 * u + r8 < chans ? (8 * u + r8) * (int)p.w_stride + chunk[u & 1] : kFar;
+#pragma unroll
+  for (int u = 0; u < XI; ++u)
+    off[2 * NT + u] = 8 * u + r8 < rows ? (8 * u + r8) * (int)p.x_stride + chunk[u & 1] : kFar;
+  const int blocks = (p.k + 127) >> 7, last = blocks - 1;
+  const int past[2] = {last * 128 + chunk[0] >= p.k ? kFar : 0, last * 128 + chunk[1] >= p.k ? kFar : 0};
+  const int count = wave < blocks ? (blocks - wave + waves - 1) / waves : 0;  // of this wave: wave, wave + waves, ...
+  const LdsBytes ring = (LdsBytes)s_dyn + wave * D * B;
+  asm volatile("s_nop 4");  // descriptor SGPRs written by VALU before the first asm load
+  auto request = [&](int i, int slot) {  // the wave's block i
+    const int at = wave + i * waves;
+    const int so = __builtin_amdgcn_readfirstlane(at * 128);
+    const int base = __builtin_amdgcn_readfirstlane(slot * B);
+    const int add[2] = {at == last ? past[0] : 0, at == last ? past[1] : 0};
+    asm volatile("s_nop 4" : : "s"(so), "s"(base));  // VALU-written SGPRs: five wait states before a VMEM reads them
+#pragma unroll
+    for (int u = 0; u < ND; ++u) dma_b128(u < 2 * NT ? rw : rx, ring + base + u * 1024, off[u] + add[u & 1], so);
+  };
+#pragma unroll
+  for (int d = 0; d < D; ++d)
+    if (d < count) request(d, d);
+  for (int i = threadIdx.x; i < MT * NT * 4 * kPlane; i += blockDim.x) s_sum[i] = 0;
+
+  // fragment of lane (ln, kg): row ln, key step s: chunk 2 kg + s
+  const int f[2] = {ln * 128 + 16 * ((2 * kg) ^ stream_swizzle(ln)), ln * 128 + 16 * ((2 * kg + 1) ^ stream_swizzle(ln))};
+  const char* const mine = s_dyn + wave * D * B;
+  i32x4 acc[NT][MT] = {};
+  int slot = 0;
+  for (int i = 0; i < count; ++i) {
+    if (count - i >= D)
+      asm volatile("s_waitcnt vmcnt(%0)" : : "n"((D - 1) * ND) : "memory");
+    else
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    i32x4 a[2][NT], b[2][MT];
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t) a[s][t] = *reinterpret_cast<const i32x4*>(mine + slot * B + t * 2048 + f[s]);
+#pragma unroll
+      for (int t = 0; t < MT; ++t) b[s][t] = *reinterpret_cast<const i32x4*>(mine + slot * B + (NT + t) * 2048 + f[s]);
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // read: the block's place is free
+    if (i + D < count) request(i + D, slot);
+    slot = slot + 1 == D ? 0 : slot + 1;
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int u = 0; u < MT; ++u) acc[t][u] = mfma_i8(a[s][t], b[s][u], acc[t][u]);
+  }
+  __syncthreads();  // the sums are cleared
+  if (count > 0) {
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int u = 0; u < MT; ++u)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          __hip_atomic_fetch_add(&s_sum[((t * MT + u) * 4 + e) * kPlane + lane], acc[t][u][e], __ATOMIC_RELAXED,
+                                 __HIP_MEMORY_SCOPE_WORKGROUP);
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < 256 * MT * NT; i += blockDim.x) {
+    const int r = i / (16 * NT), c = i % (16 * NT);
+    if (r < rows && c < chans) {
+      const int64_t m = m0 + r, n = n0 + c;
+      const int sum = s_sum[(((c >> 4) * MT + (r >> 4)) * 4 + (c & 3)) * kPlane + 16 * ((c & 15) >> 2) + (r & 15)];
+      ((TO*)p.out)[m * p.o_stride + n] =
+          (TO)scaled(sum, p.x_scale[m], p.w_scale[n], p.bias ? load_as_f32(p.bias, n, p.bias_dtype) : 0.f);
+    }
+  }
+}
+
+template <typename TO, int MT, int NT, int XI>
+int launch_stream(const W8Params& p, const StreamPlan& pl, hipStream_t stream) {
+  auto kern = w8a8_stream_kernel<TO, MT, NT, XI>;
+  const int lds = stream_lds_bytes(MT, NT, pl.waves);
+  // (each call: the attribute belongs to the function on the current device)
+  if (lds > 65536 &&
+      hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess) {
+    ss_host::set_error("w8a8 gemm: cannot reserve %d bytes of LDS", lds);
+    return SS_ERR_UNSUPPORTED;
+  }
+  const int64_t grid = ((int64_t)pl.n_tiles * pl.m_blocks + 7) / 8 * 8;
+  hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(64 * pl.waves), lds, stream, p, pl.n_tiles, pl.m_blocks);
+  return ss_host::launch_status("w8a8 gemm (stream)");
+}
+
+// 16-row tiles of tokens and of channels of a workgroup
+#define W8A8_STREAMS(X) X(1, 1) X(1, 2) X(2, 1) X(2, 2) X(4, 2) X(4, 4)
+
+template <typename TO>
+int launch_stream_typed(const W8Params& p, const StreamPlan& pl, hipStream_t stream) {
+#define W8A8_LAUNCH(MT, NT)                                                      \
+  if (pl.mt == MT && pl.nt == NT) {                                              \
+    if (MT == 1 && p.m <= 8) return launch_stream<TO, MT, NT, 1>(p, pl, stream); \
+    return launch_stream<TO, MT, NT, 2 * MT>(p, pl, stream);                     \
+  }
+  W8A8_STREAMS(W8A8_LAUNCH)
+#undef W8A8_LAUNCH
+  ss_host::set_error("w8a8 gemm: stream tile of %d x %d", pl.mt, pl.nt);
+  return SS_ERR_UNSUPPORTED;
+}
+
+}  // namespace
+
+// The tile and waves of least estimated time (us), fitted to the times of 2500 calls (every tile
+// and number of waves at 100 shapes of up to 512 tokens; 8 % off on average): a round's
+// start, a wave's blocks one after another, the adding of the sums and the results, the
+// operands' way through a CU and out of the L2, and the weights' out of the memory.
+double plan_w8a8_stream(StreamPlan& pl, int64_t m, int64_t n, int64_t k) {
+#define W8A8_SIZE(MT, NT) {MT, NT},
+  static const int kTiles[][2] = {W8A8_STREAMS(W8A8_SIZE)};
+#undef W8A8_SIZE
+  const int64_t cus = ss_host::device_cu_count(), blocks = (k + 127) / 128;
+  double best = 1e30;
+  if (m > 512) return best;
+  for (const auto& t : kTiles) {
+    const int mt = t[0], nt = t[1];
+    if (mt > 1 && 8 * mt >= m) continue;
+    const int64_t n_tiles = (n + 16 * nt - 1) / (16 * nt), m_blocks = (m + 16 * mt - 1) / (16 * mt);
+    if (n_tiles * m_blocks > 0x7ffffff) continue;
+    const int64_t groups = n_tiles * m_blocks, a_cu = (groups + cus - 1) / cus;
+    const double bytes = (16.0 * nt + (m < 16 * mt ? m : 16 * mt)) * blocks * 128;
+    // two waves only beyond 16 tokens (28672 x 4096 at m = 1 26.2 us with two, 22.3 with four)
+    for (int waves = m > 16 ? 2 : 4; waves <= 8; waves *= 2) {
+      const int64_t lds = stream_lds_bytes(mt, nt, waves);
+      if (lds > 160 * 1024) continue;
+      int64_t fit = 160 * 1024 / lds;
+      fit = fit < 32 / waves ? fit : 32 / waves;
+      const double rounds = (double)((groups + cus * fit - 1) / (cus * fit)), each = (double)((blocks + waves - 1) / waves);
+      const double us = 1.0 + rounds * (0.87 + each * (0.0134 + 0.0048 * (mt + nt) + 0.0077 * mt * nt) +
+                                        mt * nt * (0.114 + 0.68 / waves)) +
+                        a_cu * (bytes * 4.7e-6 + 0.0019 * waves) + groups * bytes * 1.08e-8 + n * k * 8.3e-8;
+      if (us < best) {
+        best = us;
+        pl = {mt, nt, waves, (int)n_tiles, (int)m_blocks};
+      }
+    }
+  }
+  return best;
+}
+
+int launch_w8a8_stream(const W8Params& p, const StreamPlan& pl, int out_dtype, hipStream_t stream) {
+  if (out_dtype == SS_DTYPE_BF16) return launch_stream_typed<bf16_t>(p, pl, stream);
+  if (out_dtype == SS_DTYPE_F16) return launch_stream_typed<f16_t>(p, pl, stream);
+  return launch_stream_typed<float>(p, pl, stream);
+}
+
+}  // namespace ss

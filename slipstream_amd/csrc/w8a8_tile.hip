@@ -1,0 +1,426 @@
+// W8A8 tile kernel: the int8 product at the sizes where the matrix cores set the time (a prefill
+// chunk's or a packed step's tokens).
+//
+// Four waves, one per SIMD, in a 2 x 2 grid multiply 32 MT tokens with 32 NT channels, wave
+// (wm, wn) 16 MT x 16 NT of them. Both operands come into LDS by DMA, 128 keys of every row a
+// stage, two stages in turn. A wave holds the fragments of half a stage (64 keys) in registers
+// while it multiplies them and reads the next half's beside the products, so a stage's LDS is
+// free again once its second half has been read, long before it is multiplied:
+//   first half's products:  the second half's fragments are read, then (barrier) the stage's
+//                           LDS is free and the DMAs of the stage after the next begin
+//   second half's products: the DMAs go on; the next stage's, a whole stage old, have landed
+//                           (wait, barrier) and its first half's fragments are read
+// One wave per SIMD has nothing to hide behind, so the order is written out: every product is
+// followed by at most one fragment read or DMA, and the scheduler is held to that order.
+#include <type_traits>
+#include <utility>
+
+#include "w8a8_common.h"
+
+namespace ss {
+namespace {
+
+// Position of 16-byte chunk c of row r within the row's 128 LDS bytes: c ^ tile_swizzle(r).
+// A 16-byte LDS read runs in four passes of sixteen lanes, lanes 0-3, 12-15, 20-27 first,
+// then 4-11, 16-19, 28-31, and the same of the upper half. The rows 2p and 2p + 1 lie in
+// different halves of the 64 banks, and the row pairs of each pass differ in p % 8.
+__device__ __forceinline__ int tile_swizzle(int r) { return (r >> 1) & 7; }
+
+template <typename F, int... I>
+__device__ __forceinline__ void static_for_impl(F&& f, std::integer_sequence<int, I...>) {
+  (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, typename F>
+__device__ __forceinline__ void static_for(F&& f) {
+  static_for_impl(f, std::make_integer_sequence<int, N>{});
+}
+
+// acc += a b on the matrix core over 32 keys: lane l's sixteen bytes of a are keys
+// 16 (l / 32) .. + 15 of channel l % 32 (of b: of token l % 32); its results are channels
+// 8 (r / 4) + 4 (l / 32) + r % 4 of token l % 32. The accumulator stays in AGPRs. Written as
+// asm because the compiler moves accumulators between the register files in every stage.
+// What it therefore does not look after: the operands come from LDS reads, which it does wait
+// for; an accumulator is touched once in MT NT products or more; and between the last
+// product and what follows the loop stand the waits there.
+typedef int i32x16 __attribute__((ext_vector_type(16)));
+__device__ __forceinline__ void mfma_acc(i32x16& acc, i32x4 a, i32x4 b) {
+  asm volatile("v_mfma_i32_32x32x32_i8 %0, %1, %2, %0" : "+a"(acc) : "v"(a), "v"(b));
+}
+
+constexpr int kFar = 0x40000000;  // a byte offset past any operand tile (host-checked)
+
+// LDS stages of the tokens and of the channels (rows of 128 bytes) for a tile: as many as 160 KB
+// hold, the tokens' first, at most six.
+constexpr int kLdsBytes = 160 * 1024;
+constexpr int channel_stages(int bm, int bn) {
+  int d = 2;
+  while (d < 6 && (d + 1) * (bm + bn) * 128 <= kLdsBytes) ++d;
+  return d;
+}
+constexpr int token_stages(int bm, int bn) {
+  const int d = channel_stages(bm, bn);
+  return d < 6 && ((d + 1) * bm + d * bn) * 128 <= kLdsBytes ? d + 1 : d;
+}
+
+// TO int: a K range's sums, for the reduce kernel
+template <typename TO, int MT, int NT, int WM>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) void w8a8_tile_kernel(
+    const W8Params p, int per, int ks, int n_tiles, int m_blocks, int band) {
+  constexpr int WN = 4 / WM, BM = 32 * MT * WM, BN = 32 * NT * WN;
+  constexpr int DX = token_stages(BM, BN), DW = channel_stages(BM, BN);
+  constexpr int XB = BM * 128, WB = BN * 128;          // LDS bytes of a stage
+  constexpr int NX = BM / 32, NW = BN / 32, ND = NX + NW;  // DMA instructions of a wave and stage
+  constexpr int NF = 2 * (MT + NT);                    // fragments of half a stage
+  extern __shared__ __attribute__((aligned(16))) char s_dyn[];
+
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int ln = lane & 31, kg = lane >> 5;
+  const int wm = wave % WM, wn = wave / WM;
+  // workgroup -> (K range, channel tile, token block): each XCD (workgroups go round robin over
+  // the eight) takes a contiguous eighth of the list. In it bands of `band` token blocks
+  // follow each other, in a band the (channel tile, K range) pairs, in those the band's blocks,
+  // so that the workgroups that run at once on an XCD share few rows of both operands.
+  const int total = ks * n_tiles * m_blocks, per_xcd = (total + 7) >> 3;
+  const int item = (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
+  if ((int)(blockIdx.x >> 3) >= per_xcd || item >= total) return;
+  const int in_band = band * n_tiles * ks;
+  const int mb0 = item / in_band * band, left = item - mb0 * n_tiles * ks;
+  const int here = min(band, m_blocks - mb0);
+  const int pair = left / here;
+  const int zr = pair % ks;
+  const int64_t n0 = (int64_t)(pair / ks) * BN;
+  const int64_t m0 = (int64_t)(mb0 + left - pair * here) * BM;
+  const int rows = (int)min((int64_t)BM, p.m - m0), chans = (int)min((int64_t)BN, p.n - n0);
+  const int stages = (p.k + 127) >> 7;
+  const int i0 = zr * per, i1 = min(stages, i0 + per);
+
+  // ---- operands: a DMA instruction brings eight LDS rows of 128 bytes; lane l byte 16 (l % 8)
+  // of row l / 8, which holds chunk (l % 8) ^ swizzle. Instruction u of wave w: LDS rows
+  // 8 (4 u + w) .. + 7. Rows past the end and, in the last stage, chunks past k get an offset
+  // outside the descriptors: zeros without an access.
+  const i32x4 rx = buffer_words(p.x + m0 * p.x_stride, (uint32_t)((rows - 1) * (int)p.x_stride + p.k));
+  const i32x4 rw = buffer_words(p.w + n0 * p.w_stride, (uint32_t)((chans - 1) * (int)p.w_stride + p.k));
+  const int row8 = 8 * wave + (lane >> 3);
+  const int chunk = 16 * ((lane & 7) ^ tile_swizzle(row8));
+  int off[ND];  // channels first
+#pragma unroll
+  for (int u = 0; u < NW; ++u) off[u] = 32 * u + row8 < chans ? (32 * u + row8) * (int)p.w_stride + chunk : kFar;
+#pragma unroll
+  for (int u = 0; u < NX; ++u) off[NW + u] = 32 * u + row8 < rows ? (32 * u + row8) * (int)p.x_stride + chunk : kFar;
+  const int past = (stages - 1) * 128 + chunk >= p.k ? kFar : 0;  // of the last stage
+  const LdsBytes lds = (LdsBytes)s_dyn + wave * 1024;
+  // DMAs of one window: the channels of a stage into their slot, then the tokens of a stage
+  struct Side {
+    int so, add, slot;  // scalar offset, tail offset, LDS slot (bytes)
+  } dw = {0, 0, 0}, dx = {0, 0, 0};
+  auto aim = [&](Side& d, int i, int next_slot) {  // stage i (past the range: the last one again, never read)
+    const int at = min(i, i1 - 1);
+    d.so = __builtin_amdgcn_readfirstlane(at * 128);
+    d.add = at == stages - 1 ? past : 0;
+    d.slot = __builtin_amdgcn_readfirstlane(next_slot);
+    asm volatile("s_nop 4" : : "s"(d.so), "s"(d.slot));  // VALU-written SGPRs: five wait states before a VMEM reads them
+  };
+  auto dma = [&](auto uc) __attribute__((always_inline)) {
+    constexpr int u = uc;
+    if constexpr (u < NW)
+      dma_b128(rw, lds + DX * XB + dw.slot + u * 4096, off[u] + dw.add, dw.so);
+    else
+      dma_b128(rx, lds + dx.slot + (u - NW) * 4096, off[u] + dx.add, dx.so);
+  };
+  auto after = [](int slot, int bytes, int depth) { return slot + bytes == depth * bytes ? 0 : slot + bytes; };
+
+  // ---- scales, requested first of all: the results wait for nothing then
+  constexpr int CL = 16 / sizeof(TO), LR = 32 * NT / CL;  // channels of a lane, lanes of a token in the store
+  const int c = lane % LR * CL;
+  const int64_t n = n0 + 32 * NT * wn + c;
+  float xs[MT], ws[CL], bias[CL];
+  if constexpr (!__is_same(TO, int)) {
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) xs[mt] = p.x_scale[min(m0 + 32 * (MT * wm + mt) + ln, p.m - 1)];
+#pragma unroll
+    for (int e = 0; e < CL; ++e) {
+      const int64_t at = min(n + e, p.n - 1);
+      ws[e] = p.w_scale[at];
+      bias[e] = p.bias ? load_as_f32(p.bias, at, p.bias_dtype) : 0.f;
+    }
+  }
+
+  // fragment of lane (ln, kg): row ln of a 32-row tile; step s of the four of a stage: chunk
+  // 2 s + kg. Half h of a stage: steps 2 h and 2 h + 1.
+  int f[4];
+#pragma unroll
+  for (int s = 0; s < 4; ++s) f[s] = ln * 128 + 16 * ((2 * s + kg) ^ tile_swizzle(ln));
+  const int xb = wm * MT * 4096, wb = DX * XB + wn * NT * 4096;
+  i32x4 a[2][2][NT], b[2][2][MT];  // channels' and tokens' fragments of the half in work and the next
+  int rxs = 0, rws = 0;            // slots of the stage that is read
+  auto read = [&](auto hc, auto uc) __attribute__((always_inline)) {
+    constexpr int h = hc, s = uc / (MT + NT), u = uc % (MT + NT);
+    const char* const at = (const char*)s_dyn + f[2 * h + s];
+    if constexpr (u < NT)
+      a[h][s][u] = *reinterpret_cast<const i32x4*>(at + wb + rws + u * 4096);
+    else
+      b[h][s][u - NT] = *reinterpret_cast<const i32x4*>(at + xb + rxs + (u - NT) * 4096);
+  };
+
+  i32x16 acc[NT][MT];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) acc[nt][mt] = i32x16{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+
+  // Slots after the P products of each half: window DMAs run from kFree of the first half to
+  // the end of the second, the channels' (whose LDS holds fewer stages) in the first P / 2.
+  constexpr int P = 2 * MT * NT;
+  constexpr int kFree = P * 5 / 8;     // the barrier after which the stage's LDS is free
+  constexpr int kLanded = P * 7 / 16;  // of the second half: the next stage has landed
+  constexpr int kSpan = 2 * P - kFree, kChan = P / 2, kRead1 = P - kLanded;
+  constexpr auto issued = [](int v) constexpr {
+    return v <= kChan ? v * NW / kChan : NW + (v - kChan) * NX / (kSpan - kChan);
+  };
+  // DMAs that may be on their way when stage i + 1 has to have landed, c of window i issued
+  constexpr auto newer = [](int c) constexpr {
+    const int w = (DW - 2) * ND + NX + c, x = (DX - 2) * ND + c;
+    return w < x ? w : x;
+  };
+
+  asm volatile("s_nop 4");  // descriptor SGPRs written by VALU before the first asm load
+  static_for<DX>([&](auto jc) __attribute__((always_inline)) {
+    constexpr int j = jc - DX;  // the window of stage i0 + j
+    if constexpr (j + DW >= 0) {
+      aim(dw, i0 + j + DW, (j + DW) * WB);
+      static_for<NW>(dma);
+    }
+    aim(dx, i0 + j + DX, (j + DX) * XB);
+    static_for<NX>([&](auto uc) __attribute__((always_inline)) { dma(std::integral_constant<int, NW + uc>{}); });
+  });
+  asm volatile("s_waitcnt vmcnt(%0)" : : "n"(newer(ND)) : "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+  static_for<NF>([&](auto uc) __attribute__((always_inline)) { read(std::integral_constant<int, 0>{}, uc); });
+  int fx = 0, fw = 0;  // slots that the next window's DMAs fill: those of the stage in work
+
+  for (int i = i0; i < i1; ++i) {
+    static_for<P>([&](auto tc) __attribute__((always_inline)) {
+      constexpr int t = tc, s = t / (MT * NT), nt = t / MT % NT, mt = t % MT;
+      if constexpr (t < kFree)
+        static_for<(t + 1) * NF / kFree - t * NF / kFree>([&](auto qc) __attribute__((always_inline)) {
+          read(std::integral_constant<int, 1>{}, std::integral_constant<int, t * NF / kFree + qc>{});
+        });
+      if constexpr (t == kFree) {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        aim(dw, i + DW, fw);
+        aim(dx, i + DX, fx);
+        rxs = fx = after(fx, XB, DX);
+        rws = fw = after(fw, WB, DW);
+      }
+      if constexpr (t >= kFree) {
+        constexpr int v = t - kFree;
+        static_for<issued(v + 1) - issued(v)>([&](auto qc) __attribute__((always_inline)) {
+          dma(std::integral_constant<int, issued(v) + qc>{});
+        });
+      }
+      mfma_acc(acc[nt][mt], a[0][s][nt], b[0][s][mt]);
+      __builtin_amdgcn_sched_barrier(0);
+    });
+    static_for<P>([&](auto tc) __attribute__((always_inline)) {
+      constexpr int t = tc, v = t + P - kFree, s = t / (MT * NT), nt = t / MT % NT, mt = t % MT;
+      if constexpr (t == kLanded) {
+        asm volatile("s_waitcnt vmcnt(%0)" : : "n"(newer(issued(v))) : "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+      }
+      if constexpr (t >= kLanded) {
+        constexpr int q0 = (t - kLanded) * NF / kRead1, q1 = (t - kLanded + 1) * NF / kRead1;
+        static_for<q1 - q0>([&](auto qc) __attribute__((always_inline)) {
+          read(std::integral_constant<int, 0>{}, std::integral_constant<int, q0 + qc>{});
+        });
+      }
+      static_for<issued(v + 1) - issued(v)>([&](auto qc) __attribute__((always_inline)) {
+        dma(std::integral_constant<int, issued(v) + qc>{});
+      });
+      mfma_acc(acc[nt][mt], a[1][s][nt], b[1][s][mt]);
+      __builtin_amdgcn_sched_barrier(0);
+    });
+  }
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");  // no DMA and no read of the LDS is on its way,
+  __builtin_amdgcn_s_barrier();                                // of any wave
+  asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");           // and the last products have landed
+
+  // ---- results: 32 tokens at a time through the wave's own part of the LDS, so that the lanes
+  // hold consecutive channels and a store writes whole rows of the wave's 32 NT channels
+  constexpr int RS = NT * 128 + 16;  // bytes of a token's sums there, and its scale behind them
+  static_assert(4 * 32 * RS <= (DX * BM + DW * BN) * 128, "the sums fit where the operands were");
+  char* const turn = s_dyn + wave * 32 * RS;
+  TO* const out = (TO*)p.out + (__is_same(TO, int) ? (int64_t)zr * p.m * p.o_stride : 0);
+  const bool vec = n + CL <= p.n && p.o_stride % CL == 0 && ((uintptr_t)p.out & 15) == 0;
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) {
+    const int64_t mb = m0 + 32 * (MT * wm + mt);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      asm volatile("" : "+a"(acc[nt][mt]));  // read behind the waits above
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        *reinterpret_cast<i32x4*>(turn + ln * RS + (32 * nt + 8 * g + 4 * kg) * 4) =
+            i32x4{acc[nt][mt][4 * g], acc[nt][mt][4 * g + 1], acc[nt][mt][4 * g + 2], acc[nt][mt][4 * g + 3]};
+    }
+    if constexpr (!__is_same(TO, int)) *reinterpret_cast<float*>(turn + ln * RS + NT * 128) = xs[mt];
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+    for (int q = 0; q < LR / 2; ++q) {
+      const int r = q * (64 / LR) + lane / LR;
+      const int64_t m = mb + r;
+      i32x4 sum[CL / 4];
+#pragma unroll
+      for (int h = 0; h < CL / 4; ++h) sum[h] = *reinterpret_cast<const i32x4*>(turn + r * RS + (c + 4 * h) * 4);
+      const float x_scale = *reinterpret_cast<const float*>(turn + r * RS + NT * 128);
+      if (m < p.m && n < p.n) {
+        TO* const o = out + m * p.o_stride + n;
+        if constexpr (__is_same(TO, int)) {
+          if (vec) {
+            *reinterpret_cast<i32x4*>(o) = sum[0];
+          } else {
+#pragma unroll
+            for (int e = 0; e < CL; ++e)
+              if (n + e < p.n) o[e] = sum[0][e];
+          }
+        } else {
+          float y[CL];
+#pragma unroll
+          for (int e = 0; e < CL; ++e) y[e] = scaled(sum[e / 4][e % 4], x_scale, ws[e], bias[e]);
+          if (vec) {
+            store_results<CL>(o, y);
+          } else {
+#pragma unroll
+            for (int e = 0; e < CL; ++e)
+              if (n + e < p.n) o[e] = (TO)y[e];
+          }
+        }
+      }
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // read before the next tokens are written
+  }
+}
+
+// The sums of ks K ranges, scaled and rounded: a thread four channels of a token.
+template <typename TO>
+__global__ __launch_bounds__(256) void w8a8_reduce_kernel(const W8Params p, const int* __restrict__ part, int ks) {
+  const int64_t quads = (p.n + 3) >> 2, total = p.m * quads, plane = p.m * p.n;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    const int64_t m = i / quads, n = 4 * (i - m * quads);
+    const int* src = part + m * p.n + n;
+    const float xs = p.x_scale[m];
+    TO* const o = (TO*)p.out + m * p.o_stride + n;
+    if (p.n % 4 == 0) {
+      i32x4 sum = *reinterpret_cast<const i32x4*>(src);
+      for (int z = 1; z < ks; ++z) sum += *reinterpret_cast<const i32x4*>(src + z * plane);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        o[e] = (TO)scaled(sum[e], xs, p.w_scale[n + e], p.bias ? load_as_f32(p.bias, n + e, p.bias_dtype) : 0.f);
+    } else {
+      for (int e = 0; e < 4 && n + e < p.n; ++e) {
+        int sum = 0;
+        for (int z = 0; z < ks; ++z) sum += src[z * plane + e];
+        o[e] = (TO)scaled(sum, xs, p.w_scale[n + e], p.bias ? load_as_f32(p.bias, n + e, p.bias_dtype) : 0.f);
+      }
+    }
+  }
+}
+
+template <typename TO, int MT, int NT, int WM>
+int launch_tile(const W8Params& p, const TilePlan& pl, hipStream_t stream) {
+  auto kern = w8a8_tile_kernel<TO, MT, NT, WM>;
+  constexpr int bm = 32 * MT * WM, bn = 32 * NT * (4 / WM);
+  constexpr int lds = (token_stages(bm, bn) * bm + channel_stages(bm, bn) * bn) * 128;
+  // (each call: the attribute belongs to the function on the current device)
+  if (lds > 65536 &&
+      hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess) {
+    ss_host::set_error("w8a8 gemm: cannot reserve %d bytes of LDS", lds);
+    return SS_ERR_UNSUPPORTED;
+  }
+  // bands of at most 8 token blocks, of one size where they can be
+  const int bands = (pl.m_blocks + 7) / 8, band = (pl.m_blocks + bands - 1) / bands;
+  const int64_t grid = ((int64_t)pl.ks * pl.n_tiles * pl.m_blocks + 7) / 8 * 8;
+  hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(256), lds, stream, p, pl.per, pl.ks, pl.n_tiles, pl.m_blocks,
+                     band);
+  return ss_host::launch_status("w8a8 gemm (tile)");
+}
+
+// A tile's tokens and channels, and its waves' 32 x 32 tiles (MT, NT) and grid (WM x 4 / WM)
+#define W8A8_TILES(X) \
+  X(256, 256, 4, 4, 2) X(224, 256, 7, 2, 1) X(192, 256, 3, 4, 2) X(160, 256, 5, 2, 1) X(128, 256, 2, 4, 2) \
+  X(256, 128, 4, 2, 2) X(192, 128, 3, 2, 2) X(128, 128, 2, 2, 2) \
+  X(96, 128, 3, 1, 1) X(64, 128, 2, 1, 1)
+
+template <typename TO>
+int launch_tile_typed(const W8Params& p, const TilePlan& pl, hipStream_t stream) {
+#define W8A8_LAUNCH(BM, BN, MT, NT, WM) \
+  if (pl.bm == BM && pl.bn == BN) return launch_tile<TO, MT, NT, WM>(p, pl, stream);
+  W8A8_TILES(W8A8_LAUNCH)
+#undef W8A8_LAUNCH
+  ss_host::set_error("w8a8 gemm: tile of %d x %d", pl.bm, pl.bn);
+  return SS_ERR_UNSUPPORTED;
+}
+
+template <typename TO>
+int launch_reduce(const W8Params& p, const int* part, int ks, hipStream_t stream) {
+  const int64_t blocks = (p.m * ((p.n + 3) / 4) + 255) / 256, cap = (int64_t)ss_host::device_cu_count() * 8;
+  hipLaunchKernelGGL(w8a8_reduce_kernel<TO>, dim3((unsigned)(blocks < cap ? blocks : cap)), dim3(256), 0, stream, p,
+                     part, ks);
+  return ss_host::launch_status("w8a8 gemm (reduce)");
+}
+
+}  // namespace
+
+// The tile and K split of least estimated time (us), fitted to the times of 3700 calls (tiles and
+// splits of 160 shapes, 1 to 2240 tokens, 0.9 to 120 million weights; 8 % off on average): what a
+// stage of a round of workgroups takes, the start and the results of each round, the operands'
+// way into the LDS, the memory's share, and for a split the sums' way out and back and
+// the launch that adds them.
+double plan_w8a8_tile(TilePlan& pl, int64_t m, int64_t n, int64_t k, bool may_split) {
+#define W8A8_SIZE(BM, BN, MT, NT, WM) {BM, BN},
+  static const int kTiles[][2] = {W8A8_TILES(W8A8_SIZE)};
+#undef W8A8_SIZE
+  const int64_t stages = (k + 127) / 128, cus = ss_host::device_cu_count();
+  double best = 1e30;
+  for (const auto& t : kTiles) {
+    const int64_t n_tiles = (n + t[1] - 1) / t[1], m_blocks = (m + t[0] - 1) / t[0];
+    if (n_tiles * m_blocks > 0x7ffffff) continue;
+    for (int64_t ks = 1; ks <= (may_split ? 14 : 1); ks += ks < 4 ? 1 : 2) {
+      const int64_t per = (stages + ks - 1) / ks, groups = ks * n_tiles * m_blocks;
+      // a split of at least four stages each, for at most two rounds and a bit
+      if (ks > 1 && (per < 4 || groups > 600 || ks * m * n * 4 >= ((int64_t)1 << 31))) break;
+      if ((stages + per - 1) / per != ks) continue;
+      const double rounds = (double)((groups + cus - 1) / cus), area = t[0] * t[1] / 65536.0, edge = t[0] + t[1];
+      double us = 1.4 + rounds * (per * (0.046 + 0.57 * area + 0.195 * edge / 512) + 2.3 + 7.9 * area) +
+                  groups * per * edge * 128 * 2.2e-8 + n * k * 4.4e-8 + m * n * 3.8e-7;
+      if (ks > 1) us += 2.5 + ks * m * n * 4 * 3.15e-7;
+      if (us < best) {
+        best = us;
+        pl = {t[0], t[1], (int)ks, (int)per, (int)n_tiles, (int)m_blocks};
+      }
+    }
+  }
+  return best;
+}
+
+int launch_w8a8_tile(const W8Params& p, const TilePlan& pl, int out_dtype, int* part, hipStream_t stream) {
+  if (pl.ks > 1) {
+    W8Params q = p;
+    q.out = part;
+    q.o_stride = p.n;
+    const int st = launch_tile_typed<int>(q, pl, stream);
+    if (st != SS_OK) return st;
+    if (out_dtype == SS_DTYPE_BF16) return launch_reduce<bf16_t>(p, part, pl.ks, stream);
+    if (out_dtype == SS_DTYPE_F16) return launch_reduce<f16_t>(p, part, pl.ks, stream);
+    return launch_reduce<float>(p, part, pl.ks, stream);
+  }
+  if (out_dtype == SS_DTYPE_BF16) return launch_tile_typed<bf16_t>(p, pl, stream);
+  if (out_dtype == SS_DTYPE_F16) return launch_tile_typed<f16_t>(p, pl, stream);
+  return launch_tile_typed<float>(p, pl, stream);
+}
+
+}  // namespace ss
