@@ -2,6 +2,8 @@
 // instruction and the scaled store of a result.
 #pragma once
 
+#include <atomic>
+
 #include "ss_common.h"
 
 namespace ss {
@@ -38,6 +40,20 @@ int launch_w8a8_stream(const W8Params& p, const StreamPlan& pl, int out_dtype, h
 
 double plan_w8a8_tile(TilePlan& pl, int64_t m, int64_t n, int64_t k, bool may_split);  // estimated us
 int launch_w8a8_tile(const W8Params& p, const TilePlan& pl, int out_dtype, int* part, hipStream_t stream);
+
+// Lets `kern` have `lds` bytes of dynamic LDS on the current device; `done` holds a bit for each
+// device where it has them already (the attribute belongs to the function on a device).
+inline int reserve_lds(const void* kern, int lds, std::atomic<uint64_t>& done) {
+  int device = 0;
+  const uint64_t bit = hipGetDevice(&device) == hipSuccess && device >= 0 && device < 64 ? 1ull << device : 0;
+  if (lds <= 65536 || (done.load(std::memory_order_relaxed) & bit)) return SS_OK;
+  if (hipFuncSetAttribute(kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess) {
+    ss_host::set_error("w8a8 gemm: cannot reserve %d bytes of LDS", lds);
+    return SS_ERR_UNSUPPORTED;
+  }
+  done.fetch_or(bit, std::memory_order_relaxed);
+  return SS_OK;
+}
 
 namespace {
 

@@ -12,6 +12,7 @@
 namespace ss {
 namespace {
 
+constexpr int kLdsBytes = 160 * 1024;
 constexpr int kFar = 0x40000000;  // a byte offset past any operand tile (host-checked)
 constexpr int kPlane = 68;        // LDS words of the 64 lanes' sums of one accumulator register
 
@@ -138,12 +139,9 @@ template <typename TO, int MT, int NT, int XI>
 int launch_stream(const W8Params& p, const StreamPlan& pl, hipStream_t stream) {
   auto kern = w8a8_stream_kernel<TO, MT, NT, XI>;
   const int lds = stream_lds_bytes(MT, NT, pl.waves);
-  // (each call: the attribute belongs to the function on the current device)
-  if (lds > 65536 &&
-      hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess) {
-    ss_host::set_error("w8a8 gemm: cannot reserve %d bytes of LDS", lds);
-    return SS_ERR_UNSUPPORTED;
-  }
+  static std::atomic<uint64_t> done{0};
+  constexpr int most = stream_lds_bytes(MT, NT, 8) < kLdsBytes ? stream_lds_bytes(MT, NT, 8) : kLdsBytes;
+  if (const int st = reserve_lds((const void*)kern, most, done); st != SS_OK) return st;
   const int64_t grid = ((int64_t)pl.n_tiles * pl.m_blocks + 7) / 8 * 8;
   hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(64 * pl.waves), lds, stream, p, pl.n_tiles, pl.m_blocks);
   return ss_host::launch_status("w8a8 gemm (stream)");
@@ -188,8 +186,8 @@ double plan_w8a8_stream(StreamPlan& pl, int64_t m, int64_t n, int64_t k) {
     // two waves only beyond 16 tokens (28672 x 4096 at m = 1 26.2 us with two, 22.3 with four)
     for (int waves = m > 16 ? 2 : 4; waves <= 8; waves *= 2) {
       const int64_t lds = stream_lds_bytes(mt, nt, waves);
-      if (lds > 160 * 1024) continue;
-      int64_t fit = 160 * 1024 / lds;
+      if (lds > kLdsBytes) continue;
+      int64_t fit = kLdsBytes / lds;
       fit = fit < 32 / waves ? fit : 32 / waves;
       const double rounds = (double)((groups + cus * fit - 1) / (cus * fit)), each = (double)((blocks + waves - 1) / waves);
       const double us = 1.0 + rounds * (0.87 + each * (0.0134 + 0.0048 * (mt + nt) + 0.0077 * mt * nt) +

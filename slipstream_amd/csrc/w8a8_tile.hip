@@ -335,12 +335,8 @@ int launch_tile(const W8Params& p, const TilePlan& pl, hipStream_t stream) {
   auto kern = w8a8_tile_kernel<TO, MT, NT, WM>;
   constexpr int bm = 32 * MT * WM, bn = 32 * NT * (4 / WM);
   constexpr int lds = (token_stages(bm, bn) * bm + channel_stages(bm, bn) * bn) * 128;
-  // (each call: the attribute belongs to the function on the current device)
-  if (lds > 65536 &&
-      hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess) {
-    ss_host::set_error("w8a8 gemm: cannot reserve %d bytes of LDS", lds);
-    return SS_ERR_UNSUPPORTED;
-  }
+  static std::atomic<uint64_t> done{0};
+  if (const int st = reserve_lds((const void*)kern, lds, done); st != SS_OK) return st;
   // bands of at most 8 token blocks, of one size where they can be
   const int bands = (pl.m_blocks + 7) / 8, band = (pl.m_blocks + bands - 1) / bands;
   const int64_t grid = ((int64_t)pl.ks * pl.n_tiles * pl.m_blocks + 7) / 8 * 8;

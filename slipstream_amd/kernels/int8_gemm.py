@@ -22,20 +22,21 @@ _WS_NEED: dict[tuple, int] = {}
 def check_w8a8_args(q: torch.Tensor, scale: torch.Tensor, qweight: torch.Tensor, w_scale: torch.Tensor,
                     bias: torch.Tensor | None) -> tuple[int, int]:
     """Shape and dtype checks; returns ``(out, in)``."""
-    if qweight.ndim != 2:
-        raise ValueError(f"qweight must be 2-D [out, in], got {tuple(qweight.shape)}")
-    n, k = qweight.shape
+    weight_shape, shape = qweight.shape, q.shape
+    if len(weight_shape) != 2:
+        raise ValueError(f"qweight must be 2-D [out, in], got {tuple(weight_shape)}")
+    n, k = weight_shape
     if q.dtype != torch.int8 or qweight.dtype != torch.int8:
         raise ValueError(f"q and qweight must be int8, got {q.dtype} and {qweight.dtype}")
     if scale.dtype != torch.float32 or w_scale.dtype != torch.float32:
         raise ValueError(f"scale and w_scale must be float32, got {scale.dtype} and {w_scale.dtype}")
-    if q.ndim == 0 or q.shape[-1] != k:
-        raise ValueError(f"q {tuple(q.shape)} does not end in the weight's {k} input features")
-    if tuple(scale.shape) != tuple(q.shape[:-1]):
-        raise ValueError(f"scale {tuple(scale.shape)} != one for each row of q {tuple(q.shape)}")
-    if tuple(w_scale.shape) != (n,):
+    if not shape or shape[-1] != k:
+        raise ValueError(f"q {tuple(shape)} does not end in the weight's {k} input features")
+    if scale.shape != shape[:-1]:
+        raise ValueError(f"scale {tuple(scale.shape)} != one for each row of q {tuple(shape)}")
+    if w_scale.shape != (n,):
         raise ValueError(f"w_scale {tuple(w_scale.shape)} != [out={n}]")
-    if bias is not None and tuple(bias.shape) != (n,):
+    if bias is not None and bias.shape != (n,):
         raise ValueError(f"bias {tuple(bias.shape)} != [out={n}]")
     return n, k
 
@@ -60,27 +61,33 @@ def w8a8_gemm(q: torch.Tensor, scale: torch.Tensor, qweight: torch.Tensor, w_sca
     n, k = check_w8a8_args(q, scale, qweight, w_scale, bias)
     dtype = _ffi.dtype_code(out_dtype)
     bias_dtype = _ffi.dtype_code(bias.dtype) if bias is not None else 0
-    out = torch.empty((*q.shape[:-1], n), dtype=out_dtype, device=q.device)
+    out = q.new_empty((*q.shape[:-1], n), dtype=out_dtype)
     if out.numel() == 0:
         return out
-    require_device("w8a8_gemm", q, scale, qweight, w_scale, *([bias] if bias is not None else []))
-    m = out.numel() // n
-    q2 = q.reshape(m, k)
-    if k and (q2.stride(1) != 1 or (m > 1 and q2.stride(0) < k)):
-        q2 = q2.contiguous()
-    if k and (qweight.stride(1) != 1 or (n > 1 and qweight.stride(0) < k)):
-        qweight = qweight.contiguous()
-    scale = scale.reshape(m).contiguous()
-    w_scale = w_scale.contiguous()
-    bias = bias.contiguous() if bias is not None else None
+    if bias is None:
+        require_device("w8a8_gemm", q, scale, qweight, w_scale)
+    else:
+        require_device("w8a8_gemm", q, scale, qweight, w_scale, bias)
+        bias = bias.contiguous()
+    m = scale.numel()
+    q_stride = w_stride = k
+    if not q.is_contiguous():
+        q = q.reshape(m, k)
+        if k and (q.stride(1) != 1 or (m > 1 and q.stride(0) < k)):
+            q = q.contiguous()
+        q_stride = q.stride(0)
+    if not qweight.is_contiguous():
+        if k and (qweight.stride(1) != 1 or (n > 1 and qweight.stride(0) < k)):
+            qweight = qweight.contiguous()
+        w_stride = qweight.stride(0)
+    scale, w_scale = scale.contiguous(), w_scale.contiguous()
     with on_device(q.device):
         need = _workspace_need(m, n, k, dtype)
         # of this call alone: nothing is shared between streams, or between captured graphs
         ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
         status = _ffi.lib().ss_w8a8_gemm(
-            q2.data_ptr(), scale.data_ptr(), qweight.data_ptr(), w_scale.data_ptr(),
-            bias.data_ptr() if bias is not None else None, out.data_ptr(), m, n, k, q2.stride(0),
-            qweight.stride(0), n, dtype, bias_dtype, ws.data_ptr() if ws is not None else None, need,
-            _ffi.stream_ptr(q.device))
+            q.data_ptr(), scale.data_ptr(), qweight.data_ptr(), w_scale.data_ptr(),
+            None if bias is None else bias.data_ptr(), out.data_ptr(), m, n, k, q_stride, w_stride, n, dtype, bias_dtype,
+            None if ws is None else ws.data_ptr(), need, _ffi.stream_ptr(q.device))
     _ffi.check(status, "w8a8_gemm")
     return out

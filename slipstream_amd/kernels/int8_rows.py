@@ -19,24 +19,30 @@ from slipstream_amd.kernels.norm_act import _rows
 
 
 def _outputs(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
-    if x.ndim == 0:
+    shape = x.shape
+    if not shape:
         raise ValueError("rows need at least one dimension")
-    q = torch.empty(x.shape, dtype=torch.int8, device=x.device)
-    make = torch.empty if x.shape[-1] else torch.zeros
-    return q, make(x.shape[:-1], dtype=torch.float32, device=x.device)
+    make = torch.empty if shape[-1] else torch.zeros
+    return x.new_empty(shape, dtype=torch.int8), make(shape[:-1], dtype=torch.float32, device=x.device)
+
+
+def _flat(x: torch.Tensor, cols: int) -> tuple[torch.Tensor, int]:
+    """``x`` itself where its rows follow each other, else ``_rows``; and the row stride."""
+    return (x, cols) if x.is_contiguous() else _rows(x, cols)
 
 
 def quantize_int8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """``x [..., K]`` -> ``(q int8 [..., K], scale fp32 [...])`` with ``x ~ q * scale[..., None]``."""
-    q, scale = _outputs(x)
     dtype = _ffi.dtype_code(x.dtype)
-    if x.numel() == 0:
+    q, scale = _outputs(x)
+    if q.numel() == 0:
         return q, scale
     require_device("quantize_int8", x)
-    x2, xs = _rows(x, x.shape[-1])
+    cols = x.shape[-1]
+    x2, xs = _flat(x, cols)
     with on_device(x.device):
-        status = _ffi.lib().ss_quantize_int8(x2.data_ptr(), q.data_ptr(), scale.data_ptr(), x2.shape[0], x2.shape[1],
-                                             xs, dtype, _ffi.stream_ptr(x.device))
+        status = _ffi.lib().ss_quantize_int8(x2.data_ptr(), q.data_ptr(), scale.data_ptr(), scale.numel(), cols, xs,
+                                             dtype, _ffi.stream_ptr(x.device))
     _ffi.check(status, "quantize_int8")
     return q, scale
 
@@ -52,21 +58,25 @@ def fused_rmsnorm_int8(x: torch.Tensor, weight: torch.Tensor, residual: torch.Te
         raise ValueError(f"weight numel {weight.numel()} != hidden {cols}")
     if residual is not None and residual.shape != x.shape:
         raise ValueError(f"residual {tuple(residual.shape)} != x {tuple(x.shape)}")
-    dtypes = {x.dtype, weight.dtype} | ({residual.dtype} if residual is not None else set())
-    if len(dtypes) != 1:
+    if weight.dtype != x.dtype or (residual is not None and residual.dtype != x.dtype):
+        dtypes = {x.dtype, weight.dtype} | ({residual.dtype} if residual is not None else set())
         raise ValueError(f"x, weight and residual must share a dtype, got {sorted(map(str, dtypes))}")
     dtype = _ffi.dtype_code(x.dtype)
-    s = torch.empty(x.shape, dtype=x.dtype, device=x.device) if residual is not None else None
-    if x.numel() == 0:
+    s = x.new_empty(x.shape) if residual is not None else None
+    if q.numel() == 0:
         return q, scale, s
-    require_device("fused_rmsnorm_int8", x, weight, *([residual] if residual is not None else []))
-    x2, xs = _rows(x, cols)
-    r2, rs = _rows(residual, cols) if residual is not None else (None, 0)
-    w = weight.reshape(cols).contiguous()
+    x2, xs = _flat(x, cols)
+    w = weight.reshape(cols) if weight.is_contiguous() else weight.reshape(cols).contiguous()
+    if residual is None:
+        require_device("fused_rmsnorm_int8", x, weight)
+        r_ptr, rs, s_ptr = None, 0, None
+    else:
+        require_device("fused_rmsnorm_int8", x, weight, residual)
+        r2, rs = _flat(residual, cols)
+        r_ptr, s_ptr = r2.data_ptr(), s.data_ptr()
     with on_device(x.device):
-        status = _ffi.lib().ss_rmsnorm_int8(x2.data_ptr(), r2.data_ptr() if r2 is not None else None, w.data_ptr(),
-                                            q.data_ptr(), scale.data_ptr(), s.data_ptr() if s is not None else None,
-                                            x2.shape[0], cols, xs, rs, float(eps), dtype, _ffi.stream_ptr(x.device))
+        status = _ffi.lib().ss_rmsnorm_int8(x2.data_ptr(), r_ptr, w.data_ptr(), q.data_ptr(), scale.data_ptr(), s_ptr,
+                                            scale.numel(), cols, xs, rs, eps, dtype, _ffi.stream_ptr(x.device))
     _ffi.check(status, "fused_rmsnorm_int8")
     return q, scale, s
 
@@ -75,16 +85,16 @@ def fused_swiglu_int8(gate: torch.Tensor, up: torch.Tensor) -> tuple[torch.Tenso
     """``silu(gate) * up`` in int8: ``(q, scale)``."""
     if gate.shape != up.shape or gate.dtype != up.dtype:
         raise ValueError("gate/up must share shape and dtype")
-    q, scale = _outputs(gate)
     dtype = _ffi.dtype_code(gate.dtype)
-    if gate.numel() == 0:
+    q, scale = _outputs(gate)
+    if q.numel() == 0:
         return q, scale
     require_device("fused_swiglu_int8", gate, up)
     cols = gate.shape[-1]
-    g2, gs = _rows(gate, cols)
-    u2, us = _rows(up, cols)
+    g2, gs = _flat(gate, cols)
+    u2, us = _flat(up, cols)
     with on_device(gate.device):
-        status = _ffi.lib().ss_swiglu_int8(g2.data_ptr(), u2.data_ptr(), q.data_ptr(), scale.data_ptr(), g2.shape[0],
+        status = _ffi.lib().ss_swiglu_int8(g2.data_ptr(), u2.data_ptr(), q.data_ptr(), scale.data_ptr(), scale.numel(),
                                            cols, gs, us, dtype, _ffi.stream_ptr(gate.device))
     _ffi.check(status, "fused_swiglu_int8")
     return q, scale
