@@ -76,20 +76,18 @@ __device__ __forceinline__ float scaled(int sum, float xs, float ws, float bias)
   return fmaf((float)sum * xs, ws, bias);
 }
 
-// N consecutive results, 16-byte aligned
+// N consecutive results (16 bytes) in the output's type
 template <int N>
-__device__ __forceinline__ void store_results(float* o, const float (&y)[N]) {
+__device__ __forceinline__ void pack_results(float (&o)[N], const float (&y)[N]) {
 #pragma unroll
-  for (int e = 0; e < N; e += 4)
-    store16(o + e, u32x4{__builtin_bit_cast(uint32_t, y[e]), __builtin_bit_cast(uint32_t, y[e + 1]),
-                         __builtin_bit_cast(uint32_t, y[e + 2]), __builtin_bit_cast(uint32_t, y[e + 3])});
+  for (int e = 0; e < N; ++e) o[e] = y[e];
 }
 template <int N, typename T>
-__device__ __forceinline__ void store_results(T* o, const float (&y)[N]) {
-#pragma unroll
-  for (int e = 0; e < N; e += 8)
-    store16(o + e, u32x4{Elem<T>::pack2(y[e], y[e + 1]), Elem<T>::pack2(y[e + 2], y[e + 3]),
-                         Elem<T>::pack2(y[e + 4], y[e + 5]), Elem<T>::pack2(y[e + 6], y[e + 7])});
+__device__ __forceinline__ void pack_results(T (&o)[N], const float (&y)[N]) {
+  static_assert(N == 8, "sixteen bytes");
+  const u32x4 w = {Elem<T>::pack2(y[0], y[1]), Elem<T>::pack2(y[2], y[3]), Elem<T>::pack2(y[4], y[5]),
+                   Elem<T>::pack2(y[6], y[7])};
+  __builtin_memcpy(o, &w, 16);
 }
 
 // A raw buffer descriptor over [base, base + bytes) as four scalars: offsets past the end read

@@ -47,6 +47,14 @@ __device__ __forceinline__ void mfma_acc(i32x16& acc, i32x4 a, i32x4 b) {
   asm volatile("v_mfma_i32_32x32x32_i8 %0, %1, %2, %0" : "+a"(acc) : "v"(a), "v"(b));
 }
 
+template <typename T, int N>
+__device__ __forceinline__ u32x4 as_words(const T (&y)[N]) {
+  u32x4 w;
+  static_assert(sizeof(y) == 16, "sixteen bytes");
+  __builtin_memcpy(&w, y, 16);
+  return w;
+}
+
 constexpr int kFar = 0x40000000;  // a byte offset past any operand tile (host-checked)
 
 // LDS stages of the tokens and of the channels (rows of 128 bytes) for a tile: as many as 160 KB
@@ -114,10 +122,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
   struct Side {
     int so, add, slot;  // scalar offset, tail offset, LDS slot (bytes)
   } dw = {0, 0, 0}, dx = {0, 0, 0};
-  auto aim = [&](Side& d, int i, int next_slot) {  // stage i (past the range: the last one again, never read)
+  auto aim = [&](Side& d, int i, int next_slot) {  // stage i; past the range zeros, which nobody reads
     const int at = min(i, i1 - 1);
     d.so = __builtin_amdgcn_readfirstlane(at * 128);
-    d.add = at == stages - 1 ? past : 0;
+    d.add = i >= i1 ? kFar : at == stages - 1 ? past : 0;
     d.slot = __builtin_amdgcn_readfirstlane(next_slot);
     asm volatile("s_nop 4" : : "s"(d.so), "s"(d.slot));  // VALU-written SGPRs: five wait states before a VMEM reads them
   };
@@ -249,55 +257,70 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
   __builtin_amdgcn_s_barrier();                                // of any wave
   asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");           // and the last products have landed
 
-  // ---- results: 32 tokens at a time through the wave's own part of the LDS, so that the lanes
-  // hold consecutive channels and a store writes whole rows of the wave's 32 NT channels
-  constexpr int RS = NT * 128 + 16;  // bytes of a token's sums there, and its scale behind them
+  // ---- results: 32 tokens at a time through the wave's own part of the LDS (as sum * x_scale, in
+  // fp32), so that the lanes hold consecutive channels and a store writes rows of the wave's
+  // 32 NT channels
+  constexpr int RS = NT * 128 + 16;  // bytes of a token there
   static_assert(4 * 32 * RS <= (DX * BM + DW * BN) * 128, "the sums fit where the operands were");
   char* const turn = s_dyn + wave * 32 * RS;
   TO* const out = (TO*)p.out + (__is_same(TO, int) ? (int64_t)zr * p.m * p.o_stride : 0);
-  const bool vec = n + CL <= p.n && p.o_stride % CL == 0 && ((uintptr_t)p.out & 15) == 0;
+  // in 16-byte pieces, through a descriptor over the wave's rows: what lies outside it is not
+  // written
+  const bool pieces = p.n % CL == 0 && p.o_stride % CL == 0 && p.o_stride <= (1 << 20) && ((uintptr_t)p.out & 15) == 0;
+  const int left_rows = rows - 32 * MT * wm, left_chans = chans - 32 * NT * wn;
+  const int row_bytes = (int)p.o_stride * (int)sizeof(TO);
+  const uint32_t bytes = left_rows > 0 && left_chans > 0 ? (min(left_rows, 32 * MT) - 1) * row_bytes +
+                                                               min(left_chans, 32 * NT) * (int)sizeof(TO)
+                                                         : 0;
+  const __amdgpu_buffer_rsrc_t ro = __builtin_amdgcn_make_buffer_rsrc(
+      out + (m0 + 32 * MT * wm) * p.o_stride + n0 + 32 * NT * wn, (short)0, (int)bytes, 0x00020000);
+  const int o_at = c < left_chans ? lane / LR * row_bytes + c * (int)sizeof(TO) : kFar;
+  int o_row = 0;  // bytes from the wave's first row
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) {
-    const int64_t mb = m0 + 32 * (MT * wm + mt);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       asm volatile("" : "+a"(acc[nt][mt]));  // read behind the waits above
 #pragma unroll
-      for (int g = 0; g < 4; ++g)
-        *reinterpret_cast<i32x4*>(turn + ln * RS + (32 * nt + 8 * g + 4 * kg) * 4) =
-            i32x4{acc[nt][mt][4 * g], acc[nt][mt][4 * g + 1], acc[nt][mt][4 * g + 2], acc[nt][mt][4 * g + 3]};
+      for (int g = 0; g < 4; ++g) {
+        u32x4 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int sum = acc[nt][mt][4 * g + e];
+          if constexpr (__is_same(TO, int))
+            v[e] = (uint32_t)sum;
+          else
+            v[e] = __builtin_bit_cast(uint32_t, (float)sum * xs[mt]);
+        }
+        store16(turn + ln * RS + (32 * nt + 8 * g + 4 * kg) * 4, v);
+      }
     }
-    if constexpr (!__is_same(TO, int)) *reinterpret_cast<float*>(turn + ln * RS + NT * 128) = xs[mt];
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 #pragma unroll
     for (int q = 0; q < LR / 2; ++q) {
       const int r = q * (64 / LR) + lane / LR;
-      const int64_t m = mb + r;
-      i32x4 sum[CL / 4];
+      u32x4 v[CL / 4];
 #pragma unroll
-      for (int h = 0; h < CL / 4; ++h) sum[h] = *reinterpret_cast<const i32x4*>(turn + r * RS + (c + 4 * h) * 4);
-      const float x_scale = *reinterpret_cast<const float*>(turn + r * RS + NT * 128);
-      if (m < p.m && n < p.n) {
-        TO* const o = out + m * p.o_stride + n;
-        if constexpr (__is_same(TO, int)) {
-          if (vec) {
-            *reinterpret_cast<i32x4*>(o) = sum[0];
-          } else {
+      for (int h = 0; h < CL / 4; ++h) v[h] = load16(turn + r * RS + (c + 4 * h) * 4);
+      TO y[CL];
+      if constexpr (__is_same(TO, int)) {
 #pragma unroll
-            for (int e = 0; e < CL; ++e)
-              if (n + e < p.n) o[e] = sum[0][e];
-          }
-        } else {
-          float y[CL];
+        for (int e = 0; e < CL; ++e) y[e] = (int)v[0][e];
+      } else {
+        float f[CL];
 #pragma unroll
-          for (int e = 0; e < CL; ++e) y[e] = scaled(sum[e / 4][e % 4], x_scale, ws[e], bias[e]);
-          if (vec) {
-            store_results<CL>(o, y);
-          } else {
+        for (int e = 0; e < CL; ++e) f[e] = fmaf(__builtin_bit_cast(float, (uint32_t)v[e / 4][e % 4]), ws[e], bias[e]);
+        pack_results<CL>(y, f);
+      }
+      if (pieces) {
+        __builtin_amdgcn_raw_buffer_store_b128(as_words(y), ro, o_at, o_row, 0);
+        o_row += 64 / LR * row_bytes;
+      } else {
+        const int64_t m = m0 + 32 * (MT * wm + mt) + r;
+        if (m < p.m) {
 #pragma unroll
-            for (int e = 0; e < CL; ++e)
-              if (n + e < p.n) o[e] = (TO)y[e];
-          }
+          for (int e = 0; e < CL; ++e)
+            if (n + e < p.n) out[m * p.o_stride + n + e] = y[e];
         }
       }
     }
