@@ -262,11 +262,14 @@ int ss_w4a16_gemm(const void* x, void* out, const int32_t* qweight, const void* 
  * The sum is exact in int32, so k must be below 131072 (else SS_ERR_UNSUPPORTED); the result
  * fma(sum * x_scale, w_scale, bias) is rounded in fp32 and once to out_dtype. It is the same
  * whatever kernel or split computes it.
- * workspace: ss_w8a8_workspace_size() bytes, 16-byte aligned, any contents; with less (or
- * NULL, 0) the call succeeds without splitting k over workgroups, more slowly. Calls that
- * share a workspace must be ordered on one stream.
+ * workspace: ss_w8a8_workspace_size() bytes, 16-byte aligned, any contents: the int32 sums of
+ * the ranges where k is split over workgroups, and copies of operands whose rows are not whole
+ * 16-byte pieces (x_whole / w_whole zero: base address or row stride not a multiple of 16,
+ * or a row stride above 2^21; with k not a multiple of 16 both operands count so). With less
+ * (or NULL, 0) the call succeeds without them, more slowly. Calls that share a workspace must
+ * be ordered on one stream.
  */
-int ss_w8a8_workspace_size(int64_t m, int64_t n, int64_t k, int out_dtype, int64_t* bytes);
+int ss_w8a8_workspace_size(int64_t m, int64_t n, int64_t k, int x_whole, int w_whole, int64_t* bytes);
 
 int ss_w8a8_gemm(const int8_t* x, const float* x_scale, const int8_t* w, const float* w_scale,
                  const void* bias, void* out, int64_t m, int64_t n, int64_t k, int64_t x_stride,

@@ -324,7 +324,7 @@ __global__ __launch_bounds__(256) void int8_rows_long_kernel(const RowArgs a) {
 bool al16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
 
 template <typename T, int MODE, bool ALIGNED>
-int launch_rows(const RowArgs& a, int64_t rows, hipStream_t stream, const char* who) {
+int launch_part(const RowArgs& a, int64_t rows, hipStream_t stream, const char* who) {
   const int pieces = (int)(((int64_t)a.cols * sizeof(T) + 15) / 16);
   const dim3 grid((unsigned)rows);
   if (pieces <= 64)
@@ -340,6 +340,23 @@ int launch_rows(const RowArgs& a, int64_t rows, hipStream_t stream, const char* 
   else
     hipLaunchKernelGGL((int8_rows_long_kernel<T, MODE>), grid, dim3(256), 0, stream, a);
   return ss_host::launch_status(who);
+}
+
+// As many rows a launch as keep its threads below 2^32
+template <typename T, int MODE, bool ALIGNED>
+int launch_rows(RowArgs a, int64_t rows, hipStream_t stream, const char* who) {
+  constexpr int64_t kMost = 1 << 23;
+  for (; rows > 0; rows -= kMost) {
+    const int64_t part = rows < kMost ? rows : kMost;
+    const int st = launch_part<T, MODE, ALIGNED>(a, part, stream, who);
+    if (st != SS_OK) return st;
+    a.x += part * a.x_stride;
+    if (a.y) a.y += part * a.y_stride;
+    a.q += part * a.cols;
+    a.scale += part;
+    if (a.s) a.s += part * a.cols * (int64_t)sizeof(T);
+  }
+  return SS_OK;
 }
 
 template <int MODE>

@@ -7,13 +7,8 @@
 namespace ss {
 namespace {
 
-// The kernel for every shape, stride and alignment: 64 x 64 results a workgroup, 64 keys at a
-// time through LDS, rows of 80 bytes there so that sixteen lanes' 16-byte reads spread over the
-// banks. Sixteen bytes are read at any alignment (global accesses need none on this
-// target); a row's last bytes one by one, zeros past its end.
-constexpr int kGenTile = 64;
-constexpr int kGenRow = 80;
-
+// Sixteen keys of a row at any alignment (global accesses need none on this target); past the
+// row's end zeros.
 __device__ __forceinline__ i32x4 load_keys(const int8_t* row, int at, int k) {
   i32x4 v = {0, 0, 0, 0};
   if (at + 16 <= k) {
@@ -26,6 +21,44 @@ __device__ __forceinline__ i32x4 load_keys(const int8_t* row, int at, int k) {
   }
   return v;
 }
+
+// The other kernels' operands begin every row on 16 bytes and end it with 16. Rows that do not
+// are copied to rows that do, zeros behind them, in the workspace: 333 x 4999 x 2051 (rows at any
+// byte) 30.4 us in the general kernel, 22.3 so, of which 7 for the copy.
+// A wave copies a row, four pieces a lane on their way.
+struct Rows {
+  const int8_t* from;
+  int8_t* to;
+  int64_t stride;  // of `from`
+  int64_t rows;
+};
+__global__ __launch_bounds__(256) void w8a8_align_kernel(Rows x, Rows w, int k, int pieces) {
+  const int lane = threadIdx.x & 63;
+  for (int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); r < x.rows + w.rows; r += (int64_t)gridDim.x * 4) {
+    const bool of_x = r < x.rows;
+    const int64_t i = of_x ? r : r - x.rows;
+    const int8_t* const from = of_x ? x.from + i * x.stride : w.from + i * w.stride;
+    int8_t* const to = (of_x ? x.to : w.to) + i * (16 * (int64_t)pieces);
+    const int full = k >> 4;
+    for (int c = lane; c < full; c += 256) {
+      i32x4 v[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (c + 64 * u < full) __builtin_memcpy(&v[u], from + 16 * (c + 64 * u), 16);
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (c + 64 * u < full) *reinterpret_cast<i32x4*>(to + 16 * (c + 64 * u)) = v[u];
+    }
+    if (full < pieces && lane < 16) to[16 * full + lane] = 16 * full + lane < k ? from[16 * full + lane] : (int8_t)0;
+  }
+}
+
+// The kernel for every shape, stride and alignment, without a workspace: 64 x 64 results a
+// workgroup, 64 keys at a time through LDS, rows of 80 bytes there so that sixteen lanes'
+// 16-byte reads spread over the banks.
+constexpr int kGenTile = 64;
+constexpr int kGenRow = 80;
+
 
 template <typename TO>
 __global__ __launch_bounds__(256) void w8a8_general_kernel(const W8Params p, int n_tiles) {
@@ -78,7 +111,7 @@ __global__ __launch_bounds__(256) void w8a8_general_kernel(const W8Params p, int
 template <typename TO>
 int launch_general(const W8Params& p, hipStream_t stream) {
   const int64_t n_tiles = (p.n + kGenTile - 1) / kGenTile, m_tiles = (p.m + kGenTile - 1) / kGenTile;
-  if (n_tiles * m_tiles > 0x7fffffff) {
+  if (n_tiles * m_tiles >= (1 << 24)) {  // of 256 threads: below 2^32
     ss_host::set_error("w8a8 gemm: %lld x %lld results are more than one launch holds", (long long)p.m, (long long)p.n);
     return SS_ERR_UNSUPPORTED;
   }
@@ -86,18 +119,17 @@ int launch_general(const W8Params& p, hipStream_t stream) {
   return ss_host::launch_status("w8a8 gemm (general)");
 }
 
-// Operands that the DMA kernels read in 16-byte pieces: every row starts on one and ends with
-// one, and a tile of 256 rows stays below a descriptor's 2^30 bytes.
-bool whole_pieces(const W8Params& p) {
-  return p.k > 0 && p.k % 16 == 0 && ((uintptr_t)p.x & 15) == 0 && ((uintptr_t)p.w & 15) == 0 &&
-         (p.m == 1 || p.x_stride % 16 == 0) && (p.n == 1 || p.w_stride % 16 == 0) && p.x_stride <= (1 << 21) &&
-         p.w_stride <= (1 << 21);
+// Rows that the DMA kernels can read in 16-byte pieces; a tile of 256 of them stays below a
+// descriptor's 2^30 bytes.
+bool whole_rows(const void* base, int64_t rows, int64_t stride, int64_t k) {
+  return k % 16 == 0 && ((uintptr_t)base & 15) == 0 && (rows == 1 || stride % 16 == 0) && stride <= (1 << 21);
 }
+int64_t round16(int64_t n) { return (n + 15) / 16 * 16; }
 
-// Which kernel a call of whole pieces takes, by the kernels' own estimates (fitted to
-// measurements, see there): for example 64 x 4096 x 4096 6.4 us streamed and 12.2 in tiles, 64 x
-// 28672 x 4096 36.7 and 28.5. Kept for the last shapes of the thread, as a plan is a few
-// hundred estimates.
+// Which kernel a call takes: up to 32 tokens the stream kernel (28672 x 4096 at m = 32 28.0 us,
+// in tiles 29.0; 4096 x 14336 11.6 and 14.9), beyond that by the kernels' own estimates, fitted to
+// measurements (at m = 64 4096 x 4096 6.5 us streamed and 10.8 in tiles, 28672 x 4096 35.4 and
+// 30.7). Kept for the last shapes of the thread, as a plan is a few hundred estimates.
 struct Plan {
   int64_t m = -1, n = 0, k = 0;
   bool may_split = false, stream = false;
@@ -116,7 +148,7 @@ const Plan& plan_for(int64_t m, int64_t n, int64_t k, bool may_split) {
   if (p.m != m || p.n != n || p.k != k || p.may_split != may_split || p.device != device) {
     p.m = m, p.n = n, p.k = k, p.may_split = may_split, p.device = device;
     const double stream = plan_w8a8_stream(p.sp, m, n, k), tile = plan_w8a8_tile(p.tp, m, n, k, may_split);
-    p.stream = stream < tile;
+    p.stream = stream < 1e29 && (m <= 32 || stream < tile);
     if (stream > 1e29 && tile > 1e29) p.tp.ks = 0;  // more results than one launch holds
   }
   return p;
@@ -143,14 +175,16 @@ int check_extents(int64_t m, int64_t n, int64_t k, int out_dtype) {
 }  // namespace
 }  // namespace ss
 
-extern "C" int ss_w8a8_workspace_size(int64_t m, int64_t n, int64_t k, int out_dtype, int64_t* bytes) {
+extern "C" int ss_w8a8_workspace_size(int64_t m, int64_t n, int64_t k, int x_whole, int w_whole, int64_t* bytes) {
   if (!bytes) {
     ss_host::set_error("w8a8 workspace: null pointer");
     return SS_ERR_INVALID;
   }
   *bytes = 0;
-  const int st = ss::check_extents(m, n, k, out_dtype);
-  if (st == SS_OK && m > 0 && n > 0 && k > 0 && k % 16 == 0) *bytes = ss::plan_for(m, n, k, true).workspace();
+  const int st = ss::check_extents(m, n, k, SS_DTYPE_BF16);
+  if (st != SS_OK || m == 0 || n == 0 || k == 0) return st;
+  const int64_t kp = ss::round16(k);
+  *bytes = ss::plan_for(m, n, kp, true).workspace() + (x_whole && kp == k ? 0 : m * kp) + (w_whole && kp == k ? 0 : n * kp);
   return st;
 }
 
@@ -173,14 +207,35 @@ extern "C" int ss_w8a8_gemm(const int8_t* x, const float* x_scale, const int8_t*
     ss_host::set_error("w8a8 gemm: row strides shorter than the rows");
     return SS_ERR_INVALID;
   }
-  const ss::W8Params p = {x, w, x_scale, w_scale, bias, out, m, n, x_stride, w_stride, o_stride, (int)k, bias_dtype};
+  ss::W8Params p = {x, w, x_scale, w_scale, bias, out, m, n, x_stride, w_stride, o_stride, (int)k, bias_dtype};
+  if (m == 1) p.x_stride = ss::round16(k), p.o_stride = ss::round16(n);  // (not used to reach a row)
+  if (n == 1) p.w_stride = ss::round16(k);
   hipStream_t s = (hipStream_t)stream;
-  if (ss::whole_pieces(p)) {
-    const ss::Plan* pl = &ss::plan_for(m, n, k, true);
-    if (pl->workspace() > 0 && (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < pl->workspace()))
-      pl = &ss::plan_for(m, n, k, false);
+  char* ws = (uintptr_t)workspace & 15 ? nullptr : (char*)workspace;
+  int64_t left = ws ? workspace_bytes : 0;
+  // rows that are not whole 16-byte pieces: their copies come first in the workspace
+  const int64_t kp = ss::round16(k);
+  const bool copy_x = !ss::whole_rows(p.x, m, p.x_stride, k), copy_w = !ss::whole_rows(p.w, n, p.w_stride, k);
+  const int64_t x_bytes = copy_x ? m * kp : 0, w_bytes = copy_w ? n * kp : 0;
+  if (k > 0 && x_bytes + w_bytes <= left) {
+    if (copy_x || copy_w) {
+      const ss::Rows rx = {p.x, (int8_t*)ws, p.x_stride, copy_x ? m : 0};
+      const ss::Rows rw = {p.w, (int8_t*)ws + x_bytes, p.w_stride, copy_w ? n : 0};
+      const int64_t blocks = (rx.rows + rw.rows + 3) / 4, cap = (int64_t)ss_host::device_cu_count() * 32;
+      hipLaunchKernelGGL(ss::w8a8_align_kernel, dim3((unsigned)(blocks < cap ? blocks : cap)), dim3(256), 0, s, rx, rw,
+                         (int)k, (int)(kp / 16));
+      const int sa = ss_host::launch_status("w8a8 gemm (align)");
+      if (sa != SS_OK) return sa;
+      if (copy_x) p.x = rx.to, p.x_stride = kp;
+      if (copy_w) p.w = rw.to, p.w_stride = kp;
+      p.k = (int)kp;
+      ws += x_bytes + w_bytes;
+      left -= x_bytes + w_bytes;
+    }
+    const ss::Plan* pl = &ss::plan_for(m, n, kp, true);
+    if (pl->workspace() > left) pl = &ss::plan_for(m, n, kp, false);
     if (pl->stream) return ss::launch_w8a8_stream(p, pl->sp, out_dtype, s);
-    if (pl->tp.ks > 0) return ss::launch_w8a8_tile(p, pl->tp, out_dtype, (int*)workspace, s);
+    if (pl->tp.ks > 0) return ss::launch_w8a8_tile(p, pl->tp, out_dtype, (int*)ws, s);
   }
   if (out_dtype == SS_DTYPE_BF16) return ss::launch_general<ss::bf16_t>(p, s);
   if (out_dtype == SS_DTYPE_F16) return ss::launch_general<ss::f16_t>(p, s);

@@ -29,6 +29,8 @@ struct TilePlan {
   int ks, per;  // K ranges and 128-key stages per range
   int n_tiles, m_blocks;
 };
+constexpr int64_t kMostGroups = 1 << 22;  // workgroups of a launch (of at most 512 threads: below 2^32)
+
 // The stream kernel (w8a8_stream.hip): a workgroup's 16-row tiles of tokens and channels, its
 // waves and its grid.
 struct StreamPlan {
@@ -70,6 +72,17 @@ __device__ __forceinline__ float load_as_f32(const void* p, int64_t i, int dtype
   return ((const float*)p)[i];
 }
 
+// c += a b over 32 keys: lane l's sixteen bytes of a are keys 16 (l / 32) .. + 15 of channel l % 32
+// (of b: of token l % 32); its results are channels 8 (r / 4) + 4 (l / 32) + r % 4 of token
+// l % 32.
+typedef int i32x16 __attribute__((ext_vector_type(16)));
+
+// Position of 16-byte chunk c of row r within the row's 128 LDS bytes: c ^ tile_swizzle(r).
+// A 16-byte LDS read runs in four passes of sixteen lanes, lanes 0-3, 12-15, 20-27 first,
+// then 4-11, 16-19, 28-31, and the same of the upper half. The rows 2p and 2p + 1 lie in
+// different halves of the 64 banks, and the row pairs of each pass differ in p % 8.
+__device__ __forceinline__ int tile_swizzle(int r) { return (r >> 1) & 7; }
+
 // The result of one output from its exact integer sum, before it is rounded to the output's
 // type: three roundings in fp32 (four with a bias).
 __device__ __forceinline__ float scaled(int sum, float xs, float ws, float bias) {
@@ -88,6 +101,38 @@ __device__ __forceinline__ void pack_results(T (&o)[N], const float (&y)[N]) {
   const u32x4 w = {Elem<T>::pack2(y[0], y[1]), Elem<T>::pack2(y[2], y[3]), Elem<T>::pack2(y[4], y[5]),
                    Elem<T>::pack2(y[6], y[7])};
   __builtin_memcpy(o, &w, 16);
+}
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_over(const void* base, uint32_t bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), (short)0, (int)bytes, 0x00020000);
+}
+
+// The biases of `chans` channels from n0 on, of whatever type, read without a branch on it (a
+// load inside such a branch makes the compiler wait for every load before it, one channel
+// after another): the aligned dword that holds a bias, through a descriptor that is empty where
+// there are none, shifted so that its bits are the low ones, and decoded under bit masks.
+struct BiasReader {
+  __amdgpu_buffer_rsrc_t rs;
+  uint32_t skew, size, f16_mask, bf16_mask;
+};
+__device__ __forceinline__ BiasReader bias_reader(const W8Params& p, int64_t n0, int chans) {
+  BiasReader b;
+  b.size = p.bias_dtype == SS_DTYPE_F32 ? 4 : 2;
+  const uint64_t at = (uint64_t)p.bias + n0 * b.size;
+  b.skew = (uint32_t)at & 3u;
+  b.rs = buffer_over((const void*)(at & ~3ull), p.bias ? (b.skew + chans * b.size + 3) & ~3u : 0u);
+  b.f16_mask = p.bias_dtype == SS_DTYPE_F16 ? ~0u : 0u;
+  b.bf16_mask = p.bias_dtype == SS_DTYPE_BF16 ? ~0u : 0u;
+  return b;
+}
+__device__ __forceinline__ uint32_t bias_bits(const BiasReader& b, int c) {  // c: from n0
+  const uint32_t off = b.skew + c * b.size;
+  return (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(b.rs, (int)(off & ~3u), 0, 0) >> (8 * (off & 2u));
+}
+__device__ __forceinline__ float bias_value(const BiasReader& b, uint32_t bits) {
+  const uint32_t f16 = __builtin_bit_cast(uint32_t, (float)__builtin_bit_cast(f16_t, (uint16_t)(bits & 0xFFFFu)));
+  const uint32_t bf16 = bits << 16;
+  return __builtin_bit_cast(float, (f16 & b.f16_mask) | (bf16 & b.bf16_mask) | (bits & ~(b.f16_mask | b.bf16_mask)));
 }
 
 // A raw buffer descriptor over [base, base + bytes) as four scalars: offsets past the end read

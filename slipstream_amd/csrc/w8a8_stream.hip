@@ -31,7 +31,7 @@ constexpr int D = 2;
 // bytes of a block (128 keys of the weights' and tokens' rows), and of a workgroup's LDS
 constexpr int block_bytes(int mt, int nt) { return (16 * nt + 16 * mt) * 128; }
 constexpr int stream_lds_bytes(int mt, int nt, int waves) {
-  return waves * D * block_bytes(mt, nt) + mt * nt * 4 * kPlane * 4;
+  return waves * D * block_bytes(mt, nt) + mt * nt * 4 * kPlane * 4 + 16 * mt * 4;
 }
 
 // XI: groups of eight tokens that are read (2 MT, or 1 of MT = 1); the rows of the others hold
@@ -44,6 +44,7 @@ __global__ __launch_bounds__(512) void w8a8_stream_kernel(const W8Params p, int 
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
   const int ln = lane & 15, kg = lane >> 4;
   int* const s_sum = reinterpret_cast<int*>(s_dyn + waves * D * B);
+  float* const s_xs = reinterpret_cast<float*>(s_sum + MT * NT * 4 * kPlane);  // and the tokens' scales
   // each XCD (workgroups go round robin over the eight) takes a contiguous eighth of the list,
   // in which the token blocks of a channel tile follow each other: its L2 serves their weights
   const int total = n_tiles * m_blocks, per_xcd = (total + 7) >> 3;
@@ -51,6 +52,16 @@ __global__ __launch_bounds__(512) void w8a8_stream_kernel(const W8Params p, int 
   if ((int)(blockIdx.x >> 3) >= per_xcd || item >= total) return;
   const int64_t n0 = (int64_t)(item / m_blocks) * (16 * NT), m0 = (int64_t)(item % m_blocks) * (16 * MT);
   const int rows = (int)min((int64_t)(16 * MT), p.m - m0), chans = (int)min((int64_t)(16 * NT), p.n - n0);
+
+  // scales, requested first of all: the results wait for nothing then. Every thread's results are
+  // of one channel (a multiple of 16 NT threads).
+  const int tc = threadIdx.x % (16 * NT);
+  const BiasReader rb = bias_reader(p, n0, chans);
+  const uint32_t bias = bias_bits(rb, tc);
+  const float ws = __builtin_bit_cast(
+      float, __builtin_amdgcn_raw_buffer_load_b32(buffer_over(p.w_scale + n0, chans * 4), tc * 4, 0, 0));
+  const uint32_t xs = __builtin_amdgcn_raw_buffer_load_b32(buffer_over(p.x_scale + m0, rows * 4),
+                                                           (threadIdx.x % (16 * MT)) * 4, 0, 0);
 
   // a DMA instruction brings eight rows of 128 bytes; lane l byte 16 (l % 8) of row l / 8, which
   // holds chunk (l % 8) ^ swizzle. Rows past the end and, in the last 128 keys, chunks past k
@@ -83,6 +94,7 @@ __global__ __launch_bounds__(512) void w8a8_stream_kernel(const W8Params p, int 
   for (int d = 0; d < D; ++d)
     if (d < count) request(d, d);
   for (int i = threadIdx.x; i < MT * NT * 4 * kPlane; i += blockDim.x) s_sum[i] = 0;
+  if (threadIdx.x < 16 * MT) s_xs[threadIdx.x] = __builtin_bit_cast(float, xs);
 
   // fragment of lane (ln, kg): row ln, key step s: chunk 2 kg + s
   const int f[2] = {ln * 128 + 16 * ((2 * kg) ^ stream_swizzle(ln)), ln * 128 + 16 * ((2 * kg + 1) ^ stream_swizzle(ln))};
@@ -124,15 +136,13 @@ __global__ __launch_bounds__(512) void w8a8_stream_kernel(const W8Params p, int 
                                  __HIP_MEMORY_SCOPE_WORKGROUP);
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < 256 * MT * NT; i += blockDim.x) {
-    const int r = i / (16 * NT), c = i % (16 * NT);
-    if (r < rows && c < chans) {
-      const int64_t m = m0 + r, n = n0 + c;
-      const int sum = s_sum[(((c >> 4) * MT + (r >> 4)) * 4 + (c & 3)) * kPlane + 16 * ((c & 15) >> 2) + (r & 15)];
-      ((TO*)p.out)[m * p.o_stride + n] =
-          (TO)scaled(sum, p.x_scale[m], p.w_scale[n], p.bias ? load_as_f32(p.bias, n, p.bias_dtype) : 0.f);
+  const float bf = bias_value(rb, bias);
+  TO* const out = (TO*)p.out + m0 * p.o_stride + n0;
+  for (int r = threadIdx.x / (16 * NT); r < rows; r += blockDim.x / (16 * NT))
+    if (tc < chans) {
+      const int sum = s_sum[(((tc >> 4) * MT + (r >> 4)) * 4 + (tc & 3)) * kPlane + 16 * ((tc & 15) >> 2) + (r & 15)];
+      out[r * p.o_stride + tc] = (TO)scaled(sum, s_xs[r], ws, bf);
     }
-  }
 }
 
 template <typename TO, int MT, int NT, int XI>
@@ -165,8 +175,8 @@ int launch_stream_typed(const W8Params& p, const StreamPlan& pl, hipStream_t str
 
 }  // namespace
 
-// The tile and waves of least estimated time (us), fitted to the times of 2500 calls (every tile
-// and number of waves at 100 shapes of up to 512 tokens; 8 % off on average): a round's
+// The tile and waves of least estimated time (us), fitted to the times of 3500 calls (every tile
+// and number of waves at 240 shapes of up to 512 tokens; 8 % off on average): a round's
 // start, a wave's blocks one after another, the adding of the sums and the results, the
 // operands' way through a CU and out of the L2, and the weights' out of the memory.
 double plan_w8a8_stream(StreamPlan& pl, int64_t m, int64_t n, int64_t k) {
@@ -180,7 +190,7 @@ double plan_w8a8_stream(StreamPlan& pl, int64_t m, int64_t n, int64_t k) {
     const int mt = t[0], nt = t[1];
     if (mt > 1 && 8 * mt >= m) continue;
     const int64_t n_tiles = (n + 16 * nt - 1) / (16 * nt), m_blocks = (m + 16 * mt - 1) / (16 * mt);
-    if (n_tiles * m_blocks > 0x7ffffff) continue;
+    if (n_tiles * m_blocks > kMostGroups) continue;
     const int64_t groups = n_tiles * m_blocks, a_cu = (groups + cus - 1) / cus;
     const double bytes = (16.0 * nt + (m < 16 * mt ? m : 16 * mt)) * blocks * 128;
     // two waves only beyond 16 tokens (28672 x 4096 at m = 1 26.2 us with two, 22.3 with four)
@@ -190,9 +200,9 @@ double plan_w8a8_stream(StreamPlan& pl, int64_t m, int64_t n, int64_t k) {
       int64_t fit = kLdsBytes / lds;
       fit = fit < 32 / waves ? fit : 32 / waves;
       const double rounds = (double)((groups + cus * fit - 1) / (cus * fit)), each = (double)((blocks + waves - 1) / waves);
-      const double us = 1.0 + rounds * (0.87 + each * (0.0134 + 0.0048 * (mt + nt) + 0.0077 * mt * nt) +
-                                        mt * nt * (0.114 + 0.68 / waves)) +
-                        a_cu * (bytes * 4.7e-6 + 0.0019 * waves) + groups * bytes * 1.08e-8 + n * k * 8.3e-8;
+      const double us = 0.94 + rounds * (1.15 + each * (0.0141 * (mt + nt) + 0.0051 * mt * nt) +
+                                         mt * nt * (0.103 + 0.416 / waves)) +
+                        a_cu * (bytes * 5.32e-6 + 0.0005 * waves) + groups * bytes * 8.4e-9 + n * k * 8.43e-8;
       if (us < best) {
         best = us;
         pl = {mt, nt, waves, (int)n_tiles, (int)m_blocks};

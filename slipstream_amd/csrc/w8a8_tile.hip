@@ -20,12 +20,6 @@
 namespace ss {
 namespace {
 
-// Position of 16-byte chunk c of row r within the row's 128 LDS bytes: c ^ tile_swizzle(r).
-// A 16-byte LDS read runs in four passes of sixteen lanes, lanes 0-3, 12-15, 20-27 first,
-// then 4-11, 16-19, 28-31, and the same of the upper half. The rows 2p and 2p + 1 lie in
-// different halves of the 64 banks, and the row pairs of each pass differ in p % 8.
-__device__ __forceinline__ int tile_swizzle(int r) { return (r >> 1) & 7; }
-
 template <typename F, int... I>
 __device__ __forceinline__ void static_for_impl(F&& f, std::integer_sequence<int, I...>) {
   (f(std::integral_constant<int, I>{}), ...);
@@ -35,14 +29,11 @@ __device__ __forceinline__ void static_for(F&& f) {
   static_for_impl(f, std::make_integer_sequence<int, N>{});
 }
 
-// acc += a b on the matrix core over 32 keys: lane l's sixteen bytes of a are keys
-// 16 (l / 32) .. + 15 of channel l % 32 (of b: of token l % 32); its results are channels
-// 8 (r / 4) + 4 (l / 32) + r % 4 of token l % 32. The accumulator stays in AGPRs. Written as
-// asm because the compiler moves accumulators between the register files in every stage.
-// What it therefore does not look after: the operands come from LDS reads, which it does wait
-// for; an accumulator is touched once in MT NT products or more; and between the last
-// product and what follows the loop stand the waits there.
-typedef int i32x16 __attribute__((ext_vector_type(16)));
+// acc += a b on the matrix core over 32 keys, the accumulator in AGPRs. Written as asm because the
+// compiler moves accumulators between the register files in every stage. What it therefore
+// does not look after: the operands come from LDS reads, which it does wait for; an
+// accumulator is touched once in MT NT products; and between the last product and what
+// follows the loop stand the waits there.
 __device__ __forceinline__ void mfma_acc(i32x16& acc, i32x4 a, i32x4 b) {
   asm volatile("v_mfma_i32_32x32x32_i8 %0, %1, %2, %0" : "+a"(acc) : "v"(a), "v"(b));
 }
@@ -57,22 +48,26 @@ __device__ __forceinline__ u32x4 as_words(const T (&y)[N]) {
 
 constexpr int kFar = 0x40000000;  // a byte offset past any operand tile (host-checked)
 
-// LDS stages of the tokens and of the channels (rows of 128 bytes) for a tile: as many as 160 KB
-// hold, the tokens' first, at most six.
+// LDS stages of the tokens and of the channels (rows of 128 bytes) for a tile: as many as its part
+// of the LDS holds, the tokens' first, at most six. Of small tiles two workgroups share a CU, so
+// that a SIMD has two waves (one has nothing to do while it waits at a barrier: 128 x 28672 x
+// 4096 33.5 us with one, 31.9 with two; 333 x 4992 x 2048 9.9 and 9.3).
 constexpr int kLdsBytes = 160 * 1024;
+constexpr int groups_of(int bm, int bn) { return bm + bn <= 256 ? 2 : 1; }
 constexpr int channel_stages(int bm, int bn) {
   int d = 2;
-  while (d < 6 && (d + 1) * (bm + bn) * 128 <= kLdsBytes) ++d;
+  while (d < 6 && (d + 1) * (bm + bn) * 128 <= kLdsBytes / groups_of(bm, bn)) ++d;
   return d;
 }
 constexpr int token_stages(int bm, int bn) {
   const int d = channel_stages(bm, bn);
-  return d < 6 && ((d + 1) * bm + d * bn) * 128 <= kLdsBytes ? d + 1 : d;
+  return d < 6 && ((d + 1) * bm + d * bn) * 128 <= kLdsBytes / groups_of(bm, bn) ? d + 1 : d;
 }
+constexpr int ring_bytes(int bm, int bn) { return (token_stages(bm, bn) * bm + channel_stages(bm, bn) * bn) * 128; }
 
 // TO int: a K range's sums, for the reduce kernel
-template <typename TO, int MT, int NT, int WM>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) void w8a8_tile_kernel(
+template <typename TO, int MT, int NT, int WM, int G>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(G, G))) void w8a8_tile_kernel(
     const W8Params p, int per, int ks, int n_tiles, int m_blocks, int band) {
   constexpr int WN = 4 / WM, BM = 32 * MT * WM, BN = 32 * NT * WN;
   constexpr int DX = token_stages(BM, BN), DW = channel_stages(BM, BN);
@@ -123,7 +118,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
     int so, add, slot;  // scalar offset, tail offset, LDS slot (bytes)
   } dw = {0, 0, 0}, dx = {0, 0, 0};
   auto aim = [&](Side& d, int i, int next_slot) {  // stage i; past the range zeros, which nobody reads
-    const int at = min(i, i1 - 1);
+    const int at = min(i, stages - 1);
     d.so = __builtin_amdgcn_readfirstlane(at * 128);
     d.add = i >= i1 ? kFar : at == stages - 1 ? past : 0;
     d.slot = __builtin_amdgcn_readfirstlane(next_slot);
@@ -140,18 +135,23 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
 
   // ---- scales, requested first of all: the results wait for nothing then
   constexpr int CL = 16 / sizeof(TO), LR = 32 * NT / CL;  // channels of a lane, lanes of a token in the store
-  const int c = lane % LR * CL;
-  const int64_t n = n0 + 32 * NT * wn + c;
-  float xs[MT], ws[CL], bias[CL];
+  const int c = lane % LR * CL, c0 = 32 * NT * wn + c;    // from the wave's first channel, and the workgroup's
+  float xs[MT];
+  u32x4 ws[CL / 4];
+  uint32_t bias[CL];
+  const BiasReader rb = bias_reader(p, n0, chans);
   if constexpr (!__is_same(TO, int)) {
+    const __amdgpu_buffer_rsrc_t rxs = buffer_over(p.x_scale + m0, rows * 4), rws = buffer_over(p.w_scale + n0, chans * 4);
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) xs[mt] = p.x_scale[min(m0 + 32 * (MT * wm + mt) + ln, p.m - 1)];
+    for (int mt = 0; mt < MT; ++mt)
+      xs[mt] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rxs, (32 * (MT * wm + mt) + ln) * 4, 0, 0));
 #pragma unroll
-    for (int e = 0; e < CL; ++e) {
-      const int64_t at = min(n + e, p.n - 1);
-      ws[e] = p.w_scale[at];
-      bias[e] = p.bias ? load_as_f32(p.bias, at, p.bias_dtype) : 0.f;
-    }
+    for (int e = 0; e < CL / 4; ++e)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        ws[e][j] = (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(rws, (c0 + 4 * e + j) * 4, 0, 0);
+#pragma unroll
+    for (int e = 0; e < CL; ++e) bias[e] = bias_bits(rb, c0 + e);
   }
 
   // fragment of lane (ln, kg): row ln of a 32-row tile; step s of the four of a stage: chunk
@@ -261,7 +261,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
   // fp32), so that the lanes hold consecutive channels and a store writes rows of the wave's
   // 32 NT channels
   constexpr int RS = NT * 128 + 16;  // bytes of a token there
-  static_assert(4 * 32 * RS <= (DX * BM + DW * BN) * 128, "the sums fit where the operands were");
+  static_assert(4 * 32 * RS <= ring_bytes(BM, BN), "the sums fit where the operands were");
   char* const turn = s_dyn + wave * 32 * RS;
   TO* const out = (TO*)p.out + (__is_same(TO, int) ? (int64_t)zr * p.m * p.o_stride : 0);
   // in 16-byte pieces, through a descriptor over the wave's rows: what lies outside it is not
@@ -276,6 +276,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
       out + (m0 + 32 * MT * wm) * p.o_stride + n0 + 32 * NT * wn, (short)0, (int)bytes, 0x00020000);
   const int o_at = c < left_chans ? lane / LR * row_bytes + c * (int)sizeof(TO) : kFar;
   int o_row = 0;  // bytes from the wave's first row
+  float biasf[CL];
+  if constexpr (!__is_same(TO, int)) {
+#pragma unroll
+    for (int e = 0; e < CL; ++e) biasf[e] = bias_value(rb, bias[e]);
+  }
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) {
 #pragma unroll
@@ -296,31 +301,48 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
       }
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    if (pieces) {
 #pragma unroll
-    for (int q = 0; q < LR / 2; ++q) {
-      const int r = q * (64 / LR) + lane / LR;
-      u32x4 v[CL / 4];
+      for (int q = 0; q < LR / 2; ++q) {
+        const int r = q * (64 / LR) + lane / LR;
+        u32x4 v[CL / 4];
 #pragma unroll
-      for (int h = 0; h < CL / 4; ++h) v[h] = load16(turn + r * RS + (c + 4 * h) * 4);
-      TO y[CL];
-      if constexpr (__is_same(TO, int)) {
+        for (int h = 0; h < CL / 4; ++h) v[h] = load16(turn + r * RS + (c + 4 * h) * 4);
+        TO y[CL];
+        if constexpr (__is_same(TO, int)) {
 #pragma unroll
-        for (int e = 0; e < CL; ++e) y[e] = (int)v[0][e];
-      } else {
-        float f[CL];
-#pragma unroll
-        for (int e = 0; e < CL; ++e) f[e] = fmaf(__builtin_bit_cast(float, (uint32_t)v[e / 4][e % 4]), ws[e], bias[e]);
-        pack_results<CL>(y, f);
-      }
-      if (pieces) {
-        __builtin_amdgcn_raw_buffer_store_b128(as_words(y), ro, o_at, o_row, 0);
-        o_row += 64 / LR * row_bytes;
-      } else {
-        const int64_t m = m0 + 32 * (MT * wm + mt) + r;
-        if (m < p.m) {
+          for (int e = 0; e < CL; ++e) y[e] = (int)v[0][e];
+        } else {
+          float y32[CL];
 #pragma unroll
           for (int e = 0; e < CL; ++e)
-            if (n + e < p.n) out[m * p.o_stride + n + e] = y[e];
+            y32[e] = fmaf(__builtin_bit_cast(float, (uint32_t)v[e / 4][e % 4]),
+                          __builtin_bit_cast(float, (uint32_t)ws[e / 4][e % 4]), biasf[e]);
+          pack_results<CL>(y, y32);
+        }
+        __builtin_amdgcn_raw_buffer_store_b128(as_words(y), ro, o_at + o_row, 0, 0);
+        o_row += 64 / LR * row_bytes;
+      }
+    } else {
+      // element by element, a lane one of consecutive channels
+      constexpr int WC = 32 * NT, PER = WC > 64 ? 64 : WC;
+      for (int h = 0; h < WC; h += PER) {
+        const int ch = h + lane % PER;
+        float ws1 = 0.f, bias1 = 0.f;
+        if constexpr (!__is_same(TO, int)) {
+          ws1 = p.w_scale[min(n0 + 32 * NT * wn + ch, p.n - 1)];
+          bias1 = bias_value(rb, bias_bits(rb, 32 * NT * wn + ch));
+        }
+#pragma unroll 4
+        for (int r = lane / PER; r < 32; r += 64 / PER) {
+          const uint32_t v = *reinterpret_cast<const uint32_t*>(turn + r * RS + ch * 4);
+          if (32 * mt + r < left_rows && ch < left_chans) {
+            TO* const o = out + (m0 + 32 * (MT * wm + mt) + r) * p.o_stride + n0 + 32 * NT * wn + ch;
+            if constexpr (__is_same(TO, int))
+              *o = (int)v;
+            else
+              *o = (TO)fmaf(__builtin_bit_cast(float, v), ws1, bias1);
+          }
         }
       }
     }
@@ -328,36 +350,54 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
   }
 }
 
-// The sums of ks K ranges, scaled and rounded: a thread four channels of a token.
-template <typename TO>
+// The sums of ks K ranges added, scaled and rounded: a thread four channels of a token. Every load
+// that does not depend on the number of ranges is on its way before the first is waited for, and
+// four ranges' at a time (past the last: outside the descriptor, zeros).
+template <typename TO, bool VEC>
 __global__ __launch_bounds__(256) void w8a8_reduce_kernel(const W8Params p, const int* __restrict__ part, int ks) {
-  const int64_t quads = (p.n + 3) >> 2, total = p.m * quads, plane = p.m * p.n;
+  const int quads = (int)((p.n + 3) >> 2);
+  const int64_t total = p.m * quads;
+  const int plane = (int)(p.m * p.n) * 4;  // bytes; ks of them below 2^31
+  const __amdgpu_buffer_rsrc_t rp = buffer_over(part, (uint32_t)(ks * plane));
+  const __amdgpu_buffer_rsrc_t rws = buffer_over(p.w_scale, (uint32_t)(p.n * 4));
+  const BiasReader rb = bias_reader(p, 0, (int)p.n);
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-    const int64_t m = i / quads, n = 4 * (i - m * quads);
-    const int* src = part + m * p.n + n;
+    const int m = (int)(i / quads), n = 4 * (int)(i - (int64_t)m * quads);
+    const int at = (m * (int)p.n + n) * 4;
     const float xs = p.x_scale[m];
-    TO* const o = (TO*)p.out + m * p.o_stride + n;
-    if (p.n % 4 == 0) {
-      i32x4 sum = *reinterpret_cast<const i32x4*>(src);
-      for (int z = 1; z < ks; ++z) sum += *reinterpret_cast<const i32x4*>(src + z * plane);
+    uint32_t ws[4], bias[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        o[e] = (TO)scaled(sum[e], xs, p.w_scale[n + e], p.bias ? load_as_f32(p.bias, n + e, p.bias_dtype) : 0.f);
-    } else {
-      for (int e = 0; e < 4 && n + e < p.n; ++e) {
-        int sum = 0;
-        for (int z = 0; z < ks; ++z) sum += src[z * plane + e];
-        o[e] = (TO)scaled(sum, xs, p.w_scale[n + e], p.bias ? load_as_f32(p.bias, n + e, p.bias_dtype) : 0.f);
-      }
+    for (int e = 0; e < 4; ++e) {
+      ws[e] = (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(rws, (n + e) * 4, 0, 0);
+      bias[e] = bias_bits(rb, n + e);
     }
+    i32x4 sum = {0, 0, 0, 0};
+    for (int z = 0; z < ks; z += 4) {
+      i32x4 v[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int off = z + j < ks ? at + (z + j) * plane : -16;
+        if constexpr (VEC) {
+          v[j] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(rp, off, 0, 0));
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[j][e] = __builtin_amdgcn_raw_buffer_load_b32(rp, off + 4 * e, 0, 0);
+        }
+      }
+      sum += (v[0] + v[1]) + (v[2] + v[3]);
+    }
+    TO* const o = (TO*)p.out + m * p.o_stride + n;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (VEC || n + e < p.n)
+        o[e] = (TO)scaled(sum[e], xs, __builtin_bit_cast(float, ws[e]), bias_value(rb, bias[e]));
   }
 }
 
 template <typename TO, int MT, int NT, int WM>
 int launch_tile(const W8Params& p, const TilePlan& pl, hipStream_t stream) {
-  auto kern = w8a8_tile_kernel<TO, MT, NT, WM>;
-  constexpr int bm = 32 * MT * WM, bn = 32 * NT * (4 / WM);
-  constexpr int lds = (token_stages(bm, bn) * bm + channel_stages(bm, bn) * bn) * 128;
+  constexpr int bm = 32 * MT * WM, bn = 32 * NT * (4 / WM), lds = ring_bytes(bm, bn);
+  auto kern = w8a8_tile_kernel<TO, MT, NT, WM, groups_of(bm, bn)>;
   static std::atomic<uint64_t> done{0};
   if (const int st = reserve_lds((const void*)kern, lds, done); st != SS_OK) return st;
   // bands of at most 8 token blocks, of one size where they can be
@@ -387,18 +427,22 @@ int launch_tile_typed(const W8Params& p, const TilePlan& pl, hipStream_t stream)
 template <typename TO>
 int launch_reduce(const W8Params& p, const int* part, int ks, hipStream_t stream) {
   const int64_t blocks = (p.m * ((p.n + 3) / 4) + 255) / 256, cap = (int64_t)ss_host::device_cu_count() * 8;
-  hipLaunchKernelGGL(w8a8_reduce_kernel<TO>, dim3((unsigned)(blocks < cap ? blocks : cap)), dim3(256), 0, stream, p,
-                     part, ks);
+  const dim3 grid((unsigned)(blocks < cap ? blocks : cap));
+  if (p.n % 4 == 0)
+    hipLaunchKernelGGL((w8a8_reduce_kernel<TO, true>), grid, dim3(256), 0, stream, p, part, ks);
+  else
+    hipLaunchKernelGGL((w8a8_reduce_kernel<TO, false>), grid, dim3(256), 0, stream, p, part, ks);
   return ss_host::launch_status("w8a8 gemm (reduce)");
 }
 
 }  // namespace
 
-// The tile and K split of least estimated time (us), fitted to the times of 3700 calls (tiles and
-// splits of 160 shapes, 1 to 2240 tokens, 0.9 to 120 million weights; 8 % off on average): what a
-// stage of a round of workgroups takes, the start and the results of each round, the operands'
-// way into the LDS, the memory's share, and for a split the sums' way out and back and
-// the launch that adds them.
+// The tile and K split of least estimated time (us), fitted to the times of 4200 calls (tiles and
+// splits of 290 shapes, 1 to 2240 tokens, 0.3 to 120 million weights; 8 % off on average): what a
+// stage takes of a round of workgroups, the results of each round, the operands' way into the
+// LDS, the memory's share, and for a split the sums' way out and back and the launch that adds
+// them. (2240 x 4096 x 14336: 224 tiles of 160 x 256 117 us, 144 of 256 x 256 140; 197 x 4096 x
+// 14336: four ranges of 128 x 128 tiles 24 us, whole rows 45.)
 double plan_w8a8_tile(TilePlan& pl, int64_t m, int64_t n, int64_t k, bool may_split) {
 #define W8A8_SIZE(BM, BN, MT, NT, WM) {BM, BN},
   static const int kTiles[][2] = {W8A8_TILES(W8A8_SIZE)};
@@ -407,16 +451,18 @@ double plan_w8a8_tile(TilePlan& pl, int64_t m, int64_t n, int64_t k, bool may_sp
   double best = 1e30;
   for (const auto& t : kTiles) {
     const int64_t n_tiles = (n + t[1] - 1) / t[1], m_blocks = (m + t[0] - 1) / t[0];
-    if (n_tiles * m_blocks > 0x7ffffff) continue;
+    const int64_t fit = groups_of(t[0], t[1]);
+    if (n_tiles * m_blocks > kMostGroups) continue;
     for (int64_t ks = 1; ks <= (may_split ? 14 : 1); ks += ks < 4 ? 1 : 2) {
       const int64_t per = (stages + ks - 1) / ks, groups = ks * n_tiles * m_blocks;
       // a split of at least four stages each, for at most two rounds and a bit
       if (ks > 1 && (per < 4 || groups > 600 || ks * m * n * 4 >= ((int64_t)1 << 31))) break;
       if ((stages + per - 1) / per != ks) continue;
       const double rounds = (double)((groups + cus - 1) / cus), area = t[0] * t[1] / 65536.0, edge = t[0] + t[1];
-      double us = 1.4 + rounds * (per * (0.046 + 0.57 * area + 0.195 * edge / 512) + 2.3 + 7.9 * area) +
-                  groups * per * edge * 128 * 2.2e-8 + n * k * 4.4e-8 + m * n * 3.8e-7;
-      if (ks > 1) us += 2.5 + ks * m * n * 4 * 3.15e-7;
+      const double turns = (double)((groups + fit * cus - 1) / (fit * cus));
+      double us = 3.13 + turns * per * 0.0844 + rounds * (per * (0.662 * area + 0.128 * edge / 512) + 0.21 + 6.33 * area) +
+                  groups * per * edge * 128 * 1.79e-8 + n * k * 4.2e-8 + m * n * 2.96e-7;
+      if (ks > 1) us += 2.03 + ks * m * n * 4 * 2.79e-7;
       if (us < best) {
         best = us;
         pl = {t[0], t[1], (int)ks, (int)per, (int)n_tiles, (int)m_blocks};

@@ -41,12 +41,17 @@ def check_w8a8_args(q: torch.Tensor, scale: torch.Tensor, qweight: torch.Tensor,
     return n, k
 
 
-def _workspace_need(m: int, n: int, k: int, dtype: int) -> int:
-    key = (torch.cuda.current_device(), m, n, k, dtype)
+def _whole(t: torch.Tensor, stride: int) -> int:
+    """Whether ``t``'s rows start on 16 bytes and are not further apart than the kernels reach."""
+    return int(not (t.data_ptr() | stride) & 15 and stride <= 1 << 21)
+
+
+def _workspace_need(m: int, n: int, k: int, x_whole: int, w_whole: int) -> int:
+    key = (torch.cuda.current_device(), m, n, k, x_whole, w_whole)
     need = _WS_NEED.get(key)
     if need is None:
         out = _ffi.ctypes.c_int64(0)
-        _ffi.check(_ffi.lib().ss_w8a8_workspace_size(m, n, k, dtype, _ffi.ctypes.byref(out)), "w8a8 workspace")
+        _ffi.check(_ffi.lib().ss_w8a8_workspace_size(m, n, k, x_whole, w_whole, _ffi.ctypes.byref(out)), "w8a8 workspace")
         if len(_WS_NEED) > 4096:  # many distinct shapes: start over
             _WS_NEED.clear()
         need = _WS_NEED[key] = int(out.value)
@@ -82,7 +87,7 @@ def w8a8_gemm(q: torch.Tensor, scale: torch.Tensor, qweight: torch.Tensor, w_sca
         w_stride = qweight.stride(0)
     scale, w_scale = scale.contiguous(), w_scale.contiguous()
     with on_device(q.device):
-        need = _workspace_need(m, n, k, dtype)
+        need = _workspace_need(m, n, k, _whole(q, q_stride), _whole(qweight, w_stride))
         # of this call alone: nothing is shared between streams, or between captured graphs
         ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
         status = _ffi.lib().ss_w8a8_gemm(

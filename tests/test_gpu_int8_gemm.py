@@ -67,6 +67,39 @@ def test_shapes(device, m, n, k, dtype):
     _check(w8a8_gemm(*args, out_dtype=dtype), *args, f"{m} x {n} x {k}")
 
 
+# sizes at which each compiled kernel is the one that runs, whole 16-byte results and others: the
+# stream kernel's tiles (16-row tiles of tokens, of channels, waves) and the tile kernel's (tokens x
+# channels), these also with k split over workgroups
+VARIANTS = [
+    ("stream 1 1 2", [(33, 8480, 944), (33, 9383, 912)]), ("stream 1 1 4", [(1, 8552, 912), (7, 8425, 912)]),
+    ("stream 1 1 8", [(1, 496, 1104), (13, 497, 1104)]), ("stream 1 2 2", [(35, 9832, 944), (36, 9671, 976)]),
+    ("stream 1 2 4", [(1, 17168, 992), (10, 17527, 912)]), ("stream 1 2 8", [(67, 840, 1808), (34, 1463, 2016)]),
+    ("stream 2 1 2", [(17, 16776, 1008), (17, 18329, 912)]), ("stream 2 1 4", [(17, 4304, 1072), (17, 4651, 1104)]),
+    ("stream 2 1 8", [(17, 2072, 816), (18, 2147, 800)]), ("stream 2 2 2", [(19, 25112, 960), (17, 25637, 928)]),
+    ("stream 2 2 4", [(17, 13520, 928), (17, 14749, 912)]), ("stream 2 2 8", [(21, 4472, 1456), (19, 4149, 1600)]),
+    ("stream 4 2 2", [(444, 2336, 4256), (346, 2699, 5616)]), ("stream 4 2 4", [(34, 5560, 3632), (33, 6051, 3296)]),
+    ("stream 4 4 4", [(33, 13456, 2848), (33, 11541, 3280)]),
+    ("tile 64 128", [(572, 16, 912), (526, 17, 1008)]), ("tile 96 128", [(67, 16784, 912), (75, 16765, 928)]),
+    ("tile 128 128", [(106, 18112, 912), (98, 18527, 912)]), ("tile 192 128", [(141, 22520, 976), (129, 22751, 960)]),
+    ("tile 256 128", [(199, 22824, 944), (203, 26691, 928)]), ("tile 128 256", [(201, 23176, 912), (196, 24009, 1008)]),
+    ("tile 160 256", [(294, 24152, 960), (257, 23769, 912)]), ("tile 192 256", [(324, 22960, 912), (348, 22249, 912)]),
+    ("tile 224 256", [(434, 22232, 992), (386, 23253, 976)]), ("tile 256 256", [(479, 23552, 928), (511, 21975, 928)]),
+    ("split 64 128", [(634, 16, 1696), (547, 17, 1728)]), ("split 96 128", [(1414, 16, 6768), (2207, 19, 4768)]),
+    ("split 128 128", [(2140, 16, 11680), (1942, 17, 12432)]), ("split 192 128", [(140, 2760, 15888), (2075, 137, 16240)]),
+    ("split 256 128", [(198, 5920, 13936), (201, 5681, 14272)]), ("split 128 256", [(201, 6136, 13168), (103, 16461, 10144)]),
+    ("split 160 256", [(132, 11080, 10128), (130, 17283, 6048)]), ("split 192 256", [(161, 16504, 11936), (164, 18613, 9200)]),
+    ("split 224 256", [(206, 11032, 13328), (218, 17533, 7984)]), ("split 256 256", [(238, 16784, 12080), (233, 17321, 12560)]),
+]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("what,shapes", VARIANTS, ids=[v[0] for v in VARIANTS])
+def test_every_kernel(device, what, shapes, dtype):
+    for i, (m, n, k) in enumerate(shapes):
+        args = _case(device, m, n, k, bias=torch.bfloat16 if i else None)
+        _check(w8a8_gemm(*args, out_dtype=dtype), *args, f"{what}: {m} x {n} x {k}")
+
+
 @pytest.mark.parametrize("m", [1, 2, 16, 17, 32, 33, 48, 49, 64, 65, 80, 100, 128, 150, 200, 256, 300, 448, 513, 1000])
 @pytest.mark.parametrize("n,k", [(896, 4864), (1536, 2560)])
 def test_token_counts(device, m, n, k):
@@ -117,9 +150,11 @@ def test_a_row_does_not_depend_on_its_batch(device, m):
 
 @pytest.mark.parametrize("m", [1, 5, 40, 70, 200, 300])
 @pytest.mark.parametrize("off", [0, 1, 4, 16])
-def test_strides_and_alignments(device, m, off):
-    """Operands inside wider buffers at any byte; what surrounds them is 127 and is not read in."""
-    k, n = 528, 190
+@pytest.mark.parametrize("k", [528, 531])
+def test_strides_and_alignments(device, m, off, k):
+    """Operands inside wider buffers at any byte; what surrounds them is 127 and is not read in.
+    (Rows that do not start on 16 bytes, or whose length is not a multiple of 16, are copied first.)"""
+    n = 190
     q, xs, w, ws, _ = _case(device, m, n, k)
     want = w8a8_gemm(q, xs, w, ws, out_dtype=torch.float32)
     bq = torch.full((m, k + 48), 127, dtype=torch.int8, device=device)
@@ -159,7 +194,7 @@ def test_zero_k(device, m):
 
 
 @pytest.mark.parametrize("m,n,k", [(1, 200, 256), (20, 72, 512), (64, 200, 256), (65, 72, 512), (200, 200, 1024),
-                                   (300, 264, 512), (9, 51, 77), (40, 4096, 14336)])
+                                   (300, 264, 512), (9, 51, 77), (90, 51, 77), (140, 2760, 15888)])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("pad", [0, 3, 8])
 def test_c_entry_writes_its_rows_only(device, m, n, k, dtype, pad):
@@ -170,7 +205,7 @@ def test_c_entry_writes_its_rows_only(device, m, n, k, dtype, pad):
     lib = _ffi.lib()
     need = _ffi.ctypes.c_int64(-1)
     code = _ffi.dtype_code(dtype)
-    _ffi.check(lib.ss_w8a8_workspace_size(m, n, k, code, _ffi.ctypes.byref(need)), "size")
+    _ffi.check(lib.ss_w8a8_workspace_size(m, n, k, 1, 1, _ffi.ctypes.byref(need)), "size")
     for nbytes in sorted({0, max(0, need.value - 1), need.value}):
         buf = torch.full((m + 2, n + pad), 77.0, dtype=dtype, device=device)
         scratch = torch.full((nbytes + 64,), 0x5A, dtype=torch.uint8, device=device)

@@ -226,3 +226,16 @@ def test_more_bytes_than_31_bits_hold(device):
     q1, scale1 = quantize_int8(tail)
     assert torch.equal(q[-3:], q1) and torch.equal(scale[-3:], scale1)
     assert not scale[:-3].any() and not q[rows // 2].any()
+
+
+def test_more_rows_than_a_launch_holds(device):
+    """17 million rows: a launch's threads stay below 2^32, so they take more than one."""
+    rows, cols = 17_000_003, 8
+    x = torch.arange(rows, device=device, dtype=torch.float32)[:, None].expand(rows, cols).contiguous()
+    x[:, 0] += 1
+    q, scale = quantize_int8(x.to(torch.bfloat16))
+    assert torch.equal(scale, x.to(torch.bfloat16).float().amax(1) / torch.full((), 127.0, device=device))
+    assert (q.amax(1) == 127).all()
+    s, one = torch.zeros_like(x), torch.ones(cols, device=device)
+    q, scale, s = fused_rmsnorm_int8(x, one, s)
+    assert torch.equal(s, x) and (q.amax(1) == 127).all() and torch.isfinite(scale).all()

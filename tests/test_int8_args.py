@@ -116,10 +116,16 @@ def test_c_abi_refusals_need_no_device():
     # 128 * 128 * 131072 = 2^31 would leave the int32 sum
     assert gemm(k=1 << 17, x_stride=1 << 17, w_stride=1 << 17) == _ffi.SS_ERR_UNSUPPORTED
     assert b"131072" in lib.ss_last_error()
-    assert lib.ss_w8a8_workspace_size(4, 8, 1 << 17, bf16, ctypes.byref(need)) == _ffi.SS_ERR_UNSUPPORTED
-    assert lib.ss_w8a8_workspace_size(-1, 8, 32, bf16, ctypes.byref(need)) == _ffi.SS_ERR_INVALID
-    assert lib.ss_w8a8_workspace_size(4, 8, 32, bf16, None) == _ffi.SS_ERR_INVALID
-    assert lib.ss_w8a8_workspace_size(4, 8, 32, bf16, ctypes.byref(need)) == _ffi.SS_OK and need.value >= 0
+    assert lib.ss_w8a8_workspace_size(4, 8, 1 << 17, 1, 1, ctypes.byref(need)) == _ffi.SS_ERR_UNSUPPORTED
+    assert lib.ss_w8a8_workspace_size(-1, 8, 32, 1, 1, ctypes.byref(need)) == _ffi.SS_ERR_INVALID
+    assert lib.ss_w8a8_workspace_size(4, 8, 32, 1, 1, None) == _ffi.SS_ERR_INVALID
+    for k, x_whole, w_whole, copies in ((32, 1, 1, 0), (32, 0, 1, 4 * 32), (32, 1, 0, 8 * 32), (33, 1, 1, 12 * 48)):
+        assert lib.ss_w8a8_workspace_size(4, 8, k, x_whole, w_whole, ctypes.byref(need)) == _ffi.SS_OK
+        assert need.value == copies
+    # 128 tokens of a long row, few tiles: int32 sums of several ranges
+    assert lib.ss_w8a8_workspace_size(197, 4096, 14336, 1, 1, ctypes.byref(need)) == _ffi.SS_OK
+    ranges, rest = divmod(need.value, 197 * 4096 * 4)
+    assert ranges > 1 and rest == 0
 
     def rows(x=FAKE, q=FAKE, scale=FAKE, m=4, k=32, stride=32, dtype=bf16):
         return (lib.ss_quantize_int8(x, q, scale, m, k, stride, dtype, None),
