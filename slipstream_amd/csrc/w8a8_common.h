@@ -146,13 +146,21 @@ __device__ __forceinline__ i32x4 buffer_words(const void* base, uint32_t bytes) 
 // LDS destination, written just before: the load may read it one wait state later). Written
 // as asm, with no register to write, so that the compiler's waits do not count it: the
 // kernel waits itself.
+// STREAM: not kept in the caches, for what is read once.
 typedef __attribute__((address_space(3))) char* LdsBytes;
+template <bool STREAM = false>
 __device__ __forceinline__ void dma_b128(i32x4 rs, LdsBytes lds, int voff, int soff) {
   const uint32_t m0 = (uint32_t)(uintptr_t)lds;
-  asm volatile("s_nop 1\n\tbuffer_load_dwordx4 %0, %1, %2 offen lds"
-               :
-               : "v"(voff), "s"(rs), "s"(soff), "{m0}"(m0)
-               : "memory");
+  if constexpr (STREAM)
+    asm volatile("s_nop 1\n\tbuffer_load_dwordx4 %0, %1, %2 offen nt lds"
+                 :
+                 : "v"(voff), "s"(rs), "s"(soff), "{m0}"(m0)
+                 : "memory");
+  else
+    asm volatile("s_nop 1\n\tbuffer_load_dwordx4 %0, %1, %2 offen lds"
+                 :
+                 : "v"(voff), "s"(rs), "s"(soff), "{m0}"(m0)
+                 : "memory");
 }
 
 }  // namespace

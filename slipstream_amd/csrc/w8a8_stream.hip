@@ -34,10 +34,19 @@ constexpr int stream_lds_bytes(int mt, int nt, int waves) {
   return waves * D * block_bytes(mt, nt) + mt * nt * 4 * kPlane * 4 + 16 * mt * 4;
 }
 
+// Whether the weights pass the caches by, as what is read once does: where no second token block
+// reads them, for 16 tokens at any size (4096 x 14336 from memory 12.7 -> 11.4 us, out of the
+// 256 MB cache 10.2 and 10.0), beyond that for weights that such a cache does not keep for the
+// next call (28672 x 4096 at m = 24 28.2 -> 25.3 us; 4096 x 14336 from memory 17.0 -> 16.0, but
+// out of the cache 11.5 -> 14.3).
+inline bool read_once(int mt, int64_t m_blocks, int64_t n, int64_t k) {
+  return m_blocks == 1 && (mt == 1 || n * k > (64 << 20));
+}
+
 // XI: groups of eight tokens that are read (2 MT, or 1 of MT = 1); the rows of the others hold
 // anything, and their sums are not stored.
 template <typename TO, int MT, int NT, int XI>
-__global__ __launch_bounds__(512) void w8a8_stream_kernel(const W8Params p, int n_tiles, int m_blocks) {
+__global__ __launch_bounds__(512) void w8a8_stream_kernel(const W8Params p, int n_tiles, int m_blocks, bool once) {
   constexpr int B = block_bytes(MT, NT), ND = 2 * NT + XI;
   extern __shared__ __attribute__((aligned(16))) char s_dyn[];  // [waves][D][B], then the sums
   const int lane = threadIdx.x & 63;
@@ -77,18 +86,28 @@ __global__ __launch_bounds__(512) void w8a8_stream_kernel(const W8Params p, int 
   for (int u = 0; u < XI; ++u)
     off[2 * NT + u] = 8 * u + r8 < rows ? (8 * u + r8) * (int)p.x_stride + chunk[u & 1] : kFar;
   const int blocks = (p.k + 127) >> 7, last = blocks - 1;
+  // channel tiles begin at different keys, so that those that run at once on an XCD do not all
+  // ask for the same cache lines (28672 x 4096 at m = 24 26.5 -> 23.1 us, at m = 1 21.3 -> 20.4)
+  const int rotation = item / m_blocks % 32 * blocks / 32;
   const int past[2] = {last * 128 + chunk[0] >= p.k ? kFar : 0, last * 128 + chunk[1] >= p.k ? kFar : 0};
   const int count = wave < blocks ? (blocks - wave + waves - 1) / waves : 0;  // of this wave: wave, wave + waves, ...
   const LdsBytes ring = (LdsBytes)s_dyn + wave * D * B;
   asm volatile("s_nop 4");  // descriptor SGPRs written by VALU before the first asm load
   auto request = [&](int i, int slot) {  // the wave's block i
-    const int at = wave + i * waves;
+    const int turn = wave + i * waves + rotation, at = turn < blocks ? turn : turn - blocks;
     const int so = __builtin_amdgcn_readfirstlane(at * 128);
     const int base = __builtin_amdgcn_readfirstlane(slot * B);
     const int add[2] = {at == last ? past[0] : 0, at == last ? past[1] : 0};
     asm volatile("s_nop 4" : : "s"(so), "s"(base));  // VALU-written SGPRs: five wait states before a VMEM reads them
+    if (once) {
 #pragma unroll
-    for (int u = 0; u < ND; ++u) dma_b128(u < 2 * NT ? rw : rx, ring + base + u * 1024, off[u] + add[u & 1], so);
+      for (int u = 0; u < 2 * NT; ++u) dma_b128<true>(rw, ring + base + u * 1024, off[u] + add[u & 1], so);
+    } else {
+#pragma unroll
+      for (int u = 0; u < 2 * NT; ++u) dma_b128(rw, ring + base + u * 1024, off[u] + add[u & 1], so);
+    }
+#pragma unroll
+    for (int u = 2 * NT; u < ND; ++u) dma_b128(rx, ring + base + u * 1024, off[u] + add[u & 1], so);
   };
 #pragma unroll
   for (int d = 0; d < D; ++d)
@@ -153,7 +172,8 @@ int launch_stream(const W8Params& p, const StreamPlan& pl, hipStream_t stream) {
   constexpr int most = stream_lds_bytes(MT, NT, 8) < kLdsBytes ? stream_lds_bytes(MT, NT, 8) : kLdsBytes;
   if (const int st = reserve_lds((const void*)kern, most, done); st != SS_OK) return st;
   const int64_t grid = ((int64_t)pl.n_tiles * pl.m_blocks + 7) / 8 * 8;
-  hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(64 * pl.waves), lds, stream, p, pl.n_tiles, pl.m_blocks);
+  hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(64 * pl.waves), lds, stream, p, pl.n_tiles, pl.m_blocks,
+                     read_once(pl.mt, pl.m_blocks, p.n, p.k));
   return ss_host::launch_status("w8a8 gemm (stream)");
 }
 
@@ -202,7 +222,7 @@ double plan_w8a8_stream(StreamPlan& pl, int64_t m, int64_t n, int64_t k) {
       const double rounds = (double)((groups + cus * fit - 1) / (cus * fit)), each = (double)((blocks + waves - 1) / waves);
       const double us = 0.94 + rounds * (1.15 + each * (0.0141 * (mt + nt) + 0.0051 * mt * nt) +
                                          mt * nt * (0.103 + 0.416 / waves)) +
-                        a_cu * (bytes * 5.32e-6 + 0.0005 * waves) + groups * bytes * 8.4e-9 + n * k * 8.43e-8;
+                        a_cu * (bytes * 5.32e-6 + 0.0005 * waves) + groups * bytes * 8.4e-9 + n * k * (read_once(mt, m_blocks, n, k) ? 7.4e-8 : 8.43e-8);
       if (us < best) {
         best = us;
         pl = {mt, nt, waves, (int)n_tiles, (int)m_blocks};
