@@ -65,8 +65,13 @@ constexpr int token_stages(int bm, int bn) {
 }
 constexpr int ring_bytes(int bm, int bn) { return (token_stages(bm, bn) * bm + channel_stages(bm, bn) * bn) * 128; }
 
-// TO int: a K range's sums, for the reduce kernel
-template <typename TO, int MT, int NT, int WM, int G>
+// TO int: a K range's sums, for the reduce kernel. ONCE: the only token block, and more weights
+// than a 256 MB cache keeps for the next call: they pass the caches by, and the channel tiles
+// begin at different stages, so that those that run at once on an XCD do not all ask for the same
+// lines of the tokens (64 x 28672 x 4096 32.2 -> 26.6 us, 256 x 28672 x 4096 44.8 -> 43.2; with
+// several token blocks, which share the weights' lines, either is slower: 512 x 4096 x 4096 14.9 us,
+// past the caches 18.0, begun apart 16.0).
+template <typename TO, int MT, int NT, int WM, int G, bool ONCE>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(G, G))) void w8a8_tile_kernel(
     const W8Params p, int per, int ks, int n_tiles, int m_blocks, int band) {
   constexpr int WN = 4 / WM, BM = 32 * MT * WM, BN = 32 * NT * WN;
@@ -117,8 +122,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(G, G))) voi
   struct Side {
     int so, add, slot;  // scalar offset, tail offset, LDS slot (bytes)
   } dw = {0, 0, 0}, dx = {0, 0, 0};
+  const int apart = ONCE ? (pair / ks) % 16 * (i1 - i0) / 16 : 0;
   auto aim = [&](Side& d, int i, int next_slot) {  // stage i; past the range zeros, which nobody reads
-    const int at = min(i, stages - 1);
+    int at = min(i, stages - 1);
+    if constexpr (ONCE)
+      if (i < i1) at = i + apart < i1 ? i + apart : i + apart - (i1 - i0);
     d.so = __builtin_amdgcn_readfirstlane(at * 128);
     d.add = i >= i1 ? kFar : at == stages - 1 ? past : 0;
     d.slot = __builtin_amdgcn_readfirstlane(next_slot);
@@ -127,7 +135,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(G, G))) voi
   auto dma = [&](auto uc) __attribute__((always_inline)) {
     constexpr int u = uc;
     if constexpr (u < NW)
-      dma_b128(rw, lds + DX * XB + dw.slot + u * 4096, off[u] + dw.add, dw.so);
+      dma_b128<ONCE>(rw, lds + DX * XB + dw.slot + u * 4096, off[u] + dw.add, dw.so);
     else
       dma_b128(rx, lds + dx.slot + (u - NW) * 4096, off[u] + dx.add, dx.so);
   };
@@ -394,10 +402,10 @@ __global__ __launch_bounds__(256) void w8a8_reduce_kernel(const W8Params p, cons
   }
 }
 
-template <typename TO, int MT, int NT, int WM>
+template <typename TO, int MT, int NT, int WM, bool ONCE>
 int launch_tile(const W8Params& p, const TilePlan& pl, hipStream_t stream) {
   constexpr int bm = 32 * MT * WM, bn = 32 * NT * (4 / WM), lds = ring_bytes(bm, bn);
-  auto kern = w8a8_tile_kernel<TO, MT, NT, WM, groups_of(bm, bn)>;
+  auto kern = w8a8_tile_kernel<TO, MT, NT, WM, groups_of(bm, bn), ONCE>;
   static std::atomic<uint64_t> done{0};
   if (const int st = reserve_lds((const void*)kern, lds, done); st != SS_OK) return st;
   // bands of at most 8 token blocks, of one size where they can be
@@ -414,10 +422,18 @@ int launch_tile(const W8Params& p, const TilePlan& pl, hipStream_t stream) {
   X(256, 128, 4, 2, 2) X(192, 128, 3, 2, 2) X(128, 128, 2, 2, 2) \
   X(96, 128, 3, 1, 1) X(64, 128, 2, 1, 1)
 
+inline bool read_once(int64_t m_blocks, int64_t ks, int64_t n, int64_t k) {
+  return m_blocks == 1 && ks == 1 && n * k > (64 << 20);
+}
+
 template <typename TO>
 int launch_tile_typed(const W8Params& p, const TilePlan& pl, hipStream_t stream) {
 #define W8A8_LAUNCH(BM, BN, MT, NT, WM) \
-  if (pl.bm == BM && pl.bn == BN) return launch_tile<TO, MT, NT, WM>(p, pl, stream);
+  if (pl.bm == BM && pl.bn == BN) {                                                             \
+    if constexpr (!__is_same(TO, int))                                                         \
+      if (read_once(pl.m_blocks, pl.ks, p.n, p.k)) return launch_tile<TO, MT, NT, WM, true>(p, pl, stream); \
+    return launch_tile<TO, MT, NT, WM, false>(p, pl, stream);                                  \
+  }
   W8A8_TILES(W8A8_LAUNCH)
 #undef W8A8_LAUNCH
   ss_host::set_error("w8a8 gemm: tile of %d x %d", pl.bm, pl.bn);
@@ -462,6 +478,7 @@ double plan_w8a8_tile(TilePlan& pl, int64_t m, int64_t n, int64_t k, bool may_sp
       const double turns = (double)((groups + fit * cus - 1) / (fit * cus));
       double us = 3.13 + turns * per * 0.0844 + rounds * (per * (0.662 * area + 0.128 * edge / 512) + 0.21 + 6.33 * area) +
                   groups * per * edge * 128 * 1.79e-8 + n * k * 4.2e-8 + m * n * 2.96e-7;
+      if (read_once(m_blocks, ks, n, k)) us -= n * k * 2e-8;
       if (ks > 1) us += 2.03 + ks * m * n * 4 * 2.79e-7;
       if (us < best) {
         best = us;

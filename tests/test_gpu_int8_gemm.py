@@ -87,8 +87,19 @@ VARIANTS = [
     ("split 64 128", [(634, 16, 1696), (547, 17, 1728)]), ("split 96 128", [(1414, 16, 6768), (2207, 19, 4768)]),
     ("split 128 128", [(2140, 16, 11680), (1942, 17, 12432)]), ("split 192 128", [(140, 2760, 15888), (2075, 137, 16240)]),
     ("split 256 128", [(198, 5920, 13936), (201, 5681, 14272)]), ("split 128 256", [(201, 6136, 13168), (103, 16461, 10144)]),
-    ("split 160 256", [(132, 11080, 10128), (130, 17283, 6048)]), ("split 192 256", [(161, 16504, 11936), (164, 18613, 9200)]),
-    ("split 224 256", [(206, 11032, 13328), (218, 17533, 7984)]), ("split 256 256", [(238, 16784, 12080), (233, 17321, 12560)]),
+    ("split 160 256", [(132, 11080, 10128), (130, 5441, 15184)]), ("split 192 256", [(161, 16504, 11936), (164, 16555, 10272)]),
+    ("split 224 256", [(206, 11032, 13328), (193, 16445, 7568)]), ("split 256 256", [(238, 16784, 12080), (233, 17321, 12560)]),
+    # one token block and more than 64 MB of weights
+    ("once 64 128", [(33, 22240, 3024), (33, 15457, 4368)]),
+    ("once 96 128", [(65, 20216, 3344), (65, 24117, 2800)]),
+    ("once 128 128", [(97, 30120, 2288), (98, 31677, 2128)]),
+    ("once 192 128", [(129, 16560, 4080), (131, 20097, 3344)]),
+    ("once 256 128", [(193, 26832, 2512), (194, 24409, 2752)]),
+    ("once 128 256", [(98, 34984, 1984), (99, 37147, 1824)]),
+    ("once 160 256", [(129, 34752, 1968), (131, 33989, 2000)]),
+    ("once 192 256", [(163, 34344, 1984), (167, 33053, 2032)]),
+    ("once 224 256", [(193, 33280, 2064), (195, 39979, 1680)]),
+    ("once 256 256", [(225, 35896, 1872), (228, 39795, 1696)]),
 ]
 
 

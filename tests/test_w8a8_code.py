@@ -38,7 +38,7 @@ def kernels(tmp_path_factory) -> dict[str, list[str]]:
             name, body = part.split(">:", 1)
             if "w8a8_tile_kernel" in name:
                 found[name] = [line.split("//")[0].strip() for line in body.splitlines() if line.startswith("\t")]
-        assert len(found) == 40  # ten tiles, three output types and the sums of a split
+        assert len(found) == 70  # ten tiles: three output types, weights kept or not, and the sums of a split
         return found
     raise AssertionError("no tile kernel in the library")
 
@@ -72,7 +72,7 @@ def test_dma_waits_leave_what_was_issued_since(kernels):
         mt, nt, wm, _ = tile
         bm, bn = 32 * mt * wm, 32 * nt * (4 // wm)
         loop = code[products[0] - 1 : products[-1] + 1]
-        loads = [i for i, line in enumerate(loop) if line.startswith("buffer_load") and line.endswith("lds")]
+        loads = [i for i, line in enumerate(loop) if line.startswith("buffer_load") and line.endswith("lds")]  # the DMAs
         assert len(loads) == (bm + bn) // 32, name
         lds = 160 * 1024 // (2 if bm + bn <= 256 else 1)
         dw = max(d for d in range(2, 7) if d * (bm + bn) * 128 <= lds)
