@@ -2,9 +2,9 @@
 
 from __future__ import annotations
 
-import contextlib
-
 import torch
+
+from slipstream_amd import _ffi
 
 
 def require_device(who: str, *tensors: torch.Tensor) -> None:
@@ -27,12 +27,13 @@ def require_device(who: str, *tensors: torch.Tensor) -> None:
             raise ValueError(f"{who}: tensors on different devices ({dev} vs {t.device})")
 
 
-_HERE = contextlib.nullcontext()
-
-
-def on_device(device: torch.device):
-    """A context in which ``device`` is the current one, as a launch on its streams needs."""
-    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+def launch(device: torch.device, entry, *args) -> int:
+    """``entry(*args, stream)`` on torch's current stream of ``device``, with ``device`` the
+    current one, as a launch on its streams needs; returns the entry's status."""
+    if device.index == torch.cuda.current_device():
+        return entry(*args, _ffi.stream_ptr(device))
+    with torch.cuda.device(device):
+        return entry(*args, _ffi.stream_ptr(device))
 
 
 def unit_last_stride(x: torch.Tensor) -> torch.Tensor:

@@ -13,7 +13,7 @@ from __future__ import annotations
 import torch
 
 from slipstream_amd import _ffi
-from slipstream_amd.kernels._common import on_device, require_device
+from slipstream_amd.kernels._common import launch, require_device
 
 # Workspace bytes the library asks for, by shape.
 _WS_NEED: dict[tuple, int] = {}
@@ -46,12 +46,14 @@ def _whole(t: torch.Tensor, stride: int) -> int:
     return int(not (t.data_ptr() | stride) & 15 and stride <= 1 << 21)
 
 
-def _workspace_need(m: int, n: int, k: int, x_whole: int, w_whole: int) -> int:
-    key = (torch.cuda.current_device(), m, n, k, x_whole, w_whole)
+def _workspace_need(device: torch.device, m: int, n: int, k: int, x_whole: int, w_whole: int) -> int:
+    key = (device.index, m, n, k, x_whole, w_whole)
     need = _WS_NEED.get(key)
     if need is None:
         out = _ffi.ctypes.c_int64(0)
-        _ffi.check(_ffi.lib().ss_w8a8_workspace_size(m, n, k, x_whole, w_whole, _ffi.ctypes.byref(out)), "w8a8 workspace")
+        with torch.cuda.device(device):
+            status = _ffi.lib().ss_w8a8_workspace_size(m, n, k, x_whole, w_whole, _ffi.ctypes.byref(out))
+        _ffi.check(status, "w8a8 workspace")
         if len(_WS_NEED) > 4096:  # many distinct shapes: start over
             _WS_NEED.clear()
         need = _WS_NEED[key] = int(out.value)
@@ -86,13 +88,11 @@ def w8a8_gemm(q: torch.Tensor, scale: torch.Tensor, qweight: torch.Tensor, w_sca
             qweight = qweight.contiguous()
         w_stride = qweight.stride(0)
     scale, w_scale = scale.contiguous(), w_scale.contiguous()
-    with on_device(q.device):
-        need = _workspace_need(m, n, k, _whole(q, q_stride), _whole(qweight, w_stride))
-        # of this call alone: nothing is shared between streams, or between captured graphs
-        ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-        status = _ffi.lib().ss_w8a8_gemm(
-            q.data_ptr(), scale.data_ptr(), qweight.data_ptr(), w_scale.data_ptr(),
-            None if bias is None else bias.data_ptr(), out.data_ptr(), m, n, k, q_stride, w_stride, n, dtype, bias_dtype,
-            None if ws is None else ws.data_ptr(), need, _ffi.stream_ptr(q.device))
+    need = _workspace_need(q.device, m, n, k, _whole(q, q_stride), _whole(qweight, w_stride))
+    # of this call alone: nothing is shared between streams, or between captured graphs
+    ws = q.new_empty(need, dtype=torch.uint8) if need else None
+    status = launch(q.device, _ffi.lib().ss_w8a8_gemm, q.data_ptr(), scale.data_ptr(), qweight.data_ptr(),
+                    w_scale.data_ptr(), None if bias is None else bias.data_ptr(), out.data_ptr(), m, n, k, q_stride,
+                    w_stride, n, dtype, bias_dtype, None if ws is None else ws.data_ptr(), need)
     _ffi.check(status, "w8a8_gemm")
     return out

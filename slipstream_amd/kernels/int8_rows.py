@@ -14,7 +14,7 @@ from __future__ import annotations
 import torch
 
 from slipstream_amd import _ffi
-from slipstream_amd.kernels._common import on_device, require_device
+from slipstream_amd.kernels._common import launch, require_device
 from slipstream_amd.kernels.norm_act import _rows
 
 
@@ -22,8 +22,8 @@ def _outputs(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     shape = x.shape
     if not shape:
         raise ValueError("rows need at least one dimension")
-    make = torch.empty if shape[-1] else torch.zeros
-    return x.new_empty(shape, dtype=torch.int8), make(shape[:-1], dtype=torch.float32, device=x.device)
+    make = x.new_empty if shape[-1] else x.new_zeros
+    return x.new_empty(shape, dtype=torch.int8), make(shape[:-1], dtype=torch.float32)
 
 
 def _flat(x: torch.Tensor, cols: int) -> tuple[torch.Tensor, int]:
@@ -40,9 +40,8 @@ def quantize_int8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     require_device("quantize_int8", x)
     cols = x.shape[-1]
     x2, xs = _flat(x, cols)
-    with on_device(x.device):
-        status = _ffi.lib().ss_quantize_int8(x2.data_ptr(), q.data_ptr(), scale.data_ptr(), scale.numel(), cols, xs,
-                                             dtype, _ffi.stream_ptr(x.device))
+    status = launch(x.device, _ffi.lib().ss_quantize_int8, x2.data_ptr(), q.data_ptr(), scale.data_ptr(), scale.numel(),
+                    cols, xs, dtype)
     _ffi.check(status, "quantize_int8")
     return q, scale
 
@@ -66,7 +65,7 @@ def fused_rmsnorm_int8(x: torch.Tensor, weight: torch.Tensor, residual: torch.Te
     if q.numel() == 0:
         return q, scale, s
     x2, xs = _flat(x, cols)
-    w = weight.reshape(cols) if weight.is_contiguous() else weight.reshape(cols).contiguous()
+    w = weight.contiguous()
     if residual is None:
         require_device("fused_rmsnorm_int8", x, weight)
         r_ptr, rs, s_ptr = None, 0, None
@@ -74,9 +73,8 @@ def fused_rmsnorm_int8(x: torch.Tensor, weight: torch.Tensor, residual: torch.Te
         require_device("fused_rmsnorm_int8", x, weight, residual)
         r2, rs = _flat(residual, cols)
         r_ptr, s_ptr = r2.data_ptr(), s.data_ptr()
-    with on_device(x.device):
-        status = _ffi.lib().ss_rmsnorm_int8(x2.data_ptr(), r_ptr, w.data_ptr(), q.data_ptr(), scale.data_ptr(), s_ptr,
-                                            scale.numel(), cols, xs, rs, eps, dtype, _ffi.stream_ptr(x.device))
+    status = launch(x.device, _ffi.lib().ss_rmsnorm_int8, x2.data_ptr(), r_ptr, w.data_ptr(), q.data_ptr(),
+                    scale.data_ptr(), s_ptr, scale.numel(), cols, xs, rs, eps, dtype)
     _ffi.check(status, "fused_rmsnorm_int8")
     return q, scale, s
 
@@ -93,8 +91,7 @@ def fused_swiglu_int8(gate: torch.Tensor, up: torch.Tensor) -> tuple[torch.Tenso
     cols = gate.shape[-1]
     g2, gs = _flat(gate, cols)
     u2, us = _flat(up, cols)
-    with on_device(gate.device):
-        status = _ffi.lib().ss_swiglu_int8(g2.data_ptr(), u2.data_ptr(), q.data_ptr(), scale.data_ptr(), scale.numel(),
-                                           cols, gs, us, dtype, _ffi.stream_ptr(gate.device))
+    status = launch(gate.device, _ffi.lib().ss_swiglu_int8, g2.data_ptr(), u2.data_ptr(), q.data_ptr(),
+                    scale.data_ptr(), scale.numel(), cols, gs, us, dtype)
     _ffi.check(status, "fused_swiglu_int8")
     return q, scale
