@@ -142,21 +142,35 @@ struct InvOf<kSwiglu> {
   typedef float type;
 };
 
-// 16 bytes at any alignment (global accesses need none on this target), and the elements of a
-// row's last, partial piece: past the row's end zeros.
+// 16 bytes at any alignment (global accesses need none on this target). A row's last, partial
+// piece is put together from the aligned words that hold its elements, read at the last one
+// where they lie behind it, zeros past the row's end: loads that are each under their own
+// condition wait for one another (SwiGLU of 11 x 4863 in fp16 3.96 us, so
+// 3.54).
 template <typename T>
 __device__ __forceinline__ u32x4 load_piece(const char* row, int i, int cols) {
   constexpr int EPP = 16 / sizeof(T);
-  u32x4 w = {0u, 0u, 0u, 0u};
+  u32x4 v = {0u, 0u, 0u, 0u};
+  const char* const at = row + (int64_t)i * sizeof(T);
   if (i + EPP <= cols) {
-    __builtin_memcpy(&w, row + (int64_t)i * sizeof(T), 16);
-  } else {
-    T t[EPP];
+    __builtin_memcpy(&v, at, 16);
+  } else if (i < cols) {
+    const int left = (cols - i) * (int)sizeof(T);
+    const uint64_t from = (uint64_t)at, last = (from + left - 1) & ~3ull;
+    uint32_t w[5];
 #pragma unroll
-    for (int e = 0; e < EPP; ++e) t[e] = i + e < cols ? reinterpret_cast<const T*>(row)[i + e] : (T)0.f;
-    __builtin_memcpy(&w, t, 16);
+    for (int e = 0; e < 5; ++e) {
+      const uint64_t word = (from & ~3ull) + 4 * e;
+      w[e] = *reinterpret_cast<const uint32_t*>(word < last ? word : last);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int bytes = left - 4 * e;  // that are left for this word
+      const uint32_t mask = bytes >= 4 ? ~0u : bytes > 0 ? (1u << (8 * bytes)) - 1u : 0u;
+      v[e] = __builtin_amdgcn_alignbyte(w[e + 1], w[e], (uint32_t)from & 3u) & mask;
+    }
   }
-  return w;
+  return v;
 }
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t row_rsrc(const char* p, uint32_t bytes) {
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(p), 0, (int)bytes, 0x00020000);

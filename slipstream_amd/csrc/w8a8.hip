@@ -2,55 +2,91 @@
 // x and w in int8. The sum is exact in int32 for k < 2^17 (128 * 128 * k < 2^31, refused
 // beyond), so a result does not depend on the kernel, the tile or the split that computed
 // it: it is rounded in fp32 by the scales and once to the output's type.
+#include <utility>
+
 #include "w8a8_common.h"
 
 namespace ss {
 namespace {
 
-// Sixteen keys of a row at any alignment (global accesses need none on this target); past the
-// row's end zeros.
+// Sixteen keys of a row at any alignment (global accesses need none on this target), past the
+// row's end zeros. A row's last, partial piece is put together from the aligned words that hold
+// its keys, read at the last one where they lie behind it: sixteen loads of a byte, each under
+// its own condition, wait for one another (the copies of 2000 rows of 1000: 6.5 us, so 4.0).
 __device__ __forceinline__ i32x4 load_keys(const int8_t* row, int at, int k) {
   i32x4 v = {0, 0, 0, 0};
   if (at + 16 <= k) {
     __builtin_memcpy(&v, row + at, 16);
   } else if (at < k) {
-    int8_t b[16];
+    const uint64_t from = (uint64_t)(row + at), last = (uint64_t)(row + k - 1) & ~3ull;
+    uint32_t w[5];
 #pragma unroll
-    for (int e = 0; e < 16; ++e) b[e] = at + e < k ? row[at + e] : (int8_t)0;
-    __builtin_memcpy(&v, b, 16);
+    for (int e = 0; e < 5; ++e) {
+      const uint64_t word = (from & ~3ull) + 4 * e;
+      w[e] = *reinterpret_cast<const uint32_t*>(word < last ? word : last);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int keys = k - at - 4 * e;  // that are left for this word
+      const uint32_t mask = keys >= 4 ? ~0u : keys > 0 ? (1u << (8 * keys)) - 1u : 0u;
+      v[e] = (int)(__builtin_amdgcn_alignbyte(w[e + 1], w[e], (uint32_t)from & 3u) & mask);
+    }
   }
   return v;
 }
 
 // The other kernels' operands begin every row on 16 bytes and end it with 16. Rows that do not
 // are copied to rows that do, zeros behind them, in the workspace: 333 x 4999 x 2051 (rows at any
-// byte) 30.4 us in the general kernel, 22.3 so, of which 7 for the copy.
-// A wave copies a row, four pieces a lane on their way.
+// byte) 30.4 us in the general kernel, 20.7 so, of which 8 for the copies.
+// Two pieces a thread, both on their way before the first is written.
 struct Rows {
   const int8_t* from;
   int8_t* to;
   int64_t stride;  // of `from`
-  int64_t rows;
+  int rows;
 };
-__global__ __launch_bounds__(256) void w8a8_align_kernel(Rows x, Rows w, int k, int pieces) {
-  const int lane = threadIdx.x & 63;
-  for (int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); r < x.rows + w.rows; r += (int64_t)gridDim.x * 4) {
-    const bool of_x = r < x.rows;
-    const int64_t i = of_x ? r : r - x.rows;
-    const int8_t* const from = of_x ? x.from + i * x.stride : w.from + i * w.stride;
-    int8_t* const to = (of_x ? x.to : w.to) + i * (16 * (int64_t)pieces);
-    const int full = k >> 4;
-    for (int c = lane; c < full; c += 256) {
-      i32x4 v[4];
+__global__ __launch_bounds__(256) void w8a8_align_kernel(Rows x, Rows w, int k, uint32_t pieces) {
+  const uint32_t total = (uint32_t)(x.rows + w.rows) * pieces, half = (total + 1) >> 1;
+  const uint32_t i = blockIdx.x * 256 + threadIdx.x;
+  if (i >= half) return;
+  i32x4 v[2];
+  int8_t* to[2];
 #pragma unroll
-      for (int u = 0; u < 4; ++u)
-        if (c + 64 * u < full) __builtin_memcpy(&v[u], from + 16 * (c + 64 * u), 16);
-#pragma unroll
-      for (int u = 0; u < 4; ++u)
-        if (c + 64 * u < full) *reinterpret_cast<i32x4*>(to + 16 * (c + 64 * u)) = v[u];
-    }
-    if (full < pieces && lane < 16) to[16 * full + lane] = 16 * full + lane < k ? from[16 * full + lane] : (int8_t)0;
+  for (int u = 0; u < 2; ++u) {
+    const uint32_t j = i + u * half;
+    to[u] = nullptr;
+    if (j >= total) continue;
+    const uint32_t r = j / pieces, c = 16 * (j - r * pieces);
+    const bool of_x = r < (uint32_t)x.rows;
+    const int64_t row = of_x ? r : r - x.rows;
+    to[u] = (of_x ? x.to : w.to) + row * (16 * (int64_t)pieces) + c;
+    v[u] = load_keys((of_x ? x.from : w.from) + row * (of_x ? x.stride : w.stride), (int)c, k);
   }
+#pragma unroll
+  for (int u = 0; u < 2; ++u)
+    if (to[u]) *reinterpret_cast<i32x4*>(to[u]) = v[u];
+}
+
+// The copies of both operands (0 rows: none), as many rows a launch as its 32-bit piece numbers hold
+int align_rows(Rows x, Rows w, int k, hipStream_t stream) {
+  const int pieces = (k + 15) / 16;
+  const int most = (1 << 30) / pieces;
+  for (int64_t left = (int64_t)x.rows + w.rows; left > 0;) {
+    const Rows px = {x.from, x.to, x.stride, x.rows < most ? x.rows : most};
+    const Rows pw = {w.from, w.to, w.stride, w.rows < most - px.rows ? w.rows : most - px.rows};
+    const int64_t half = ((int64_t)(px.rows + pw.rows) * pieces + 1) / 2;
+    hipLaunchKernelGGL(w8a8_align_kernel, dim3((unsigned)((half + 255) / 256)), dim3(256), 0, stream, px, pw, k,
+                       (uint32_t)pieces);
+    const int st = ss_host::launch_status("w8a8 gemm (align)");
+    if (st != SS_OK) return st;
+    for (auto [all, part] : {std::pair<Rows*, const Rows*>{&x, &px}, {&w, &pw}}) {
+      all->from += part->rows * all->stride;
+      all->to += part->rows * (16 * (int64_t)pieces);
+      all->rows -= part->rows;
+    }
+    left -= px.rows + pw.rows;
+  }
+  return SS_OK;
 }
 
 // The kernel for every shape, stride and alignment, without a workspace: 64 x 64 results a
@@ -217,14 +253,11 @@ extern "C" int ss_w8a8_gemm(const int8_t* x, const float* x_scale, const int8_t*
   const int64_t kp = ss::round16(k);
   const bool copy_x = !ss::whole_rows(p.x, m, p.x_stride, k), copy_w = !ss::whole_rows(p.w, n, p.w_stride, k);
   const int64_t x_bytes = copy_x ? m * kp : 0, w_bytes = copy_w ? n * kp : 0;
-  if (k > 0 && x_bytes + w_bytes <= left) {
+  if (k > 0 && x_bytes + w_bytes <= left && m <= INT32_MAX && n <= INT32_MAX) {
     if (copy_x || copy_w) {
-      const ss::Rows rx = {p.x, (int8_t*)ws, p.x_stride, copy_x ? m : 0};
-      const ss::Rows rw = {p.w, (int8_t*)ws + x_bytes, p.w_stride, copy_w ? n : 0};
-      const int64_t blocks = (rx.rows + rw.rows + 3) / 4, cap = (int64_t)ss_host::device_cu_count() * 32;
-      hipLaunchKernelGGL(ss::w8a8_align_kernel, dim3((unsigned)(blocks < cap ? blocks : cap)), dim3(256), 0, s, rx, rw,
-                         (int)k, (int)(kp / 16));
-      const int sa = ss_host::launch_status("w8a8 gemm (align)");
+      const ss::Rows rx = {p.x, (int8_t*)ws, p.x_stride, copy_x ? (int)m : 0};
+      const ss::Rows rw = {p.w, (int8_t*)ws + x_bytes, p.w_stride, copy_w ? (int)n : 0};
+      const int sa = ss::align_rows(rx, rw, (int)k, s);
       if (sa != SS_OK) return sa;
       if (copy_x) p.x = rx.to, p.x_stride = kp;
       if (copy_w) p.w = rw.to, p.w_stride = kp;

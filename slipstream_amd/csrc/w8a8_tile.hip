@@ -309,48 +309,44 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(G, G))) voi
       }
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    auto results = [&](int r, TO (&y)[CL]) __attribute__((always_inline)) {
+      u32x4 v[CL / 4];
+#pragma unroll
+      for (int h = 0; h < CL / 4; ++h) v[h] = load16(turn + r * RS + (c + 4 * h) * 4);
+      if constexpr (__is_same(TO, int)) {
+#pragma unroll
+        for (int e = 0; e < CL; ++e) y[e] = (int)v[0][e];
+      } else {
+        float y32[CL];
+#pragma unroll
+        for (int e = 0; e < CL; ++e)
+          y32[e] = fmaf(__builtin_bit_cast(float, (uint32_t)v[e / 4][e % 4]),
+                        __builtin_bit_cast(float, (uint32_t)ws[e / 4][e % 4]), biasf[e]);
+        pack_results<CL>(y, y32);
+      }
+    };
     if (pieces) {
 #pragma unroll
       for (int q = 0; q < LR / 2; ++q) {
-        const int r = q * (64 / LR) + lane / LR;
-        u32x4 v[CL / 4];
-#pragma unroll
-        for (int h = 0; h < CL / 4; ++h) v[h] = load16(turn + r * RS + (c + 4 * h) * 4);
         TO y[CL];
-        if constexpr (__is_same(TO, int)) {
-#pragma unroll
-          for (int e = 0; e < CL; ++e) y[e] = (int)v[0][e];
-        } else {
-          float y32[CL];
-#pragma unroll
-          for (int e = 0; e < CL; ++e)
-            y32[e] = fmaf(__builtin_bit_cast(float, (uint32_t)v[e / 4][e % 4]),
-                          __builtin_bit_cast(float, (uint32_t)ws[e / 4][e % 4]), biasf[e]);
-          pack_results<CL>(y, y32);
-        }
+        results(q * (64 / LR) + lane / LR, y);
         __builtin_amdgcn_raw_buffer_store_b128(as_words(y), ro, o_at + o_row, 0, 0);
         o_row += 64 / LR * row_bytes;
       }
     } else {
-      // element by element, a lane one of consecutive channels
-      constexpr int WC = 32 * NT, PER = WC > 64 ? 64 : WC;
-      for (int h = 0; h < WC; h += PER) {
-        const int ch = h + lane % PER;
-        float ws1 = 0.f, bias1 = 0.f;
-        if constexpr (!__is_same(TO, int)) {
-          ws1 = p.w_scale[min(n0 + 32 * NT * wn + ch, p.n - 1)];
-          bias1 = bias_value(rb, bias_bits(rb, 32 * NT * wn + ch));
-        }
-#pragma unroll 4
-        for (int r = lane / PER; r < 32; r += 64 / PER) {
-          const uint32_t v = *reinterpret_cast<const uint32_t*>(turn + r * RS + ch * 4);
-          if (32 * mt + r < left_rows && ch < left_chans) {
-            TO* const o = out + (m0 + 32 * (MT * wm + mt) + r) * p.o_stride + n0 + 32 * NT * wn + ch;
-            if constexpr (__is_same(TO, int))
-              *o = (int)v;
-            else
-              *o = (TO)fmaf(__builtin_bit_cast(float, v), ws1, bias1);
-          }
+      // at any alignment (global accesses need none on this target), a row's last ones one by one
+#pragma unroll 2
+      for (int r = lane / LR; r < 32; r += 64 / LR) {
+        TO y[CL];
+        results(r, y);
+        if (32 * mt + r >= left_rows || c >= left_chans) continue;
+        TO* const o = out + (m0 + 32 * (MT * wm + mt) + r) * p.o_stride + n0 + c0;
+        if (c + CL <= left_chans) {
+          __builtin_memcpy(o, y, sizeof(y));
+        } else {
+#pragma unroll
+          for (int e = 0; e < CL; ++e)
+            if (c + e < left_chans) o[e] = y[e];
         }
       }
     }
@@ -363,14 +359,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(G, G))) voi
 // four ranges' at a time (past the last: outside the descriptor, zeros).
 template <typename TO, bool VEC>
 __global__ __launch_bounds__(256) void w8a8_reduce_kernel(const W8Params p, const int* __restrict__ part, int ks) {
-  const int quads = (int)((p.n + 3) >> 2);
-  const int64_t total = p.m * quads;
+  const uint32_t quads = (uint32_t)((p.n + 3) >> 2), total = (uint32_t)p.m * quads;  // m n below 2^29
   const int plane = (int)(p.m * p.n) * 4;  // bytes; ks of them below 2^31
   const __amdgpu_buffer_rsrc_t rp = buffer_over(part, (uint32_t)(ks * plane));
   const __amdgpu_buffer_rsrc_t rws = buffer_over(p.w_scale, (uint32_t)(p.n * 4));
   const BiasReader rb = bias_reader(p, 0, (int)p.n);
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-    const int m = (int)(i / quads), n = 4 * (int)(i - (int64_t)m * quads);
+  for (uint32_t i = blockIdx.x * 256 + threadIdx.x; i < total; i += gridDim.x * 256) {
+    const int m = (int)(i / quads), n = 4 * (int)(i - m * quads);
     const int at = (m * (int)p.n + n) * 4;
     const float xs = p.x_scale[m];
     uint32_t ws[4], bias[4];

@@ -23,7 +23,12 @@ def _outputs(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     if not shape:
         raise ValueError("rows need at least one dimension")
     make = x.new_empty if shape[-1] else x.new_zeros
-    return x.new_empty(shape, dtype=torch.int8), make(shape[:-1], dtype=torch.float32)
+    return _like(x, torch.int8), make(shape[:-1], dtype=torch.float32)
+
+
+def _like(x: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    """A contiguous tensor of ``x``'s shape (``empty_like`` is the cheaper call)."""
+    return torch.empty_like(x, dtype=dtype) if x.is_contiguous() else x.new_empty(x.shape, dtype=dtype)
 
 
 def _flat(x: torch.Tensor, cols: int) -> tuple[torch.Tensor, int]:
@@ -61,7 +66,7 @@ def fused_rmsnorm_int8(x: torch.Tensor, weight: torch.Tensor, residual: torch.Te
         dtypes = {x.dtype, weight.dtype} | ({residual.dtype} if residual is not None else set())
         raise ValueError(f"x, weight and residual must share a dtype, got {sorted(map(str, dtypes))}")
     dtype = _ffi.dtype_code(x.dtype)
-    s = x.new_empty(x.shape) if residual is not None else None
+    s = _like(x, x.dtype) if residual is not None else None
     if q.numel() == 0:
         return q, scale, s
     x2, xs = _flat(x, cols)
