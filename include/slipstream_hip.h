@@ -285,7 +285,8 @@ int ss_w8a8_gemm(const int8_t* x, const float* x_scale, const int8_t* w, const f
  * elements; dtype SS_DTYPE_BF16/F16/F32, arithmetic in fp32 or wider. cols < 2^29.
  *   ss_quantize_int8: y = x.
  *   ss_rmsnorm_int8: the norm of ss_rmsnorm with an int8 output: s = x + residual rounded to
- *     dtype and written to sum [rows, cols] (contiguous; residual and sum NULL: s = x),
+ *     dtype and written to sum [rows, cols] (contiguous; it may be residual itself, or x, where
+ *     that is; residual and sum NULL: s = x),
  *     y = s * weight / sqrt(mean(s^2) + eps), not rounded before it is quantized.
  *   ss_swiglu_int8: y = silu(gate) * up, not rounded before it is quantized.
  */

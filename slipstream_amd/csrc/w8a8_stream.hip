@@ -113,7 +113,6 @@ __global__ __launch_bounds__(512) void w8a8_stream_kernel(const W8Params p, int 
   for (int d = 0; d < D; ++d)
     if (d < count) request(d, d);
   for (int i = threadIdx.x; i < MT * NT * 4 * kPlane; i += blockDim.x) s_sum[i] = 0;
-  if (threadIdx.x < 16 * MT) s_xs[threadIdx.x] = __builtin_bit_cast(float, xs);
 
   // fragment of lane (ln, kg): row ln, key step s: chunk 2 kg + s
   const int f[2] = {ln * 128 + 16 * ((2 * kg) ^ stream_swizzle(ln)), ln * 128 + 16 * ((2 * kg + 1) ^ stream_swizzle(ln))};
@@ -143,6 +142,7 @@ __global__ __launch_bounds__(512) void w8a8_stream_kernel(const W8Params p, int 
 #pragma unroll
         for (int u = 0; u < MT; ++u) acc[t][u] = mfma_i8(a[s][t], b[s][u], acc[t][u]);
   }
+  if (threadIdx.x < 16 * MT) s_xs[threadIdx.x] = __builtin_bit_cast(float, xs);
   __syncthreads();  // the sums are cleared
   if (count > 0) {
 #pragma unroll

@@ -1,17 +1,22 @@
 // W8A8 tile kernel: the int8 product at the sizes where the matrix cores set the time (a prefill
 // chunk's or a packed step's tokens).
 //
-// Four waves, one per SIMD, in a 2 x 2 grid multiply 32 MT tokens with 32 NT channels, wave
-// (wm, wn) 16 MT x 16 NT of them. Both operands come into LDS by DMA, 128 keys of every row a
-// stage, two stages in turn. A wave holds the fragments of half a stage (64 keys) in registers
-// while it multiplies them and reads the next half's beside the products, so a stage's LDS is
-// free again once its second half has been read, long before it is multiplied:
+// Four waves multiply 32 MT WM tokens with 32 NT (4 / WM) channels, wave (wm, wn) 32 MT x 32 NT
+// of them. Both operands come into LDS by DMA, 128 keys of every row a stage, into rings of as
+// many stages as fit (256 x 256: three of the tokens', two of the channels'). A wave holds the
+// fragments of half a stage (64 keys) in registers while it multiplies them and reads the next
+// half's beside the products, so a stage's LDS is free again once its second half has been
+// read, long before it is multiplied:
 //   first half's products:  the second half's fragments are read, then (barrier) the stage's
-//                           LDS is free and the DMAs of the stage after the next begin
-//   second half's products: the DMAs go on; the next stage's, a whole stage old, have landed
+//                           LDS is free and the DMAs into it begin
+//   second half's products: the DMAs go on; the next stage's, a stage or more old, have landed
 //                           (wait, barrier) and its first half's fragments are read
 // One wave per SIMD has nothing to hide behind, so the order is written out: every product is
-// followed by at most one fragment read or DMA, and the scheduler is held to that order.
+// followed by at most a fragment read or two and a DMA, and the scheduler is held to that
+// order. At 2240 x 28672 x 4096 (231 to 239 us) the products are under way in 60 % of the cycles
+// and the card's power holds the clock at 1.86 GHz; the products alone, with nothing read, take
+// 187 us. Small tiles are bound by their LDS reads: a 64 x 128 tile's 72 KB a stage take the 570
+// cycles that a stage does.
 #include <type_traits>
 #include <utility>
 

@@ -216,6 +216,25 @@ def test_nothing_is_written_past_the_rows(device):
             assert (got[:edge] == 77).all() and (got[edge + n :] == 77).all()
 
 
+@pytest.mark.parametrize("cols", [64, 1003, 4096, 40001])
+@pytest.mark.parametrize("into", ["residual", "x"])
+def test_sum_in_place(device, cols, into):
+    """The C entry with the sum written over one of its addends."""
+    from slipstream_amd import _ffi
+
+    g = torch.Generator(device=device).manual_seed(cols)
+    x, r = (_rand(g, (5, cols), torch.bfloat16, device) for _ in range(2))
+    w = torch.ones(cols, device=device, dtype=torch.bfloat16)
+    want = fused_rmsnorm_int8(x, w, r)
+    q = torch.empty((5, cols), dtype=torch.int8, device=device)
+    scale = torch.empty(5, device=device)
+    s = r if into == "residual" else x
+    _ffi.check(_ffi.lib().ss_rmsnorm_int8(x.data_ptr(), r.data_ptr(), w.data_ptr(), q.data_ptr(), scale.data_ptr(),
+                                          s.data_ptr(), 5, cols, cols, cols, 1e-6, _ffi.dtype_code(x.dtype),
+                                          _ffi.stream_ptr(device)), "norm")
+    assert torch.equal(q, want[0]) and torch.equal(scale, want[1]) and torch.equal(s, want[2])
+
+
 def test_more_bytes_than_31_bits_hold(device):
     """Rows whose addresses pass 2^31 and 2^32 bytes: the last ones are as they are alone."""
     rows, cols = 280_000, 8192  # 4.6 GB in bf16
