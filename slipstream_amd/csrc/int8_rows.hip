@@ -4,6 +4,8 @@
 //
 // Mathematics, for a row y of fp32 values:
 //   a = max |y|;  scale = a / 127;  q = rint(y * 127 / a), half to even;  y ~ q * scale.
+//   Plain rows and SwiGLU: 1 / a, its product with 127 and the product with y are each rounded to
+//   fp32, so that elementary operations on the same y give the same q. Norms: in 64 bits.
 //   A row whose scale would be subnormal (a < 127 * 2^-126) is zeros with scale zero: 127 / a
 //   stays finite, and what is dropped is below 1.5e-36.
 //   A row that holds a NaN or an infinity gets zeros and the scale NaN, so that every product
@@ -15,7 +17,7 @@
 //   q = rint(p * 127 / a) and scale = r * a / 127. So both reductions, the sum of squares and
 //   the maximum, share one exchange between the waves, and q is the same whatever the order
 //   of the sum. Nothing is rounded to 16 bits between the norm and its int8 values.
-// SwiGLU: y = g / (1 + exp(-g)) * u in fp32, not rounded before it is quantized.
+// SwiGLU: y = g / (1 + exp(-g)) * u, each operation rounded to fp32 and none to 16 bits.
 #include "ss_common.h"
 
 namespace {
@@ -104,11 +106,15 @@ __device__ __forceinline__ float wave_sum(float x) {
   return add_dpp<0xB1>(x);
 }
 
-// g / (1 + exp(-g)) by the hardware's exp2 and reciprocal (one unit in the last place each; the
-// product with log2 e adds |g| 2^-24): a step of int8 is 2^-8 of the row's largest value.
-// exp overflows to infinity below g = -88.7, where the value is under 2^-120 and becomes -0.
+// g / (1 + exp(-g)), the quotient rounded to nearest: a reciprocal refined by one Newton step, and
+// Markstein's correction of the quotient by its remainder (the range scaling that a general
+// division adds has nothing to do for a divisor from 1 on: 2240 x 14336 38.1 us with it, 34.7 so,
+// 28.0 with the hardware's exp2 and reciprocal alone, whose last bits moved some tens of q by a
+// step). From a divisor of 2^100 on, where the value is below 1e-28, g times the plain reciprocal.
 __device__ __forceinline__ float silu(float g) {
-  return g * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-ss::kLog2e * g));
+  const float d = 1.f + expf(-g);
+  const float r0 = __builtin_amdgcn_rcpf(d), r = fmaf(fmaf(-d, r0, 1.f), r0, r0), q = g * r;
+  return d < 0x1p100f ? fmaf(fmaf(-d, q, g), r, q) : g * r0;
 }
 
 // The low bytes of four words in a dword.
@@ -116,15 +122,14 @@ __device__ __forceinline__ uint32_t low_bytes(uint32_t b0, uint32_t b1, uint32_t
   return __builtin_amdgcn_perm(b1, b0, 0x0C0C0400u) | __builtin_amdgcn_perm(b3, b2, 0x04000C0Cu);
 }
 // Four values times 127 / a -> four int8 in a dword. A product plus 1.5 * 2^23 (2^52) is rounded to
-// an integer, half to even, whose two's complement is the sum's low bits. Rows and norms do this
-// in 64 bits, where 127 / a has no error that could put a value on the other side of a half: a
-// step of one normalised value changes every output of its row behind the next product.
-// (2240 x 4096: rows 5.95 us in 32 bits, 6.30 so; norms 10.69 and 10.74.) SwiGLU's values are
-// known to some 2^-21 only, and stay in 32.
+// an integer, half to even, whose two's complement is the sum's low bits. Rows and SwiGLU round
+// the product to fp32 first, as an elementary product does. Norms do it in 64 bits, where nothing
+// puts a value on the other side of a half: a step of one normalised value changes every output of
+// its row behind the next product (2240 x 4096 10.69 us in 32 bits, 10.74 so).
 __device__ __forceinline__ uint32_t quant4(const float* p, float inv) {
   uint32_t b[4];
 #pragma unroll
-  for (int e = 0; e < 4; ++e) b[e] = __builtin_bit_cast(uint32_t, fmaf(p[e], inv, 12582912.f));
+  for (int e = 0; e < 4; ++e) b[e] = __builtin_bit_cast(uint32_t, pin(p[e] * inv) + 12582912.f);
   return low_bytes(b[0], b[1], b[2], b[3]);
 }
 __device__ __forceinline__ uint32_t quant4(const float* p, double inv) {
@@ -135,11 +140,15 @@ __device__ __forceinline__ uint32_t quant4(const float* p, double inv) {
 }
 template <int MODE>
 struct InvOf {
+  typedef float type;
+};
+template <>
+struct InvOf<kNorm> {
   typedef double type;
 };
 template <>
-struct InvOf<kSwiglu> {
-  typedef float type;
+struct InvOf<kNormRes> {
+  typedef double type;
 };
 
 // 16 bytes at any alignment (global accesses need none on this target). A row's last, partial
@@ -237,7 +246,13 @@ __device__ __forceinline__ typename InvOf<MODE>::type finish_row(uint32_t top, f
   const float peak = __builtin_bit_cast(float, top);
   const bool finite = top < 0x7F800000u, live = finite && peak >= kSmallest;
   typedef typename InvOf<MODE>::type Inv;
-  const Inv inv = live ? (Inv)kLevels / (Inv)peak : (Inv)0;
+  Inv inv = (Inv)0;
+  if (live) {
+    if constexpr (__is_same(Inv, double))
+      inv = (double)kLevels / (double)peak;
+    else  // 1 / a is subnormal, so short of bits, from 2^126 on
+      inv = peak < 0x1p126f ? kLevels * (1.f / peak) : kLevels / peak;
+  }
   if (threadIdx.x == 0) {
     float scale = live ? peak / kLevels : 0.f;
     if constexpr (MODE == kNorm || MODE == kNormRes) scale *= 1.f / __builtin_sqrtf(sq / (float)a.cols + a.eps);
