@@ -5,7 +5,7 @@
 // Mathematics, for a row y of fp32 values:
 //   a = max |y|;  scale = a / 127;  q = rint(y * 127 / a), half to even;  y ~ q * scale.
 //   Plain rows and SwiGLU: 1 / a, its product with 127 and the product with y are each rounded to
-//   fp32, so that elementary operations on the same y give the same q. Norms: in 64 bits.
+//   fp32, so that elementary operations on the same y give the same q. Norms: the exact q.
 //   A row whose scale would be subnormal (a < 127 * 2^-126) is zeros with scale zero: 127 / a
 //   stays finite, and what is dropped is below 1.5e-36.
 //   A row that holds a NaN or an infinity gets zeros and the scale NaN, so that every product
@@ -123,9 +123,12 @@ __device__ __forceinline__ uint32_t low_bytes(uint32_t b0, uint32_t b1, uint32_t
 }
 // Four values times 127 / a -> four int8 in a dword. A product plus 1.5 * 2^23 (2^52) is rounded to
 // an integer, half to even, whose two's complement is the sum's low bits. Rows and SwiGLU round
-// the product to fp32 first, as an elementary product does. Norms do it in 64 bits, where nothing
-// puts a value on the other side of a half: a step of one normalised value changes every output of
-// its row behind the next product (2240 x 4096 10.69 us in 32 bits, 10.74 so).
+// the product to fp32 first, as an elementary product does. Norms do it in 64 bits, where q is the
+// exact quotient's nearest, half to even: the product is first rounded to multiples of 2^-40. With
+// 24 bits in p and a, a quotient that is no half is 2^-33 away from one at least (|p| > a / 254 there,
+// so p 254 - a (2 n + 1), over 2 a, counts units of a 2^-32), and the error of 127 / a moves it by
+// 2^-46 at most. A step of one normalised value changes every output of its row behind the next
+// product, and 16-bit rows hold many exact halves (2240 x 4096 10.69 us in 32 bits, 10.8 so).
 __device__ __forceinline__ uint32_t quant4(const float* p, float inv) {
   uint32_t b[4];
 #pragma unroll
@@ -135,7 +138,10 @@ __device__ __forceinline__ uint32_t quant4(const float* p, float inv) {
 __device__ __forceinline__ uint32_t quant4(const float* p, double inv) {
   uint32_t b[4];
 #pragma unroll
-  for (int e = 0; e < 4; ++e) b[e] = (uint32_t)__builtin_bit_cast(uint64_t, fma((double)p[e], inv, 6755399441055744.0));
+  for (int e = 0; e < 4; ++e) {
+    const double fine = fma((double)p[e], inv, 6144.0);  // 1.5 * 2^12
+    b[e] = (uint32_t)__builtin_bit_cast(uint64_t, fine + (6755399441055744.0 - 6144.0));
+  }
   return low_bytes(b[0], b[1], b[2], b[3]);
 }
 template <int MODE>

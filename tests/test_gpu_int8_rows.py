@@ -144,6 +144,26 @@ def test_row_counts_agree(device, rows):
     _check(q, scale, y, 0.0, _norm_scale_err(1024), f"{rows} rows")
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("cols", [64, 4096, 40001])
+def test_norm_rounds_exact_halves_to_even(device, dtype, cols):
+    """Normalised rows of few bits hold many exact halves of a step, and q is the nearest integer of
+    the exact quotient, found here in whole numbers: with p = x * w and a = max |p|,
+    |q| = floor((254 |p| + a) / 2 a), less one where that was a half and gives an odd number."""
+    g = torch.Generator(device="cpu").manual_seed(cols)
+    x = torch.randint(-254, 255, (33, cols), generator=g)
+    w = torch.randint(1, 4, (cols,), generator=g)
+    q, scale, _ = fused_rmsnorm_int8(x.to(device, dtype), w.to(device, dtype))
+    p = x * w
+    top = p.abs().amax(-1, keepdim=True)
+    num = 254 * p.abs() + top
+    n = num // (2 * top)
+    half = (num % (2 * top) == 0) & (top > 0)
+    n = torch.where(half & (n % 2 == 1), n - 1, n)
+    assert half.sum().item() > 0
+    assert torch.equal(q.cpu().long(), n * p.sign())
+
+
 def test_norm_in_int8_is_the_norm(device):
     """The int8 rows stand for what ``fused_rmsnorm`` gives: within half a step and that
     op's two roundings to bf16 (2^-8 of the value each)."""
