@@ -7,7 +7,7 @@
 //   Plain rows and SwiGLU: 1 / a, its product with 127 and the product with y are each rounded to
 //   fp32, so that elementary operations on the same y give the same q. Norms: the exact q.
 //   A row whose scale would be subnormal (a < 127 * 2^-126) is zeros with scale zero: 127 / a
-//   stays finite, and what is dropped is below 1.5e-36.
+//   stays finite, and what is dropped is below 1.5e-36. Norms go by p below, before r is known.
 //   A row that holds a NaN or an infinity gets zeros and the scale NaN, so that every product
 //   with it is NaN and none is silently finite. The maximum is taken over the magnitudes' bit
 //   patterns as unsigned integers, in which infinity follows every number and NaN infinity.
