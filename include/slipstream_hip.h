@@ -283,8 +283,8 @@ int ss_w8a8_gemm(const int8_t* x, const float* x_scale, const int8_t* w, const f
  * holds a NaN or an infinity is zeros with scale NaN. q [rows, cols] and scale [rows] are
  * contiguous; x, residual, gate and up have row strides in elements and unit column strides, at
  * any alignment of their elements; dtype SS_DTYPE_BF16/F16/F32, arithmetic in fp32 or wider: the
- * norm's q is exact for s * weight in fp32, the others round 1 / a, its product with 127 and that
- * with y to fp32. cols < 2^29.
+ * norm's q is exact for s * weight in fp32; the others' is that of fp32 operations, with the
+ * reciprocal of a, its product with 127 and the product with y rounded each. cols < 2^29.
  *   ss_quantize_int8: y = x.
  *   ss_rmsnorm_int8: the norm of ss_rmsnorm with an int8 output: s = x + residual rounded to
  *     dtype and written to sum [rows, cols] (contiguous; it may be residual itself, or x, where
