@@ -307,3 +307,34 @@ def test_more_rows_than_a_launch_holds(device):
     s, one = torch.zeros_like(x), torch.ones(cols, device=device)
     q, scale, s = fused_rmsnorm_int8(x, one, s)
     assert torch.equal(s, x) and (q.amax(1) == 127).all() and torch.isfinite(scale).all()
+
+
+@pytest.mark.parametrize("rows,cols,with_residual", [(2240, 4096, True), (300, 4096, False), (300, 1003, True)])
+def test_norm_differs_from_elementary_operations_at_halves_only(device, rows, cols, with_residual):
+    """Rows in bf16 in which a few channels are large: the call repeats itself bit for bit, its sum is
+    the elementary one, and where its q is not that of ``s * rsqrt(mean(s^2) + eps) * w`` in fp32, the
+    exact quotient s w 127 / max|s w| is a half of a step, which that chain's last bits send either
+    way and the kernel sends to even. s and w have 8 bits each, so doubles hold s w, 254 s w and the
+    remainder exactly."""
+    g = torch.Generator(device=device).manual_seed(rows + cols)
+
+    def states():
+        x = torch.randn(rows, cols, generator=g, device=device) * torch.exp(0.5 * torch.randn(rows, 1, generator=g, device=device))
+        return (x * torch.where(torch.rand(cols, generator=g, device=device) < 0.004, 12.0, 1.0)).to(torch.bfloat16)
+
+    x, r = states(), states() if with_residual else None
+    w = (1 + 0.1 * torch.randn(cols, generator=g, device=device)).to(torch.bfloat16)
+    first = fused_rmsnorm_int8(x, w, r)
+    for _ in range(3):
+        assert all(a is b or torch.equal(a, b) for a, b in zip(first, fused_rmsnorm_int8(x, w, r)))
+    q, scale, s = first
+    hidden = x if r is None else (x.float() + r.float()).to(torch.bfloat16)
+    assert s is None or torch.equal(s, hidden)
+    y = hidden.float()
+    y = y * torch.rsqrt(y.square().mean(-1, keepdim=True) + 1e-6) * w.float()
+    plain = torch.round(y * (127 / y.abs().amax(-1, keepdim=True)))
+    row, col = (q.float() != plain).nonzero(as_tuple=True)
+    p = hidden.double() * w.double()
+    top, p = p.abs().amax(-1)[row], p[row, col].abs()
+    assert (torch.remainder(254 * p + top, 2 * top) == 0).all()
+    assert (q[row, col] % 2 == 0).all() and (q[row, col].float() - plain[row, col]).abs().eq(1).all()
