@@ -279,8 +279,8 @@ int ss_w8a8_gemm(const int8_t* x, const float* x_scale, const int8_t* w, const f
 /*
  * Rows quantized to int8 with one fp32 scale each, the inputs of ss_w8a8_gemm:
  *   a = max |y|, scale = a / 127, q = rint(y * 127 / a) (half to even), y ~ q * scale.
- * A row with a < 127 * 2^-126 (the norm: the a of s * weight) is zeros with scale 0; a row that
- * holds a NaN or an infinity is zeros with scale NaN. q [rows, cols] and scale [rows] are
+ * A row with a < 127 * 2^-126 (the norm: the a of s * weight, whatever eps) is zeros with scale 0;
+ * a row that holds a NaN or an infinity (the norm: in s * weight, in fp32) is zeros with scale NaN. q [rows, cols] and scale [rows] are
  * contiguous; x, residual, gate and up have row strides in elements and unit column strides, at
  * any alignment of their elements; dtype SS_DTYPE_BF16/F16/F32, arithmetic in fp32 or wider: the
  * norm's q is exact for s * weight in fp32; the others' is that of fp32 operations, with the
@@ -289,7 +289,8 @@ int ss_w8a8_gemm(const int8_t* x, const float* x_scale, const int8_t* w, const f
  *   ss_rmsnorm_int8: the norm of ss_rmsnorm with an int8 output: s = x + residual rounded to
  *     dtype and written to sum [rows, cols] (contiguous; it may be residual itself, or x, where
  *     that is; residual and sum NULL: s = x),
- *     y = s * weight / sqrt(mean(s^2) + eps), not rounded before it is quantized.
+ *     y = s * weight / sqrt(mean(s^2) + eps), not rounded before it is quantized; also where the
+ *     squares' sum is more or less than fp32 holds.
  *   ss_swiglu_int8: y = silu(gate) * up, not rounded before it is quantized.
  */
 int ss_quantize_int8(const void* x, int8_t* q, float* scale, int64_t rows, int64_t cols, int64_t x_stride,

@@ -16,7 +16,8 @@
 //   not depend on it: with p = s * w (exact in fp32 for 16-bit types) and a = max |p|,
 //   q = rint(p * 127 / a) and scale = r * a / 127. So both reductions, the sum of squares and
 //   the maximum, share one exchange between the waves, and q is the same whatever the order
-//   of the sum. Nothing is rounded to 16 bits between the norm and its int8 values.
+//   of the sum. Nothing is rounded to 16 bits between the norm and its int8 values. A row whose
+//   squares' sum fp32 does not hold has it taken again, of s times a power of two.
 // SwiGLU: y = g / (1 + exp(-g)) * u, each operation rounded to fp32 and none to 16 bits.
 #include "ss_common.h"
 
@@ -228,9 +229,16 @@ __device__ __forceinline__ void fold(u32x4& xw, const u32x4& yw, const u32x4& ww
   for (int e = 0; e < EPP; ++e) top = umax(top, magnitude(v[e]));
 }
 
+template <int MODE>
+struct RowEnd {
+  typename InvOf<MODE>::type inv;  // 127 / a, zero where q is
+  float peak;                      // a
+  float by;                        // norms: not zero where the scale is still to be found, by scale_again
+};
+
 // The row's largest magnitude and sum over the workgroup, then 127 / a, and the scale written.
 template <int MODE, int WAVES>
-__device__ __forceinline__ typename InvOf<MODE>::type finish_row(uint32_t top, float sq, const RowArgs& a, int64_t row) {
+__device__ __forceinline__ RowEnd<MODE> finish_row(uint32_t top, float sq, const RowArgs& a, int64_t row) {
   __shared__ uint32_t s_top[WAVES];
   __shared__ float s_sq[WAVES];
   top = wave_umax(top);
@@ -249,22 +257,58 @@ __device__ __forceinline__ typename InvOf<MODE>::type finish_row(uint32_t top, f
       sq += s_sq[i];
     }
   }
-  const float peak = __builtin_bit_cast(float, top);
-  const bool finite = top < 0x7F800000u, live = finite && peak >= kSmallest;
-  typedef typename InvOf<MODE>::type Inv;
-  Inv inv = (Inv)0;
+  RowEnd<MODE> end = {0, __builtin_bit_cast(float, top), 0.f};
+  const bool finite = top < 0x7F800000u, live = finite && end.peak >= kSmallest;
   if (live) {
-    if constexpr (__is_same(Inv, double))
-      inv = (double)kLevels / (double)peak;
+    if constexpr (__is_same(decltype(end.inv), double))
+      end.inv = (double)kLevels / (double)end.peak;
     else  // 1 / a is subnormal, so short of bits, from 2^126 on
-      inv = peak < 0x1p126f ? kLevels * (1.f / peak) : kLevels / peak;
+      end.inv = end.peak < 0x1p126f ? kLevels * (1.f / end.peak) : kLevels / end.peak;
   }
+  if constexpr (MODE == kNorm || MODE == kNormRes)
+    if (live) {
+      if (sq > 0x1.fffffep127f) end.by = 0x1p-96f;
+      if (sq < 0x1p-96f && a.eps < 0x1p-60f) end.by = 0x1p96f;
+    }
   if (threadIdx.x == 0) {
-    float scale = live ? peak / kLevels : 0.f;
-    if constexpr (MODE == kNorm || MODE == kNormRes) scale *= 1.f / __builtin_sqrtf(sq / (float)a.cols + a.eps);
+    float scale = live ? end.peak / kLevels : 0.f;
+    if constexpr (MODE == kNorm || MODE == kNormRes)
+      if (live) scale *= 1.f / __builtin_sqrtf(sq / (float)a.cols + a.eps);
     a.scale[row] = finite ? scale : __builtin_nanf("");
   }
-  return inv;
+  return end;
+}
+
+// The scale of a norm's row whose sum of squares is not one that fp32 holds: infinite, or below 2^-96,
+// where squares that were subnormal count (unless eps outweighs them all). Of s times 2^-96 (2^96) the
+// squares that count are from 2^-106 on and their sum is below 2^125; the rest is done in
+// doubles. It comes after the row's stores, where no registers are held for it, so the sum
+// written there is read again, each thread what it wrote itself.
+template <typename T, int MODE, int WAVES>
+__device__ __forceinline__ void scale_again(const RowEnd<MODE>& end, const RowArgs& a, int64_t row) {
+  constexpr int EPP = 16 / sizeof(T);
+  __shared__ float s_sq[WAVES];
+  const char* const s = MODE == kNormRes ? a.s + row * a.cols * (int64_t)sizeof(T) : a.x + row * a.x_stride;
+  float sq = 0.f;
+#pragma unroll 1
+  for (int64_t i = (int64_t)threadIdx.x * EPP; i < a.cols; i += 64 * WAVES * EPP) {
+    float v[EPP];
+    unpack<T>(load_piece<T>(s, (int)i, a.cols), v);
+#pragma unroll
+    for (int e = 0; e < EPP; ++e) sq = fmaf(v[e] * end.by, v[e] * end.by, sq);
+  }
+  sq = wave_sum(sq);
+  if constexpr (WAVES > 1) {
+    if ((threadIdx.x & 63) == 0) s_sq[threadIdx.x >> 6] = sq;
+    __syncthreads();
+    sq = s_sq[0];
+#pragma unroll
+    for (int i = 1; i < WAVES; ++i) sq += s_sq[i];
+  }
+  if (threadIdx.x == 0) {
+    const double mean = (double)sq / (double)a.cols / ((double)end.by * (double)end.by);
+    a.scale[row] = (float)((double)end.peak / (double)kLevels / __builtin_sqrt(mean + (double)a.eps));
+  }
 }
 
 template <typename T, typename Inv>
@@ -298,9 +342,12 @@ __device__ __forceinline__ void store_s(char* s, int i, int cols, const u32x4& w
 // One workgroup per row, PPT 16-byte pieces a thread, held in registers between the reduction
 // and the write, so that the row is read once. Bound by memory for many rows and by its
 // latency for few: with ALIGNED rows every piece is requested before the first is used, through
-// descriptors that end with the row (a piece past it reads zeros without an access).
+// descriptors that end with the row (a piece past it reads zeros without an access). Two waves a
+// SIMD at least, which the compiler does not keep to by itself (fp16 norms of 2240 x 16384 62 us, so
+// 45); of rows that are not aligned the longest would spill then.
 template <typename T, int MODE, int TPB, int PPT, bool ALIGNED>
-__global__ __launch_bounds__(TPB) void int8_rows_kernel(const RowArgs a) {
+__global__ __launch_bounds__(TPB) __attribute__((amdgpu_waves_per_eu(ALIGNED ? 2 : 1))) void int8_rows_kernel(
+    const RowArgs a) {
   constexpr int EPP = 16 / sizeof(T);
   const int64_t row = blockIdx.x;
   const char* const xr = a.x + row * a.x_stride;
@@ -335,17 +382,19 @@ __global__ __launch_bounds__(TPB) void int8_rows_kernel(const RowArgs a) {
   float sq = 0.f;
 #pragma unroll
   for (int u = 0; u < PPT; ++u) fold<T, MODE>(xw[u], yw[u], ww[u], v[u], top, sq);
-  const auto inv = finish_row<MODE, TPB / 64>(top, sq, a, row);
+  const auto end = finish_row<MODE, TPB / 64>(top, sq, a, row);
   int8_t* const q = a.q + row * a.cols;
   char* const s = a.s + row * a.cols * (int64_t)sizeof(T);
 #pragma unroll
   for (int u = 0; u < PPT; ++u) {
     const int i = (threadIdx.x + TPB * u) * EPP;
     if (i < a.cols) {
-      store_q<T>(q, i, a.cols, v[u], inv);
+      store_q<T>(q, i, a.cols, v[u], end.inv);
       if constexpr (MODE == kNormRes) store_s<T>(s, i, a.cols, xw[u]);
     }
   }
+  if constexpr (MODE == kNorm || MODE == kNormRes)
+    if (end.by != 0.f) scale_again<T, MODE, TPB / 64>(end, a, row);
 }
 
 // Rows longer than the registers hold: the same pieces in two passes over the row, the second
@@ -368,14 +417,16 @@ __global__ __launch_bounds__(256) void int8_rows_long_kernel(const RowArgs a) {
   u32x4 xw;
   float v[EPP];
   for (int64_t i = (int64_t)threadIdx.x * EPP; i < a.cols; i += 256 * EPP) piece((int)i, xw, v, top, sq);
-  const auto inv = finish_row<MODE, 4>(top, sq, a, row);
+  const auto end = finish_row<MODE, 4>(top, sq, a, row);
   int8_t* const q = a.q + row * a.cols;
   char* const s = a.s + row * a.cols * (int64_t)sizeof(T);
   for (int64_t i = (int64_t)threadIdx.x * EPP; i < a.cols; i += 256 * EPP) {
     piece((int)i, xw, v, top, sq);
-    store_q<T>(q, (int)i, a.cols, v, inv);
+    store_q<T>(q, (int)i, a.cols, v, end.inv);
     if constexpr (MODE == kNormRes) store_s<T>(s, (int)i, a.cols, xw);
   }
+  if constexpr (MODE == kNorm || MODE == kNormRes)
+    if (end.by != 0.f) scale_again<T, MODE, 4>(end, a, row);
 }
 
 bool al16(const void* p) { return ((uintptr_t)p & 15u) == 0; }

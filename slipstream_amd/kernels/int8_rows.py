@@ -7,8 +7,8 @@ residual's addition, ``fused_swiglu_int8`` behind SwiGLU; the names and argument
 ops, nothing is rounded to the inputs' type on the way, except the residual sum that is
 returned. The norm's ``q`` is the exact quotient's (of ``s * weight`` in fp32); the others round
 ``1 / max|y|``, its product with 127 and that with ``y`` to fp32. A row of zeros (or of ``y``, for
-the norm ``s * weight``, below 1.5e-36) has scale 0, a row with a NaN or an infinity has zeros
-and scale NaN. Device tensors only.
+the norm ``s * weight``, below 1.5e-36) has scale 0, whatever the norm's eps; a row with a NaN or
+an infinity (for the norm in ``s * weight``) has zeros and scale NaN. Device tensors only.
 """
 
 from __future__ import annotations

@@ -338,3 +338,30 @@ def test_norm_differs_from_elementary_operations_at_halves_only(device, rows, co
     top, p = p.abs().amax(-1)[row], p[row, col].abs()
     assert (torch.remainder(254 * p + top, 2 * top) == 0).all()
     assert (q[row, col] % 2 == 0).all() and (q[row, col].float() - plain[row, col]).abs().eq(1).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("cols", [64, 1003, 4096, 40001])
+@pytest.mark.parametrize("with_residual", [False, True])
+@pytest.mark.parametrize("eps", [0.0, 1e-6])
+def test_norm_of_zeros_and_of_rows_whose_squares_leave_fp32(device, dtype, cols, with_residual, eps):
+    """A row of zeros has scale 0 whatever eps is, and rows whose squares' sum is above or below what
+    fp32 holds have the norm's value as any other: the sum is taken again of the row times a power
+    of two, which rounds as it does elsewhere, and the rest in doubles."""
+    g = torch.Generator(device=device).manual_seed(cols)
+    sizes = torch.tensor([1.0, 0.0, 2.0**60, 2.0**64, 2.0**70, 2.0**122, 2.0**-40, 2.0**-46, 2.0**-60, 2.0**-70, 2.0**-100, 0.0],
+                         dtype=torch.float64, device=device)
+    if dtype == torch.float16:  # from its smallest to its largest
+        sizes = torch.tensor([1.0, 0.0, 2.0**12, 2.0**-10, 2.0**-24, 0.0], dtype=torch.float64, device=device)
+    x = torch.randn(len(sizes), cols, generator=g, device=device).clamp(-7, 7).double()
+    x = (x * sizes[:, None]).to(dtype)
+    w = (1 + 0.1 * _rand(g, (cols,), torch.float32, device)).to(dtype)
+    r = (x * 0.25).flip(-1) if with_residual else None
+    q, scale, s = fused_rmsnorm_int8(x, w, r, eps)
+    y, want = _norm64(x, w, r, eps)
+    assert s is None or torch.equal(s, want)
+    assert torch.isfinite(scale).all()
+    p = want.double() * w.double()
+    if with_residual and dtype == torch.float16:  # the sum of the smallest may be zero everywhere
+        y = torch.where(p.abs().amax(-1, keepdim=True) > 0, y, 0.0)
+    _check(q, scale, y, U if dtype == torch.float32 else 0.0, _norm_scale_err(cols), f"norm {cols} {dtype} {eps}")
