@@ -107,15 +107,15 @@ __device__ __forceinline__ float wave_sum(float x) {
   return add_dpp<0xB1>(x);
 }
 
-// g / (1 + exp(-g)), the quotient rounded to nearest: a reciprocal refined by one Newton step, and
+// g / d for a divisor d = 1 + exp(-g), rounded to nearest: a reciprocal refined by one Newton step, and
 // Markstein's correction of the quotient by its remainder (the range scaling that a general
-// division adds has nothing to do for a divisor from 1 on: 2240 x 14336 38.1 us with it, 34.7 so,
-// 28.0 with the hardware's exp2 and reciprocal alone, whose last bits moved some tens of q by a
-// step). From a divisor of 2^100 on, where the value is below 1e-28, g times the plain reciprocal.
-__device__ __forceinline__ float silu(float g) {
-  const float d = 1.f + expf(-g);
+// division adds has nothing to do for a divisor from 1 to kFarDivisor, up to which the reciprocal is no
+// subnormal: 2240 x 14336 38.1 us with it, 32.6 so, 28.0 with the hardware's exp2 and reciprocal
+// alone, whose last bits moved some tens of q by a step).
+constexpr float kFarDivisor = 0x1p126f;
+__device__ __forceinline__ float silu_quotient(float g, float d) {
   const float r0 = __builtin_amdgcn_rcpf(d), r = fmaf(fmaf(-d, r0, 1.f), r0, r0), q = g * r;
-  return d < 0x1p100f ? fmaf(fmaf(-d, q, g), r, q) : g * r0;
+  return fmaf(fmaf(-d, q, g), r, q);
 }
 
 // The low bytes of four words in a dword.
@@ -220,10 +220,19 @@ __device__ __forceinline__ void fold(u32x4& xw, const u32x4& yw, const u32x4& ww
     }
   }
   if constexpr (MODE == kSwiglu) {
-    float u[EPP];
+    float u[EPP], g[EPP], d[EPP], far = 0.f;
     unpack<T>(yw, u);
 #pragma unroll
-    for (int e = 0; e < EPP; ++e) v[e] = silu(v[e]) * u[e];
+    for (int e = 0; e < EPP; ++e) {
+      g[e] = v[e];
+      d[e] = 1.f + expf(-g[e]);
+      far = fmaxf(far, d[e]);
+      v[e] = silu_quotient(g[e], d[e]) * u[e];
+    }
+    if (far > kFarDivisor) {  // gates below -87.3: the general division, in pieces that hold such a gate
+#pragma unroll
+      for (int e = 0; e < EPP; ++e) v[e] = g[e] / d[e] * u[e];
+    }
   }
 #pragma unroll
   for (int e = 0; e < EPP; ++e) top = umax(top, magnitude(v[e]));

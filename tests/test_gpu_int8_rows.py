@@ -365,3 +365,60 @@ def test_norm_of_zeros_and_of_rows_whose_squares_leave_fp32(device, dtype, cols,
     if with_residual and dtype == torch.float16:  # the sum of the smallest may be zero everywhere
         y = torch.where(p.abs().amax(-1, keepdim=True) > 0, y, 0.0)
     _check(q, scale, y, U if dtype == torch.float32 else 0.0, _norm_scale_err(cols), f"norm {cols} {dtype} {eps}")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("cols", [16, 1001, 40001])
+def test_swiglu_of_far_negative_gates(device, dtype, cols):
+    """Gates whose divisor 1 + exp(-g) is next to fp32's largest number (its reciprocal a subnormal
+    one), beside an ``up`` that makes the product a normal one: values as near as anywhere, and
+    from where exp(-g) is infinite zeros, as elementary operations have them."""
+    at = torch.tensor([-60.0, -69.0, -70.0, -80.0, -87.0, -87.3, -87.5, -88.0, -88.5, -88.7], device=device).to(dtype)
+    gate = at[:, None].expand(-1, cols).contiguous()
+    up = torch.linspace(-1, 1, cols, device=device).mul(3e4 if dtype == torch.float16 else 1e30).to(dtype).expand(len(at), -1)
+    q, scale = fused_swiglu_int8(gate, up)
+    g64 = gate.double()
+    y = g64 / (1 + torch.exp(-g64)) * up.double()
+    assert (y.abs().amax(-1) >= SMALLEST).all()
+    _check(q, scale, y, 7 * U, 9 * U, f"far {dtype}")
+    gone = torch.full_like(gate[:1], -89.0)
+    q, scale = fused_swiglu_int8(gone, up[:1])
+    assert not q.any() and not scale.any()
+    gone[0, cols // 2] = float("-inf")  # -inf / inf
+    q, scale = fused_swiglu_int8(gone, up[:1])
+    assert torch.isnan(scale).all() and not q.any()
+
+
+def _elementary_swiglu(gate, up):
+    g = gate.float()
+    return (g / (1 + torch.exp(-g)) * up.float()).contiguous()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,cols", [(333, 2051), (65, 14336), (3, 40001)])
+def test_swiglu_is_what_elementary_operations_give(device, dtype, rows, cols):
+    """Bit for bit, on rows as a projection leaves them: q and scale of ``g / (1 + exp(-g)) * u``, every
+    operation rounded to fp32, through ``quantize_int8``; some gates far below zero."""
+    g = torch.Generator(device=device).manual_seed(cols)
+    gate, up = 3 * _rand(g, (rows, cols), dtype, device), _rand(g, (rows, cols), dtype, device)
+    gate[:, ::97] = (torch.rand(gate[:, ::97].shape, generator=g, device=device) * -90).to(dtype)
+    for a, b in zip(fused_swiglu_int8(gate, up), quantize_int8(_elementary_swiglu(gate, up))):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("up", [1.0, 3.0, -1e4, 1e30])
+def test_every_gate_is_what_elementary_operations_give(device, dtype, up):
+    """Rows of one value, so that the scale is the value's magnitude over 127 and shows its last bits:
+    every 16-bit gate, and fp32 gates all over the range."""
+    if dtype == torch.float32:
+        gen = torch.Generator(device=device).manual_seed(1)
+        spans = [(-105, -86), (-90, -60), (-60, 0), (-1, 1), (0, 90)]
+        gate = torch.cat([lo + (hi - lo) * torch.rand(1 << 20, generator=gen, device=device) for lo, hi in spans])
+    else:
+        gate = torch.arange(1 << 16, dtype=torch.int32, device=device).to(torch.int16).view(dtype)
+    gate = gate[:, None].contiguous()
+    up = torch.full_like(gate, min(up, 6e4) if dtype == torch.float16 else up)
+    for a, b in zip(fused_swiglu_int8(gate, up), quantize_int8(_elementary_swiglu(gate, up))):
+        assert torch.equal(torch.nan_to_num(a, nan=-1.0), torch.nan_to_num(b, nan=-1.0))
+        assert torch.equal(torch.isnan(a), torch.isnan(b))
