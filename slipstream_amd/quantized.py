@@ -244,9 +244,11 @@ class W4A16MLP(nn.Module):
 
 def quantize_weight_int8(weight: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """Per output channel (row) of ``weight [N, K]``: ``scale = max|w| / 127``,
-    ``q = round(w * 127 / max|w|)`` (half to even), the rule of ``quantize_int8``. Returns
-    ``(qweight int8 [N, K], scales fp32 [N])``; a channel of zeros (or below 1.5e-36) has
-    scale 0. Torch ops on the weight's device, once at load."""
+    ``q = round(w * 127 / max|w|)`` (half to even), with ``127 / max|w|`` and its product with ``w``
+    rounded to fp32 (``quantize_int8`` rounds ``1 / max|w|`` and its product with 127: of a 16-bit
+    weight's values about one in 8000 differs by a step). Returns ``(qweight int8 [N, K], scales fp32
+    [N])``, the same on every device; a channel of zeros (or below 1.5e-36) has scale 0. Torch ops
+    on the weight's device, once at load."""
     if weight.ndim != 2:
         raise ValueError(f"weight must be 2-D [out, in], got {tuple(weight.shape)}")
     w = weight.float()

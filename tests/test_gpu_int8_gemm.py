@@ -14,7 +14,7 @@ import torch.nn.functional as F
 
 from slipstream_amd import _ffi
 from slipstream_amd.kernels import fused_rmsnorm_int8, fused_swiglu_int8, quantize_int8, w8a8_gemm
-from slipstream_amd.quantized import W8A8Linear, W8A8MLP
+from slipstream_amd.quantized import W8A8Linear, W8A8MLP, quantize_weight_int8
 
 pytestmark = pytest.mark.gpu
 
@@ -380,3 +380,10 @@ def test_two_streams_at_once(device):
     torch.cuda.synchronize()
     for i in range(2):
         assert all(torch.equal(y, want[i]) for y in got[i])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_weights_are_quantized_alike_on_every_device(device, dtype):
+    w = torch.randn(513, 1000, generator=torch.Generator().manual_seed(3)).to(dtype)
+    for on_gpu, on_cpu in zip(quantize_weight_int8(w.to(device)), quantize_weight_int8(w)):
+        assert torch.equal(on_gpu.cpu(), on_cpu)

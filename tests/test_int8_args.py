@@ -159,6 +159,19 @@ def test_weight_quantizer(dtype):
     assert torch.equal(q[live].abs().amax(1), torch.full((36,), 127, dtype=torch.int8))
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_weight_quantizer_rounds_twice(dtype):
+    """Bit for bit ``127 / max`` rounded to fp32, its product with the weight rounded to fp32, and that to
+    an integer: both roundings here by doubles, which hold a product of two fp32 values and round
+    a quotient of two so that rounding it again to fp32 is the quotient's nearest."""
+    w = torch.randn(67, 1021, generator=torch.Generator().manual_seed(2)).to(dtype)
+    q, scale = quantize_weight_int8(w)
+    top = w.double().abs().amax(1, keepdim=True)
+    steps = (w.double() * (127 / top).float().double()).float()
+    assert torch.equal(q, torch.round(steps).to(torch.int8))
+    assert torch.equal(scale, (top / 127).float()[:, 0])
+
+
 def test_weight_quantizer_and_modules_refuse():
     with pytest.raises(ValueError, match="2-D"):
         quantize_weight_int8(torch.zeros(4))
