@@ -43,6 +43,16 @@ int launch_w8a8_stream(const W8Params& p, const StreamPlan& pl, int out_dtype, h
 double plan_w8a8_tile(TilePlan& pl, int64_t m, int64_t n, int64_t k, bool may_split);  // estimated us
 int launch_w8a8_tile(const W8Params& p, const TilePlan& pl, int out_dtype, int* part, hipStream_t stream);
 
+// Weights that one token block reads pass the caches by beyond this many bytes. Out of the memory that
+// is 2 to 16 % faster at any size (24 x 28672 x 4096 25.1 -> 23.2 us, 24 x 4096 x 14336 18.0 ->
+// 17.3, 64 x 28672 x 4096 30.8 -> 25.9, 64 x 14336 x 4096 20.5 -> 19.7), but up to 46 % slower for
+// weights that the 256 MB cache still has from the call before (24 x 4096 x 14336 11.5 -> 14.5, 64 x
+// 14336 x 4096 13.2 -> 19.3). A call does not know which it is. Three such weights in turn are
+// kept at 59 MB and not at 117 (28672 x 4096 takes the same time either way: 25.0 and 25.1), so the
+// size of one weight decides: a model whose weights are all below it and more than the cache
+// altogether loses 2 to 8 %.
+constexpr int64_t kKeptWeights = 64 << 20;
+
 // Lets `kern` have `lds` bytes of dynamic LDS on the current device; `done` holds a bit for each
 // device where it has them already (the attribute belongs to the function on a device).
 inline int reserve_lds(const void* kern, int lds, std::atomic<uint64_t>& done) {

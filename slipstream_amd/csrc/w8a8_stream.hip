@@ -36,11 +36,9 @@ constexpr int stream_lds_bytes(int mt, int nt, int waves) {
 
 // Whether the weights pass the caches by, as what is read once does: where no second token block
 // reads them, for 16 tokens at any size (4096 x 14336 from memory 12.7 -> 11.4 us, out of the
-// 256 MB cache 10.2 and 10.0), beyond that for weights that such a cache does not keep for the
-// next call (28672 x 4096 at m = 24 28.2 -> 25.3 us; 4096 x 14336 from memory 17.0 -> 16.0, but
-// out of the cache 11.5 -> 14.3).
+// 256 MB cache 10.2 and 10.0), beyond that above kKeptWeights.
 inline bool read_once(int mt, int64_t m_blocks, int64_t n, int64_t k) {
-  return m_blocks == 1 && (mt == 1 || n * k > (64 << 20));
+  return m_blocks == 1 && (mt == 1 || n * k > kKeptWeights);
 }
 
 // XI: groups of eight tokens that are read (2 MT, or 1 of MT = 1); the rows of the others hold

@@ -70,10 +70,10 @@ constexpr int token_stages(int bm, int bn) {
 }
 constexpr int ring_bytes(int bm, int bn) { return (token_stages(bm, bn) * bm + channel_stages(bm, bn) * bn) * 128; }
 
-// TO int: a K range's sums, for the reduce kernel. ONCE: the only token block, and more weights
-// than a 256 MB cache keeps for the next call: they pass the caches by, and the channel tiles
-// begin at different stages, so that those that run at once on an XCD do not all ask for the same
-// lines of the tokens (64 x 28672 x 4096 32.2 -> 26.6 us, 256 x 28672 x 4096 44.8 -> 43.2; with
+// TO int: a K range's sums, for the reduce kernel. ONCE: the only token block, and more than
+// kKeptWeights: the weights pass the caches by, and the channel tiles begin at different
+// stages, so that those that run at once on an XCD do not all ask for the same lines of the
+// tokens (64 x 28672 x 4096 30.8 -> 25.9 us, 256 x 28672 x 4096 44.6 -> 41.6; with
 // several token blocks, which share the weights' lines, either is slower: 512 x 4096 x 4096 14.9 us,
 // past the caches 18.0, begun apart 16.0).
 template <typename TO, int MT, int NT, int WM, int G, bool ONCE>
@@ -423,7 +423,7 @@ int launch_tile(const W8Params& p, const TilePlan& pl, hipStream_t stream) {
   X(96, 128, 3, 1, 1) X(64, 128, 2, 1, 1)
 
 inline bool read_once(int64_t m_blocks, int64_t ks, int64_t n, int64_t k) {
-  return m_blocks == 1 && ks == 1 && n * k > (64 << 20);
+  return m_blocks == 1 && ks == 1 && n * k > kKeptWeights;
 }
 
 template <typename TO>
