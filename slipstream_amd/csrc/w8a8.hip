@@ -162,10 +162,12 @@ bool whole_rows(const void* base, int64_t rows, int64_t stride, int64_t k) {
 }
 int64_t round16(int64_t n) { return (n + 15) / 16 * 16; }
 
-// Which kernel a call takes: up to 32 tokens the stream kernel (28672 x 4096 at m = 32 28.0 us,
-// in tiles 29.0; 4096 x 14336 11.6 and 14.9), beyond that by the kernels' own estimates, fitted to
-// measurements (at m = 64 4096 x 4096 6.5 us streamed and 10.8 in tiles, 28672 x 4096 35.4 and
-// 30.7). Kept for the last shapes of the thread, as a plan is a few hundred estimates.
+// Which kernel a call takes: up to 32 tokens the stream kernel, which is the faster one there (at m =
+// 32 28672 x 4096 22.9 us, in tiles 24.1; 4096 x 14336 12.1 and 14.9; 57344 x 8192 86 and 91),
+// beyond that by the kernels' own estimates, fitted to measurements (at m = 64 4096 x 4096 6.3 us
+// streamed and 10.8 in tiles, 28672 x 4096 31.2 and 25.0, 4096 x 14336 14.1 and 16.0; wrong where
+// they are close: m = 48 4096 x 14336 goes in tiles, 15.9 us, streamed 13.4). Kept for the last
+// shapes of the thread, as a plan is a few hundred estimates.
 struct Plan {
   int64_t m = -1, n = 0, k = 0;
   bool may_split = false, stream = false;

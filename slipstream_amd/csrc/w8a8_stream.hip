@@ -194,7 +194,9 @@ int launch_stream_typed(const W8Params& p, const StreamPlan& pl, hipStream_t str
 }  // namespace
 
 // The tile and waves of least estimated time (us), fitted to the times of 3500 calls (every tile
-// and number of waves at 240 shapes of up to 512 tokens; 8 % off on average): a round's
+// and number of waves at 240 shapes of up to 512 tokens); 8 % off on average over 3177 calls of the
+// kernel as it is, too low for weights of hundreds of MB (8192 x 28672 at m = 32 36 us, takes 44;
+// 57344 x 8192 73, takes 86 with the two waves so chosen and 76 with four): a round's
 // start, a wave's blocks one after another, the adding of the sums and the results, the
 // operands' way through a CU and out of the L2, and the weights' out of the memory.
 double plan_w8a8_stream(StreamPlan& pl, int64_t m, int64_t n, int64_t k) {

@@ -454,7 +454,10 @@ int launch_reduce(const W8Params& p, const int* part, int ks, hipStream_t stream
 }  // namespace
 
 // The tile and K split of least estimated time (us), fitted to the times of 4200 calls (tiles and
-// splits of 290 shapes, 1 to 2240 tokens, 0.3 to 120 million weights; 8 % off on average): what a
+// splits of 290 shapes, 1 to 2240 tokens, 0.3 to 120 million weights); 7 % off on average over 5025
+// calls of the kernel as it is, but 30 % too low for one token block of more than kKeptWeights,
+// whose term was put in by hand (64 x 28672 x 4096 17 us, takes 25; among those the choice is
+// mostly right, at worst 96 x 57344 x 8192 108 us in tiles of 96 x 128, 80 in 128 x 256): what a
 // stage takes of a round of workgroups, the results of each round, the operands' way into the
 // LDS, the memory's share, and for a split the sums' way out and back and the launch that adds
 // them. (2240 x 4096 x 14336: 224 tiles of 160 x 256 117 us, 144 of 256 x 256 140; 197 x 4096 x
