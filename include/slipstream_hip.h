@@ -271,6 +271,14 @@ int ss_w4a16_gemm(const void* x, void* out, const int32_t* qweight, const void* 
  */
 int ss_w8a8_workspace_size(int64_t m, int64_t n, int64_t k, int x_whole, int w_whole, int64_t* bytes);
 
+/*
+ * What ss_w8a8_gemm with its whole workspace runs on the current device, as five numbers: the
+ * kernel (0 general, 1 stream, 2 tile; each after a copy of operands that are not whole), the
+ * tokens and channels of a workgroup, its waves (stream) or the ranges that k is split into (tile),
+ * and whether the weights pass the caches by. Launches nothing.
+ */
+int ss_w8a8_plan(int64_t m, int64_t n, int64_t k, int32_t* plan);
+
 int ss_w8a8_gemm(const int8_t* x, const float* x_scale, const int8_t* w, const float* w_scale,
                  const void* bias, void* out, int64_t m, int64_t n, int64_t k, int64_t x_stride,
                  int64_t w_stride, int64_t o_stride, int out_dtype, int bias_dtype, void* workspace,

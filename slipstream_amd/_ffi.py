@@ -80,6 +80,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i32, _i64, _i64, _i32, _i32, _vp, _i64, _vp],
     ),
     "ss_w8a8_workspace_size": (_i32, [_i64, _i64, _i64, _i32, _i32, _c_i64p]),
+    "ss_w8a8_plan": (_i32, [_i64, _i64, _i64, ctypes.POINTER(_i32)]),
     "ss_w8a8_gemm": (
         _i32,
         [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i32, _i32, _vp, _i64, _vp],

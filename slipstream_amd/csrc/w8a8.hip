@@ -226,6 +226,26 @@ extern "C" int ss_w8a8_workspace_size(int64_t m, int64_t n, int64_t k, int x_who
   return st;
 }
 
+extern "C" int ss_w8a8_plan(int64_t m, int64_t n, int64_t k, int32_t* plan) {
+  if (!plan) {
+    ss_host::set_error("w8a8 plan: null pointer");
+    return SS_ERR_INVALID;
+  }
+  for (int i = 0; i < 5; ++i) plan[i] = 0;
+  const int st = ss::check_extents(m, n, k, SS_DTYPE_BF16);
+  if (st != SS_OK || m == 0 || n == 0) return st;
+  if (k == 0 || m > INT32_MAX || n > INT32_MAX) return SS_OK;
+  const ss::Plan& p = ss::plan_for(m, n, ss::round16(k), true);
+  if (p.stream) {
+    const int32_t is[5] = {1, 16 * p.sp.mt, 16 * p.sp.nt, p.sp.waves, p.sp.once};
+    for (int i = 0; i < 5; ++i) plan[i] = is[i];
+  } else if (p.tp.ks > 0) {
+    const int32_t is[5] = {2, p.tp.bm, p.tp.bn, p.tp.ks, p.tp.once};
+    for (int i = 0; i < 5; ++i) plan[i] = is[i];
+  }
+  return SS_OK;
+}
+
 extern "C" int ss_w8a8_gemm(const int8_t* x, const float* x_scale, const int8_t* w, const float* w_scale,
                             const void* bias, void* out, int64_t m, int64_t n, int64_t k, int64_t x_stride,
                             int64_t w_stride, int64_t o_stride, int out_dtype, int bias_dtype, void* workspace,

@@ -28,6 +28,7 @@ struct TilePlan {
   int bm, bn;
   int ks, per;  // K ranges and 128-key stages per range
   int n_tiles, m_blocks;
+  bool once;    // the weights pass the caches by
 };
 constexpr int64_t kMostGroups = 1 << 22;  // workgroups of a launch (of at most 512 threads: below 2^32)
 
@@ -36,6 +37,7 @@ constexpr int64_t kMostGroups = 1 << 22;  // workgroups of a launch (of at most 
 struct StreamPlan {
   int mt, nt, waves;
   int n_tiles, m_blocks;
+  bool once;    // the weights pass the caches by
 };
 double plan_w8a8_stream(StreamPlan& pl, int64_t m, int64_t n, int64_t k);  // estimated us
 int launch_w8a8_stream(const W8Params& p, const StreamPlan& pl, int out_dtype, hipStream_t stream);

@@ -171,7 +171,7 @@ int launch_stream(const W8Params& p, const StreamPlan& pl, hipStream_t stream) {
   if (const int st = reserve_lds((const void*)kern, most, done); st != SS_OK) return st;
   const int64_t grid = ((int64_t)pl.n_tiles * pl.m_blocks + 7) / 8 * 8;
   hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(64 * pl.waves), lds, stream, p, pl.n_tiles, pl.m_blocks,
-                     read_once(pl.mt, pl.m_blocks, p.n, p.k));
+                     pl.once);
   return ss_host::launch_status("w8a8 gemm (stream)");
 }
 
@@ -212,6 +212,7 @@ double plan_w8a8_stream(StreamPlan& pl, int64_t m, int64_t n, int64_t k) {
     const int64_t n_tiles = (n + 16 * nt - 1) / (16 * nt), m_blocks = (m + 16 * mt - 1) / (16 * mt);
     if (n_tiles * m_blocks > kMostGroups) continue;
     const int64_t groups = n_tiles * m_blocks, a_cu = (groups + cus - 1) / cus;
+    const bool once = read_once(mt, m_blocks, n, k);
     const double bytes = (16.0 * nt + (m < 16 * mt ? m : 16 * mt)) * blocks * 128;
     // two waves only beyond 16 tokens (28672 x 4096 at m = 1 26.2 us with two, 22.3 with four)
     for (int waves = m > 16 ? 2 : 4; waves <= 8; waves *= 2) {
@@ -222,10 +223,10 @@ double plan_w8a8_stream(StreamPlan& pl, int64_t m, int64_t n, int64_t k) {
       const double rounds = (double)((groups + cus * fit - 1) / (cus * fit)), each = (double)((blocks + waves - 1) / waves);
       const double us = 0.94 + rounds * (1.15 + each * (0.0141 * (mt + nt) + 0.0051 * mt * nt) +
                                          mt * nt * (0.103 + 0.416 / waves)) +
-                        a_cu * (bytes * 5.32e-6 + 0.0005 * waves) + groups * bytes * 8.4e-9 + n * k * (read_once(mt, m_blocks, n, k) ? 7.4e-8 : 8.43e-8);
+                        a_cu * (bytes * 5.32e-6 + 0.0005 * waves) + groups * bytes * 8.4e-9 + n * k * (once ? 7.4e-8 : 8.43e-8);
       if (us < best) {
         best = us;
-        pl = {mt, nt, waves, (int)n_tiles, (int)m_blocks};
+        pl = {mt, nt, waves, (int)n_tiles, (int)m_blocks, once};
       }
     }
   }

@@ -431,7 +431,7 @@ int launch_tile_typed(const W8Params& p, const TilePlan& pl, hipStream_t stream)
 #define W8A8_LAUNCH(BM, BN, MT, NT, WM) \
   if (pl.bm == BM && pl.bn == BN) {                                                             \
     if constexpr (!__is_same(TO, int))                                                         \
-      if (read_once(pl.m_blocks, pl.ks, p.n, p.k)) return launch_tile<TO, MT, NT, WM, true>(p, pl, stream); \
+      if (pl.once) return launch_tile<TO, MT, NT, WM, true>(p, pl, stream); \
     return launch_tile<TO, MT, NT, WM, false>(p, pl, stream);                                  \
   }
   W8A8_TILES(W8A8_LAUNCH)
@@ -481,11 +481,12 @@ double plan_w8a8_tile(TilePlan& pl, int64_t m, int64_t n, int64_t k, bool may_sp
       const double turns = (double)((groups + fit * cus - 1) / (fit * cus));
       double us = 3.13 + turns * per * 0.0844 + rounds * (per * (0.662 * area + 0.128 * edge / 512) + 0.21 + 6.33 * area) +
                   groups * per * edge * 128 * 1.79e-8 + n * k * 4.2e-8 + m * n * 2.96e-7;
-      if (read_once(m_blocks, ks, n, k)) us -= n * k * 2e-8;
+      const bool once = read_once(m_blocks, ks, n, k);
+      if (once) us -= n * k * 2e-8;
       if (ks > 1) us += 2.03 + ks * m * n * 4 * 2.79e-7;
       if (us < best) {
         best = us;
-        pl = {t[0], t[1], (int)ks, (int)per, (int)n_tiles, (int)m_blocks};
+        pl = {t[0], t[1], (int)ks, (int)per, (int)n_tiles, (int)m_blocks, once};
       }
     }
   }

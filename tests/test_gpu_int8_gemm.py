@@ -387,3 +387,21 @@ def test_weights_are_quantized_alike_on_every_device(device, dtype):
     w = torch.randn(513, 1000, generator=torch.Generator().manual_seed(3)).to(dtype)
     for on_gpu, on_cpu in zip(quantize_weight_int8(w.to(device)), quantize_weight_int8(w)):
         assert torch.equal(on_gpu.cpu(), on_cpu)
+
+
+# the stream kernel with one block of more than 16 tokens and weights that pass the caches by
+ONCE_STREAMS = [
+    ("stream 2 1 2", [(20, 18016, 3744), (23, 41409, 1664)]), ("stream 2 1 4", [(19, 12024, 5616), (18, 11835, 5856)]),
+    ("stream 2 1 8", [(20, 1984, 33872), (19, 2169, 30960)]),
+    ("stream 2 2 2", [(24, 28672, 4096), (29, 38581, 1744)]), ("stream 2 2 4", [(23, 15632, 4352), (29, 10633, 6464)]),
+    ("stream 2 2 8", [(20, 4336, 15712), (29, 5609, 12112)]),
+    ("stream 4 2 4", [(46, 7776, 9216), (39, 8015, 8416)]), ("stream 4 4 4", [(42, 12664, 5312), (44, 11135, 6064)]),
+]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("what,shapes", ONCE_STREAMS, ids=[v[0] for v in ONCE_STREAMS])
+def test_streams_past_the_caches(device, what, shapes, dtype):
+    for i, (m, n, k) in enumerate(shapes):
+        args = _case(device, m, n, k, bias=torch.bfloat16 if i else None)
+        _check(w8a8_gemm(*args, out_dtype=dtype), *args, f"{what}: {m} x {n} x {k}")

@@ -91,6 +91,49 @@ def test_rows_refuse_shapes_and_dtypes():
             quantize_int8(torch.zeros(2, 32, dtype=bad))
 
 
+def _plan(m, n, k):
+    plan = (ctypes.c_int32 * 5)()
+    assert _ffi.lib().ss_w8a8_plan(m, n, k, plan) == _ffi.SS_OK
+    return list(plan)
+
+
+def test_gpu_tests_reach_the_kernels_they_name():
+    """The shapes of the product's GPU tests lie where the fitted estimates choose the kernel, tile, waves
+    and split that their names say."""
+    from tests.test_gpu_int8_gemm import ONCE_STREAMS, VARIANTS
+
+    seen = set()
+    for once_only, variants in ((False, VARIANTS), (True, ONCE_STREAMS)):
+        for what, shapes in variants:
+            name, *numbers = what.split()
+            numbers = [int(v) for v in numbers]
+            for shape in shapes:
+                kernel, tokens, channels, parts, once = _plan(*shape)
+                if name == "stream":
+                    mt, nt, waves = numbers
+                    assert [kernel, tokens, channels, parts] == [1, 16 * mt, 16 * nt, waves], (what, shape)
+                    assert once or not once_only, (what, shape)
+                else:
+                    assert [kernel, tokens, channels] == [2, *numbers], (what, shape)
+                    assert (parts > 1, once) == (name == "split", name == "once"), (what, shape)
+            seen.add((name, *numbers))
+    tiles = {(256, 256), (224, 256), (192, 256), (160, 256), (128, 256), (256, 128), (192, 128), (128, 128), (96, 128),
+             (64, 128)}
+    for name in ("tile", "split", "once"):
+        assert {v[1:] for v in seen if v[0] == name} == tiles
+
+
+def test_plan_of_calls_without_one():
+    assert _plan(0, 8, 32) == _plan(4, 0, 32) == _plan(4, 8, 0) == [0] * 5
+    assert _plan(1, 28672, 4095) == _plan(1, 28672, 4096)  # a copy of whole rows first
+    lib, plan = _ffi.lib(), (ctypes.c_int32 * 5)()
+    assert lib.ss_w8a8_plan(4, 8, 32, None) == _ffi.SS_ERR_INVALID
+    assert lib.ss_w8a8_plan(-1, 8, 32, plan) == _ffi.SS_ERR_INVALID
+    assert lib.ss_w8a8_plan(4, 8, 1 << 17, plan) == _ffi.SS_ERR_UNSUPPORTED
+    # more results than the tile kernel's launches hold: the general kernel's refusal, or its work
+    assert _plan((1 << 31) - 1, (1 << 31) - 1, 16)[0] == 0
+
+
 def test_c_abi_refusals_need_no_device():
     lib = _ffi.lib()
     bf16 = _ffi.SS_DTYPE_BF16
