@@ -23,7 +23,6 @@
 
 namespace {
 
-using ss::u32x2;
 using ss::u32x4;
 
 enum Mode { kRows, kNorm, kNormRes, kSwiglu };

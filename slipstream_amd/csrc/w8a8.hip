@@ -95,7 +95,6 @@ int align_rows(Rows x, Rows w, int k, hipStream_t stream) {
 constexpr int kGenTile = 64;
 constexpr int kGenRow = 80;
 
-
 template <typename TO>
 __global__ __launch_bounds__(256) void w8a8_general_kernel(const W8Params p, int n_tiles) {
   __shared__ __attribute__((aligned(16))) int8_t s_x[kGenTile * kGenRow];

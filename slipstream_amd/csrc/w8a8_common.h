@@ -84,9 +84,6 @@ __device__ __forceinline__ float load_as_f32(const void* p, int64_t i, int dtype
   return ((const float*)p)[i];
 }
 
-// c += a b over 32 keys: lane l's sixteen bytes of a are keys 16 (l / 32) .. + 15 of channel l % 32
-// (of b: of token l % 32); its results are channels 8 (r / 4) + 4 (l / 32) + r % 4 of token
-// l % 32.
 typedef int i32x16 __attribute__((ext_vector_type(16)));
 
 // Position of 16-byte chunk c of row r within the row's 128 LDS bytes: c ^ tile_swizzle(r).
@@ -96,7 +93,8 @@ typedef int i32x16 __attribute__((ext_vector_type(16)));
 __device__ __forceinline__ int tile_swizzle(int r) { return (r >> 1) & 7; }
 
 // The result of one output from its exact integer sum, before it is rounded to the output's
-// type: three roundings in fp32 (four with a bias).
+// type: three roundings in fp32, the sum's, the product's and that of the second product with the
+// bias.
 __device__ __forceinline__ float scaled(int sum, float xs, float ws, float bias) {
   return fmaf((float)sum * xs, ws, bias);
 }

@@ -34,7 +34,9 @@ __device__ __forceinline__ void static_for(F&& f) {
   static_for_impl(f, std::make_integer_sequence<int, N>{});
 }
 
-// acc += a b on the matrix core over 32 keys, the accumulator in AGPRs. Written as asm because the
+// acc += a b on the matrix core over 32 keys, the accumulator in AGPRs: lane l's sixteen bytes of a are
+// keys 16 (l / 32) .. + 15 of channel l % 32 (of b: of token l % 32); its result r is channel
+// 8 (r / 4) + 4 (l / 32) + r % 4 of token l % 32. Written as asm because the
 // compiler moves accumulators between the register files in every stage. What it therefore
 // does not look after: the operands come from LDS reads, which it does wait for; an
 // accumulator is touched once in MT NT products; and between the last product and what
