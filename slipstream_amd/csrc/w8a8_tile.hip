@@ -13,8 +13,8 @@
 //                           (wait, barrier) and its first half's fragments are read
 // One wave per SIMD has nothing to hide behind, so the order is written out: every product is
 // followed by at most a fragment read or two and a DMA, and the scheduler is held to that
-// order. At 2240 x 28672 x 4096 (231 to 239 us) the products are under way in 60 % of the cycles
-// and the card's power holds the clock at 1.86 GHz; the products alone, with nothing read, take
+// order. At 2240 x 28672 x 4096 (231 to 239 us) the products are under way in 61 % of the cycles
+// and the card's power holds the clock at 1.85 GHz; the products alone, with nothing read, take
 // 187 us. Small tiles are bound by their LDS reads: a 64 x 128 tile's 72 KB a stage take the 570
 // cycles that a stage does.
 #include <type_traits>
