@@ -5,8 +5,7 @@ Tolerances, in units of u = 2^-24 (a fp32 rounding, relative):
   q: the value in steps is y * 127 / a; 1 / a, its product with 127 and the product with y are
      rounded once each, the norm's s * w once in y and once in a (exact for 16-bit types), so
      |q - steps| <= 1/2 + 127 * 5 u. SwiGLU: exp is within 2 u, 1 + exp and the quotient round
-     once each, or the reciprocal is within 2 u and its product rounds once (1 + exp from 2^100
-     on), then * u: 7 u in y and the same in a.
+     once each, then * u: within 7 u in y and the same in a.
   scale: a / 127 once (a as above); the norm's sum of squares adds each of a thread's
      cols / 256 values and 16 partial sums with a rounding each, halved by the root, and the
      mean, eps, root, reciprocal and two products round once each.
