@@ -421,3 +421,24 @@ def test_every_gate_is_what_elementary_operations_give(device, dtype, up):
     for a, b in zip(fused_swiglu_int8(gate, up), quantize_int8(_elementary_swiglu(gate, up))):
         assert torch.equal(torch.nan_to_num(a, nan=-1.0), torch.nan_to_num(b, nan=-1.0))
         assert torch.equal(torch.isnan(a), torch.isnan(b))
+
+
+@pytest.mark.parametrize("cols", [64, 1003, 16384, 40001])
+@pytest.mark.parametrize("into", ["residual", "x"])
+def test_sum_in_place_of_rows_whose_squares_leave_fp32(device, cols, into):
+    """The sum over one of its addends, in rows whose squares are summed again after it is written."""
+    from slipstream_amd import _ffi
+
+    g = torch.Generator(device=device).manual_seed(cols)
+    sizes = torch.tensor([1.0, 2.0**70, 0.0, 2.0**-70, 2.0**100], device=device)[:, None]
+    x, r = ((torch.randn(5, cols, generator=g, device=device) * sizes).to(torch.bfloat16) for _ in range(2))
+    w = torch.ones(cols, device=device, dtype=torch.bfloat16)
+    want = fused_rmsnorm_int8(x, w, r, 0.0)
+    _check(*want[:2], _norm64(x, w, r, 0.0)[0], 0.0, _norm_scale_err(cols), f"far {cols}")
+    q = torch.empty((5, cols), dtype=torch.int8, device=device)
+    scale = torch.empty(5, device=device)
+    s = r if into == "residual" else x
+    _ffi.check(_ffi.lib().ss_rmsnorm_int8(x.data_ptr(), r.data_ptr(), w.data_ptr(), q.data_ptr(), scale.data_ptr(),
+                                          s.data_ptr(), 5, cols, cols, cols, 0.0, _ffi.dtype_code(x.dtype),
+                                          _ffi.stream_ptr(device)), "norm")
+    assert torch.equal(q, want[0]) and torch.equal(scale, want[1]) and torch.equal(s, want[2])
