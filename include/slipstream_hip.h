@@ -312,6 +312,39 @@ int ss_swiglu_int8(const void* gate, const void* up, int8_t* q, float* scale, in
                    int64_t g_stride, int64_t u_stride, int dtype, void* stream);
 
 /*
+ * Rows quantized to 8-bit floating point (e4m3) with an fp32 scale for every 128 columns, the inputs of
+ * ss_fp8_gemm: for a block x of a row (the last one may be shorter) a = max |x|, scale = a / 448,
+ * q = e4m3(x * 448 / a): the exact quotient (of fp32 x up to its own 2^-24) rounded to the nearest,
+ * half to even. A block with a < 448 * 2^-126 is zeros with scale 0, one that holds a NaN or an
+ * infinity zeros with scale NaN. x [rows, cols], row stride x_stride (elements, unit column stride, any
+ * alignment of its elements), dtype SS_DTYPE_BF16/F16/F32; q [rows, cols] contiguous; scale (row, block)
+ * at block * scale_stride + row, scale_stride >= rows. No counterpart in the reference.
+ */
+int ss_quantize_fp8(const void* x, uint8_t* q, float* scale, int64_t rows, int64_t cols, int64_t x_stride,
+                    int64_t scale_stride, int dtype, void* stream);
+
+/*
+ * Linear layer in 8-bit floating point: out[m, n] = sum_b x_scale(m, b) w_scale(n / 128, b)
+ * (sum_{k in block b} x[m, k] w[n, k]) (+ bias[n]), blocks of 128 k. No counterpart in the reference,
+ * whose quantized linear is W4A16 (slipstream/kernels/quant_gemm.py:23-42).
+ *   x [m, k], w [n, k] e4m3, row strides x_stride, w_stride (unit column stride); x_scale (row, block) at
+ *   row * xs_strides[0] + block * xs_strides[1]; w_scale (block of 128 n, block of 128 k) at
+ *   ws_strides[0], ws_strides[1] likewise; bias [n] of bias_dtype, or NULL; out [m, n], row stride
+ *   o_stride, of out_dtype (SS_DTYPE_BF16/F16/F32). k below 2^30.
+ * A block's sum is in fp32, is multiplied with fl(x_scale w_scale) and added in one fp32 rounding; the
+ * result is rounded once to out_dtype.
+ * workspace: ss_fp8_workspace_size() bytes, 16-byte aligned, any contents (x_whole, w_whole as in
+ * ss_w8a8_workspace_size). With less (or NULL, 0) the call succeeds without it, more slowly. Calls that
+ * share a workspace must be ordered on one stream.
+ */
+int ss_fp8_workspace_size(int64_t m, int64_t n, int64_t k, int x_whole, int w_whole, int64_t* bytes);
+
+int ss_fp8_gemm(const uint8_t* x, const float* x_scale, const uint8_t* w, const float* w_scale,
+                const void* bias, void* out, int64_t m, int64_t n, int64_t k, int64_t x_stride,
+                int64_t w_stride, int64_t o_stride, const int64_t xs_strides[2], const int64_t ws_strides[2],
+                int out_dtype, int bias_dtype, void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
  * KV page copies: for each pair i, page pairs[2i + 1] of dst <- page pairs[2i] of
  * src, in every plane p in [0, planes) (a plane is one (layer, K/V) of
  * kv_cache[L, 2, NB, ...], so planes = 2L for a contiguous cache). Page b of plane
@@ -404,6 +437,68 @@ int ss_rmsnorm(const void* x, const void* residual, const void* weight, void* ou
  */
 int ss_swiglu(const void* gate, const void* up, void* out, int64_t rows, int cols, int64_t g_stride,
               int64_t u_stride, int64_t o_stride, int dtype, void* stream);
+
+/*
+ * The write of a paged cache of latents: per token [c | rope(k)], shared by all heads, and the rotated
+ * queries. c = latent * weight / sqrt(mean(latent^2) + eps), or latent itself with weight NULL;
+ * rope(x) = x * cos + cat(-x2, x1) * sin. fp32, rounded once to dtype (SS_DTYPE_BF16/F16/F32, of every
+ * tensor). No counterpart in the reference, which caches keys and values of heads
+ * (slipstream/kernels/reshape_and_cache.py:10-27).
+ *   q, q_out [n_tok, heads, rope_dim] with (token, head) strides, q_out may be q; latent [n_tok,
+ *   latent_dim], k_rope, cos, sin [n_tok, rope_dim] with token strides; weight [latent_dim]; cache rows
+ *   [latent_dim + rope_dim] at c_strides (block, position); strides in elements, unit last strides.
+ * Slots < 0 or >= num_slots are skipped; of a slot given twice the row may hold parts of both.
+ */
+int ss_latent_rope_and_cache(const void* q, void* q_out, const void* latent, const void* k_rope,
+                             const void* cos, const void* sin, const void* weight, void* cache,
+                             const int64_t* slot_mapping, int64_t n_tok, int heads, int latent_dim,
+                             int rope_dim, int block_size, int64_t num_slots, const int64_t q_strides[2],
+                             const int64_t o_strides[2], int64_t latent_stride, int64_t k_stride,
+                             int64_t cos_stride, int64_t sin_stride, const int64_t c_strides[2], float eps,
+                             int dtype, void* stream);
+
+/*
+ * Attention over a paged cache of latents, absorbed form: rows [c | r] of latent_dim + rope_dim values
+ * are the keys of all heads, their latents the values.
+ *   score = scale * q . [c | r], out = sum softmax(score) c
+ * q(b, t, h) = q + b*q_strides[0] + t*q_strides[1] + h*q_strides[2] (packed, with cu_seqlens: token
+ * cu_seqlens[b] + t, q_strides[0] unused), latent_dim + rope_dim values; out likewise, latent_dim
+ * values; cache row (block, position) at c_strides; strides in elements, unit last strides. Query t of a
+ * sequence's n sees the keys [0, context_lens[b] - n + t]; n is tq, or of cu_seqlens, whose entries
+ * are clamped into [0, total_tokens]; with it tq only tells how long sequences are likely to be, and
+ * rows of no sequence are left as they are. Table entries outside [0, num_blocks) are masked, a row
+ * that sees no key gives zeros. latent_dim 1..512, rope_dim 0..256, dtype SS_DTYPE_BF16/F16/F32. The
+ * conventions of ss_paged_attention_varlen; no counterpart in the reference.
+ * workspace: ss_latent_attention_workspace_size() bytes (total_tokens = batch * tq without cu_seqlens),
+ * any contents: partial rows of keys split over workgroups. Too small a one is SS_ERR_WORKSPACE.
+ */
+int ss_latent_attention_workspace_size(int64_t batch, int64_t total_tokens, int heads, int latent_dim,
+                                       int rope_dim, int dtype, int64_t* bytes);
+
+int ss_latent_attention(const void* q, void* out, const void* cache, const int32_t* block_tables,
+                        const int32_t* cu_seqlens, const int32_t* context_lens, int64_t batch,
+                        int64_t total_tokens, int tq, int heads, int latent_dim, int rope_dim, int max_blocks,
+                        int block_size, int64_t num_blocks, const int64_t q_strides[3],
+                        const int64_t o_strides[3], const int64_t c_strides[2], int64_t bt_stride,
+                        float scale, int dtype, void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * Attention over latents, expanded form: for every token of the context kv(i, h) = [k | v] of nope_dim +
+ * value_dim values (its latent projected) and k_rope(i) of rope_dim values, shared by the heads.
+ *   score = scale * q . [k | k_rope], out = sum softmax(score) v
+ * q, out (token, head), kv (token, head) and k_rope (token) strides in elements, unit last strides; the
+ * tokens of sequence b are [cu_seqlens[b], cu_seqlens[b + 1]) of q and out, its context (these
+ * tokens last) [cu_context[b], cu_context[b + 1]) of kv and k_rope; both are clamped to total_tokens and
+ * total_keys, and rows of no sequence are left as they are. max_query_len only tells how long
+ * sequences are likely to be. nope_dim and value_dim 1..512, rope_dim 0..256, dtype
+ * SS_DTYPE_BF16/F16/F32.
+ */
+int ss_latent_attention_expanded(const void* q, void* out, const void* kv, const void* k_rope,
+                                 const int32_t* cu_seqlens, const int32_t* cu_context, int64_t batch,
+                                 int64_t total_tokens, int64_t total_keys, int max_query_len, int heads,
+                                 int nope_dim, int rope_dim, int value_dim, const int64_t q_strides[2],
+                                 const int64_t o_strides[2], const int64_t kv_strides[2], int64_t k_stride,
+                                 float scale, int dtype, void* stream);
 
 #ifdef __cplusplus
 }

@@ -91,6 +91,15 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, ctypes.c_float, _i32, _vp],
     ),
     "ss_swiglu_int8": (_i32, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i32, _vp]),
+    "ss_quantize_fp8": (_i32, [_vp, _vp, _vp, _i64, _i64, _i64, _i64, _i32, _vp]),
+    "ss_fp8_workspace_size": (_i32, [_i64, _i64, _i64, _i32, _i32, _c_i64p]),
+    "ss_fp8_gemm": (
+        _i32,
+        [
+            _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _c_i64p, _c_i64p, _i32, _i32,
+            _vp, _i64, _vp,
+        ],
+    ),
     "ss_copy_blocks": (_i32, [_vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _i64, _vp]),
     "ss_build_step_metadata": (_i32, [_vp, _i64, _i32, _vp, _vp, _i32, _i32, _vp, _vp, _vp, _i64, _vp]),
     "ss_rmsnorm": (_i32, [_vp, _vp, _vp, _vp, _i64, _i32, _i64, _i64, _i64, ctypes.c_float, _i32, _vp]),
@@ -100,6 +109,28 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         [
             _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i32, _i32, _i32, _i32, _i64,
             _c_i64p, _c_i64p, _c_i64p, _c_i64p, _c_i64p, _c_i64p, _c_i64p, _i32, _vp,
+        ],
+    ),
+    "ss_latent_rope_and_cache": (
+        _i32,
+        [
+            _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _i64, _c_i64p, _c_i64p,
+            _i64, _i64, _i64, _i64, _c_i64p, ctypes.c_float, _i32, _vp,
+        ],
+    ),
+    "ss_latent_attention_workspace_size": (_i32, [_i64, _i64, _i32, _i32, _i32, _i32, _c_i64p]),
+    "ss_latent_attention": (
+        _i32,
+        [
+            _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i32, _i32, _i32, _i32, _i32, _i32, _i64,
+            _c_i64p, _c_i64p, _c_i64p, _i64, ctypes.c_float, _i32, _vp, _i64, _vp,
+        ],
+    ),
+    "ss_latent_attention_expanded": (
+        _i32,
+        [
+            _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i32, _i32, _i32, _i32, _i32,
+            _c_i64p, _c_i64p, _c_i64p, _i64, ctypes.c_float, _i32, _vp,
         ],
     ),
 }

@@ -33,6 +33,22 @@ def allocate_kv_cache(
     )
 
 
+def allocate_latent_cache(
+    num_layers: int,
+    num_blocks: int,
+    block_size: int,
+    latent_dim: int,
+    rope_dim: int,
+    *,
+    dtype: torch.dtype,
+    device: torch.device,
+) -> torch.Tensor:
+    """Zeros ``[L, num_blocks, block_size, latent_dim + rope_dim]``: the pool that
+    ``latent_rope_and_cache`` writes and the absorbed latent attention reads. Blocks, slots and tables
+    are those of ``allocate_kv_cache``'s pool."""
+    return torch.zeros((num_layers, num_blocks, block_size, latent_dim + rope_dim), dtype=dtype, device=device)
+
+
 def slots_from_pairs(pairs: list[tuple[int, int]], block_size: int) -> list[int]:
     """``block * block_size + offset`` (``paged_cache.py:31-32``)."""
     return [block_id * block_size + offset for block_id, offset in pairs]

@@ -13,6 +13,9 @@ format at load (the quantized-model loading the reference plans, ``MASTERPLAN.md
 per output channel, activations quantized on the way in with a scale per token
 (``quantize_int8``, ``fused_swiglu_int8``) and multiplied by ``w8a8_gemm``; their
 ``forward_int8`` takes rows that are int8 already, as ``fused_rmsnorm_int8`` leaves them.
+``FP8Linear`` and ``FP8MLP`` are the same in 8-bit floating point (e4m3) with a scale for every 128 x
+128 weights and every 128 columns of an activation row (``quantize_fp8``, ``fp8_gemm``), the format that
+block-scaled checkpoints store.
 The forward passes are the HIP kernels only.
 """
 
@@ -21,6 +24,8 @@ from __future__ import annotations
 import torch
 from torch import nn
 
+from slipstream_amd.kernels.fp8_gemm import fp8_gemm
+from slipstream_amd.kernels.fp8_rows import BLOCK, FP8, blocks_of, quantize_fp8
 from slipstream_amd.kernels.int8_gemm import w8a8_gemm
 from slipstream_amd.kernels.int8_rows import fused_swiglu_int8, quantize_int8
 from slipstream_amd.kernels.norm_act import fused_swiglu
@@ -336,3 +341,113 @@ class W8A8MLP(nn.Module):
         gu = self.gate_up_proj.forward_int8(q, scale, out_dtype)
         i = self.intermediate
         return self.down_proj.forward_int8(*fused_swiglu_int8(gu[..., :i], gu[..., i:]), out_dtype)
+
+
+def quantize_weight_fp8(weight: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """For each 128 x 128 values of ``weight [N, K]`` (the last ones of a row or column of blocks may be
+    fewer): ``scale = max|w| / 448``, ``q = e4m3(w * 448 / max|w|)`` with the quotient taken in 64 bits.
+    Returns ``(qweight float8_e4m3fn [N, K], scales fp32 [ceil(N / 128), ceil(K / 128)])``; a block of
+    zeros (or below 5.3e-36) has scale 0. Torch ops on the weight's device, once at load."""
+    if weight.ndim != 2:
+        raise ValueError(f"weight must be 2-D [out, in], got {tuple(weight.shape)}")
+    n, k = weight.shape
+    w = weight.float()
+    if not torch.isfinite(w).all():
+        raise ValueError("weight has infinities or NaN")
+    nb, kb = blocks_of(n), blocks_of(k)
+    q = torch.empty((n, k), dtype=FP8, device=w.device)
+    scales = torch.zeros((nb, kb), dtype=torch.float32, device=w.device)
+    top_value = torch.full((), 448.0, device=w.device)  # a tensor: a true division, as in quantize_weight
+    for b in range(nb):  # a row of blocks at a time: 64-bit copies of the whole weight would be large
+        rows = torch.nn.functional.pad(w[b * BLOCK : (b + 1) * BLOCK], (0, kb * BLOCK - k)).unflatten(1, (kb, BLOCK))
+        top = rows.abs().amax(dim=(0, 2)) if rows.numel() else scales[b]
+        live = top >= 448 * 2.0**-126
+        safe = torch.where(live, top, 1.0)
+        exact = rows.double() * 448.0 / safe.double()[None, :, None] * live[None, :, None]
+        # rounded to e4m3 here: a conversion by way of fp32 would round twice
+        step = torch.exp2(torch.frexp(exact).exponent.clamp_min(-5) - 4.0)
+        q[b * BLOCK : (b + 1) * BLOCK] = (torch.round(exact / step) * step).flatten(1)[:, :k].float().to(FP8)
+        scales[b] = torch.where(live, safe / top_value, 0.0)
+    return q, scales
+
+
+class FP8Linear(nn.Module):
+    """``y = x @ dequant(qweight).T (+ bias)`` with ``x`` quantized in blocks of 128, through ``fp8_gemm``."""
+
+    def __init__(self, qweight: torch.Tensor, scales: torch.Tensor, bias: torch.Tensor | None = None) -> None:
+        super().__init__()
+        if qweight.ndim != 2 or qweight.dtype != FP8:
+            raise ValueError(f"qweight must be float8_e4m3fn [out, in], got {qweight.dtype} {tuple(qweight.shape)}")
+        self.out_features, self.in_features = qweight.shape
+        want = (blocks_of(self.out_features), blocks_of(self.in_features))
+        if tuple(scales.shape) != want or scales.dtype != torch.float32:
+            raise ValueError(f"scales must be float32 {want}, got {scales.dtype} {tuple(scales.shape)}")
+        self.register_buffer("qweight", qweight)
+        self.register_buffer("scales", scales)
+        self.register_buffer("bias", bias)
+
+    def _apply(self, fn, recurse: bool = True):
+        # .half() or .to(dtype) of a model: the weight stays e4m3 and its scales fp32
+        kept = {"qweight": self.qweight, "scales": self.scales}
+        super()._apply(fn, recurse)
+        for name, before in kept.items():
+            now = getattr(self, name)
+            if now.dtype != before.dtype:
+                setattr(self, name, before.to(now.device))
+        return self
+
+    @classmethod
+    def from_linear(cls, linear: nn.Linear) -> "FP8Linear":
+        bias = linear.bias.detach().clone() if linear.bias is not None else None
+        return cls(*quantize_weight_fp8(linear.weight.detach()), bias)
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        return self.forward_fp8(*quantize_fp8(x), x.dtype)
+
+    def forward_fp8(self, q: torch.Tensor, scale: torch.Tensor,
+                    out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+        """The product alone, for rows quantized already."""
+        return fp8_gemm(q, scale, self.qweight, self.scales, self.bias, out_dtype)
+
+    def extra_repr(self) -> str:
+        return f"in={self.in_features}, out={self.out_features}"
+
+
+class FP8MLP(nn.Module):
+    """SwiGLU MLP (``mlp.py:12-40``) on FP8 linears, gate and up held as one linear (as in ``W4A16MLP``)
+    where a block of scales does not reach over both (``out_features`` a multiple of 128)."""
+
+    def __init__(self, gate_proj: FP8Linear, up_proj: FP8Linear, down_proj: FP8Linear) -> None:
+        super().__init__()
+        if (gate_proj.in_features, gate_proj.out_features) != (up_proj.in_features, up_proj.out_features):
+            raise ValueError("gate_proj and up_proj must share in/out features")
+        if down_proj.in_features != gate_proj.out_features:
+            raise ValueError(f"down_proj reads {down_proj.in_features} features, gate_proj has {gate_proj.out_features}")
+        if gate_proj.out_features % BLOCK:
+            raise ValueError(f"{gate_proj.out_features} features of gate_proj are not whole blocks of {BLOCK}")
+        bias = None
+        if gate_proj.bias is not None or up_proj.bias is not None:
+            like = gate_proj.bias if gate_proj.bias is not None else up_proj.bias
+            bias = torch.cat([lin.bias if lin.bias is not None else torch.zeros_like(like)
+                              for lin in (gate_proj, up_proj)])
+        self.intermediate = gate_proj.out_features
+        self.gate_up_proj = FP8Linear(torch.cat([gate_proj.qweight.view(torch.uint8),
+                                                 up_proj.qweight.view(torch.uint8)]).view(FP8),
+                                      torch.cat([gate_proj.scales, up_proj.scales]), bias)
+        self.down_proj = down_proj
+
+    @classmethod
+    def from_mlp(cls, mlp: nn.Module) -> "FP8MLP":
+        """Quantize a module with ``gate_proj`` / ``up_proj`` / ``down_proj`` linears (the
+        reference's ``MLP``, HF names)."""
+        return cls(*(FP8Linear.from_linear(lin) for lin in (mlp.gate_proj, mlp.up_proj, mlp.down_proj)))
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        return self.forward_fp8(*quantize_fp8(x), x.dtype)
+
+    def forward_fp8(self, q: torch.Tensor, scale: torch.Tensor,
+                    out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+        """The MLP for rows quantized already."""
+        gu = self.gate_up_proj.forward_fp8(q, scale, out_dtype)
+        i = self.intermediate
+        return self.down_proj.forward_fp8(*quantize_fp8(fused_swiglu(gu[..., :i], gu[..., i:])), out_dtype)
