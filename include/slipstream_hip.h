@@ -472,7 +472,7 @@ int ss_latent_rope_and_cache(const void* q, void* q_out, const void* latent, con
  * workspace: ss_latent_attention_workspace_size() bytes (total_tokens = batch * tq without cu_seqlens),
  * any contents: partial rows of keys split over workgroups. Too small a one is SS_ERR_WORKSPACE.
  */
-int ss_latent_attention_workspace_size(int64_t batch, int64_t total_tokens, int heads, int latent_dim,
+int ss_latent_attention_workspace_size(int64_t batch, int64_t total_tokens, int tq, int heads, int latent_dim,
                                        int rope_dim, int dtype, int64_t* bytes);
 
 int ss_latent_attention(const void* q, void* out, const void* cache, const int32_t* block_tables,

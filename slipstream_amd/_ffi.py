@@ -118,7 +118,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
             _i64, _i64, _i64, _i64, _c_i64p, ctypes.c_float, _i32, _vp,
         ],
     ),
-    "ss_latent_attention_workspace_size": (_i32, [_i64, _i64, _i32, _i32, _i32, _i32, _c_i64p]),
+    "ss_latent_attention_workspace_size": (_i32, [_i64, _i64, _i32, _i32, _i32, _i32, _i32, _c_i64p]),
     "ss_latent_attention": (
         _i32,
         [

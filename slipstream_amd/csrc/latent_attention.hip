@@ -236,15 +236,19 @@ int check_call(const char* who, int64_t batch, int64_t total, int64_t keys, int 
 }  // namespace
 }  // namespace ss
 
-extern "C" int ss_latent_attention_workspace_size(int64_t batch, int64_t total_tokens, int heads, int latent_dim,
-                                                  int rope_dim, int dtype, int64_t* bytes) {
+extern "C" int ss_latent_attention_workspace_size(int64_t batch, int64_t total_tokens, int tq, int heads,
+                                                  int latent_dim, int rope_dim, int dtype, int64_t* bytes) {
   if (!bytes) {
     ss_host::set_error("latent attention workspace: null pointer");
     return SS_ERR_INVALID;
   }
   *bytes = 0;
-  return ss::check_call("latent attention workspace", batch, total_tokens, 0, heads, latent_dim, rope_dim, latent_dim,
-                        dtype);
+  const int st = ss::check_call("latent attention workspace", batch, total_tokens, 0, heads, latent_dim, rope_dim,
+                                latent_dim, dtype);
+  if (st != SS_OK || batch == 0 || heads == 0 || total_tokens == 0) return st;
+  if (dtype != SS_DTYPE_F32 && (latent_dim == 256 || latent_dim == 512))
+    *bytes = ss::latent_tile_bytes(batch, total_tokens, tq, heads, latent_dim);
+  return SS_OK;
 }
 
 extern "C" int ss_latent_attention(const void* q, void* out, const void* cache, const int32_t* block_tables,
@@ -279,7 +283,15 @@ extern "C" int ss_latent_attention(const void* q, void* out, const void* cache, 
   p.max_blocks = num_blocks > 0 ? max_blocks : 0, p.block_size = block_size;
   p.total = (int)total_tokens;
   p.scale_log2 = scale * ss::kLog2e;
-  (void)workspace, (void)workspace_bytes;
+  if (ss::latent_tile_takes(p, dtype)) {
+    const int64_t need = ss::latent_tile_bytes(batch, p.cu ? total_tokens : batch * tq, tq, heads, latent_dim);
+    if (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < need) {
+      ss_host::set_error("%s: workspace of %lld bytes, needs %lld (16-byte aligned)", who,
+                         (long long)(workspace ? workspace_bytes : 0), (long long)need);
+      return SS_ERR_WORKSPACE;
+    }
+    return ss::launch_latent_tile(p, dtype, (char*)workspace, (hipStream_t)stream);
+  }
   return ss::launch_general<true>(p, dtype, (hipStream_t)stream);
 }
 

@@ -58,4 +58,10 @@ __device__ __forceinline__ int latent_keys(const LatentParams& p, int b, int& fi
   return (int)min((int64_t)length, (int64_t)p.max_blocks * p.block_size);
 }
 
+// latent_tile.hip: whether the matrix-core kernels take a call of the absorbed form, the workspace they
+// need for it, and the call
+bool latent_tile_takes(const LatentParams& p, int dtype);
+int64_t latent_tile_bytes(int64_t batch, int64_t total, int tq, int heads, int latent_dim);
+int launch_latent_tile(const LatentParams& p, int dtype, char* ws, hipStream_t stream);
+
 }  // namespace ss

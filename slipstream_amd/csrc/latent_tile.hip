@@ -1,0 +1,621 @@
+// Attention over latents, absorbed form, on the matrix cores: bf16 and fp16, latents of 256 or 512
+// values, rotated keys of 64, pages of 8, 16, 32, ... tokens.
+//
+// All heads share a sequence's keys, so the query rows of a (sequence, few tokens) are its tokens' heads,
+// and a tile of keys that is in the LDS serves them all. A workgroup takes ROWS = 16 RT rows and walks the
+// keys in tiles of 32:
+//   S^T = K Q^T     a wave its 16 rows against the tile's 32 keys; the queries stay in registers
+//   softmax         in fp32 over the wave's rows; P^T goes to the LDS in the order in which the next
+//                   product's operand wants it (16 bytes a lane, no bank twice), with the factors by which
+//                   the rows' earlier outputs shrink
+//   O^T += C^T P^T  a wave all the workgroup's rows, but R / NW of the latents' values: so a latent is
+//                   read from the LDS once by each wave for the scores and once in all for the outputs
+//                   (whole rows a wave would take twice the LDS reads, which bound the kernel then)
+// The tiles come by DMA into a ring of four (latents) and three (rotated keys); a step multiplies tile
+// t's outputs and tile t + 1's scores while tiles t + 2 and t + 3 are on their way, with one barrier.
+//
+// In the LDS the 16-byte chunk c of a latent's row r lies at c ^ swizzle(r) (the four bits of r, two of
+// them swapped): a score operand's sixteen rows then lie in different banks, and so do the 8-byte pieces of
+// eight rows that a transposing read (ds_read_b64_tr_b16) takes of four chunks.
+//
+// Work: a sequence's tokens are cut into tiles of J (J heads <= ROWS, a power of two), one item each, or
+// where there are more heads than rows into slices of heads. An item's length is its number of key
+// tiles; the items in a row are cut into as many equal ranges as there are workgroups, so every
+// workgroup has the same number of tiles whatever the lengths are. Each finds its range by a scan over the
+// sequences' lengths in closed form. An item that is cut leaves fp32 partial rows, which
+// latent_merge_kernel adds in order: results repeat themselves to the bit.
+#include <type_traits>
+#include <utility>
+
+#include "latent_common.h"
+#include "w8a8_common.h"
+
+namespace ss {
+namespace {
+
+constexpr int kRopeDim = 64;
+constexpr float kSlack = 8.f;  // by which (log2) a score may exceed the running maximum before it is raised
+
+typedef short tr16x4 __attribute__((ext_vector_type(4)));
+
+template <int R_, int RT_, int NW_>
+struct LatTile {
+  static constexpr int R = R_, RT = RT_, NW = NW_;
+  static constexpr int KT = 32, ROWS = 16 * RT;
+  static constexpr int ROWB = 2 * R, LPLANE = KT * ROWB;  // latents of a tile in the LDS
+  static constexpr int RPLANE = KT * 2 * kRopeDim;
+  static constexpr int NS = 4, NR = 3;                    // ring depths
+  static constexpr int DT = R / (16 * NW);                // 16-value output tiles of a wave
+  static constexpr int PB = RT * 1024;                    // bytes of a tile's P
+  static constexpr int RPI = 1024 / ROWB;                 // latents a DMA instruction brings
+  static constexpr int NL = KT / RPI / NW;                // DMA instructions of a wave and tile, latents
+  static constexpr int kP = NS * LPLANE + NR * RPLANE, kAlpha = kP + 2 * PB, kMl = kAlpha + 2 * ROWS * 4,
+                       kGrew = kMl + ROWS * 8, kScan = kGrew + 64, LDS = kScan + 128;
+  static_assert(LDS <= 160 * 1024, "one workgroup a CU");
+};
+
+__device__ __forceinline__ int lat_swizzle(int r) { return (r & 3) | ((r & 4) << 1) | ((r & 8) >> 1); }
+
+// The latents' chunk of 8 values that output tile dt of wave w takes for lanes of row group g: bit 2 from
+// g >> 1, so that the four pieces of a transposing read lie in different banks whatever dt and w are
+template <typename C>
+__device__ __forceinline__ int out_chunk(int dt, int gh, int w) {
+  if constexpr (C::DT == 8)
+    return (dt & 3) + 4 * gh + 8 * (dt >> 2) + 16 * w;
+  else if constexpr (C::DT == 4)
+    return dt + 4 * gh + 8 * w;
+  else
+    return dt + 2 * (w & 1) + 4 * gh + 8 * (w >> 1);
+}
+
+// 16 bytes a lane straight into LDS at lds + 16 lane, zeros past the descriptor's end. As asm, so that
+// the compiler's waits do not count it; the wait states are those of a descriptor that a VALU
+// instruction wrote.
+__device__ __forceinline__ void lat_dma(i32x4 rs, LdsBytes lds, int voff) {
+  const uint32_t m0 = (uint32_t)(uintptr_t)lds;
+  asm volatile("s_nop 4\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" : : "v"(voff), "s"(rs), "{m0}"(m0) : "memory");
+}
+template <int N>
+__device__ __forceinline__ void lat_wait() {
+  asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory");
+}
+
+// ---- items ----------------------------------------------------------------------------------
+
+// How rows are made of tokens and heads: items of J tokens (1 << js), or HS slices of one token's heads
+struct RowShape {
+  int js, hs;
+};
+template <int ROWS>
+__host__ __device__ inline RowShape row_shape(int heads) {
+  RowShape s = {0, (heads + ROWS - 1) / ROWS};
+  while ((heads << (s.js + 1)) <= ROWS) ++s.js;
+  return s;
+}
+
+// A sequence as the items see it: n query tokens, `length` keys of which the table reaches `keys`
+struct SeqView {
+  int n, start, length, keys;
+};
+// lo < n heads <= hi, else the sequence counts as empty (another launch takes it)
+__device__ __forceinline__ SeqView seq_view(const LatentParams& p, int b, int lo, int hi) {
+  SeqView v;
+  latent_queries(p, b, v.n, v.start);
+  int first;
+  v.keys = latent_keys(p, b, first, v.length);
+  const int64_t rows = (int64_t)v.n * p.heads;
+  if (rows <= lo || rows > hi) v.n = 0;
+  return v;
+}
+
+// sum of floor(i / 2^s) over i < x
+__device__ __forceinline__ int64_t steps_below(int64_t x, int s) {
+  const int64_t q = x >> s;
+  return ((q * (q - 1) / 2) << s) + q * (x - (q << s));
+}
+// Key tiles of the token tiles before the i-th of a sequence's nt: tile i ends at key length - n +
+// (i + 1) J (the last one at `length`) and counts at least one. With a table that does not reach the
+// length, all of them as long as the table.
+__device__ __forceinline__ int64_t tiles_before(const SeqView& v, int i, int nt, int js) {
+  if (v.length > v.keys) return (int64_t)i * max(1, (v.keys + 31) >> 5);
+  const int m = min(i, nt - 1);  // of those that end with a whole tile of tokens
+  const int base = v.length - v.n + (1 << js);
+  const int none = base >= 1 ? 0 : min(m, (-base >> js) + 1);  // that see no key
+  int64_t sum = none;
+  const int64_t count = m - none, at = (int64_t)base + ((int64_t)none << js) + 31;
+  if (count > 0) {
+    if (js >= 5) {
+      sum += count * (at >> 5) + ((count * (count - 1) / 2) << (js - 5));
+    } else {
+      const int64_t c = at >> js;
+      sum += steps_below(c + count, 5 - js) - steps_below(c, 5 - js);
+    }
+  }
+  return i > m ? sum + max(1, (v.length + 31) >> 5) : sum;
+}
+__device__ __forceinline__ int64_t seq_tiles(const SeqView& v, RowShape s) {
+  if (v.n <= 0) return 0;
+  const int nt = (v.n + (1 << s.js) - 1) >> s.js;
+  return tiles_before(v, nt, nt, s.js) * s.hs;
+}
+
+// The same in every lane, kept in scalar registers
+__device__ __forceinline__ int64_t uniform(int64_t x) {
+  return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32 |
+                   (uint32_t)__builtin_amdgcn_readfirstlane((int)x));
+}
+
+struct LatentWork {
+  float* o;   // [2 groups][ROWS][R] partial rows
+  float* ml;  // [2 groups][ROWS][2] maximum (log2) and sum
+  int* rec;   // [groups][4] the item that begins before a group's range and is merged there
+  int lo, hi;  // the launch's sequences: lo < n heads <= hi
+};
+
+template <typename T, typename C>
+__device__ __forceinline__ void latent_segment(const LatentParams& p, const LatentWork& work, char* const lds,
+                                               const SeqView v, const int b, const int tok0, const int head0,
+                                               const int js, const int t0, const int t1, const bool whole,
+                                               const int slot) {
+  constexpr int R = C::R, RT = C::RT, NW = C::NW, DT = C::DT, KS = R / 32, KR = kRopeDim / 32;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n = lane & 15, g = lane >> 4;
+  const int heads = min(p.heads - head0, C::ROWS);  // of a token in this item
+  const int tokens = min(1 << js, v.n - tok0);
+  const int kv_end = max(0, min(v.keys, v.length - v.n + tok0 + tokens));
+  const int tend = min(t1, (kv_end + 31) >> 5);
+
+  // the row of this lane in row tile rt: token and head, or none
+  auto row_of = [&](int rt, int& tok, int& head) {
+    const int rr = 16 * rt + n, j = rr / heads;
+    tok = tok0 + j;
+    head = head0 + rr - j * heads;
+    return j < tokens;
+  };
+  const bool scores = wave < RT;
+  // queries: scaled inside the exponent, which needs a positive scale (a negative one is the query's sign)
+  u32x4 qop[KS + KR];
+  int lim = 0x7FFFFFFF;
+  if (scores) {
+    int tok, head;
+    const bool ok = row_of(wave, tok, head);
+    if (ok) lim = min(v.keys, v.length - v.n + tok + 1);
+    const T* const q = (const T*)p.q + (p.cu ? 0 : b * p.q_sb) + (v.start + tok) * p.q_st + head * p.q_sh + 8 * g;
+    const uint32_t flip = p.scale_log2 < 0.f ? 0x80008000u : 0u;
+#pragma unroll
+    for (int s = 0; s < KS + KR; ++s)
+      qop[s] = (ok ? load16(q + 32 * s) : u32x4{0, 0, 0, 0}) ^ u32x4{flip, flip, flip, flip};
+  }
+  const float cscale = fabsf(p.scale_log2);
+  int least = lim;  // of the wave's rows: tiles that end before it need no mask
+#pragma unroll
+  for (int o = 1; o < 16; o <<= 1) least = min(least, __shfl_xor(least, o));
+  least = __builtin_amdgcn_readfirstlane(least);
+
+  const int32_t* const table = p.bt + (int64_t)b * p.bt_stride;
+  const ConstInts stable = (ConstInts)table;
+  const int shift = __builtin_ctz((unsigned)p.block_size);
+  bool bad = false;
+  for (int i = ((t0 * 32) >> shift) + threadIdx.x; (int64_t)i << shift < min(kv_end, tend * 32); i += 64 * NW) {
+    const int e = table[i];
+    bad |= e < 0 || e >= p.num_blocks;
+  }
+  const bool holes = __syncthreads_or(bad);
+
+  // DMA of tile t: this wave brings the latents of 32 / NW keys, and waves 0 .. 3 the rotated keys of eight
+  // (in the same page as its latents)
+  const int key8 = 8 * (wave & 3), key_l = NW == 8 ? 4 * (wave >> 2) : 0;  // first key of the eight; latents from there
+  const int tok_bytes = (int)(p.kv_s1 * 2);
+  int voff_l[C::NL], voff_r;
+#pragma unroll
+  for (int u = 0; u < C::NL; ++u) {
+    const int k = key_l + u * C::RPI + lane * 16 / C::ROWB;  // of the eight
+    voff_l[u] = k * tok_bytes + 16 * ((lane & (R / 8 - 1)) ^ lat_swizzle(key8 + k));
+  }
+  voff_r = (lane >> 3) * tok_bytes + C::ROWB + 16 * ((lane & 7) ^ tile_swizzle(key8 + (lane >> 3)));
+  auto entry = [&](int t) { return stable[max(0, min((t * 32 + key8) >> shift, p.max_blocks - 1))]; };
+  auto issue = [&](int t, int e, int ls, int rs) {
+    const int key = t * 32 + key8, live = min(8, kv_end - key);
+    const bool there = e >= 0 && e < p.num_blocks && live > 0 && t < tend;
+    const int64_t off = there ? (int64_t)e * p.kv_s0 + (int64_t)(key & (p.block_size - 1)) * p.kv_s1 : 0;
+    const uint64_t at = (uint64_t)p.kv + 2 * off;
+    const i32x4 rsrc = {__builtin_amdgcn_readfirstlane((int)(uint32_t)at),
+                        __builtin_amdgcn_readfirstlane((int)(uint32_t)(at >> 32) & 0xFFFF),
+                        __builtin_amdgcn_readfirstlane(there ? (live - 1) * tok_bytes + C::ROWB + 2 * kRopeDim : 0),
+                        0x00020000};
+    const LdsBytes base = (LdsBytes)lds;
+#pragma unroll
+    for (int u = 0; u < C::NL; ++u)
+      lat_dma(rsrc, base + ls * C::LPLANE + (key8 + key_l + u * C::RPI) * C::ROWB, voff_l[u]);
+    if (wave < 4) lat_dma(rsrc, base + C::NS * C::LPLANE + rs * C::RPLANE + key8 * 2 * kRopeDim, voff_r);
+  };
+  auto landed = [&](auto tiles) {  // all but the youngest `tiles` tiles
+    if (wave < 4)
+      lat_wait<decltype(tiles)::value*(C::NL + 1)>();
+    else
+      lat_wait<decltype(tiles)::value * C::NL>();
+  };
+
+  f32x4 acc[RT][DT];
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) acc[rt][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float m = kNegBig, l = 0.f;  // of row n; l: of this lane's keys
+
+  // ---- scores and softmax of tile t in ring slots ls, rs; P and the rows' factors into buffer `buf`
+  auto score = [&](int t, int ls, int rs, int buf) {
+    const int sw = lat_swizzle(n);
+    const char* const kl = lds + ls * C::LPLANE + n * C::ROWB;
+    const char* const kr = lds + C::NS * C::LPLANE + rs * C::RPLANE + n * 2 * kRopeDim;
+    f32x4 s2[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+        s2[x] = Elem<T>::mfma(load16(kl + 16 * x * C::ROWB + 16 * ((4 * s + g) ^ sw)), qop[s], s2[x]);
+#pragma unroll
+    for (int s = 0; s < KR; ++s)
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+        s2[x] = Elem<T>::mfma(load16(kr + 16 * x * 2 * kRopeDim + 16 * ((4 * s + g) ^ tile_swizzle(n))), qop[KS + s], s2[x]);
+    float sv[8];
+#pragma unroll
+    for (int x = 0; x < 2; ++x)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sv[4 * x + e] = s2[x][e];
+    if (holes || t * 32 + 32 > least) {
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const int key = t * 32 + 16 * x + 4 * g;  // four keys of one page
+        bool there = true;
+        if (holes && key < kv_end) {
+          const int e = table[key >> shift];
+          there = e >= 0 && e < p.num_blocks;
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (!there || key + e >= min(lim, kv_end)) sv[4 * x + e] = -__builtin_inff();
+      }
+    }
+    float top = fmaxf(fmaxf(fmaxf(sv[0], sv[1]), fmaxf(sv[2], sv[3])), fmaxf(fmaxf(sv[4], sv[5]), fmaxf(sv[6], sv[7])));
+    top = max_across_rows(top);
+    const float want = fmaxf(m, top * cscale);
+    const bool grew = __any(want > m + kSlack);
+    const float mn = grew ? want : m;
+    float pv[8], sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) pv[i] = fast_exp2(fmaf(sv[i], cscale, -mn));
+    if (cscale == 0.f) {  // (a masked key's is then not a number)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) pv[i] = sv[i] == -__builtin_inff() ? 0.f : pv[i];
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum += pv[i];
+    const float alpha = fast_exp2(m - mn);
+    l = l * alpha + sum;
+    m = mn;
+    store16(lds + C::kP + buf * C::PB + wave * 1024 + lane * 16,
+            u32x4{Elem<T>::pack2(pv[0], pv[1]), Elem<T>::pack2(pv[2], pv[3]), Elem<T>::pack2(pv[4], pv[5]),
+                  Elem<T>::pack2(pv[6], pv[7])});
+    if (g == 0) *reinterpret_cast<float*>(lds + C::kAlpha + (buf * C::ROWS + 16 * wave + n) * 4) = alpha;
+    if (lane == 0) *reinterpret_cast<int*>(lds + C::kGrew + (buf * RT + wave) * 4) = grew;
+  };
+  // ---- outputs of the tile in ring slot ls with the probabilities in buffer `buf`
+  const int vrow = 4 * g + (n >> 2);
+  auto output = [&](int ls, int buf) {
+    if (__any(*reinterpret_cast<const int*>(lds + C::kGrew + (buf * RT + (lane & (RT - 1))) * 4))) {
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        const float alpha = *reinterpret_cast<const float*>(lds + C::kAlpha + (buf * C::ROWS + 16 * rt + n) * 4);
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) acc[rt][dt] *= alpha;
+      }
+    }
+    const LdsBytes vp = (LdsBytes)lds + ls * C::LPLANE + vrow * C::ROWB + 8 * (n & 1);
+    const int sw = lat_swizzle(vrow);
+    u32x4 c[DT];
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) {
+      const LdsBytes at = vp + 16 * (out_chunk<C>(dt, (n >> 1) & 1, wave) ^ sw);
+      const u32x2 lo = __builtin_bit_cast(
+          u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) tr16x4*)at));
+      const u32x2 hi = __builtin_bit_cast(
+          u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) tr16x4*)(at + 16 * C::ROWB)));
+      c[dt] = u32x4{lo[0], lo[1], hi[0], hi[1]};
+    }
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      const u32x4 pr = load16(lds + C::kP + buf * C::PB + rt * 1024 + lane * 16);
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) acc[rt][dt] = Elem<T>::mfma(c[dt], pr, acc[rt][dt]);
+    }
+  };
+
+  if (t0 < tend) {
+    int e3 = entry(t0 + 3);
+    issue(t0, entry(t0), 0, 0);
+    issue(t0 + 1, entry(t0 + 1), 1, 1);
+    issue(t0 + 2, entry(t0 + 2), 2, 2);
+    landed(std::integral_constant<int, 2>{});
+    __syncthreads();
+    if (scores) score(t0, 0, 0, 0);
+    int ls = 0, rs = 0;  // slots of tile t
+    for (int t = t0; t < tend; ++t) {
+      landed(std::integral_constant<int, 1>{});
+      __syncthreads();  // tile t + 1 is there, P of tile t too, and tile t - 1's slots are free
+      issue(t + 3, e3, (ls + 3) & 3, rs);
+      e3 = entry(t + 4);
+      const int rn = rs == 2 ? 0 : rs + 1;
+      if (scores && t + 1 < tend) score(t + 1, (ls + 1) & 3, rn, (t + 1 - t0) & 1);
+      output(ls, (t - t0) & 1);
+      ls = (ls + 1) & 3;
+      rs = rn;
+    }
+    lat_wait<0>();
+  }
+
+  // ---- the rows' sums, then the rows themselves
+  if (scores) {
+    const float total = sum_across_rows(l);
+    if (g == 0) *reinterpret_cast<float2*>(lds + C::kMl + (16 * wave + n) * 8) = float2{m, total};
+  }
+  __syncthreads();
+  if (whole) {
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      int tok, head;
+      if (!row_of(rt, tok, head)) continue;
+      const float total = reinterpret_cast<const float2*>(lds + C::kMl + (16 * rt + n) * 8)->y;
+      const float inv = total == 0.f ? 0.f : 1.f / total;
+      T* const o = (T*)p.out + (p.cu ? 0 : b * p.o_sb) + (v.start + tok) * p.o_st + head * p.o_sh + 4 * (g & 1);
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) {
+        const f32x4 y = acc[rt][dt] * inv;
+        *reinterpret_cast<u32x2*>(o + 8 * out_chunk<C>(dt, g >> 1, wave)) =
+            u32x2{Elem<T>::pack2(y[0], y[1]), Elem<T>::pack2(y[2], y[3])};
+      }
+    }
+  } else {
+    float* const o = work.o + (int64_t)slot * C::ROWS * R + 4 * (g & 1);
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+        *reinterpret_cast<f32x4*>(o + (16 * rt + n) * R + 8 * out_chunk<C>(dt, g >> 1, wave)) = acc[rt][dt];
+    float* const ml = work.ml + (int64_t)slot * C::ROWS * 2;
+    for (int i = threadIdx.x; i < 2 * C::ROWS; i += 64 * NW) ml[i] = *reinterpret_cast<const float*>(lds + C::kMl + 4 * i);
+  }
+  __syncthreads();  // the LDS is free for the next item
+}
+
+extern __shared__ __attribute__((aligned(1024))) char s_lat[];
+
+template <typename T, typename C>
+__global__ __launch_bounds__(64 * C::NW) void latent_tile_kernel(const LatentParams p, const LatentWork work) {
+  constexpr int NT = 64 * C::NW;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const RowShape shape = row_shape<C::ROWS>(p.heads);
+  // workgroups go round robin over the eight XCDs: each XCD takes a contiguous eighth of the ranges, whose
+  // items share keys
+  const int all = gridDim.x, per_xcd = all >> 3;
+  const int w = all & 7 ? (int)blockIdx.x : (int)(blockIdx.x & 7) * per_xcd + (int)(blockIdx.x >> 3);
+
+  // the sequences' lengths in tiles, summed: where this workgroup's range begins
+  int64_t* const s_sum = reinterpret_cast<int64_t*>(s_lat + C::kScan);  // [NW], then the sequence found
+  auto scan = [&](int b, int64_t& mine) {  // the sum up to and with sequence b, and that of the NT
+    mine = 0;
+    if (b < p.batch) mine = seq_tiles(seq_view(p, b, work.lo, work.hi), shape);
+    int64_t sum = mine;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int64_t below = __shfl_up(sum, o);
+      sum += lane >= o ? below : 0;
+    }
+    __syncthreads();
+    if (lane == 63) s_sum[wave] = sum;
+    __syncthreads();
+    for (int i = 0; i < wave; ++i) sum += s_sum[i];
+    return sum;
+  };
+  int64_t mine, upto = 0, total = 0;
+  for (int b0 = 0; b0 < p.batch; b0 += NT) {
+    upto = total + scan(b0 + threadIdx.x, mine);
+    for (int i = 0; i < C::NW; ++i) total += s_sum[i];
+  }
+  total = uniform(total);
+  const int groups = (int)min((int64_t)all, total);
+  int* const rec = work.rec + 4 * w;
+  if (w >= groups) {
+    if (threadIdx.x == 0) rec[0] = -1;
+    return;
+  }
+  int64_t u = total * w / groups;
+  const int64_t u1 = total * (w + 1) / groups;
+  int64_t before = 0;  // tiles of the sequences before b
+  int b = 0;
+  for (int64_t b0 = 0, done = 0; b0 < p.batch; b0 += NT) {
+    if (p.batch > NT) {
+      upto = done + scan((int)b0 + threadIdx.x, mine);
+      for (int i = 0; i < C::NW; ++i) done += s_sum[i];
+    }
+    if (upto - mine <= u && u < upto) {
+      s_sum[C::NW] = b0 + threadIdx.x;
+      s_sum[C::NW + 1] = upto - mine;
+    }
+    __syncthreads();
+    if (p.batch <= NT || u < done) break;
+  }
+  b = __builtin_amdgcn_readfirstlane((int)s_sum[C::NW]);
+  before = uniform(s_sum[C::NW + 1]);
+  __syncthreads();
+
+  const int64_t u0 = u;
+  for (; u < u1; ++b) {
+    const SeqView v = seq_view(p, b, work.lo, work.hi);
+    const int nt = (v.n + (1 << shape.js) - 1) >> shape.js;
+    const int64_t end = before + seq_tiles(v, shape);
+    if (u >= end) continue;  // no rows of this launch
+    // the token tile that tile u is in: a search 64 at a time
+    int i = 0;
+    for (int span = nt; span > 1;) {
+      const int step = (span + 63) >> 6, at = i + lane * step;
+      const bool below = at < i + span && tiles_before(v, at, nt, shape.js) * shape.hs <= u - before;
+      i += (__popcll(__ballot(below)) - 1) * step;
+      span = min(step, nt - i);
+    }
+    i = __builtin_amdgcn_readfirstlane(i);
+    for (; i < nt && u < u1; ++i) {
+      const int64_t first = before + tiles_before(v, i, nt, shape.js) * shape.hs;
+      const int64_t each = tiles_before(v, i + 1, nt, shape.js) - tiles_before(v, i, nt, shape.js);
+      for (int h = shape.hs > 1 ? (int)((u - first) / each) : 0; h < shape.hs && u < u1; ++h) {
+        const int64_t s = first + h * each, e = min(s + each, u1);
+        const int t0 = (int)(u - s), t1 = (int)(e - s);
+        if (u == u0 && threadIdx.x == 0) {  // an item begun in the range before: merged from here on
+          const int from = (int)(((s + 1) * groups - 1) / total), to = (int)(((s + each) * groups - 1) / total);
+          rec[0] = t0 > 0 && from + 1 == w ? b : -1;
+          rec[1] = i * shape.hs + h;
+          rec[2] = to;
+        }
+        latent_segment<T, C>(p, work, s_lat, v, b, i << shape.js, h * C::ROWS, shape.js, t0, t1,
+                             t0 == 0 && t1 == each, 2 * w + (t0 == 0));
+        u = e;
+      }
+    }
+    before = end;
+  }
+}
+
+// The partial rows of an item that is cut, added in the order of its ranges: workgroup (w, part) 16 rows of
+// the item whose first cut is the begin of range w.
+template <typename T, int R, int ROWS>
+__global__ __launch_bounds__(256) void latent_merge_kernel(const LatentParams p, const LatentWork work) {
+  const int w = blockIdx.x;
+  const int* const rec = work.rec + 4 * w;
+  const int b = rec[0];
+  if (b < 0) return;
+  const RowShape shape = row_shape<ROWS>(p.heads);
+  const int item = rec[1], last = rec[2];
+  const SeqView v = seq_view(p, b, work.lo, work.hi);
+  const int tok0 = item / shape.hs << shape.js, head0 = item % shape.hs * ROWS;
+  const int heads = min(p.heads - head0, ROWS), tokens = min(1 << shape.js, v.n - tok0);
+  constexpr int PER = R / 64;  // values of a lane
+  const int lane = threadIdx.x & 63;
+#pragma unroll 1
+  for (int k = 0; k < 4; ++k) {
+    const int rr = 16 * blockIdx.y + 4 * (threadIdx.x >> 6) + k, j = rr / heads;
+    if (j >= tokens) continue;
+    float top = kNegBig;
+    for (int i = w - 1; i <= last; ++i) {
+      const int slot = i == w - 1 ? 2 * i + 1 : 2 * i;
+      top = fmaxf(top, work.ml[((int64_t)slot * ROWS + rr) * 2]);
+    }
+    float sum = 0.f, o[PER] = {};
+    for (int i = w - 1; i <= last; ++i) {
+      const int64_t row = (int64_t)(i == w - 1 ? 2 * i + 1 : 2 * i) * ROWS + rr;
+      const float2 ml = *reinterpret_cast<const float2*>(work.ml + 2 * row);
+      const float f = fast_exp2(ml.x - top);
+      sum = fmaf(ml.y, f, sum);
+#pragma unroll
+      for (int d = 0; d < PER; d += 4) {
+        const f32x4 x = *reinterpret_cast<const f32x4*>(work.o + row * R + d * 64 + 4 * lane);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) o[d + q] = fmaf(x[q], f, o[d + q]);
+      }
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    T* const out = (T*)p.out + (p.cu ? 0 : b * p.o_sb) + (v.start + tok0 + j) * p.o_st + (head0 + rr - j * heads) * p.o_sh;
+#pragma unroll
+    for (int d = 0; d < PER; d += 4)
+      *reinterpret_cast<u32x2*>(out + d * 64 + 4 * lane) =
+          u32x2{Elem<T>::pack2(o[d] * inv, o[d + 1] * inv), Elem<T>::pack2(o[d + 2] * inv, o[d + 3] * inv)};
+  }
+}
+
+// ---- host ---------------------------------------------------------------------------------------
+
+constexpr int64_t kAlign = 256;
+int64_t up(int64_t n) { return (n + kAlign - 1) / kAlign * kAlign; }
+
+int64_t part_bytes(int rows, int r) {
+  const int64_t groups = ss_host::device_cu_count();
+  return up(groups * 2 * rows * r * 4) + up(groups * 2 * rows * 2 * 4) + up(groups * 4 * 4);
+}
+
+template <typename T, int R, int RT, int NW>
+int launch_rows(const LatentParams& p, int lo, int hi, char* ws, hipStream_t stream) {
+  typedef LatTile<R, RT, NW> C;
+  const int64_t groups = ss_host::device_cu_count();
+  LatentWork work;
+  work.o = (float*)ws;
+  work.ml = (float*)(ws + up(groups * 2 * C::ROWS * R * 4));
+  work.rec = (int*)((char*)work.ml + up(groups * 2 * C::ROWS * 2 * 4));
+  work.lo = lo, work.hi = hi;
+  auto kern = latent_tile_kernel<T, C>;
+  static std::atomic<uint64_t> done{0};
+  if (const int st = reserve_lds((const void*)kern, C::LDS, done); st != SS_OK) return st;
+  hipLaunchKernelGGL(kern, dim3((unsigned)groups), dim3(64 * NW), C::LDS, stream, p, work);
+  if (const int st = ss_host::launch_status("latent attention"); st != SS_OK) return st;
+  hipLaunchKernelGGL((latent_merge_kernel<T, R, C::ROWS>), dim3((unsigned)groups, RT), dim3(256), 0, stream, p, work);
+  return ss_host::launch_status("latent attention (merge)");
+}
+
+template <typename T, int R>
+int launch_for(const LatentParams& p, int rows, int lo, int hi, char* ws, hipStream_t stream) {
+  if (rows <= 16) return launch_rows<T, R, 1, 4>(p, lo, hi, ws, stream);
+  if (rows <= 32) return launch_rows<T, R, 2, 4>(p, lo, hi, ws, stream);
+  if (rows <= 64) return launch_rows<T, R, 4, 8>(p, lo, hi, ws, stream);
+  return launch_rows<T, R, 8, 8>(p, lo, hi, ws, stream);
+}
+
+// Rows of the launches of a call: of sequences of few rows (0: no such launch), and of the others. Where
+// some sequences are shorter than the longest, those of one token take tiles of one token's heads.
+void plan_rows(int64_t batch, int64_t total, int tq, int heads, int& few, int& many) {
+  const int64_t rows = (int64_t)(tq < 1 ? 1 : tq) * heads;
+  many = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
+  few = tq > 1 && total < batch * tq && heads <= 64 ? (heads <= 16 ? 16 : heads <= 32 ? 32 : 64) : 0;
+  if (few >= many) few = 0;
+}
+
+}  // namespace
+
+bool latent_tile_takes(const LatentParams& p, int dtype) {
+  const bool pow2 = (p.block_size & (p.block_size - 1)) == 0;
+  if (dtype != SS_DTYPE_BF16 && dtype != SS_DTYPE_F16) return false;
+  if ((p.key_dim != 512 && p.key_dim != 256) || p.rope_dim != kRopeDim || !pow2 || p.block_size < 8) return false;
+  if (p.max_blocks < 1) return false;
+  for (int64_t s : {p.q_sb, p.q_st, p.q_sh, p.kv_s0, p.kv_s1})
+    if (s % 8) return false;
+  for (int64_t s : {p.o_sb, p.o_st, p.o_sh})
+    if (s % 4) return false;
+  return ((uintptr_t)p.q | (uintptr_t)p.kv) % 16 == 0 && (uintptr_t)p.out % 8 == 0 &&
+         p.kv_s1 >= p.key_dim + p.rope_dim && p.kv_s1 < (1 << 24);
+}
+
+int64_t latent_tile_bytes(int64_t batch, int64_t total, int tq, int heads, int latent_dim) {
+  int few, many;
+  plan_rows(batch, total, tq, heads, few, many);
+  return part_bytes(many, latent_dim) + (few ? part_bytes(few, latent_dim) : 0);
+}
+
+int launch_latent_tile(const LatentParams& p, int dtype, char* ws, hipStream_t stream) {
+  int few, many;
+  plan_rows(p.batch, p.cu ? p.total : (int64_t)p.batch * p.tq, p.tq, p.heads, few, many);
+  constexpr int kAll = 0x7FFFFFFF;
+  const int lo = few ? p.heads : 0;  // the first launch's sequences: of one token
+#define LATENT_LAUNCH(T, R)                                                                           \
+  do {                                                                                                \
+    if (few)                                                                                          \
+      if (const int st = launch_for<T, R>(p, few, 0, lo, ws, stream); st != SS_OK) return st;         \
+    return launch_for<T, R>(p, many, lo, kAll, ws + (few ? part_bytes(few, R) : 0), stream);          \
+  } while (0)
+  if (dtype == SS_DTYPE_BF16) {
+    if (p.key_dim == 512) LATENT_LAUNCH(bf16_t, 512);
+    LATENT_LAUNCH(bf16_t, 256);
+  }
+  if (p.key_dim == 512) LATENT_LAUNCH(f16_t, 512);
+  LATENT_LAUNCH(f16_t, 256);
+#undef LATENT_LAUNCH
+}
+
+}  // namespace ss

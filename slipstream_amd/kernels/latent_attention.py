@@ -24,21 +24,21 @@ import torch
 from slipstream_amd import _ffi
 from slipstream_amd.kernels._common import launch, require_device, unit_last_stride
 from slipstream_amd.kernels.latent_cache import check_latent_cache, layer_ptr
-from slipstream_amd.kernels.paged_attention import _check_stream, _debug, _int32
+from slipstream_amd.kernels.paged_attention import _check_stream, _debug, _int32, _strides
 
 _WS_BYTES: dict[tuple, int] = {}
 
 
-def _workspace(device: torch.device, batch: int, tokens: int, heads: int, latent_dim: int, rope_dim: int,
+def _workspace(device: torch.device, batch: int, tokens: int, tq: int, heads: int, latent_dim: int, rope_dim: int,
                dtype: int) -> torch.Tensor:
     """Scratch of this call alone, sized by the library: partial rows of keys split over workgroups."""
-    key = (device.index, batch, tokens, heads, latent_dim, rope_dim, dtype)
+    key = (device.index, batch, tokens, tq, heads, latent_dim, rope_dim, dtype)
     nbytes = _WS_BYTES.get(key)
     if nbytes is None:
         need = _ffi.ctypes.c_int64(0)
         with torch.cuda.device(device):
-            status = _ffi.lib().ss_latent_attention_workspace_size(batch, tokens, heads, latent_dim, rope_dim, dtype,
-                                                                   _ffi.ctypes.byref(need))
+            status = _ffi.lib().ss_latent_attention_workspace_size(batch, tokens, tq, heads, latent_dim, rope_dim,
+                                                                   dtype, _ffi.ctypes.byref(need))
         _ffi.check(status, "latent attention workspace")
         if len(_WS_BYTES) > 4096:  # many distinct shapes: start over
             _WS_BYTES.clear()
@@ -55,7 +55,7 @@ def _absorbed(who: str, q: torch.Tensor, out: torch.Tensor, latent_cache: torch.
     if latent_cache.stride(3) != 1:
         raise _ffi.KernelError(f"{who}: latent_cache must have a unit last stride")
     rope_dim = q.shape[-1] - latent_dim
-    ws = _workspace(q.device, batch, tokens, heads, latent_dim, rope_dim, dtype)
+    ws = _workspace(q.device, batch, tokens, tq, heads, latent_dim, rope_dim, dtype)
     block_tables = _int32(block_tables)
     ctx = _int32(ctx.reshape(-1))
     cst = latent_cache.stride()
@@ -101,9 +101,9 @@ def latent_attention_decode(
         return out
     require_device("latent_attention_decode", q, latent_cache, block_tables, seq_lens)
     q = unit_last_stride(q)
-    st, so = q.stride(), out.stride()
+    so = out.stride()
     return _absorbed("latent_attention_decode", q, out, latent_cache, block_tables, None, seq_lens, layer_idx, scale,
-                     block_size, latent_dim, batch, batch * tq, tq, heads, (st[0], st[2], st[1]), (so[0], so[1], so[2]))
+                     block_size, latent_dim, batch, batch * tq, tq, heads, _strides(q, (0, 2, 1)), so[:3])
 
 
 def latent_attention_varlen(
@@ -150,9 +150,8 @@ def latent_attention_varlen(
     cu = _int32(cu_seqlens.reshape(-1))
     if _debug():
         _check_stream(cu, total, max_query_len)
-    st, so = q.stride(), out.stride()
     return _absorbed("latent_attention_varlen", q, out, latent_cache, block_tables, cu, context_lens, layer_idx, scale,
-                     block_size, latent_dim, batch, total, max_query_len, heads, (0, st[0], st[1]), (0, so[0], so[1]))
+                     block_size, latent_dim, batch, total, max_query_len, heads, (0, *_strides(q, (0, 1))), (0, *_strides(out, (0, 1))))
 
 
 def latent_attention_expanded(

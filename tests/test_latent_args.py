@@ -134,9 +134,9 @@ def test_c_entries_refuse_before_any_launch():
     assert absorbed(tq=0, q=None) == _ffi.SS_OK and absorbed(cu=FAKE, total=0, q=None) == _ffi.SS_OK
     need = ctypes.c_int64(-1)
     size = lib.ss_latent_attention_workspace_size
-    assert size(1, 1, 16, 512, 64, 1, None) == _ffi.SS_ERR_INVALID
-    assert size(1, 1, 16, 513, 64, 1, ctypes.byref(need)) == _ffi.SS_ERR_UNSUPPORTED
-    assert size(-1, 1, 16, 512, 64, 1, ctypes.byref(need)) == _ffi.SS_ERR_INVALID
+    assert size(1, 1, 1, 16, 512, 64, 1, None) == _ffi.SS_ERR_INVALID
+    assert size(1, 1, 1, 16, 513, 64, 1, ctypes.byref(need)) == _ffi.SS_ERR_UNSUPPORTED
+    assert size(-1, 1, 1, 16, 512, 64, 1, ctypes.byref(need)) == _ffi.SS_ERR_INVALID
 
     def expanded(batch=1, total=1, keys=1, heads=2, n=128, d=64, v=128, dtype=1, kv=FAKE, rope=FAKE):
         return lib.ss_latent_attention_expanded(FAKE, FAKE, kv, rope, FAKE, FAKE, batch, total, keys, 1, heads, n, d, v, two,
