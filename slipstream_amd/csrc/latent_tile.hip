@@ -34,6 +34,7 @@ namespace ss {
 namespace {
 
 constexpr int kRopeDim = 64;
+constexpr int kLeastTiles = 4;
 constexpr float kSlack = 8.f;  // by which (log2) a score may exceed the running maximum before it is raised
 
 typedef short tr16x4 __attribute__((ext_vector_type(4)));
@@ -54,6 +55,21 @@ struct LatTile {
   static_assert(LDS <= 160 * 1024, "one workgroup a CU");
 };
 
+// The same for 128 rows, four waves (one a SIMD, with all its registers) of 32 rows and R / 4 values
+template <int R_>
+struct LatWide {
+  static constexpr int R = R_, NW = 4, ROWS = 128;
+  static constexpr int KT = 32;
+  static constexpr int ROWB = 2 * R, LPLANE = KT * ROWB, RPLANE = KT * 2 * kRopeDim;
+  static constexpr int NS = 4, NR = 3;
+  static constexpr int DT = R / 128;      // 32-value output tiles of a wave
+  static constexpr int PB = 4 * 2048;     // bytes of a tile's P
+  static constexpr int RPI = 1024 / ROWB, NL = KT / RPI / NW;
+  static constexpr int kP = NS * LPLANE + NR * RPLANE, kAlpha = kP + 2 * PB, kMl = kAlpha + 2 * ROWS * 4,
+                       kGrew = kMl + ROWS * 8, kScan = kGrew + 64, LDS = kScan + 128;
+  static_assert(LDS <= 160 * 1024, "one workgroup a CU");
+};
+
 __device__ __forceinline__ int lat_swizzle(int r) { return (r & 3) | ((r & 4) << 1) | ((r & 8) >> 1); }
 
 // The latents' chunk of 8 values that output tile dt of wave w takes for lanes of row group g: bit 2 from
@@ -68,16 +84,18 @@ __device__ __forceinline__ int out_chunk(int dt, int gh, int w) {
     return dt + 2 * (w & 1) + 4 * gh + 8 * (w >> 1);
 }
 
-// 16 bytes a lane straight into LDS at lds + 16 lane, zeros past the descriptor's end. As asm, so that
-// the compiler's waits do not count it; the wait states are those of a descriptor that a VALU
-// instruction wrote.
-__device__ __forceinline__ void lat_dma(i32x4 rs, LdsBytes lds, int voff) {
-  const uint32_t m0 = (uint32_t)(uintptr_t)lds;
-  asm volatile("s_nop 4\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" : : "v"(voff), "s"(rs), "{m0}"(m0) : "memory");
-}
 template <int N>
 __device__ __forceinline__ void lat_wait() {
   asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory");
+}
+
+template <typename F, int... I>
+__device__ __forceinline__ void static_for_impl(F&& f, std::integer_sequence<int, I...>) {
+  (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, typename F>
+__device__ __forceinline__ void static_for(F&& f) {
+  static_for_impl(f, std::make_integer_sequence<int, N>{});
 }
 
 // ---- items ----------------------------------------------------------------------------------
@@ -152,6 +170,78 @@ struct LatentWork {
   int lo, hi;  // the launch's sequences: lo < n heads <= hi
 };
 
+// ---- a wave's part of the tiles' way into the LDS ------------------------------------------------
+//
+// 32 / NW keys' latents, and waves 0 .. 3 eight rotated keys, of one page each (pages hold eight tokens at
+// least): one descriptor a tile, which ends with the keys that are there; behind its end, for absent
+// pages and for tiles past the last one the DMA writes zeros without an access. The page table is
+// read 64 tiles at a time, an entry a lane.
+template <typename C>
+struct Feed {
+  const LatentParams& p;
+  const int32_t* table;
+  uint32_t lds;
+  int shift, kv_end, tend, key8, tok_bytes, base, at8;  // at8: the wave's first of the eight keys
+  int entries;                                          // of tile base + lane
+  int l16, first;
+  int voff_r;
+  i32x4 rsrc;
+  uint32_t to_l, to_r;
+
+  __device__ __forceinline__ Feed(const LatentParams& params, int b, char* mem, int kv_end_, int t0, int tend_)
+      : p(params), kv_end(kv_end_), tend(tend_) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    table = p.bt + (int64_t)b * p.bt_stride;
+    lds = (uint32_t)(uintptr_t)(LdsBytes)mem;
+    shift = __builtin_ctz((unsigned)p.block_size);
+    key8 = 8 * (wave & 3);
+    at8 = C::NW == 8 ? 4 * (wave >> 2) : 0;
+    tok_bytes = (int)(p.kv_s1 * 2);
+    const int hi = lane / (C::R / 8);  // 0 where an instruction brings one latent
+    l16 = 16 * ((lane & (C::R / 8 - 1)) ^ lat_swizzle(key8 + at8) ^ hi);
+    first = (at8 + hi) * tok_bytes;
+    voff_r = (lane >> 3) * tok_bytes + C::ROWB + 16 * ((lane & 7) ^ tile_swizzle(key8 + (lane >> 3)));
+    load(t0);
+  }
+  __device__ __forceinline__ void load(int t) {
+    base = t;
+    const int i = (int)min(((int64_t)(t + (int)(threadIdx.x & 63)) * 32 + key8) >> shift, (int64_t)p.max_blocks - 1);
+    entries = table[i];
+    asm volatile("" : "+v"(entries));  // waited for here, not where every tile's entry is read
+  }
+  // tile t into ring slots ls and rs; ready for dma
+  __device__ __forceinline__ void aim(int t, int ls, int rs) {
+    if (t - base >= 64) load(t);
+    const int e = __builtin_amdgcn_readlane(entries, t - base);
+    const int key = t * 32 + key8, live = min(8, kv_end - key);
+    const bool there = (uint32_t)e < (uint32_t)p.num_blocks && live > 0 && t < tend;
+    const uint64_t off = 2 * (uint64_t)p.kv_s0 * (uint32_t)e + (uint32_t)((key & (p.block_size - 1)) * tok_bytes);
+    const uint64_t at = (uint64_t)p.kv + (there ? off : 0);
+    rsrc = i32x4{__builtin_amdgcn_readfirstlane((int)(uint32_t)at),
+                 __builtin_amdgcn_readfirstlane((int)(uint32_t)(at >> 32) & 0xFFFF),
+                 __builtin_amdgcn_readfirstlane(there ? (live - 1) * tok_bytes + C::ROWB + 2 * kRopeDim : 0), 0x00020000};
+    to_l = lds + ls * C::LPLANE + (key8 + at8) * C::ROWB;
+    to_r = lds + C::NS * C::LPLANE + rs * C::RPLANE + key8 * 2 * kRopeDim;
+    asm volatile("s_nop 4" : : "s"(rsrc));  // SGPRs that a VALU wrote: five wait states before a VMEM reads them
+  }
+  // instruction u of C::NL (latents), and C::NL (rotated keys; waves 0 .. 3 alone)
+  template <int u>
+  __device__ __forceinline__ void dma() const {
+    if constexpr (u < C::NL) {
+      constexpr int k = u * C::RPI, sw = 16 * ((k & 3) | ((k & 4) << 1));
+      int at = l16;
+      asm volatile("" : "+v"(at));  // made anew each time: the offsets would take registers that the queries need
+      dma_b128(rsrc, (LdsBytes)(uintptr_t)(to_l + k * C::ROWB), (at ^ sw) + (first + k * tok_bytes), 0);
+    } else {
+      dma_b128(rsrc, (LdsBytes)(uintptr_t)to_r, voff_r, 0);
+    }
+  }
+  __device__ __forceinline__ void all() const {
+    static_for<C::NL>([&](auto u) __attribute__((always_inline)) { dma<decltype(u)::value>(); });
+    if (C::NW == 4 || threadIdx.x < 256) dma<C::NL>();
+  }
+};
+
 template <typename T, typename C>
 __device__ __forceinline__ void latent_segment(const LatentParams& p, const LatentWork& work, char* const lds,
                                                const SeqView v, const int b, const int tok0, const int head0,
@@ -173,6 +263,11 @@ __device__ __forceinline__ void latent_segment(const LatentParams& p, const Late
     return j < tokens;
   };
   const bool scores = wave < RT;
+  Feed<C> feed(p, b, lds, kv_end, t0, tend);
+  for (int i = 0; i < 3; ++i) {
+    feed.aim(t0 + i, i, i);
+    feed.all();
+  }
   // queries: scaled inside the exponent, which needs a positive scale (a negative one is the query's sign)
   u32x4 qop[KS + KR];
   int lim = 0x7FFFFFFF;
@@ -192,43 +287,12 @@ __device__ __forceinline__ void latent_segment(const LatentParams& p, const Late
   for (int o = 1; o < 16; o <<= 1) least = min(least, __shfl_xor(least, o));
   least = __builtin_amdgcn_readfirstlane(least);
 
-  const int32_t* const table = p.bt + (int64_t)b * p.bt_stride;
-  const ConstInts stable = (ConstInts)table;
-  const int shift = __builtin_ctz((unsigned)p.block_size);
+  // absent pages among this item's: its tiles are masked key by key then
   bool bad = false;
-  for (int i = ((t0 * 32) >> shift) + threadIdx.x; (int64_t)i << shift < min(kv_end, tend * 32); i += 64 * NW) {
-    const int e = table[i];
-    bad |= e < 0 || e >= p.num_blocks;
-  }
+  for (int i = ((t0 * 32) >> feed.shift) + threadIdx.x; (int64_t)i << feed.shift < min(kv_end, tend * 32); i += 64 * NW)
+    bad |= (uint32_t)feed.table[i] >= (uint32_t)p.num_blocks;
   const bool holes = __syncthreads_or(bad);
 
-  // DMA of tile t: this wave brings the latents of 32 / NW keys, and waves 0 .. 3 the rotated keys of eight
-  // (in the same page as its latents)
-  const int key8 = 8 * (wave & 3), key_l = NW == 8 ? 4 * (wave >> 2) : 0;  // first key of the eight; latents from there
-  const int tok_bytes = (int)(p.kv_s1 * 2);
-  int voff_l[C::NL], voff_r;
-#pragma unroll
-  for (int u = 0; u < C::NL; ++u) {
-    const int k = key_l + u * C::RPI + lane * 16 / C::ROWB;  // of the eight
-    voff_l[u] = k * tok_bytes + 16 * ((lane & (R / 8 - 1)) ^ lat_swizzle(key8 + k));
-  }
-  voff_r = (lane >> 3) * tok_bytes + C::ROWB + 16 * ((lane & 7) ^ tile_swizzle(key8 + (lane >> 3)));
-  auto entry = [&](int t) { return stable[max(0, min((t * 32 + key8) >> shift, p.max_blocks - 1))]; };
-  auto issue = [&](int t, int e, int ls, int rs) {
-    const int key = t * 32 + key8, live = min(8, kv_end - key);
-    const bool there = e >= 0 && e < p.num_blocks && live > 0 && t < tend;
-    const int64_t off = there ? (int64_t)e * p.kv_s0 + (int64_t)(key & (p.block_size - 1)) * p.kv_s1 : 0;
-    const uint64_t at = (uint64_t)p.kv + 2 * off;
-    const i32x4 rsrc = {__builtin_amdgcn_readfirstlane((int)(uint32_t)at),
-                        __builtin_amdgcn_readfirstlane((int)(uint32_t)(at >> 32) & 0xFFFF),
-                        __builtin_amdgcn_readfirstlane(there ? (live - 1) * tok_bytes + C::ROWB + 2 * kRopeDim : 0),
-                        0x00020000};
-    const LdsBytes base = (LdsBytes)lds;
-#pragma unroll
-    for (int u = 0; u < C::NL; ++u)
-      lat_dma(rsrc, base + ls * C::LPLANE + (key8 + key_l + u * C::RPI) * C::ROWB, voff_l[u]);
-    if (wave < 4) lat_dma(rsrc, base + C::NS * C::LPLANE + rs * C::RPLANE + key8 * 2 * kRopeDim, voff_r);
-  };
   auto landed = [&](auto tiles) {  // all but the youngest `tiles` tiles
     if (wave < 4)
       lat_wait<decltype(tiles)::value*(C::NL + 1)>();
@@ -270,8 +334,7 @@ __device__ __forceinline__ void latent_segment(const LatentParams& p, const Late
         const int key = t * 32 + 16 * x + 4 * g;  // four keys of one page
         bool there = true;
         if (holes && key < kv_end) {
-          const int e = table[key >> shift];
-          there = e >= 0 && e < p.num_blocks;
+          there = (uint32_t)feed.table[key >> feed.shift] < (uint32_t)p.num_blocks;
         }
 #pragma unroll
         for (int e = 0; e < 4; ++e)
@@ -286,10 +349,6 @@ __device__ __forceinline__ void latent_segment(const LatentParams& p, const Late
     float pv[8], sum = 0.f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) pv[i] = fast_exp2(fmaf(sv[i], cscale, -mn));
-    if (cscale == 0.f) {  // (a masked key's is then not a number)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) pv[i] = sv[i] == -__builtin_inff() ? 0.f : pv[i];
-    }
 #pragma unroll
     for (int i = 0; i < 8; ++i) sum += pv[i];
     const float alpha = fast_exp2(m - mn);
@@ -333,10 +392,6 @@ __device__ __forceinline__ void latent_segment(const LatentParams& p, const Late
   };
 
   if (t0 < tend) {
-    int e3 = entry(t0 + 3);
-    issue(t0, entry(t0), 0, 0);
-    issue(t0 + 1, entry(t0 + 1), 1, 1);
-    issue(t0 + 2, entry(t0 + 2), 2, 2);
     landed(std::integral_constant<int, 2>{});
     __syncthreads();
     if (scores) score(t0, 0, 0, 0);
@@ -344,16 +399,16 @@ __device__ __forceinline__ void latent_segment(const LatentParams& p, const Late
     for (int t = t0; t < tend; ++t) {
       landed(std::integral_constant<int, 1>{});
       __syncthreads();  // tile t + 1 is there, P of tile t too, and tile t - 1's slots are free
-      issue(t + 3, e3, (ls + 3) & 3, rs);
-      e3 = entry(t + 4);
+      feed.aim(t + 3, (ls + 3) & 3, rs);
+      feed.all();
       const int rn = rs == 2 ? 0 : rs + 1;
       if (scores && t + 1 < tend) score(t + 1, (ls + 1) & 3, rn, (t + 1 - t0) & 1);
       output(ls, (t - t0) & 1);
       ls = (ls + 1) & 3;
       rs = rn;
     }
-    lat_wait<0>();
   }
+  lat_wait<0>();
 
   // ---- the rows' sums, then the rows themselves
   if (scores) {
@@ -389,10 +444,349 @@ __device__ __forceinline__ void latent_segment(const LatentParams& p, const Late
   __syncthreads();  // the LDS is free for the next item
 }
 
+// ---- 128 rows: 32 x 32 products --------------------------------------------------------------
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+// acc += a b, the accumulator in AGPRs. As asm, because the compiler moves accumulators between the register
+// files when it needs more than half of the registers. What it therefore does not look after: the
+// operands come from LDS reads, which it does wait for; an accumulator is touched again sixteen products
+// later; and what reads the accumulators waits first (settled).
+template <typename T>
+__device__ __forceinline__ void mfma32_acc(f32x16& acc, u32x4 a, u32x4 b) {
+  if constexpr (std::is_same<T, bf16_t>::value)
+    asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+a"(acc) : "v"(a), "v"(b));
+  else
+    asm volatile("v_mfma_f32_32x32x16_f16 %0, %1, %2, %0" : "+a"(acc) : "v"(a), "v"(b));
+}
+// s = a b (FIRST) or s += a b, chained; reading s is for the caller to wait for
+template <typename T, bool FIRST>
+__device__ __forceinline__ void mfma32_sum(f32x16& s, u32x4 a, u32x4 b) {
+  if constexpr (std::is_same<T, bf16_t>::value) {
+    if constexpr (FIRST)
+      asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, 0" : "=&v"(s) : "v"(a), "v"(b));
+    else
+      asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+v"(s) : "v"(a), "v"(b));
+  } else {
+    if constexpr (FIRST)
+      asm volatile("v_mfma_f32_32x32x16_f16 %0, %1, %2, 0" : "=&v"(s) : "v"(a), "v"(b));
+    else
+      asm volatile("v_mfma_f32_32x32x16_f16 %0, %1, %2, %0" : "+v"(s) : "v"(a), "v"(b));
+  }
+}
+template <typename T>
+__device__ __forceinline__ void clear_acc(f32x16& acc) {  // a product of zeros: no other registers take part
+  const u32x4 z = {0, 0, 0, 0};
+  if constexpr (std::is_same<T, bf16_t>::value)
+    asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %1, 0" : "=a"(acc) : "v"(z));
+  else
+    asm volatile("v_mfma_f32_32x32x16_f16 %0, %1, %1, 0" : "=a"(acc) : "v"(z));
+}
+template <int N>
+__device__ __forceinline__ void settled(f32x16 (&acc)[4][N]) {
+  asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
+#pragma unroll
+  for (int rt = 0; rt < 4; ++rt)
+#pragma unroll
+    for (int dt = 0; dt < N; ++dt) asm volatile("" : "+a"(acc[rt][dt]));
+}
+
+typedef __attribute__((address_space(3))) const u32x4* LdsWords;
+
+// A wave takes 32 rows' scores against all 32 keys (as S^T: lane l row l % 32, its result r key 8 (r / 4) +
+// 4 (l / 32) + r % 4) and all 128 rows' outputs of R / 4 values. Four waves: with 32 rows each a key is
+// read from the LDS four times for the scores instead of eight, which bound the kernel.
+template <typename T, typename C>
+__device__ __forceinline__ void latent_segment_wide(const LatentParams& p, const LatentWork& work, char* const lds,
+                                                    const SeqView v, const int b, const int tok0, const int head0,
+                                                    const int js, const int t0, const int t1, const bool whole,
+                                                    const int slot) {
+  constexpr int R = C::R, DT = C::DT, KS = R / 16, KR = kRopeDim / 16;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n = lane & 31, h = lane >> 5;
+  const int heads = min(p.heads - head0, C::ROWS);
+  const int tokens = min(1 << js, v.n - tok0);
+  const int kv_end = max(0, min(v.keys, v.length - v.n + tok0 + tokens));
+  const int tend = min(t1, (kv_end + 31) >> 5);
+  auto row_of = [&](int rt, int& tok, int& head) {
+    const int rr = 32 * rt + n, j = rr / heads;
+    tok = tok0 + j;
+    head = head0 + rr - j * heads;
+    return j < tokens;
+  };
+
+  Feed<C> feed(p, b, lds, kv_end, t0, tend);  // begun before anything else is waited for
+  for (int i = 0; i < 3; ++i) {
+    feed.aim(t0 + i, i, i);
+    feed.all();
+  }
+
+  u32x4 qop[KS + KR];
+  int lim = min(kv_end, t1 * 32);  // keys of this lane's row up to here (its part of the item's)
+  {
+    int tok, head;
+    const bool ok = row_of(wave, tok, head);
+    if (ok) lim = min(lim, v.length - v.n + tok + 1);
+    // a lane without a row reads the item's first one and takes zeros
+    const T* const q = (const T*)p.q + (p.cu ? 0 : b * p.q_sb) + (v.start + (ok ? tok : tok0)) * p.q_st +
+                       (ok ? head : head0) * p.q_sh + 8 * h;
+    const uint32_t flip = p.scale_log2 < 0.f ? 0x80008000u : 0u, keep = ok ? ~0u : 0u;
+#pragma unroll
+    for (int s = 0; s < KS + KR; ++s) qop[s] = (load16(q + 16 * s) ^ u32x4{flip, flip, flip, flip}) & u32x4{keep, keep, keep, keep};
+  }
+  const float cscale = fabsf(p.scale_log2);
+  int least = lim;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) least = min(least, __shfl_xor(least, o));
+  least = __builtin_amdgcn_readfirstlane(least);
+  bool bad = false;
+  for (int i = ((t0 * 32) >> feed.shift) + threadIdx.x; (int64_t)i << feed.shift < min(kv_end, tend * 32); i += 256)
+    bad |= (uint32_t)feed.table[i] >= (uint32_t)p.num_blocks;
+  const bool holes = __syncthreads_or(bad);
+
+  f32x16 acc[4][DT];
+#pragma unroll
+  for (int rt = 0; rt < 4; ++rt)
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) clear_acc<T>(acc[rt][dt]);
+  float m = kNegBig, l = 0.f;
+
+  const uint32_t lbase = (uint32_t)(uintptr_t)(LdsBytes)lds;
+  // LDS addresses: the 16-byte chunk's bits 4 .. 7 under the swizzle are the low bits of an address (planes
+  // begin on 512 bytes), so another chunk's address is an exclusive or away
+  const uint32_t kaddr = lbase + n * C::ROWB + 16 * (h ^ lat_swizzle(n));
+  const uint32_t raddr = lbase + C::NS * C::LPLANE + n * 2 * kRopeDim + 16 * (h ^ tile_swizzle(n));
+  const int sl = lane & 15, vrow = 4 * h + (sl >> 2), quad = 2 * ((lane >> 4) & 1) + ((sl & 3) >> 1);
+  const uint32_t vaddr = lbase + vrow * C::ROWB + 8 * (sl & 1) + 16 * ((4 * quad) ^ lat_swizzle(vrow)) +
+                         (DT == 4 ? 256 * wave : 256 * (wave >> 1) + 0);
+  const uint32_t vflip = DT == 4 ? 0 : 32 * (wave & 1);  // the wave's bit of the chunk
+  const uint32_t paddr = lbase + C::kP;
+
+  // a lane's number that the compiler cannot build addresses from ahead of time: they would take registers
+  // that the queries need
+  auto fresh = [&]() {
+    int ln = lane;
+    asm volatile("" : "+v"(ln));
+    return ln;
+  };
+  auto word = [](uint32_t at) { return *(LdsWords)(uintptr_t)at; };
+  auto vread = [&](uint32_t slot, int s, int dt) {  // 16 keys from 16 s on, output tile dt
+    const uint32_t at = (vaddr + slot) ^ (16 * dt) ^ vflip;
+    typedef __attribute__((address_space(3))) tr16x4* Tr;
+    const u32x2 lo = __builtin_bit_cast(
+        u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Tr)(uintptr_t)(at + 16 * s * C::ROWB)));
+    const u32x2 hi = __builtin_bit_cast(
+        u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Tr)(uintptr_t)((at ^ 64) + (16 * s + 8) * C::ROWB)));
+    return u32x4{lo[0], lo[1], hi[0], hi[1]};
+  };
+
+  // One step: the scores of tile t + 1 from ring slots kl, kr, then the outputs of tile t in slot vl with the
+  // probabilities in buffer `buf` (OUT), and between their products the softmax of t + 1, whose
+  // probabilities go into the other buffer (SCORE). One wave a SIMD has nothing to hide behind, so the order
+  // is written out: an operand is read from the LDS a few products ahead of its own.
+  constexpr int NQ = KS + KR, AHEAD = 4, P = 8 * DT;  // products of the scores and of the outputs
+  u32x4 kring[AHEAD];
+  uint32_t ka = 0, ra = 0;
+  auto kread = [&](auto sc) __attribute__((always_inline)) {
+    constexpr int s = sc;
+    if constexpr (s < KS)
+      kring[s % AHEAD] = word((ka ^ (32 * (s & 7))) + 256 * (s >> 3));
+    else if constexpr (s < NQ)
+      kring[s % AHEAD] = word(ra ^ (32 * (s - KS)));
+  };
+  auto begin = [&](int kl, int kr) __attribute__((always_inline)) {
+    ka = kaddr + kl * C::LPLANE;
+    ra = raddr + kr * C::RPLANE;
+    static_for<AHEAD>(kread);
+  };
+  auto step = [&](auto outc, int t, int vl, int vr, int buf) __attribute__((always_inline)) {
+    constexpr bool OUT = decltype(outc)::value;
+    f32x16 s16;
+    u32x4 cv[DT], pr[2];
+    const uint32_t vslot = vl * C::LPLANE, pa = paddr + buf * C::PB + fresh() * 16;
+    __builtin_amdgcn_sched_barrier(0);
+    static_for<NQ>([&](auto sc) __attribute__((always_inline)) {
+      constexpr int s = sc;
+      mfma32_sum<T, s == 0>(s16, kring[s % AHEAD], qop[s]);
+      kread(std::integral_constant<int, s + AHEAD>{});
+      if constexpr (OUT && s == 1) feed.aim(t + 3, (vl + 3) & 3, vr);
+      if constexpr (OUT && s >= 3 && s % 2 == 1 && (s - 3) / 2 <= C::NL) feed.template dma<(s - 3) / 2>();
+      if constexpr (OUT) {
+        constexpr int u = s - (NQ - DT - 1);  // the first outputs' operands behind the last scores'
+        if constexpr (u >= 0 && u < DT) cv[u] = vread(vslot, 0, u);
+        if constexpr (u == DT) pr[0] = word(pa);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    });
+    if (holes || t * 32 + 64 > least) {
+      asm volatile("s_nop 15\n\ts_nop 7" : "+v"(s16));  // the last product is through
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const int key = (t + 1) * 32 + 8 * x + 4 * h;  // four keys of one page
+        bool there = true;
+        if (holes && key < kv_end) {
+          there = (uint32_t)feed.table[key >> feed.shift] < (uint32_t)p.num_blocks;
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (!there || key + e >= lim) s16[4 * x + e] = -__builtin_inff();
+      }
+    }
+    float top = 0.f, mn = 0.f, sum = 0.f;
+    bool grew = false;
+    uint32_t pk[8];
+    // the softmax in 19 parts of a few instructions
+    auto part = [&](auto ic) __attribute__((always_inline)) {
+      constexpr int i = ic;
+      if constexpr (i == 0) {
+        asm volatile("s_nop 15\n\ts_nop 7" : "+v"(s16));  // the last score's product is through
+        top = fmaxf(fmaxf(fmaxf(s16[0], s16[1]), fmaxf(s16[2], s16[3])), fmaxf(fmaxf(s16[4], s16[5]), fmaxf(s16[6], s16[7])));
+      } else if constexpr (i == 1) {
+        top = fmaxf(top, fmaxf(fmaxf(fmaxf(s16[8], s16[9]), fmaxf(s16[10], s16[11])),
+                               fmaxf(fmaxf(s16[12], s16[13]), fmaxf(s16[14], s16[15]))));
+      } else if constexpr (i == 2) {
+        const uint32_t tb = __builtin_bit_cast(uint32_t, top);
+        auto sw = __builtin_amdgcn_permlane32_swap(tb, tb, false, false);
+        top = fmaxf(__builtin_bit_cast(float, (uint32_t)sw[0]), __builtin_bit_cast(float, (uint32_t)sw[1]));
+        top = fmaxf(m, top * cscale);
+        grew = __any(top > m + kSlack);
+      } else if constexpr (i == 3) {
+        mn = grew ? top : m;
+      } else if constexpr (i < 12) {
+        constexpr int e = 2 * (i - 4);
+        const float a = s16[e], c = s16[e + 1];
+        s16[e] = fast_exp2(fmaf(a, cscale, -mn));
+        s16[e + 1] = fast_exp2(fmaf(c, cscale, -mn));
+      } else if constexpr (i < 16) {
+        constexpr int e = 4 * (i - 12);
+        sum += (s16[e] + s16[e + 1]) + (s16[e + 2] + s16[e + 3]);
+        pk[e / 2] = Elem<T>::pack2(s16[e], s16[e + 1]);
+        pk[e / 2 + 1] = Elem<T>::pack2(s16[e + 2], s16[e + 3]);
+      } else if constexpr (i == 16) {
+        const float alpha = fast_exp2(m - mn);
+        l = fmaf(l, alpha, sum);
+        m = mn;
+        const int ln = fresh();
+        if (ln < 32) *reinterpret_cast<float*>(lds + C::kAlpha + ((buf ^ 1) * C::ROWS + 32 * wave + ln) * 4) = alpha;
+        if (ln == 0) *reinterpret_cast<int*>(lds + C::kGrew + ((buf ^ 1) * 4 + wave) * 4) = grew;
+      } else if constexpr (i < 19) {
+        constexpr int q = i - 17;
+        store16(lds + C::kP + (buf ^ 1) * C::PB + (2 * wave + q) * 1024 + fresh() * 16,
+                u32x4{pk[4 * q], pk[4 * q + 1], pk[4 * q + 2], pk[4 * q + 3]});
+      }
+    };
+    if constexpr (!OUT) {
+      static_for<19>(part);
+    } else {
+      __builtin_amdgcn_sched_barrier(0);
+      static_for<P>([&](auto ic) __attribute__((always_inline)) {
+        constexpr int i = ic, q = i / (4 * DT), rt = i / DT % 4, dt = i % DT, g = i / DT;  // g: group of DT products
+        if constexpr (dt == 0 && g + 1 < 8) pr[(g + 1) & 1] = word(pa + (2 * ((g + 1) & 3) + ((g + 1) >> 2)) * 1024);
+        mfma32_acc<T>(acc[rt][dt], cv[dt], pr[g & 1]);
+        if constexpr (q == 0 && rt == 3) cv[dt] = vread(vslot, 1, dt);  // its last product of these 16 keys
+        // from the third product on, in as many places as there are
+        constexpr int from = i < 2 ? 0 : (i - 2) * 19 / (P - 3), to = i < 2 ? 0 : (i - 1) * 19 / (P - 3);
+        static_for<(to < 19 ? to : 19) - (from < 19 ? from : 19)>(
+            [&](auto jc) __attribute__((always_inline)) { part(std::integral_constant<int, from + jc>{}); });
+        __builtin_amdgcn_sched_barrier(0);
+      });
+    }
+  };
+  auto shrink = [&](int buf) {
+    if (__any(*reinterpret_cast<const int*>(lds + C::kGrew + (buf * 4 + (fresh() & 3)) * 4))) {
+      settled(acc);
+#pragma unroll
+      for (int rt = 0; rt < 4; ++rt) {
+        const float alpha = *reinterpret_cast<const float*>(lds + C::kAlpha + (buf * C::ROWS + 32 * rt + (fresh() & 31)) * 4);
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+          acc[rt][dt] *= alpha;
+          asm volatile("" : "+a"(acc[rt][dt]));
+        }
+      }
+      asm volatile("s_nop 4" ::: "memory");
+    }
+  };
+
+  if (t0 < tend) {
+    lat_wait<2 * (C::NL + 1)>();
+    __syncthreads();
+    begin(0, 0);
+    step(std::false_type{}, t0 - 1, 0, 0, 1);
+    int ls = 0, rs = 0;
+    for (int t = t0; t < tend; ++t) {
+      lat_wait<C::NL + 1>();
+      __syncthreads();
+      const int buf = (t - t0) & 1, rn = rs == 2 ? 0 : rs + 1;
+      begin((ls + 1) & 3, rn);
+      shrink(buf);
+      // (the last step's scores are those of a tile of zeros behind every row's keys)
+      step(std::true_type{}, t, ls, rs, buf);
+      ls = (ls + 1) & 3;
+      rs = rn;
+    }
+  }
+  lat_wait<0>();
+  settled(acc);
+
+  {
+    const uint32_t u = __builtin_bit_cast(uint32_t, l);
+    auto sw = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    const float sum = __builtin_bit_cast(float, (uint32_t)sw[0]) + __builtin_bit_cast(float, (uint32_t)sw[1]);
+    if (h == 0) *reinterpret_cast<float2*>(lds + C::kMl + (32 * wave + n) * 8) = float2{m, sum};
+  }
+  __syncthreads();
+  // result r of output tile dt: value 8 chunk + 4 h + r % 4 of row n
+  auto chunk = [&](int dt, int x) {
+    return DT == 4 ? dt + 4 * x + 16 * wave : dt + 2 * (wave & 1) + 4 * x + 16 * (wave >> 1);
+  };
+  if (whole) {
+#pragma unroll
+    for (int rt = 0; rt < 4; ++rt) {
+      int tok, head;
+      const bool ok = row_of(rt, tok, head);
+      const float total = reinterpret_cast<const float2*>(lds + C::kMl + (32 * rt + n) * 8)->y;
+      const float inv = total == 0.f ? 0.f : 1.f / total;
+      T* const o = (T*)p.out + (p.cu ? 0 : b * p.o_sb) + (v.start + tok) * p.o_st + head * p.o_sh;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int x = 0; x < 4; x += 2) {
+          // the halves of chunks x and x + 1 change places so that a lane holds one whole
+          uint32_t w[2][2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const uint32_t even = Elem<T>::pack2(acc[rt][dt][4 * x + 2 * e] * inv, acc[rt][dt][4 * x + 2 * e + 1] * inv);
+            const uint32_t odd = Elem<T>::pack2(acc[rt][dt][4 * x + 4 + 2 * e] * inv, acc[rt][dt][4 * x + 5 + 2 * e] * inv);
+            auto sw = __builtin_amdgcn_permlane32_swap(even, odd, false, false);
+            w[e][0] = sw[0], w[e][1] = sw[1];
+          }
+          if (ok) {
+            const u32x4 y = {w[0][0], w[1][0], w[0][1], w[1][1]};
+            __builtin_memcpy(o + 8 * chunk(dt, x + h), &y, 16);
+          }
+        }
+    }
+  } else {
+    float* const o = work.o + (int64_t)slot * C::ROWS * R + 4 * h;
+#pragma unroll
+    for (int rt = 0; rt < 4; ++rt)
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+          *reinterpret_cast<f32x4*>(o + (32 * rt + n) * R + 8 * chunk(dt, x)) =
+              f32x4{acc[rt][dt][4 * x], acc[rt][dt][4 * x + 1], acc[rt][dt][4 * x + 2], acc[rt][dt][4 * x + 3]};
+    float* const ml = work.ml + (int64_t)slot * C::ROWS * 2;
+    ml[threadIdx.x] = *reinterpret_cast<const float*>(lds + C::kMl + 4 * threadIdx.x);
+  }
+  __syncthreads();
+}
+
 extern __shared__ __attribute__((aligned(1024))) char s_lat[];
 
 template <typename T, typename C>
-__global__ __launch_bounds__(64 * C::NW) void latent_tile_kernel(const LatentParams p, const LatentWork work) {
+__global__ __launch_bounds__(64 * C::NW) __attribute__((amdgpu_waves_per_eu(C::NW / 4, C::NW / 4))) void latent_tile_kernel(const LatentParams p, const LatentWork work) {
   constexpr int NT = 64 * C::NW;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const RowShape shape = row_shape<C::ROWS>(p.heads);
@@ -424,7 +818,8 @@ __global__ __launch_bounds__(64 * C::NW) void latent_tile_kernel(const LatentPar
     for (int i = 0; i < C::NW; ++i) total += s_sum[i];
   }
   total = uniform(total);
-  const int groups = (int)min((int64_t)all, total);
+  // as many ranges as there are workgroups, so long as they have kLeastTiles tiles or a sequence each
+  const int groups = (int)min((int64_t)all, max(total / kLeastTiles, min(total, (int64_t)p.batch)));
   int* const rec = work.rec + 4 * w;
   if (w >= groups) {
     if (threadIdx.x == 0) rec[0] = -1;
@@ -477,8 +872,12 @@ __global__ __launch_bounds__(64 * C::NW) void latent_tile_kernel(const LatentPar
           rec[1] = i * shape.hs + h;
           rec[2] = to;
         }
-        latent_segment<T, C>(p, work, s_lat, v, b, i << shape.js, h * C::ROWS, shape.js, t0, t1,
-                             t0 == 0 && t1 == each, 2 * w + (t0 == 0));
+        if constexpr (std::is_same<C, LatWide<C::R>>::value)
+          latent_segment_wide<T, C>(p, work, s_lat, v, b, i << shape.js, h * C::ROWS, shape.js, t0, t1,
+                                    t0 == 0 && t1 == each, 2 * w + (t0 == 0));
+        else
+          latent_segment<T, C>(p, work, s_lat, v, b, i << shape.js, h * C::ROWS, shape.js, t0, t1,
+                               t0 == 0 && t1 == each, 2 * w + (t0 == 0));
         u = e;
       }
     }
@@ -486,8 +885,9 @@ __global__ __launch_bounds__(64 * C::NW) void latent_tile_kernel(const LatentPar
   }
 }
 
-// The partial rows of an item that is cut, added in the order of its ranges: workgroup (w, part) 16 rows of
-// the item whose first cut is the begin of range w.
+// The partial rows of an item that is cut, added in the order of its ranges: a wave one row of the item
+// whose first cut is the begin of range w. The parts' maxima and sums are read 64 at a time, a part a
+// lane; then the rows, eight parts' on their way at once.
 template <typename T, int R, int ROWS>
 __global__ __launch_bounds__(256) void latent_merge_kernel(const LatentParams p, const LatentWork work) {
   const int w = blockIdx.x;
@@ -495,41 +895,54 @@ __global__ __launch_bounds__(256) void latent_merge_kernel(const LatentParams p,
   const int b = rec[0];
   if (b < 0) return;
   const RowShape shape = row_shape<ROWS>(p.heads);
-  const int item = rec[1], last = rec[2];
+  const int item = rec[1], parts = rec[2] - w + 2;  // ranges w - 1 .. rec[2]
   const SeqView v = seq_view(p, b, work.lo, work.hi);
   const int tok0 = item / shape.hs << shape.js, head0 = item % shape.hs * ROWS;
   const int heads = min(p.heads - head0, ROWS), tokens = min(1 << shape.js, v.n - tok0);
+  const int rr = __builtin_amdgcn_readfirstlane(4 * blockIdx.y + (threadIdx.x >> 6)), j = rr / heads;
+  if (j >= tokens) return;
   constexpr int PER = R / 64;  // values of a lane
   const int lane = threadIdx.x & 63;
-#pragma unroll 1
-  for (int k = 0; k < 4; ++k) {
-    const int rr = 16 * blockIdx.y + 4 * (threadIdx.x >> 6) + k, j = rr / heads;
-    if (j >= tokens) continue;
-    float top = kNegBig;
-    for (int i = w - 1; i <= last; ++i) {
-      const int slot = i == w - 1 ? 2 * i + 1 : 2 * i;
-      top = fmaxf(top, work.ml[((int64_t)slot * ROWS + rr) * 2]);
-    }
-    float sum = 0.f, o[PER] = {};
-    for (int i = w - 1; i <= last; ++i) {
-      const int64_t row = (int64_t)(i == w - 1 ? 2 * i + 1 : 2 * i) * ROWS + rr;
-      const float2 ml = *reinterpret_cast<const float2*>(work.ml + 2 * row);
-      const float f = fast_exp2(ml.x - top);
-      sum = fmaf(ml.y, f, sum);
+  auto row = [&](int i) { return (int64_t)(i == 0 ? 2 * w - 1 : 2 * (w - 1 + i)) * ROWS + rr; };
+  float top = kNegBig, sum = 0.f, o[PER] = {};
+  for (int i0 = 0; i0 < parts; i0 += 64) {
+    float2 ml = {kNegBig, 0.f};
+    if (i0 + lane < parts) ml = *reinterpret_cast<const float2*>(work.ml + 2 * row(i0 + lane));
+    float most = ml.x;
 #pragma unroll
-      for (int d = 0; d < PER; d += 4) {
-        const f32x4 x = *reinterpret_cast<const f32x4*>(work.o + row * R + d * 64 + 4 * lane);
+    for (int x = 32; x > 0; x >>= 1) most = fmaxf(most, __shfl_xor(most, x));
+    most = fmaxf(most, top);
+    const float before = fast_exp2(top - most), f = fast_exp2(ml.x - most);
+    float add = ml.y * f;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) o[d + q] = fmaf(x[q], f, o[d + q]);
+    for (int x = 32; x > 0; x >>= 1) add += __shfl_xor(add, x);
+    sum = fmaf(sum, before, add);
+    top = most;
+#pragma unroll
+    for (int d = 0; d < PER; ++d) o[d] *= before;
+    const int here = min(64, parts - i0);
+    for (int i = 0; i < here; i += 8) {
+      f32x4 x[8][PER / 4];
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+#pragma unroll
+        for (int d = 0; d < PER / 4; ++d)
+          x[k][d] = *reinterpret_cast<const f32x4*>(work.o + row(i0 + min(i + k, here - 1)) * R + d * 256 + 4 * lane);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        if (i + k >= here) continue;
+        const float fk = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), i + k));
+#pragma unroll
+        for (int d = 0; d < PER; ++d) o[d] = fmaf(x[k][d >> 2][d & 3], fk, o[d]);
       }
     }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    T* const out = (T*)p.out + (p.cu ? 0 : b * p.o_sb) + (v.start + tok0 + j) * p.o_st + (head0 + rr - j * heads) * p.o_sh;
-#pragma unroll
-    for (int d = 0; d < PER; d += 4)
-      *reinterpret_cast<u32x2*>(out + d * 64 + 4 * lane) =
-          u32x2{Elem<T>::pack2(o[d] * inv, o[d + 1] * inv), Elem<T>::pack2(o[d + 2] * inv, o[d + 3] * inv)};
   }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  T* const out = (T*)p.out + (p.cu ? 0 : b * p.o_sb) + (v.start + tok0 + j) * p.o_st + (head0 + rr - j * heads) * p.o_sh;
+#pragma unroll
+  for (int d = 0; d < PER; d += 4)
+    *reinterpret_cast<u32x2*>(out + d * 64 + 4 * lane) =
+        u32x2{Elem<T>::pack2(o[d] * inv, o[d + 1] * inv), Elem<T>::pack2(o[d + 2] * inv, o[d + 3] * inv)};
 }
 
 // ---- host ---------------------------------------------------------------------------------------
@@ -542,9 +955,9 @@ int64_t part_bytes(int rows, int r) {
   return up(groups * 2 * rows * r * 4) + up(groups * 2 * rows * 2 * 4) + up(groups * 4 * 4);
 }
 
-template <typename T, int R, int RT, int NW>
+template <typename T, typename C>
 int launch_rows(const LatentParams& p, int lo, int hi, char* ws, hipStream_t stream) {
-  typedef LatTile<R, RT, NW> C;
+  constexpr int R = C::R, NW = C::NW;
   const int64_t groups = ss_host::device_cu_count();
   LatentWork work;
   work.o = (float*)ws;
@@ -556,16 +969,17 @@ int launch_rows(const LatentParams& p, int lo, int hi, char* ws, hipStream_t str
   if (const int st = reserve_lds((const void*)kern, C::LDS, done); st != SS_OK) return st;
   hipLaunchKernelGGL(kern, dim3((unsigned)groups), dim3(64 * NW), C::LDS, stream, p, work);
   if (const int st = ss_host::launch_status("latent attention"); st != SS_OK) return st;
-  hipLaunchKernelGGL((latent_merge_kernel<T, R, C::ROWS>), dim3((unsigned)groups, RT), dim3(256), 0, stream, p, work);
+  hipLaunchKernelGGL((latent_merge_kernel<T, R, C::ROWS>), dim3((unsigned)groups, C::ROWS / 4), dim3(256), 0, stream, p,
+                     work);
   return ss_host::launch_status("latent attention (merge)");
 }
 
 template <typename T, int R>
 int launch_for(const LatentParams& p, int rows, int lo, int hi, char* ws, hipStream_t stream) {
-  if (rows <= 16) return launch_rows<T, R, 1, 4>(p, lo, hi, ws, stream);
-  if (rows <= 32) return launch_rows<T, R, 2, 4>(p, lo, hi, ws, stream);
-  if (rows <= 64) return launch_rows<T, R, 4, 8>(p, lo, hi, ws, stream);
-  return launch_rows<T, R, 8, 8>(p, lo, hi, ws, stream);
+  if (rows <= 16) return launch_rows<T, LatTile<R, 1, 4>>(p, lo, hi, ws, stream);
+  if (rows <= 32) return launch_rows<T, LatTile<R, 2, 4>>(p, lo, hi, ws, stream);
+  if (rows <= 64) return launch_rows<T, LatTile<R, 4, 8>>(p, lo, hi, ws, stream);
+  return launch_rows<T, LatWide<R>>(p, lo, hi, ws, stream);
 }
 
 // Rows of the launches of a call: of sequences of few rows (0: no such launch), and of the others. Where
@@ -583,13 +997,14 @@ bool latent_tile_takes(const LatentParams& p, int dtype) {
   const bool pow2 = (p.block_size & (p.block_size - 1)) == 0;
   if (dtype != SS_DTYPE_BF16 && dtype != SS_DTYPE_F16) return false;
   if ((p.key_dim != 512 && p.key_dim != 256) || p.rope_dim != kRopeDim || !pow2 || p.block_size < 8) return false;
-  if (p.max_blocks < 1) return false;
+  if (p.max_blocks < 1 || p.scale_log2 == 0.f) return false;  // (masked scores are -inf, times the scale)
   for (int64_t s : {p.q_sb, p.q_st, p.q_sh, p.kv_s0, p.kv_s1})
     if (s % 8) return false;
   for (int64_t s : {p.o_sb, p.o_st, p.o_sh})
     if (s % 4) return false;
   return ((uintptr_t)p.q | (uintptr_t)p.kv) % 16 == 0 && (uintptr_t)p.out % 8 == 0 &&
-         p.kv_s1 >= p.key_dim + p.rope_dim && p.kv_s1 < (1 << 24);
+         p.kv_s1 >= p.key_dim + p.rope_dim && p.block_size * p.kv_s1 < (1 << 29) && p.kv_s0 >= 0 &&
+         p.num_blocks < (1ll << 31);
 }
 
 int64_t latent_tile_bytes(int64_t batch, int64_t total, int tq, int heads, int latent_dim) {
