@@ -474,6 +474,12 @@ __device__ __forceinline__ void mfma32_sum(f32x16& s, u32x4 a, u32x4 b) {
       asm volatile("v_mfma_f32_32x32x16_f16 %0, %1, %2, %0" : "+v"(s) : "v"(a), "v"(b));
   }
 }
+// (without the quieting of NaNs that fmaxf has: a score that is none makes its row one anyway)
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
 template <typename T>
 __device__ __forceinline__ void clear_acc(f32x16& acc) {  // a product of zeros: no other registers take part
   const u32x4 z = {0, 0, 0, 0};
@@ -580,11 +586,17 @@ __device__ __forceinline__ void latent_segment_wide(const LatentParams& p, const
     return u32x4{lo[0], lo[1], hi[0], hi[1]};
   };
 
-  // One step: the scores of tile t + 1 from ring slots kl, kr, then the outputs of tile t in slot vl with the
-  // probabilities in buffer `buf` (OUT), and between their products the softmax of t + 1, whose
-  // probabilities go into the other buffer (SCORE). One wave a SIMD has nothing to hide behind, so the order
-  // is written out: an operand is read from the LDS a few products ahead of its own.
+  // One step: the scores of tile t + 1, then the outputs of tile t (OUT), whose latents are in ring slot vl and
+  // whose probabilities in buffer `buf`, and between their products the softmax of t + 1, whose probabilities
+  // go into the other buffer. One wave a SIMD has nothing to hide behind, so the order is written out: an
+  // operand is read from the LDS a few products ahead of its own, and the two barriers stand where
+  // products go on behind them:
+  //   among the scores: the other waves are done with the step before. Their probabilities can be read, and
+  //     the LDS of tile t - 1 is free: tile t + 3 is sent for.
+  //   among the outputs: tile t + 2 has landed, and its first operands are read.
   constexpr int NQ = KS + KR, AHEAD = 4, P = 8 * DT;  // products of the scores and of the outputs
+  constexpr int kShared = NQ / 3, kLanded = P / 2;    // where the barriers are
+  static_assert(kShared + 3 + 2 * C::NL < NQ || C::NL < 8, "the DMAs fit among the scores");
   u32x4 kring[AHEAD];
   uint32_t ka = 0, ra = 0;
   auto kread = [&](auto sc) __attribute__((always_inline)) {
@@ -594,106 +606,40 @@ __device__ __forceinline__ void latent_segment_wide(const LatentParams& p, const
     else if constexpr (s < NQ)
       kring[s % AHEAD] = word(ra ^ (32 * (s - KS)));
   };
-  auto begin = [&](int kl, int kr) __attribute__((always_inline)) {
+  auto at_keys = [&](int kl, int kr) {  // of the tile in ring slots kl, kr
     ka = kaddr + kl * C::LPLANE;
     ra = raddr + kr * C::RPLANE;
-    static_for<AHEAD>(kread);
   };
   auto step = [&](auto outc, int t, int vl, int vr, int buf) __attribute__((always_inline)) {
     constexpr bool OUT = decltype(outc)::value;
     f32x16 s16;
     u32x4 cv[DT], pr[2];
+    int flags = 0;
     const uint32_t vslot = vl * C::LPLANE, pa = paddr + buf * C::PB + fresh() * 16;
     __builtin_amdgcn_sched_barrier(0);
     static_for<NQ>([&](auto sc) __attribute__((always_inline)) {
       constexpr int s = sc;
       mfma32_sum<T, s == 0>(s16, kring[s % AHEAD], qop[s]);
       kread(std::integral_constant<int, s + AHEAD>{});
-      if constexpr (OUT && s == 1) feed.aim(t + 3, (vl + 3) & 3, vr);
-      if constexpr (OUT && s >= 3 && s % 2 == 1 && (s - 3) / 2 <= C::NL) feed.template dma<(s - 3) / 2>();
       if constexpr (OUT) {
+        if constexpr (s == kShared) {
+          asm volatile("s_waitcnt lgkmcnt(%0)" : : "n"(AHEAD) : "memory");  // all but the scores' operands
+          __builtin_amdgcn_s_barrier();
+          asm volatile("" ::: "memory");
+        }
+        if constexpr (s == kShared + 1) {
+          flags = *reinterpret_cast<const int*>(lds + C::kGrew + (buf * 4 + (fresh() & 3)) * 4);
+          feed.aim(t + 3, (vl + 3) & 3, vr);
+        }
+        constexpr int gap = C::NL < 8 ? 1 : 2, d = s - kShared - 3;
+        if constexpr (d >= 0 && d % gap == 0 && d / gap <= C::NL) feed.template dma<d / gap>();
         constexpr int u = s - (NQ - DT - 1);  // the first outputs' operands behind the last scores'
         if constexpr (u >= 0 && u < DT) cv[u] = vread(vslot, 0, u);
         if constexpr (u == DT) pr[0] = word(pa);
       }
       __builtin_amdgcn_sched_barrier(0);
     });
-    if (holes || t * 32 + 64 > least) {
-      asm volatile("s_nop 15\n\ts_nop 7" : "+v"(s16));  // the last product is through
-#pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        const int key = (t + 1) * 32 + 8 * x + 4 * h;  // four keys of one page
-        bool there = true;
-        if (holes && key < kv_end) {
-          there = (uint32_t)feed.table[key >> feed.shift] < (uint32_t)p.num_blocks;
-        }
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (!there || key + e >= lim) s16[4 * x + e] = -__builtin_inff();
-      }
-    }
-    float top = 0.f, mn = 0.f, sum = 0.f;
-    bool grew = false;
-    uint32_t pk[8];
-    // the softmax in 19 parts of a few instructions
-    auto part = [&](auto ic) __attribute__((always_inline)) {
-      constexpr int i = ic;
-      if constexpr (i == 0) {
-        asm volatile("s_nop 15\n\ts_nop 7" : "+v"(s16));  // the last score's product is through
-        top = fmaxf(fmaxf(fmaxf(s16[0], s16[1]), fmaxf(s16[2], s16[3])), fmaxf(fmaxf(s16[4], s16[5]), fmaxf(s16[6], s16[7])));
-      } else if constexpr (i == 1) {
-        top = fmaxf(top, fmaxf(fmaxf(fmaxf(s16[8], s16[9]), fmaxf(s16[10], s16[11])),
-                               fmaxf(fmaxf(s16[12], s16[13]), fmaxf(s16[14], s16[15]))));
-      } else if constexpr (i == 2) {
-        const uint32_t tb = __builtin_bit_cast(uint32_t, top);
-        auto sw = __builtin_amdgcn_permlane32_swap(tb, tb, false, false);
-        top = fmaxf(__builtin_bit_cast(float, (uint32_t)sw[0]), __builtin_bit_cast(float, (uint32_t)sw[1]));
-        top = fmaxf(m, top * cscale);
-        grew = __any(top > m + kSlack);
-      } else if constexpr (i == 3) {
-        mn = grew ? top : m;
-      } else if constexpr (i < 12) {
-        constexpr int e = 2 * (i - 4);
-        const float a = s16[e], c = s16[e + 1];
-        s16[e] = fast_exp2(fmaf(a, cscale, -mn));
-        s16[e + 1] = fast_exp2(fmaf(c, cscale, -mn));
-      } else if constexpr (i < 16) {
-        constexpr int e = 4 * (i - 12);
-        sum += (s16[e] + s16[e + 1]) + (s16[e + 2] + s16[e + 3]);
-        pk[e / 2] = Elem<T>::pack2(s16[e], s16[e + 1]);
-        pk[e / 2 + 1] = Elem<T>::pack2(s16[e + 2], s16[e + 3]);
-      } else if constexpr (i == 16) {
-        const float alpha = fast_exp2(m - mn);
-        l = fmaf(l, alpha, sum);
-        m = mn;
-        const int ln = fresh();
-        if (ln < 32) *reinterpret_cast<float*>(lds + C::kAlpha + ((buf ^ 1) * C::ROWS + 32 * wave + ln) * 4) = alpha;
-        if (ln == 0) *reinterpret_cast<int*>(lds + C::kGrew + ((buf ^ 1) * 4 + wave) * 4) = grew;
-      } else if constexpr (i < 19) {
-        constexpr int q = i - 17;
-        store16(lds + C::kP + (buf ^ 1) * C::PB + (2 * wave + q) * 1024 + fresh() * 16,
-                u32x4{pk[4 * q], pk[4 * q + 1], pk[4 * q + 2], pk[4 * q + 3]});
-      }
-    };
-    if constexpr (!OUT) {
-      static_for<19>(part);
-    } else {
-      __builtin_amdgcn_sched_barrier(0);
-      static_for<P>([&](auto ic) __attribute__((always_inline)) {
-        constexpr int i = ic, q = i / (4 * DT), rt = i / DT % 4, dt = i % DT, g = i / DT;  // g: group of DT products
-        if constexpr (dt == 0 && g + 1 < 8) pr[(g + 1) & 1] = word(pa + (2 * ((g + 1) & 3) + ((g + 1) >> 2)) * 1024);
-        mfma32_acc<T>(acc[rt][dt], cv[dt], pr[g & 1]);
-        if constexpr (q == 0 && rt == 3) cv[dt] = vread(vslot, 1, dt);  // its last product of these 16 keys
-        // from the third product on, in as many places as there are
-        constexpr int from = i < 2 ? 0 : (i - 2) * 19 / (P - 3), to = i < 2 ? 0 : (i - 1) * 19 / (P - 3);
-        static_for<(to < 19 ? to : 19) - (from < 19 ? from : 19)>(
-            [&](auto jc) __attribute__((always_inline)) { part(std::integral_constant<int, from + jc>{}); });
-        __builtin_amdgcn_sched_barrier(0);
-      });
-    }
-  };
-  auto shrink = [&](int buf) {
-    if (__any(*reinterpret_cast<const int*>(lds + C::kGrew + (buf * 4 + (fresh() & 3)) * 4))) {
+    if (OUT && __any(flags)) {  // some row's maximum grew with tile t
       settled(acc);
 #pragma unroll
       for (int rt = 0; rt < 4; ++rt) {
@@ -706,24 +652,104 @@ __device__ __forceinline__ void latent_segment_wide(const LatentParams& p, const
       }
       asm volatile("s_nop 4" ::: "memory");
     }
+    if (holes || t * 32 + 64 > least) {
+      asm volatile("s_nop 15\n\ts_nop 7" : "+v"(s16));  // the last product is through
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const int key = (t + 1) * 32 + 8 * x + 4 * h;  // four keys of one page
+        bool there = true;
+        if (holes && key < kv_end) there = (uint32_t)feed.table[key >> feed.shift] < (uint32_t)p.num_blocks;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (!there || key + e >= lim) s16[4 * x + e] = -__builtin_inff();
+      }
+    }
+    float top = 0.f, mn = 0.f, sum = 0.f;
+    bool grew = false;
+    uint32_t pk[8];
+    // the softmax in parts of a few instructions
+    constexpr int kParts = 19;
+    auto part = [&](auto ic) __attribute__((always_inline)) {
+      constexpr int i = ic;
+      if constexpr (i == 0) {
+        asm volatile("s_nop 15\n\ts_nop 7" : "+v"(s16));  // the last score's product is through
+        top = max3(max3(max3(s16[0], s16[1], s16[2]), s16[3], s16[4]), s16[5], s16[6]);
+      } else if constexpr (i == 1) {
+        top = max3(max3(max3(top, s16[7], s16[8]), s16[9], s16[10]), s16[11], s16[12]);
+      } else if constexpr (i == 2) {
+        top = max3(max3(top, s16[13], s16[14]), s16[15], s16[15]);
+        const uint32_t tb = __builtin_bit_cast(uint32_t, top);
+        auto sw = __builtin_amdgcn_permlane32_swap(tb, tb, false, false);
+        top = max3(__builtin_bit_cast(float, (uint32_t)sw[0]), __builtin_bit_cast(float, (uint32_t)sw[1]),
+                   __builtin_bit_cast(float, (uint32_t)sw[1]));
+      } else if constexpr (i == 3) {
+        top = fmaxf(m, top * cscale);
+        grew = __any(top > m + kSlack);
+        mn = grew ? top : m;
+      } else if constexpr (i < 12) {
+        constexpr int e = 2 * (i - 4);
+        float a = fast_exp2(fmaf(s16[e], cscale, -mn)), c = fast_exp2(fmaf(s16[e + 1], cscale, -mn));
+        asm volatile("" : "+v"(a), "+v"(c));  // made here
+        s16[e] = a, s16[e + 1] = c;
+      } else if constexpr (i < 16) {
+        constexpr int e = 4 * (i - 12);
+        sum += (s16[e] + s16[e + 1]) + (s16[e + 2] + s16[e + 3]);
+        pk[e / 2] = Elem<T>::pack2(s16[e], s16[e + 1]);
+        pk[e / 2 + 1] = Elem<T>::pack2(s16[e + 2], s16[e + 3]);
+      } else if constexpr (i == 16) {
+        const float alpha = fast_exp2(m - mn);
+        l = fmaf(l, alpha, sum);
+        m = mn;
+        // (by every lane, without a branch: behind one the compiler would gather the parts before it)
+        *reinterpret_cast<float*>(lds + C::kAlpha + ((buf ^ 1) * C::ROWS + 32 * wave + (fresh() & 31)) * 4) = alpha;
+        *reinterpret_cast<int*>(lds + C::kGrew + ((buf ^ 1) * 4 + wave) * 4) = grew;
+      } else if constexpr (i < kParts) {
+        constexpr int q = i - 17;
+        store16(lds + C::kP + (buf ^ 1) * C::PB + (2 * wave + q) * 1024 + fresh() * 16,
+                u32x4{pk[4 * q], pk[4 * q + 1], pk[4 * q + 2], pk[4 * q + 3]});
+      }
+    };
+    if constexpr (!OUT) {
+      static_for<kParts>(part);
+    } else {
+      __builtin_amdgcn_sched_barrier(0);
+      static_for<P>([&](auto ic) __attribute__((always_inline)) {
+        constexpr int i = ic, q = i / (4 * DT), rt = i / DT % 4, dt = i % DT, g = i / DT;  // g: group of DT products
+        if constexpr (dt == 0 && g + 1 < 8) pr[(g + 1) & 1] = word(pa + (2 * ((g + 1) & 3) + ((g + 1) >> 2)) * 1024);
+        if constexpr (i == kLanded) {
+          lat_wait<C::NL + 1>();
+          __builtin_amdgcn_s_barrier();
+          asm volatile("" ::: "memory");
+          at_keys((vl + 2) & 3, vr == 0 ? 2 : vr - 1);
+        }
+        mfma32_acc<T>(acc[rt][dt], cv[dt], pr[g & 1]);
+        if constexpr (q == 0 && rt == 3) cv[dt] = vread(vslot, 1, dt);  // its last product of these 16 keys
+        if constexpr (i >= P - AHEAD) kread(std::integral_constant<int, i - (P - AHEAD)>{});
+        // from the third product on, in as many places as there are
+        constexpr int from = i < 2 ? 0 : (i - 2) * kParts / (P - 2), to = i < 2 ? 0 : (i - 1) * kParts / (P - 2);
+        static_for<to - from>(
+            [&](auto jc) __attribute__((always_inline)) { part(std::integral_constant<int, from + jc>{}); });
+        __builtin_amdgcn_sched_barrier(0);
+      });
+    }
   };
 
   if (t0 < tend) {
     lat_wait<2 * (C::NL + 1)>();
     __syncthreads();
-    begin(0, 0);
+    at_keys(0, 0);
+    static_for<AHEAD>(kread);
     step(std::false_type{}, t0 - 1, 0, 0, 1);
+    lat_wait<C::NL + 1>();
+    __syncthreads();
+    at_keys(1, 1);
+    static_for<AHEAD>(kread);
     int ls = 0, rs = 0;
     for (int t = t0; t < tend; ++t) {
-      lat_wait<C::NL + 1>();
-      __syncthreads();
-      const int buf = (t - t0) & 1, rn = rs == 2 ? 0 : rs + 1;
-      begin((ls + 1) & 3, rn);
-      shrink(buf);
       // (the last step's scores are those of a tile of zeros behind every row's keys)
-      step(std::true_type{}, t, ls, rs, buf);
+      step(std::true_type{}, t, ls, rs, (t - t0) & 1);
       ls = (ls + 1) & 3;
-      rs = rn;
+      rs = rs == 2 ? 0 : rs + 1;
     }
   }
   lat_wait<0>();
