@@ -319,5 +319,6 @@ extern "C" int ss_latent_attention_expanded(const void* q, void* out, const void
   p.block_size = 1;
   p.total = (int)total_tokens, p.total_keys = (int)total_keys;
   p.scale_log2 = scale * ss::kLog2e;
+  if (ss::latent_expanded_takes(p, dtype)) return ss::launch_latent_expanded(p, dtype, (hipStream_t)stream);
   return ss::launch_general<false>(p, dtype, (hipStream_t)stream);
 }

@@ -24,20 +24,12 @@
 // workgroup has the same number of tiles whatever the lengths are. Each finds its range by a scan over the
 // sequences' lengths in closed form. An item that is cut leaves fp32 partial rows, which
 // latent_merge_kernel adds in order: results repeat themselves to the bit.
-#include <type_traits>
-#include <utility>
-
-#include "latent_common.h"
-#include "w8a8_common.h"
+#include "latent_mma.h"
 
 namespace ss {
 namespace {
 
-constexpr int kRopeDim = 64;
 constexpr int kLeastTiles = 4;
-constexpr float kSlack = 8.f;  // by which (log2) a score may exceed the running maximum before it is raised
-
-typedef short tr16x4 __attribute__((ext_vector_type(4)));
 
 template <int R_, int RT_, int NW_>
 struct LatTile {
@@ -70,8 +62,6 @@ struct LatWide {
   static_assert(LDS <= 160 * 1024, "one workgroup a CU");
 };
 
-__device__ __forceinline__ int lat_swizzle(int r) { return (r & 3) | ((r & 4) << 1) | ((r & 8) >> 1); }
-
 // The latents' chunk of 8 values that output tile dt of wave w takes for lanes of row group g: bit 2 from
 // g >> 1, so that the four pieces of a transposing read lie in different banks whatever dt and w are
 template <typename C>
@@ -82,20 +72,6 @@ __device__ __forceinline__ int out_chunk(int dt, int gh, int w) {
     return dt + 4 * gh + 8 * w;
   else
     return dt + 2 * (w & 1) + 4 * gh + 8 * (w >> 1);
-}
-
-template <int N>
-__device__ __forceinline__ void lat_wait() {
-  asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory");
-}
-
-template <typename F, int... I>
-__device__ __forceinline__ void static_for_impl(F&& f, std::integer_sequence<int, I...>) {
-  (f(std::integral_constant<int, I>{}), ...);
-}
-template <int N, typename F>
-__device__ __forceinline__ void static_for(F&& f) {
-  static_for_impl(f, std::make_integer_sequence<int, N>{});
 }
 
 // ---- items ----------------------------------------------------------------------------------
@@ -371,17 +347,13 @@ __device__ __forceinline__ void latent_segment(const LatentParams& p, const Late
         for (int dt = 0; dt < DT; ++dt) acc[rt][dt] *= alpha;
       }
     }
-    const LdsBytes vp = (LdsBytes)lds + ls * C::LPLANE + vrow * C::ROWB + 8 * (n & 1);
+    const uint32_t vp = lds_address(lds) + ls * C::LPLANE + vrow * C::ROWB + 8 * (n & 1);
     const int sw = lat_swizzle(vrow);
     u32x4 c[DT];
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) {
-      const LdsBytes at = vp + 16 * (out_chunk<C>(dt, (n >> 1) & 1, wave) ^ sw);
-      const u32x2 lo = __builtin_bit_cast(
-          u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) tr16x4*)at));
-      const u32x2 hi = __builtin_bit_cast(
-          u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) tr16x4*)(at + 16 * C::ROWB)));
-      c[dt] = u32x4{lo[0], lo[1], hi[0], hi[1]};
+      const uint32_t at = vp + 16 * (out_chunk<C>(dt, (n >> 1) & 1, wave) ^ sw);
+      c[dt] = lds_keys(at, at + 16 * C::ROWB);
     }
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
@@ -446,8 +418,6 @@ __device__ __forceinline__ void latent_segment(const LatentParams& p, const Late
 
 // ---- 128 rows: 32 x 32 products --------------------------------------------------------------
 
-typedef float f32x16 __attribute__((ext_vector_type(16)));
-
 // acc += a b, the accumulator in AGPRs. As asm, because the compiler moves accumulators between the register
 // files when it needs more than half of the registers. What it therefore does not look after: the
 // operands come from LDS reads, which it does wait for; an accumulator is touched again sixteen products
@@ -459,34 +429,13 @@ __device__ __forceinline__ void mfma32_acc(f32x16& acc, u32x4 a, u32x4 b) {
   else
     asm volatile("v_mfma_f32_32x32x16_f16 %0, %1, %2, %0" : "+a"(acc) : "v"(a), "v"(b));
 }
-// s = a b (FIRST) or s += a b, chained; reading s is for the caller to wait for
-template <typename T, bool FIRST>
-__device__ __forceinline__ void mfma32_sum(f32x16& s, u32x4 a, u32x4 b) {
-  if constexpr (std::is_same<T, bf16_t>::value) {
-    if constexpr (FIRST)
-      asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, 0" : "=&v"(s) : "v"(a), "v"(b));
-    else
-      asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+v"(s) : "v"(a), "v"(b));
-  } else {
-    if constexpr (FIRST)
-      asm volatile("v_mfma_f32_32x32x16_f16 %0, %1, %2, 0" : "=&v"(s) : "v"(a), "v"(b));
-    else
-      asm volatile("v_mfma_f32_32x32x16_f16 %0, %1, %2, %0" : "+v"(s) : "v"(a), "v"(b));
-  }
-}
-// (without the quieting of NaNs that fmaxf has: a score that is none makes its row one anyway)
-__device__ __forceinline__ float max3(float a, float b, float c) {
-  float r;
-  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
-  return r;
-}
 template <typename T>
-__device__ __forceinline__ void clear_acc(f32x16& acc) {  // a product of zeros: no other registers take part
+__device__ __forceinline__ void clear_acc(f32x16& acc) {  // a product of zeros (two wait states after they are written): no other registers take part
   const u32x4 z = {0, 0, 0, 0};
   if constexpr (std::is_same<T, bf16_t>::value)
-    asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %1, 0" : "=a"(acc) : "v"(z));
+    asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %1, 0" : "=a"(acc) : "v"(z));
   else
-    asm volatile("v_mfma_f32_32x32x16_f16 %0, %1, %1, 0" : "=a"(acc) : "v"(z));
+    asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_f16 %0, %1, %1, 0" : "=a"(acc) : "v"(z));
 }
 template <int N>
 __device__ __forceinline__ void settled(f32x16 (&acc)[4][N]) {
@@ -497,7 +446,6 @@ __device__ __forceinline__ void settled(f32x16 (&acc)[4][N]) {
     for (int dt = 0; dt < N; ++dt) asm volatile("" : "+a"(acc[rt][dt]));
 }
 
-typedef __attribute__((address_space(3))) const u32x4* LdsWords;
 
 // A wave takes 32 rows' scores against all 32 keys (as S^T: lane l row l % 32, its result r key 8 (r / 4) +
 // 4 (l / 32) + r % 4) and all 128 rows' outputs of R / 4 values. Four waves: with 32 rows each a key is
@@ -575,15 +523,10 @@ __device__ __forceinline__ void latent_segment_wide(const LatentParams& p, const
     asm volatile("" : "+v"(ln));
     return ln;
   };
-  auto word = [](uint32_t at) { return *(LdsWords)(uintptr_t)at; };
+  auto word = [](uint32_t at) { return lds_word(at); };
   auto vread = [&](uint32_t slot, int s, int dt) {  // 16 keys from 16 s on, output tile dt
     const uint32_t at = (vaddr + slot) ^ (16 * dt) ^ vflip;
-    typedef __attribute__((address_space(3))) tr16x4* Tr;
-    const u32x2 lo = __builtin_bit_cast(
-        u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Tr)(uintptr_t)(at + 16 * s * C::ROWB)));
-    const u32x2 hi = __builtin_bit_cast(
-        u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Tr)(uintptr_t)((at ^ 64) + (16 * s + 8) * C::ROWB)));
-    return u32x4{lo[0], lo[1], hi[0], hi[1]};
+    return lds_keys(at + 16 * s * C::ROWB, (at ^ 64) + (16 * s + 8) * C::ROWB);
   };
 
   // One step: the scores of tile t + 1, then the outputs of tile t (OUT), whose latents are in ring slot vl and
