@@ -337,7 +337,8 @@ int ss_quantize_fp8(const void* x, uint8_t* q, float* scale, int64_t rows, int64
  * ss_w8a8_workspace_size). With less (or NULL, 0) the call succeeds without it, more slowly. Calls that
  * share a workspace must be ordered on one stream.
  */
-int ss_fp8_workspace_size(int64_t m, int64_t n, int64_t k, int x_whole, int w_whole, int64_t* bytes);
+int ss_fp8_workspace_size(int64_t m, int64_t n, int64_t k, int x_whole, int w_whole, int out_dtype,
+                          int64_t* bytes);
 
 int ss_fp8_gemm(const uint8_t* x, const float* x_scale, const uint8_t* w, const float* w_scale,
                 const void* bias, void* out, int64_t m, int64_t n, int64_t k, int64_t x_stride,

@@ -92,7 +92,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     ),
     "ss_swiglu_int8": (_i32, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i32, _vp]),
     "ss_quantize_fp8": (_i32, [_vp, _vp, _vp, _i64, _i64, _i64, _i64, _i32, _vp]),
-    "ss_fp8_workspace_size": (_i32, [_i64, _i64, _i64, _i32, _i32, _c_i64p]),
+    "ss_fp8_workspace_size": (_i32, [_i64, _i64, _i64, _i32, _i32, _i32, _c_i64p]),
     "ss_fp8_gemm": (
         _i32,
         [

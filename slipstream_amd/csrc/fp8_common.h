@@ -20,6 +20,15 @@ struct F8Params {
   int bias_dtype;
 };
 
+// The tile kernel (fp8_tile.hip): a workgroup's tokens and channels, its grid and K split.
+struct F8TilePlan {
+  int bm, bn;
+  int ks, per;  // K ranges and blocks of 128 keys per range
+  int n_tiles, m_blocks;
+};
+double plan_fp8_tile(F8TilePlan& pl, int64_t m, int64_t n, int64_t k, bool wide, bool may_split);  // estimated us
+int launch_fp8_tile(const F8Params& p, const F8TilePlan& pl, int out_dtype, float* part, hipStream_t stream);
+
 namespace {
 
 typedef int i32x8 __attribute__((ext_vector_type(8)));

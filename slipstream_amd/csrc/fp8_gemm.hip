@@ -115,16 +115,51 @@ int check_extents(int64_t m, int64_t n, int64_t k, int out_dtype) {
   return SS_OK;
 }
 
+// Rows that the DMA kernels can read in 16-byte pieces; a tile of 256 of them stays below a descriptor's 2^30
+// bytes.
+bool whole_rows(const void* base, int64_t rows, int64_t stride, int64_t k) {
+  return k % 16 == 0 && ((uintptr_t)base & 15) == 0 && (rows == 1 || stride % 16 == 0) && stride <= (1 << 21);
+}
+int64_t round16(int64_t n) { return (n + 15) / 16 * 16; }
+
+// What a call runs on the current device. Kept for the last shapes of the thread.
+struct Plan {
+  int64_t m = -1, n = 0, k = 0;
+  bool wide = false, may_split = false;
+  int device = -1;
+  F8TilePlan tp = {};
+  int64_t workspace() const { return tp.ks > 1 ? (int64_t)tp.ks * m * n * 4 : 0; }
+};
+const Plan& plan_for(int64_t m, int64_t n, int64_t k, bool wide, bool may_split) {
+  static thread_local Plan kept[64];
+  int device = 0;
+  if (hipGetDevice(&device) != hipSuccess) device = 0;
+  const uint64_t h = ((uint64_t)m * 0x9E3779B97F4A7C15ull) ^ ((uint64_t)n * 0xC2B2AE3D27D4EB4Full) ^
+                     ((uint64_t)k * 0x165667B19E3779F9ull) ^ (may_split ? 0 : ~0ull) ^ (wide ? 0xFFFFull << 40 : 0);
+  Plan& p = kept[h >> 58];
+  if (p.m != m || p.n != n || p.k != k || p.wide != wide || p.may_split != may_split || p.device != device) {
+    p.m = m, p.n = n, p.k = k, p.wide = wide, p.may_split = may_split, p.device = device;
+    plan_fp8_tile(p.tp, m, n, k, wide, may_split);
+  }
+  return p;
+}
+
 }  // namespace
 }  // namespace ss
 
-extern "C" int ss_fp8_workspace_size(int64_t m, int64_t n, int64_t k, int x_whole, int w_whole, int64_t* bytes) {
+extern "C" int ss_fp8_workspace_size(int64_t m, int64_t n, int64_t k, int x_whole, int w_whole, int out_dtype,
+                                     int64_t* bytes) {
   if (!bytes) {
     ss_host::set_error("fp8 workspace: null pointer");
     return SS_ERR_INVALID;
   }
   *bytes = 0;
-  return ss::check_extents(m, n, k, SS_DTYPE_BF16);
+  const int st = ss::check_extents(m, n, k, out_dtype);
+  if (st != SS_OK || m == 0 || n == 0 || k == 0) return st;
+  const int64_t kp = ss::round16(k);
+  *bytes = ss::plan_for(m, n, kp, out_dtype != SS_DTYPE_BF16, true).workspace() + (x_whole && kp == k ? 0 : m * kp) +
+           (w_whole && kp == k ? 0 : n * kp);
+  return SS_OK;
 }
 
 extern "C" int ss_fp8_gemm(const uint8_t* x, const float* x_scale, const uint8_t* w, const float* w_scale,
@@ -146,11 +181,39 @@ extern "C" int ss_fp8_gemm(const uint8_t* x, const float* x_scale, const uint8_t
     ss_host::set_error("fp8 gemm: row strides shorter than the rows");
     return SS_ERR_INVALID;
   }
-  const ss::F8Params p = {x,        w,        x_scale,       w_scale,       bias,          out,           m,      n,
+  ss::F8Params p = {x,        w,        x_scale,       w_scale,       bias,          out,           m,      n,
                           x_stride, w_stride, o_stride,      xs_strides[0], xs_strides[1], ws_strides[0], ws_strides[1],
                           (int)k,   bias_dtype};
+  if (m == 1) p.x_stride = ss::round16(k), p.o_stride = ss::round16(n), p.xs_row = 1;  // (not used to reach a row)
+  if (n == 1) p.w_stride = ss::round16(k);
+  if (n <= 128) p.ws_row = 1;
   hipStream_t s = (hipStream_t)stream;
-  (void)workspace, (void)workspace_bytes;
+  char* ws = (uintptr_t)workspace & 15 ? nullptr : (char*)workspace;
+  int64_t left = ws ? workspace_bytes : 0;
+  // rows that are not whole 16-byte pieces: their copies come first in the workspace
+  const int64_t kp = ss::round16(k), blocks = (k + 127) / 128;
+  const bool copy_x = !ss::whole_rows(p.x, m, p.x_stride, k), copy_w = !ss::whole_rows(p.w, n, p.w_stride, k);
+  const int64_t x_bytes = copy_x ? m * kp : 0, w_bytes = copy_w ? n * kp : 0;
+  // a tile's scales within a descriptor's reach
+  const int64_t reach = (int64_t)1 << 27;
+  const bool scales = p.xs_row >= 0 && p.xs_blk >= 0 && p.ws_row >= 0 && p.ws_blk >= 0 &&
+                      256 * p.xs_row + blocks * p.xs_blk < reach && 2 * p.ws_row + blocks * p.ws_blk < reach;
+  if (k > 0 && scales && x_bytes + w_bytes <= left && m <= INT32_MAX && n <= INT32_MAX) {
+    const bool wide = out_dtype != SS_DTYPE_BF16;
+    const ss::Plan* pl = &ss::plan_for(m, n, kp, wide, true);
+    if (pl->workspace() > left - x_bytes - w_bytes) pl = &ss::plan_for(m, n, kp, wide, false);
+    if (pl->tp.ks > 0) {
+      if (copy_x || copy_w) {
+        const ss::ByteRows rx = {(const int8_t*)p.x, (int8_t*)ws, p.x_stride, copy_x ? (int)m : 0};
+        const ss::ByteRows rw = {(const int8_t*)p.w, (int8_t*)ws + x_bytes, p.w_stride, copy_w ? (int)n : 0};
+        if (const int sa = ss::align_rows(rx, rw, (int)k, s); sa != SS_OK) return sa;
+        if (copy_x) p.x = (const uint8_t*)rx.to, p.x_stride = kp;
+        if (copy_w) p.w = (const uint8_t*)rw.to, p.w_stride = kp;
+        p.k = (int)kp;
+      }
+      return ss::launch_fp8_tile(p, pl->tp, out_dtype, (float*)(ws + x_bytes + w_bytes), s);
+    }
+  }
   if (out_dtype == SS_DTYPE_BF16) return ss::launch_general<ss::bf16_t>(p, s);
   if (out_dtype == SS_DTYPE_F16) return ss::launch_general<ss::f16_t>(p, s);
   return ss::launch_general<float>(p, s);

@@ -238,7 +238,7 @@ latent_expanded_kernel(const LatentParams p, int tiles) {
 
   f32x16 sa[2], sb[2];
   if (tend > 0) {
-    lat_wait<(C::D - 1) * C::PER>();
+    wait_dma<(C::D - 1) * C::PER>();
     __syncthreads();
     if (most > 0) step(std::false_type{}, -1, 0, 0, sb, sa);
     int ks = 0, vs = 0;  // slots of the keys and of the values of tile t
@@ -246,7 +246,7 @@ latent_expanded_kernel(const LatentParams p, int tiles) {
     // t + D's keys and t + D - 1's values take their places. Waves whose rows see nothing of a tile do
     // nothing else.
     auto turn = [&](int t, f32x16 (&cur)[2], f32x16 (&next)[2]) __attribute__((always_inline)) {
-      lat_wait<(C::D - 2) * C::PER>();
+      wait_dma<(C::D - 2) * C::PER>();
       __syncthreads();
       const int kn = ks + 1 == C::D ? 0 : ks + 1;
       issue(t + C::D, ks, vs == 0 ? C::D - 1 : vs - 1);
@@ -259,7 +259,7 @@ latent_expanded_kernel(const LatentParams p, int tiles) {
       if (t + 1 < tend) turn(t + 1, sb, sa);
     }
   }
-  lat_wait<0>();  // no DMA may land after the workgroup has ended
+  wait_dma<0>();  // no DMA may land after the workgroup has ended
   asm volatile("s_nop 15\n\ts_nop 7" : "+v"(acc[0]), "+v"(acc[1]), "+v"(acc[2]), "+v"(acc[3]));
 
   const uint32_t lb = __builtin_bit_cast(uint32_t, l);

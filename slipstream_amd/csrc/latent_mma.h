@@ -1,11 +1,9 @@
 // Device helpers shared by the matrix-core kernels of attention over latents: products of 32 x 32 x 16,
-// the swizzle of rows in the LDS, waits.
+// the swizzle of rows in the LDS.
 #pragma once
-#include <type_traits>
-#include <utility>
 
 #include "latent_common.h"
-#include "w8a8_common.h"
+#include "tile_order.h"
 
 namespace ss {
 namespace {
@@ -15,27 +13,11 @@ constexpr float kSlack = 8.f;  // by which (log2) a score may exceed the running
 
 typedef short tr16x4 __attribute__((ext_vector_type(4)));typedef float f32x16 __attribute__((ext_vector_type(16)));
 
-typedef __attribute__((address_space(3))) const u32x4* LdsWords;
-
 // Where the 16-byte chunk c of a row r of 256 bytes and more lies in the LDS: at c ^ lat_swizzle(r). The 16
 // lanes of a pass of a 16-byte read have different rows (mod 16) and lie in different banks; of
 // eight rows in order the low two bits and the highest differ, so that the 8-byte pieces of four
 // chunks that differ in bit 2 (and their halves) do so too.
 __device__ __forceinline__ int lat_swizzle(int r) { return (r & 3) | ((r & 4) << 1) | ((r & 8) >> 1); }
-
-template <int N>
-__device__ __forceinline__ void lat_wait() {
-  asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory");
-}
-
-template <typename F, int... I>
-__device__ __forceinline__ void static_for_impl(F&& f, std::integer_sequence<int, I...>) {
-  (f(std::integral_constant<int, I>{}), ...);
-}
-template <int N, typename F>
-__device__ __forceinline__ void static_for(F&& f) {
-  static_for_impl(f, std::make_integer_sequence<int, N>{});
-}
 
 // s = a b (FIRST) or s += a b, chained; reading s is for the caller to wait for
 template <typename T, bool FIRST>
@@ -59,9 +41,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return r;
 }
 
-// An address space 3 address as a number, and the transposing read of four keys' values there
-__device__ __forceinline__ uint32_t lds_address(char* p) { return (uint32_t)(uintptr_t)(LdsBytes)p; }
-__device__ __forceinline__ u32x4 lds_word(uint32_t at) { return *(LdsWords)(uintptr_t)at; }
 // The operand of 16 keys of a product over keys, from rows of the LDS: the lane's four keys at `lo`, and
 // those eight rows on at `hi`. Within sixteen lanes, lane i receives element i % 4 of the 8-byte reads of
 // lanes i / 4 + 4 e (e = 0 .. 3).

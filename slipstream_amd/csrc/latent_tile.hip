@@ -271,9 +271,9 @@ __device__ __forceinline__ void latent_segment(const LatentParams& p, const Late
 
   auto landed = [&](auto tiles) {  // all but the youngest `tiles` tiles
     if (wave < 4)
-      lat_wait<decltype(tiles)::value*(C::NL + 1)>();
+      wait_dma<decltype(tiles)::value*(C::NL + 1)>();
     else
-      lat_wait<decltype(tiles)::value * C::NL>();
+      wait_dma<decltype(tiles)::value * C::NL>();
   };
 
   f32x4 acc[RT][DT];
@@ -380,7 +380,7 @@ __device__ __forceinline__ void latent_segment(const LatentParams& p, const Late
       rs = rn;
     }
   }
-  lat_wait<0>();
+  wait_dma<0>();
 
   // ---- the rows' sums, then the rows themselves
   if (scores) {
@@ -660,7 +660,7 @@ __device__ __forceinline__ void latent_segment_wide(const LatentParams& p, const
         constexpr int i = ic, q = i / (4 * DT), rt = i / DT % 4, dt = i % DT, g = i / DT;  // g: group of DT products
         if constexpr (dt == 0 && g + 1 < 8) pr[(g + 1) & 1] = word(pa + (2 * ((g + 1) & 3) + ((g + 1) >> 2)) * 1024);
         if constexpr (i == kLanded) {
-          lat_wait<C::NL + 1>();
+          wait_dma<C::NL + 1>();
           __builtin_amdgcn_s_barrier();
           asm volatile("" ::: "memory");
           at_keys((vl + 2) & 3, vr == 0 ? 2 : vr - 1);
@@ -678,12 +678,12 @@ __device__ __forceinline__ void latent_segment_wide(const LatentParams& p, const
   };
 
   if (t0 < tend) {
-    lat_wait<2 * (C::NL + 1)>();
+    wait_dma<2 * (C::NL + 1)>();
     __syncthreads();
     at_keys(0, 0);
     static_for<AHEAD>(kread);
     step(std::false_type{}, t0 - 1, 0, 0, 1);
-    lat_wait<C::NL + 1>();
+    wait_dma<C::NL + 1>();
     __syncthreads();
     at_keys(1, 1);
     static_for<AHEAD>(kread);
@@ -695,7 +695,7 @@ __device__ __forceinline__ void latent_segment_wide(const LatentParams& p, const
       rs = rs == 2 ? 0 : rs + 1;
     }
   }
-  lat_wait<0>();
+  wait_dma<0>();
   settled(acc);
 
   {

@@ -39,13 +39,7 @@ __device__ __forceinline__ i32x4 load_keys(const int8_t* row, int at, int k) {
 // are copied to rows that do, zeros behind them, in the workspace: 333 x 4999 x 2051 (rows at any
 // byte; bf16, no bias) 30.4 us in the general kernel, 20.8 so, of which 8 for the copies.
 // Two pieces a thread, both on their way before the first is written.
-struct Rows {
-  const int8_t* from;
-  int8_t* to;
-  int64_t stride;  // of `from`
-  int rows;
-};
-__global__ __launch_bounds__(256) void w8a8_align_kernel(Rows x, Rows w, int k, uint32_t pieces) {
+__global__ __launch_bounds__(256) void w8a8_align_kernel(ByteRows x, ByteRows w, int k, uint32_t pieces) {
   const uint32_t total = (uint32_t)(x.rows + w.rows) * pieces, half = (total + 1) >> 1;
   const uint32_t i = blockIdx.x * 256 + threadIdx.x;
   if (i >= half) return;
@@ -65,28 +59,6 @@ __global__ __launch_bounds__(256) void w8a8_align_kernel(Rows x, Rows w, int k, 
 #pragma unroll
   for (int u = 0; u < 2; ++u)
     if (to[u]) *reinterpret_cast<i32x4*>(to[u]) = v[u];
-}
-
-// The copies of both operands (0 rows: none), as many rows a launch as its 32-bit piece numbers hold
-int align_rows(Rows x, Rows w, int k, hipStream_t stream) {
-  const int pieces = (k + 15) / 16;
-  const int most = (1 << 30) / pieces;
-  for (int64_t left = (int64_t)x.rows + w.rows; left > 0;) {
-    const Rows px = {x.from, x.to, x.stride, x.rows < most ? x.rows : most};
-    const Rows pw = {w.from, w.to, w.stride, w.rows < most - px.rows ? w.rows : most - px.rows};
-    const int64_t half = ((int64_t)(px.rows + pw.rows) * pieces + 1) / 2;
-    hipLaunchKernelGGL(w8a8_align_kernel, dim3((unsigned)((half + 255) / 256)), dim3(256), 0, stream, px, pw, k,
-                       (uint32_t)pieces);
-    const int st = ss_host::launch_status("w8a8 gemm (align)");
-    if (st != SS_OK) return st;
-    for (auto [all, part] : {std::pair<Rows*, const Rows*>{&x, &px}, {&w, &pw}}) {
-      all->from += part->rows * all->stride;
-      all->to += part->rows * (16 * (int64_t)pieces);
-      all->rows -= part->rows;
-    }
-    left -= px.rows + pw.rows;
-  }
-  return SS_OK;
 }
 
 // The kernel for every shape, stride and alignment, without a workspace: 64 x 64 results a
@@ -210,6 +182,28 @@ int check_extents(int64_t m, int64_t n, int64_t k, int out_dtype) {
 }
 
 }  // namespace
+
+int align_rows(ByteRows x, ByteRows w, int k, hipStream_t stream) {
+  const int pieces = (k + 15) / 16;
+  const int most = (1 << 30) / pieces;
+  for (int64_t left = (int64_t)x.rows + w.rows; left > 0;) {
+    const ByteRows px = {x.from, x.to, x.stride, x.rows < most ? x.rows : most};
+    const ByteRows pw = {w.from, w.to, w.stride, w.rows < most - px.rows ? w.rows : most - px.rows};
+    const int64_t half = ((int64_t)(px.rows + pw.rows) * pieces + 1) / 2;
+    hipLaunchKernelGGL(w8a8_align_kernel, dim3((unsigned)((half + 255) / 256)), dim3(256), 0, stream, px, pw, k,
+                       (uint32_t)pieces);
+    const int st = ss_host::launch_status("8-bit gemm (align)");
+    if (st != SS_OK) return st;
+    for (auto [all, part] : {std::pair<ByteRows*, const ByteRows*>{&x, &px}, {&w, &pw}}) {
+      all->from += part->rows * all->stride;
+      all->to += part->rows * (16 * (int64_t)pieces);
+      all->rows -= part->rows;
+    }
+    left -= px.rows + pw.rows;
+  }
+  return SS_OK;
+}
+
 }  // namespace ss
 
 extern "C" int ss_w8a8_workspace_size(int64_t m, int64_t n, int64_t k, int x_whole, int w_whole, int64_t* bytes) {
@@ -276,8 +270,8 @@ extern "C" int ss_w8a8_gemm(const int8_t* x, const float* x_scale, const int8_t*
   const int64_t x_bytes = copy_x ? m * kp : 0, w_bytes = copy_w ? n * kp : 0;
   if (k > 0 && x_bytes + w_bytes <= left && m <= INT32_MAX && n <= INT32_MAX) {
     if (copy_x || copy_w) {
-      const ss::Rows rx = {p.x, (int8_t*)ws, p.x_stride, copy_x ? (int)m : 0};
-      const ss::Rows rw = {p.w, (int8_t*)ws + x_bytes, p.w_stride, copy_w ? (int)n : 0};
+      const ss::ByteRows rx = {p.x, (int8_t*)ws, p.x_stride, copy_x ? (int)m : 0};
+      const ss::ByteRows rw = {p.w, (int8_t*)ws + x_bytes, p.w_stride, copy_w ? (int)n : 0};
       const int sa = ss::align_rows(rx, rw, (int)k, s);
       if (sa != SS_OK) return sa;
       if (copy_x) p.x = rx.to, p.x_stride = kp;

@@ -45,6 +45,16 @@ int launch_w8a8_stream(const W8Params& p, const StreamPlan& pl, int out_dtype, h
 double plan_w8a8_tile(TilePlan& pl, int64_t m, int64_t n, int64_t k, bool may_split);  // estimated us
 int launch_w8a8_tile(const W8Params& p, const TilePlan& pl, int out_dtype, int* part, hipStream_t stream);
 
+// Rows of bytes that are copied (w8a8.hip) to ones that begin on 16 bytes and end with 16, zeros behind them;
+// 0 rows: none. As many rows a launch as its 32-bit piece numbers hold.
+struct ByteRows {
+  const int8_t* from;
+  int8_t* to;
+  int64_t stride;  // of `from`
+  int rows;
+};
+int align_rows(ByteRows x, ByteRows w, int k, hipStream_t stream);
+
 // Weights that one token block reads pass the caches by beyond this many bytes. Out of the memory that
 // is 2 to 16 % faster at any size (24 x 28672 x 4096 25.1 -> 23.2 us, 24 x 4096 x 14336 18.0 ->
 // 17.3, 64 x 28672 x 4096 30.8 -> 25.9, 64 x 14336 x 4096 20.5 -> 19.7), but up to 46 % slower for

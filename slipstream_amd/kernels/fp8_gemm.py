@@ -48,13 +48,14 @@ def _whole(t: torch.Tensor, stride: int) -> int:
     return int(not (t.data_ptr() | stride) & 15 and stride <= 1 << 21)
 
 
-def _workspace_need(device: torch.device, m: int, n: int, k: int, x_whole: int, w_whole: int) -> int:
-    key = (device.index, m, n, k, x_whole, w_whole)
+def _workspace_need(device: torch.device, m: int, n: int, k: int, x_whole: int, w_whole: int, dtype: int) -> int:
+    key = (device.index, m, n, k, x_whole, w_whole, dtype)
     need = _WS_NEED.get(key)
     if need is None:
         out = _ffi.ctypes.c_int64(0)
         with torch.cuda.device(device):
-            status = _ffi.lib().ss_fp8_workspace_size(m, n, k, x_whole, w_whole, _ffi.ctypes.byref(out))
+            status = _ffi.lib().ss_fp8_workspace_size(m, n, k, x_whole, w_whole, dtype,
+                                                        _ffi.ctypes.byref(out))
         _ffi.check(status, "fp8 workspace")
         if len(_WS_NEED) > 4096:  # many distinct shapes: start over
             _WS_NEED.clear()
@@ -99,7 +100,7 @@ def fp8_gemm(q: torch.Tensor, scale: torch.Tensor, qweight: torch.Tensor, w_scal
             qweight = qweight.contiguous()
         w_stride = qweight.stride(0)
     scale = _scale_rows(scale, m)
-    need = _workspace_need(q.device, m, n, k, _whole(q, q_stride), _whole(qweight, w_stride))
+    need = _workspace_need(q.device, m, n, k, _whole(q, q_stride), _whole(qweight, w_stride), dtype)
     # of this call alone: nothing is shared between streams, or between captured graphs
     ws = q.new_empty(need, dtype=torch.uint8) if need else None
     status = launch(q.device, _ffi.lib().ss_fp8_gemm, q.data_ptr(), scale.data_ptr(), qweight.data_ptr(),

@@ -97,8 +97,8 @@ def test_c_entries_refuse_before_any_launch():
     assert rows(1 << 40, 256) == _ffi.SS_ERR_UNSUPPORTED
     assert rows(0, 8, x=None) == _ffi.SS_OK
     need = ctypes.c_int64(-1)
-    assert lib.ss_fp8_workspace_size(4, 8, -1, 1, 1, ctypes.byref(need)) == _ffi.SS_ERR_INVALID
-    assert lib.ss_fp8_workspace_size(4, 8, 8, 1, 1, None) == _ffi.SS_ERR_INVALID
+    assert lib.ss_fp8_workspace_size(4, 8, -1, 1, 1, 1, ctypes.byref(need)) == _ffi.SS_ERR_INVALID
+    assert lib.ss_fp8_workspace_size(4, 8, 8, 1, 1, 1, None) == _ffi.SS_ERR_INVALID
 
 
 def test_oracle_rounds_as_the_type_does():
