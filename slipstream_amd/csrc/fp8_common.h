@@ -26,6 +26,15 @@ struct F8TilePlan {
   int ks, per;  // K ranges and blocks of 128 keys per range
   int n_tiles, m_blocks;
 };
+// The stream kernel (fp8_stream.hip): a workgroup's 16-row tiles of tokens and channels, its waves and its grid.
+struct F8StreamPlan {
+  int mt, nt, waves;
+  int n_tiles, m_blocks;
+  bool once;  // the weights pass the caches by
+};
+double plan_fp8_stream(F8StreamPlan& pl, int64_t m, int64_t n, int64_t k);  // estimated us
+int launch_fp8_stream(const F8Params& p, const F8StreamPlan& pl, int out_dtype, hipStream_t stream);
+
 double plan_fp8_tile(F8TilePlan& pl, int64_t m, int64_t n, int64_t k, bool wide, bool may_split);  // estimated us
 int launch_fp8_tile(const F8Params& p, const F8TilePlan& pl, int out_dtype, float* part, hipStream_t stream);
 
@@ -87,6 +96,15 @@ struct Block<bf16_t> {
 
 __device__ __forceinline__ i32x8 join8(i32x4 lo, i32x4 hi) {
   return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+// 16-byte chunk c of row r of a 16-row tile lies at chunk c ^ f8_swizzle(r) of its 128 LDS bytes: a 16-byte
+// read takes rows 0-3 and 12-15 of one key group with rows 4-11 of the next, whose chunk differs by 2, in a
+// pass; rows 2p and 2p + 1 lie in different halves of the banks, and this value keeps the row pairs of a pass
+// apart.
+__device__ __forceinline__ int f8_swizzle(int r) {
+  const int p = r >> 1;
+  return (((p >> 2) ^ (p >> 1)) & 1) << 2 | ((p >> 2) & 1) << 1 | (p & 1);
 }
 
 // Sixteen keys of a row at any alignment, zeros past the row's end

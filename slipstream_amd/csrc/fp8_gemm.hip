@@ -127,8 +127,10 @@ struct Plan {
   int64_t m = -1, n = 0, k = 0;
   bool wide = false, may_split = false;
   int device = -1;
+  bool stream = false;
+  F8StreamPlan sp = {};
   F8TilePlan tp = {};
-  int64_t workspace() const { return tp.ks > 1 ? (int64_t)tp.ks * m * n * 4 : 0; }
+  int64_t workspace() const { return !stream && tp.ks > 1 ? (int64_t)tp.ks * m * n * 4 : 0; }
 };
 const Plan& plan_for(int64_t m, int64_t n, int64_t k, bool wide, bool may_split) {
   static thread_local Plan kept[64];
@@ -139,7 +141,8 @@ const Plan& plan_for(int64_t m, int64_t n, int64_t k, bool wide, bool may_split)
   Plan& p = kept[h >> 58];
   if (p.m != m || p.n != n || p.k != k || p.wide != wide || p.may_split != may_split || p.device != device) {
     p.m = m, p.n = n, p.k = k, p.wide = wide, p.may_split = may_split, p.device = device;
-    plan_fp8_tile(p.tp, m, n, k, wide, may_split);
+    const double stream = plan_fp8_stream(p.sp, m, n, k), tile = plan_fp8_tile(p.tp, m, n, k, wide, may_split);
+    p.stream = stream < 1e29 && (m <= 32 || stream < tile);
   }
   return p;
 }
@@ -202,7 +205,7 @@ extern "C" int ss_fp8_gemm(const uint8_t* x, const float* x_scale, const uint8_t
     const bool wide = out_dtype != SS_DTYPE_BF16;
     const ss::Plan* pl = &ss::plan_for(m, n, kp, wide, true);
     if (pl->workspace() > left - x_bytes - w_bytes) pl = &ss::plan_for(m, n, kp, wide, false);
-    if (pl->tp.ks > 0) {
+    if (pl->stream || pl->tp.ks > 0) {
       if (copy_x || copy_w) {
         const ss::ByteRows rx = {(const int8_t*)p.x, (int8_t*)ws, p.x_stride, copy_x ? (int)m : 0};
         const ss::ByteRows rw = {(const int8_t*)p.w, (int8_t*)ws + x_bytes, p.w_stride, copy_w ? (int)n : 0};
@@ -211,6 +214,7 @@ extern "C" int ss_fp8_gemm(const uint8_t* x, const float* x_scale, const uint8_t
         if (copy_w) p.w = (const uint8_t*)rw.to, p.w_stride = kp;
         p.k = (int)kp;
       }
+      if (pl->stream) return ss::launch_fp8_stream(p, pl->sp, out_dtype, s);
       return ss::launch_fp8_tile(p, pl->tp, out_dtype, (float*)(ws + x_bytes + w_bytes), s);
     }
   }

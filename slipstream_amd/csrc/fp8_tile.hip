@@ -15,15 +15,6 @@ namespace {
 constexpr int kLdsBytes = 160 * 1024;
 constexpr int kFar = 0x40000000;  // a byte offset past any operand tile (host-checked)
 
-// 16-byte chunk c of row r of a 16-row tile lies at chunk c ^ f8_swizzle(r) of its 128 LDS bytes: a 16-byte
-// read takes rows 0-3 and 12-15 of one key group with rows 4-11 of the next, whose chunk differs by 2, in a
-// pass; rows 2p and 2p + 1 lie in different halves of the banks, and this value keeps the row pairs of a pass
-// apart.
-__device__ __forceinline__ int f8_swizzle(int r) {
-  const int p = r >> 1;
-  return (((p >> 2) ^ (p >> 1)) & 1) << 2 | ((p >> 2) & 1) << 1 | (p & 1);
-}
-
 constexpr int stage_bytes(int bm, int bn) { return (bm + bn) * 128 + bm * 4 + 256; }
 constexpr int ring_depth(int bm, int bn) {
   int d = 2;
