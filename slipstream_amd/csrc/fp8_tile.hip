@@ -158,7 +158,12 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       static_for<(q + 1) * ND / P - q * ND / P>([&](auto uc) __attribute__((always_inline)) {
         dma(std::integral_constant<int, q * ND / P + decltype(uc)::value>{});
       });
-      if constexpr (q >= 2) add(std::integral_constant<int, q - 2>{});
+      if constexpr (q >= 2) {
+        // not before this product's issue: it waits for the matrix cores to be done with the two before it. (Left
+        // to the compiler, which does not know the asm's latency, the sums were read one product too early.)
+        if constexpr (__is_same(TO, bf16_t)) asm volatile("" : "+v"(part[(q - 2) % 3]));
+        add(std::integral_constant<int, q - 2>{});
+      }
       __builtin_amdgcn_sched_barrier(0);
     });
     asm volatile("s_nop 15\n\ts_nop 3" : "+v"(part[0]), "+v"(part[1]), "+v"(part[2]));  // the last products are through

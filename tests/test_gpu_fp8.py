@@ -236,3 +236,11 @@ def test_linear_and_mlp_together(device):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(y, lin(x)) and torch.equal(z, mlp(x))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("m,n,k", [(2048, 8192, 640), (1000, 16384 + 200, 384), (768, 4096, 2048 + 48), (500, 1280, 4096)])
+def test_gemm_of_many_tokens(device, m, n, k, dtype):
+    """The widest tiles, whole ones and cut ones, and keys split over workgroups."""
+    q, scale, qw, ws = _operands(m, n, k, m + n + k)
+    _check_gemm(fp8_gemm(q, scale, qw, ws, None, dtype), q, scale, qw, ws)
