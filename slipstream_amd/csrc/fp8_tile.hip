@@ -155,8 +155,10 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         part[q % 3] = Block<TO>::sum(a[i & 1], b[j]);
       }
       if constexpr (j == 0 && i + 1 < IT) a[(i + 1) & 1] = Block<TO>::operand(frag(wb + (i + 1) * 2048));
-      static_for<(q + 1) * ND / P - q * ND / P>([&](auto uc) __attribute__((always_inline)) {
-        dma(std::integral_constant<int, q * ND / P + decltype(uc)::value>{});
+      // the DMAs early, so that most of the stage is left for them to land in
+      constexpr int kOver = P < 16 ? P : P / 4, from = q < kOver ? q * ND / kOver : ND, to = q < kOver ? (q + 1) * ND / kOver : ND;
+      static_for<to - from>([&](auto uc) __attribute__((always_inline)) {
+        dma(std::integral_constant<int, from + decltype(uc)::value>{});
       });
       if constexpr (q >= 2) {
         // not before this product's issue: it waits for the matrix cores to be done with the two before it. (Left
