@@ -82,31 +82,43 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   const LdsBytes lds = (LdsBytes)s_dyn;
   const uint32_t base = lds_address(s_dyn);
   struct {
-    int so, add, ss, slot;
+    int so, ss, slot;
   } to;
   auto aim = [&](int i, int slot) {  // stage i into ring slot `slot`; past the range zeros, which nobody reads
     const int at = min(i, stages - 1);
     to.so = __builtin_amdgcn_readfirstlane(at * 128);
     to.ss = __builtin_amdgcn_readfirstlane(4 * at * (int)sc_blk);
-    to.add = i >= i1 ? kFar : at == stages - 1 ? past : 0;
     to.slot = __builtin_amdgcn_readfirstlane(slot * SB);
+    if (i >= min(i1, stages - 1)) {  // the last stage's chunks past k, and all past the range, from here on
+      const int add = i >= i1 ? kFar : past;
+#pragma unroll
+      for (int u = 0; u < NX + NW; ++u) off[u] |= add;
+    }
     asm volatile("s_nop 4" : : "s"(to.so), "s"(to.ss), "s"(to.slot));  // VALU-written SGPRs: five wait states
   };
   auto dma = [&](auto uc) __attribute__((always_inline)) {
     constexpr int u = decltype(uc)::value;
     if constexpr (u < NX) {
-      dma_b128(rx, lds + to.slot + u * 8192 + wave * 1024, off[u] + to.add, to.so);
+      dma_b128(rx, lds + to.slot + u * 8192 + wave * 1024, off[u], to.so);
     } else if constexpr (u < NX + NW) {
-      dma_b128(rw, lds + to.slot + XB + (u - NX) * 8192 + wave * 1024, off[u] + to.add, to.so);
+      dma_b128(rw, lds + to.slot + XB + (u - NX) * 8192 + wave * 1024, off[u], to.so);
     } else {
       dma_b32(rs, base + to.slot + XB + WB + (of_x ? wave * 256 : BM * 4), off_s, to.ss);
     }
   };
 
-  // fragment of lane (ln, kg): row ln of a 16-row tile, chunks 2 kg and 2 kg + 1
-  const uint32_t f0 = base + ln * 128 + 16 * ((2 * kg) ^ f8_swizzle(ln)), f1 = base + ln * 128 + 16 * ((2 * kg + 1) ^ f8_swizzle(ln));
-  auto frag = [&](uint32_t at) __attribute__((always_inline)) {
-    return join8(__builtin_bit_cast(i32x4, lds_word(f0 + at)), __builtin_bit_cast(i32x4, lds_word(f1 + at)));
+  // fragment of lane (ln, kg): row ln of a 16-row tile, chunks 2 kg and 2 kg + 1. The addresses of a stage's
+  // first fragments and scales are kept; the others are a constant away.
+  const uint32_t chunk0 = ln * 128 + 16 * ((2 * kg) ^ f8_swizzle(ln)), chunk1 = ln * 128 + 16 * ((2 * kg + 1) ^ f8_swizzle(ln));
+  uint32_t x0, x1, w0, w1, sx, sw;
+  auto look_at = [&](int slot) __attribute__((always_inline)) {
+    const uint32_t at = base + slot * SB, xb = at + wm * JT * 2048, wb = at + XB + wn * IT * 2048;
+    x0 = xb + chunk0, x1 = xb + chunk1, w0 = wb + chunk0, w1 = wb + chunk1;
+    sx = at + XB + WB + 4 * (16 * JT * wm + ln), sw = at + XB + WB + BM * 4 + 4 * ((wn * IT * 16) >> 7);
+    asm volatile("" : "+v"(x0), "+v"(x1), "+v"(w0), "+v"(w1), "+v"(sx), "+v"(sw));
+  };
+  auto frag = [&](uint32_t lo, uint32_t hi) __attribute__((always_inline)) {
+    return join8(__builtin_bit_cast(i32x4, lds_word(lo)), __builtin_bit_cast(i32x4, lds_word(hi)));
   };
 
   f32x4 acc[IT][JT];
@@ -121,58 +133,88 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     aim(i0 + j, j);
     static_for<ND>(dma);
   });
+
+  // The products of a stage in the order of the channels' tiles. What the next stage begins with is read behind
+  // the last channels' products, once it has landed for all waves (kReady); the DMAs of the stage D - 1 on
+  // follow the first product, when all waves are past the stage whose place they take, and are through early,
+  // so that most of the stage is left for them to land in. A product's results are added two products later, the
+  // last two's in the next stage.
+  constexpr int P = IT * JT, kReady = P - JT, kSent = P >= 16 ? P / 4 : 1;
+  static_assert(P % 4 == 0 && IT % 2 == 0 && JT >= 2 && kSent <= kReady, "order");
+  i32x8 next_a, next_b[JT];  // a stage's first operands and its scales, as they lie in the LDS
+  float next_sc[JT], next_ws, sc[JT];
+  f32x4 part[4];
+#pragma unroll
+  for (int j = 0; j < JT; ++j) sc[j] = 0.f;
+  part[2] = part[3] = f32x4{0.f, 0.f, 0.f, 0.f};
+  auto add = [&](auto ic) __attribute__((always_inline)) {
+    constexpr int q = decltype(ic)::value, i = q / JT, j = q % JT;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[i][j][e] = fmaf(part[q % 4][e], sc[j], acc[i][j][e]);
+  };
+  auto begin_a = [&]() __attribute__((always_inline)) {
+    next_a = frag(w0, w1);
+    next_ws = lds_float(sw);
+  };
+  auto begin_b = [&](int j) __attribute__((always_inline)) {
+    next_b[j] = frag(x0 + j * 2048, x1 + j * 2048);
+    next_sc[j] = lds_float(sx + 64 * j);
+  };
+  wait_dma<(D - 2) * ND>();
+  __syncthreads();
+  look_at(0);
+  begin_a();
+#pragma unroll
+  for (int j = 0; j < JT; ++j) begin_b(j);
   int slot = 0;
   for (int st = i0; st < i1; ++st) {
-    wait_dma<(D - 2) * ND>();
-    __syncthreads();  // the stage has landed, and the one before is read
-    const uint32_t xb = slot * SB + wm * JT * 2048, wb = slot * SB + XB + wn * IT * 2048;
-    const uint32_t sb = base + slot * SB + XB + WB;
     typename Block<TO>::Operand b[JT], a[2];
-    float sc[JT];
-    const float ws = lds_float(sb + BM * 4 + 4 * ((wn * IT * 16) >> 7));
-    a[0] = Block<TO>::operand(frag(wb));
+    a[0] = Block<TO>::operand(next_a);
 #pragma unroll
-    for (int j = 0; j < JT; ++j) {
-      b[j] = Block<TO>::operand(frag(xb + j * 2048));
-      sc[j] = lds_float(sb + 4 * (16 * (JT * wm + j) + ln));
-    }
-    aim(st + D - 1, slot == 0 ? D - 1 : slot - 1);
-#pragma unroll
-    for (int j = 0; j < JT; ++j) sc[j] *= ws;
-    constexpr int P = IT * JT;
-    f32x4 part[3];
-    auto add = [&](auto ic) __attribute__((always_inline)) {
-      constexpr int q = decltype(ic)::value, i = q / JT, j = q % JT;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) acc[i][j][e] = fmaf(part[q % 3][e], sc[j], acc[i][j][e]);
-    };
+    for (int j = 0; j < JT; ++j) b[j] = Block<TO>::operand(next_b[j]);
+    const int before = slot == 0 ? D - 1 : slot - 1, after = slot + 1 == D ? 0 : slot + 1;
     __builtin_amdgcn_sched_barrier(0);
     static_for<P>([&](auto qc) __attribute__((always_inline)) {
       constexpr int q = decltype(qc)::value, i = q / JT, j = q % JT;
       if constexpr (__is_same(TO, bf16_t)) {
-        mfma_block<TO>(part[q % 3], a[i & 1], b[j]);
+        mfma_block<TO>(part[q % 4], a[i & 1], b[j]);
       } else {
-        part[q % 3] = Block<TO>::sum(a[i & 1], b[j]);
+        part[q % 4] = Block<TO>::sum(a[i & 1], b[j]);
       }
-      if constexpr (j == 0 && i + 1 < IT) a[(i + 1) & 1] = Block<TO>::operand(frag(wb + (i + 1) * 2048));
-      // the DMAs early, so that most of the stage is left for them to land in
-      constexpr int kOver = P < 16 ? P : P / 4, from = q < kOver ? q * ND / kOver : ND, to = q < kOver ? (q + 1) * ND / kOver : ND;
+      if constexpr (q == kReady) {
+        wait_dma<(D - 2) * ND>();
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        look_at(after);
+        begin_a();
+      }
+      if constexpr (j == 0 && i + 1 < IT) a[(i + 1) & 1] = Block<TO>::operand(frag(w0 + (i + 1) * 2048, w1 + (i + 1) * 2048));
+      if constexpr (q >= kReady) begin_b(j);
+      if constexpr (q == 0) {
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        aim(st + D - 1, before);
+      }
+      constexpr int from = q < kSent ? q * ND / kSent : ND, to = q < kSent ? (q + 1) * ND / kSent : ND;
       static_for<to - from>([&](auto uc) __attribute__((always_inline)) {
         dma(std::integral_constant<int, from + decltype(uc)::value>{});
       });
-      if constexpr (q >= 2) {
-        // not before this product's issue: it waits for the matrix cores to be done with the two before it. (Left
-        // to the compiler, which does not know the asm's latency, the sums were read one product too early.)
-        if constexpr (__is_same(TO, bf16_t)) asm volatile("" : "+v"(part[(q - 2) % 3]));
-        add(std::integral_constant<int, q - 2>{});
+      // not before this product's issue: it waits for the matrix cores to be done with the two before it. (Left
+      // to the compiler, which does not know the asm's latency, the sums were read one product too early.)
+      constexpr int done = (q + P - 2) % P;
+      if constexpr (__is_same(TO, bf16_t)) asm volatile("" : "+v"(part[done % 4]));
+      add(std::integral_constant<int, done>{});
+      if constexpr (q == 1) {
+#pragma unroll
+        for (int t = 0; t < JT; ++t) sc[t] = next_sc[t] * next_ws;
       }
       __builtin_amdgcn_sched_barrier(0);
     });
-    asm volatile("s_nop 15\n\ts_nop 3" : "+v"(part[0]), "+v"(part[1]), "+v"(part[2]));  // the last products are through
-    if constexpr (P >= 2) add(std::integral_constant<int, P - 2>{});
-    add(std::integral_constant<int, P - 1>{});
-    slot = slot + 1 == D ? 0 : slot + 1;
+    slot = after;
   }
+  asm volatile("s_nop 15\n\ts_nop 3" : "+v"(part[2]), "+v"(part[3]));  // the last products are through
+  add(std::integral_constant<int, P - 2>{});
+  add(std::integral_constant<int, P - 1>{});
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");  // no DMA and no read of the LDS is on its way,
   __syncthreads();                                              // of any wave
 
