@@ -66,35 +66,40 @@ def latent_rope_and_cache(
     if latent.shape[0] != n_tok or k_rope.shape != (n_tok, rope):
         raise ValueError(f"latent {tuple(latent.shape)} and k_rope {tuple(k_rope.shape)} do not match q_rope "
                          f"{tuple(q_rope.shape)}")
-    for c, name in ((cos, "cos"), (sin, "sin")):
-        if c.shape != (n_tok, rope):
-            raise ValueError(f"{name} {tuple(c.shape)} != [{n_tok}, {rope}]")
+    if cos.shape != (n_tok, rope) or sin.shape != cos.shape:
+        raise ValueError(f"cos {tuple(cos.shape)} and sin {tuple(sin.shape)} must be [{n_tok}, {rope}]")
     if norm_weight is not None and norm_weight.shape != (width,):
         raise ValueError(f"norm_weight {tuple(norm_weight.shape)} != [{width}]")
     if slot_mapping.numel() != n_tok:
         raise ValueError(f"slot_mapping {slot_mapping.numel()} != tokens {n_tok}")
     check_latent_cache(latent_cache, layer_idx, block_size, width + rope)
-    given = [q_rope, latent, k_rope, cos, sin, latent_cache] + ([] if norm_weight is None else [norm_weight])
-    if any(t.dtype != q_rope.dtype for t in given):
-        raise ValueError(f"all tensors must share one dtype, got {sorted({str(t.dtype) for t in given})}")
-    dtype = _ffi.dtype_code(q_rope.dtype)
+    weight = latent if norm_weight is None else norm_weight
+    dtype, device = q_rope.dtype, q_rope.device
+    if not dtype == latent.dtype == k_rope.dtype == cos.dtype == sin.dtype == latent_cache.dtype == weight.dtype:
+        raise ValueError(f"all tensors must share one dtype, got {dtype}, {latent.dtype}, {k_rope.dtype}, {cos.dtype}, "
+                         f"{sin.dtype}, {latent_cache.dtype} and {weight.dtype}")
+    code = _ffi.dtype_code(dtype)
     if out is None:
-        out = torch.empty((n_tok, heads, rope), dtype=q_rope.dtype, device=q_rope.device)
-    elif out.shape != q_rope.shape or out.dtype != q_rope.dtype or out.device != q_rope.device:
-        raise ValueError(f"out must be {tuple(q_rope.shape)} {q_rope.dtype} on {q_rope.device}")
+        out = torch.empty((n_tok, heads, rope), dtype=dtype, device=device)
+    elif out.shape != q_rope.shape or out.dtype != dtype or out.device != device:
+        raise ValueError(f"out must be {tuple(q_rope.shape)} {dtype} on {device}")
     if n_tok == 0:
         return out
-    require_device("latent_rope_and_cache", *given, slot_mapping)
-    if any(t.shape[-1] > 1 and t.stride(-1) != 1 for t in (*given, out)):
+    require_device("latent_rope_and_cache", q_rope, latent, k_rope, cos, sin, latent_cache, weight, slot_mapping)
+    qs, os, ls, ks, cs, ss, cst = (q_rope.stride(), out.stride(), latent.stride(), k_rope.stride(), cos.stride(),
+                                   sin.stride(), latent_cache.stride())
+    # (of a tensor of one column any last stride will do)
+    if (rope > 1 and not qs[2] == os[2] == ks[1] == cs[1] == ss[1] == 1) or cst[3] != 1 or (
+            width > 1 and not ls[1] == weight.stride(-1) == 1):
         raise ValueError("every tensor needs a unit last stride")
-    slots = slot_mapping.to(torch.int64).reshape(-1).contiguous()
-    cst = latent_cache.stride()
+    slots = slot_mapping
+    if slots.dtype != torch.int64 or not slots.is_contiguous():
+        slots = slots.to(torch.int64).contiguous()
     status = launch(
-        q_rope.device, _ffi.lib().ss_latent_rope_and_cache, q_rope.data_ptr(), out.data_ptr(), latent.data_ptr(),
+        device, _ffi.lib().ss_latent_rope_and_cache, q_rope.data_ptr(), out.data_ptr(), latent.data_ptr(),
         k_rope.data_ptr(), cos.data_ptr(), sin.data_ptr(), None if norm_weight is None else norm_weight.data_ptr(),
         layer_ptr(latent_cache, layer_idx), slots.data_ptr(), n_tok, heads, width, rope, block_size,
-        latent_cache.shape[1] * block_size, _ffi.i64x2(q_rope.stride(0), q_rope.stride(1)),
-        _ffi.i64x2(out.stride(0), out.stride(1)), latent.stride(0), k_rope.stride(0), cos.stride(0), sin.stride(0),
-        _ffi.i64x2(cst[1], cst[2]), eps, dtype)
+        latent_cache.shape[1] * block_size, _ffi.i64x2(qs[0], qs[1]), _ffi.i64x2(os[0], os[1]), ls[0], ks[0], cs[0],
+        ss[0], _ffi.i64x2(cst[1], cst[2]), eps, code)
     _ffi.check(status, "latent_rope_and_cache")
     return out
