@@ -29,7 +29,10 @@
 namespace ss {
 namespace {
 
-constexpr int kLeastTiles = 4;
+// Ranges of a call of few tiles: a range of t tiles takes t steps, and its partial rows are written and read
+// again, rows a tile at a time, by as many workgroups as there are: the least of tiles / ranges * kStep + ranges * rows
+// * kRow, in us (a step 1.6 .. 2; 4 KB a row written and read at some 5 TB/s)
+constexpr float kStep = 1.8f, kRow = 0.5e-3f;
 
 template <int R_, int RT_, int NW_>
 struct LatTile {
@@ -765,10 +768,11 @@ __global__ __launch_bounds__(64 * C::NW) __attribute__((amdgpu_waves_per_eu(C::N
   const int w = all & 7 ? (int)blockIdx.x : (int)(blockIdx.x & 7) * per_xcd + (int)(blockIdx.x >> 3);
 
   // the sequences' lengths in tiles, summed: where this workgroup's range begins
-  int64_t* const s_sum = reinterpret_cast<int64_t*>(s_lat + C::kScan);  // [NW], then the sequence found
+  int64_t* const s_sum = reinterpret_cast<int64_t*>(s_lat + C::kScan);  // [NW], then what was found
+  SeqView view = {0, 0, 0, 0};
   auto scan = [&](int b, int64_t& mine) {  // the sum up to and with sequence b, and that of the NT
     mine = 0;
-    if (b < p.batch) mine = seq_tiles(seq_view(p, b, work.lo, work.hi), shape);
+    if (b < p.batch) view = seq_view(p, b, work.lo, work.hi), mine = seq_tiles(view, shape);
     int64_t sum = mine;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
@@ -787,8 +791,8 @@ __global__ __launch_bounds__(64 * C::NW) __attribute__((amdgpu_waves_per_eu(C::N
     for (int i = 0; i < C::NW; ++i) total += s_sum[i];
   }
   total = uniform(total);
-  // as many ranges as there are workgroups, so long as they have kLeastTiles tiles or a sequence each
-  const int groups = (int)min((int64_t)all, max(total / kLeastTiles, min(total, (int64_t)p.batch)));
+  const int64_t most = max((int64_t)sqrtf((float)total * (kStep / (kRow * C::ROWS))), min(total, (int64_t)p.batch));
+  const int groups = (int)min(min((int64_t)all, total), most);
   int* const rec = work.rec + 4 * w;
   if (w >= groups) {
     if (threadIdx.x == 0) rec[0] = -1;
@@ -806,17 +810,20 @@ __global__ __launch_bounds__(64 * C::NW) __attribute__((amdgpu_waves_per_eu(C::N
     if (upto - mine <= u && u < upto) {
       s_sum[C::NW] = b0 + threadIdx.x;
       s_sum[C::NW + 1] = upto - mine;
+      *reinterpret_cast<SeqView*>(s_sum + C::NW + 2) = view;
     }
     __syncthreads();
     if (p.batch <= NT || u < done) break;
   }
   b = __builtin_amdgcn_readfirstlane((int)s_sum[C::NW]);
   before = uniform(s_sum[C::NW + 1]);
+  SeqView v = *reinterpret_cast<SeqView*>(s_sum + C::NW + 2);
+  v.n = __builtin_amdgcn_readfirstlane(v.n), v.start = __builtin_amdgcn_readfirstlane(v.start);
+  v.length = __builtin_amdgcn_readfirstlane(v.length), v.keys = __builtin_amdgcn_readfirstlane(v.keys);
   __syncthreads();
 
   const int64_t u0 = u;
-  for (; u < u1; ++b) {
-    const SeqView v = seq_view(p, b, work.lo, work.hi);
+  for (;; v = seq_view(p, ++b, work.lo, work.hi)) {
     const int nt = (v.n + (1 << shape.js) - 1) >> shape.js;
     const int64_t end = before + seq_tiles(v, shape);
     if (u >= end) continue;  // no rows of this launch
@@ -850,29 +857,48 @@ __global__ __launch_bounds__(64 * C::NW) __attribute__((amdgpu_waves_per_eu(C::N
         u = e;
       }
     }
+    if (u >= u1) break;
     before = end;
   }
 }
 
-// The partial rows of an item that is cut, added in the order of its ranges: a wave one row of the item
-// whose first cut is the begin of range w. The parts' maxima and sums are read 64 at a time, a part a
-// lane; then the rows, eight parts' on their way at once.
-template <typename T, int R, int ROWS>
-__global__ __launch_bounds__(256) void latent_merge_kernel(const LatentParams p, const LatentWork work) {
-  const int w = blockIdx.x;
+// The partial rows of an item that is cut, added in the order of its ranges: WPR waves one row of the item
+// whose first cut is the begin of range w, each an equal part of the ranges. The parts' maxima and sums are read
+// 64 at a time, a part a lane; then the rows, eight parts' on their way at once. With one wave a row blockIdx.x is w;
+// else it counts the ranges at whose begin an item is merged, of which there are at most as many as items.
+template <typename T, int R, int ROWS, int WPR>
+__global__ __launch_bounds__(WPR == 1 ? 256 : 64 * WPR) void latent_merge_kernel(const LatentParams p, const LatentWork work,
+                                                                                int groups) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int w = blockIdx.x;
+  if constexpr (WPR > 1) {
+    int left = w;
+    w = -1;
+    for (int w0 = 0; w0 < groups && w < 0; w0 += 64) {
+      const bool here = w0 + lane < groups && work.rec[4 * (w0 + lane)] >= 0;
+      uint64_t m = __ballot(here);
+      if (__popcll(m) <= left) {
+        left -= __popcll(m);
+        continue;
+      }
+      for (; left > 0; --left) m &= m - 1;
+      w = w0 + __builtin_ctzll(m);
+    }
+    if (w < 0) return;
+  }
   const int* const rec = work.rec + 4 * w;
   const int b = rec[0];
   if (b < 0) return;
   const RowShape shape = row_shape<ROWS>(p.heads);
-  const int item = rec[1], parts = rec[2] - w + 2;  // ranges w - 1 .. rec[2]
+  const int item = rec[1], all = rec[2] - w + 2;  // ranges w - 1 .. rec[2]
   const SeqView v = seq_view(p, b, work.lo, work.hi);
   const int tok0 = item / shape.hs << shape.js, head0 = item % shape.hs * ROWS;
   const int heads = min(p.heads - head0, ROWS), tokens = min(1 << shape.js, v.n - tok0);
-  const int rr = __builtin_amdgcn_readfirstlane(4 * blockIdx.y + (threadIdx.x >> 6)), j = rr / heads;
+  const int rr = WPR == 1 ? 4 * blockIdx.y + wave : blockIdx.y, j = rr / heads;
   if (j >= tokens) return;
   constexpr int PER = R / 64;  // values of a lane
-  const int lane = threadIdx.x & 63;
-  auto row = [&](int i) { return (int64_t)(i == 0 ? 2 * w - 1 : 2 * (w - 1 + i)) * ROWS + rr; };
+  const int each = (all + WPR - 1) / WPR, from = wave % WPR * each, parts = min(all - from, each);  // (none or less: none)
+  auto row = [&](int i) { return (int64_t)(from + i == 0 ? 2 * w - 1 : 2 * (w - 1 + from + i)) * ROWS + rr; };
   float top = kNegBig, sum = 0.f, o[PER] = {};
   for (int i0 = 0; i0 < parts; i0 += 64) {
     float2 ml = {kNegBig, 0.f};
@@ -890,33 +916,63 @@ __global__ __launch_bounds__(256) void latent_merge_kernel(const LatentParams p,
 #pragma unroll
     for (int d = 0; d < PER; ++d) o[d] *= before;
     const int here = min(64, parts - i0);
-    for (int i = 0; i < here; i += 8) {
-      f32x4 x[8][PER / 4];
+    auto take = [&](int i, auto count) {
+      constexpr int N = decltype(count)::value;
+      f32x4 x[N][PER / 4];
 #pragma unroll
-      for (int k = 0; k < 8; ++k)
+      for (int k = 0; k < N; ++k)
 #pragma unroll
         for (int d = 0; d < PER / 4; ++d)
-          x[k][d] = *reinterpret_cast<const f32x4*>(work.o + row(i0 + min(i + k, here - 1)) * R + d * 256 + 4 * lane);
+          x[k][d] = *reinterpret_cast<const f32x4*>(work.o + row(i0 + i + k) * R + d * 256 + 4 * lane);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        if (i + k >= here) continue;
+      for (int k = 0; k < N; ++k) {
         const float fk = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), i + k));
 #pragma unroll
         for (int d = 0; d < PER; ++d) o[d] = fmaf(x[k][d >> 2][d & 3], fk, o[d]);
       }
-    }
+    };
+    int i = 0;
+    for (; i + 8 <= here; i += 8) take(i, std::integral_constant<int, 8>{});
+    if (here - i >= 4) take(i, std::integral_constant<int, 4>{}), i += 4;
+    if (here - i >= 2) take(i, std::integral_constant<int, 2>{}), i += 2;
+    if (here > i) take(i, std::integral_constant<int, 1>{});
   }
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
   T* const out = (T*)p.out + (p.cu ? 0 : b * p.o_sb) + (v.start + tok0 + j) * p.o_st + (head0 + rr - j * heads) * p.o_sh;
+  if constexpr (WPR > 1) {  // the waves' sums, in their order
+    __shared__ float s_o[WPR][R];
+    __shared__ float2 s_ml[WPR];
 #pragma unroll
-  for (int d = 0; d < PER; d += 4)
-    *reinterpret_cast<u32x2*>(out + d * 64 + 4 * lane) =
-        u32x2{Elem<T>::pack2(o[d] * inv, o[d + 1] * inv), Elem<T>::pack2(o[d + 2] * inv, o[d + 3] * inv)};
+    for (int d = 0; d < PER; d += 4)
+      *reinterpret_cast<f32x4*>(&s_o[wave][d * 64 + 4 * lane]) = f32x4{o[d], o[d + 1], o[d + 2], o[d + 3]};
+    if (lane == 0) s_ml[wave] = float2{top, sum};
+    __syncthreads();
+    if ((int)threadIdx.x >= R / 2) return;
+    float most = kNegBig;
+#pragma unroll
+    for (int k = 0; k < WPR; ++k) most = fmaxf(most, s_ml[k].x);
+    float2 y = {0.f, 0.f};
+    sum = 0.f;
+#pragma unroll
+    for (int k = 0; k < WPR; ++k) {
+      const float f = fast_exp2(s_ml[k].x - most);
+      const float2 x = *reinterpret_cast<const float2*>(&s_o[k][2 * threadIdx.x]);
+      sum = fmaf(s_ml[k].y, f, sum);
+      y.x = fmaf(x.x, f, y.x), y.y = fmaf(x.y, f, y.y);
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    *reinterpret_cast<uint32_t*>(out + 2 * threadIdx.x) = Elem<T>::pack2(y.x * inv, y.y * inv);
+  } else {
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+    for (int d = 0; d < PER; d += 4)
+      *reinterpret_cast<u32x2*>(out + d * 64 + 4 * lane) =
+          u32x2{Elem<T>::pack2(o[d] * inv, o[d + 1] * inv), Elem<T>::pack2(o[d + 2] * inv, o[d + 3] * inv)};
+  }
 }
 
 // ---- host ---------------------------------------------------------------------------------------
 
-constexpr int64_t kAlign = 256;
+constexpr int64_t kAlign = 256, kFewRows = 2048;
 int64_t up(int64_t n) { return (n + kAlign - 1) / kAlign * kAlign; }
 
 int64_t part_bytes(int rows, int r) {
@@ -938,8 +994,16 @@ int launch_rows(const LatentParams& p, int lo, int hi, char* ws, hipStream_t str
   if (const int st = reserve_lds((const void*)kern, C::LDS, done); st != SS_OK) return st;
   hipLaunchKernelGGL(kern, dim3((unsigned)groups), dim3(64 * NW), C::LDS, stream, p, work);
   if (const int st = ss_host::launch_status("latent attention"); st != SS_OK) return st;
-  hipLaunchKernelGGL((latent_merge_kernel<T, R, C::ROWS>), dim3((unsigned)groups, C::ROWS / 4), dim3(256), 0, stream, p,
-                     work);
+  // Many items are cut once or twice each: a wave a row (of 256 decodes of 128 heads). Few are cut often: sixteen
+  // waves a row, and no more workgroups than there may be items.
+  const RowShape shape = row_shape<C::ROWS>(p.heads);
+  const int64_t tiles = p.cu ? (int64_t)p.batch + (p.total >> shape.js) : (int64_t)p.batch * (((p.tq - 1) >> shape.js) + 1);
+  if (tiles * shape.hs * C::ROWS <= kFewRows)
+    hipLaunchKernelGGL((latent_merge_kernel<T, R, C::ROWS, 16>), dim3((unsigned)(tiles * shape.hs), C::ROWS), dim3(1024), 0,
+                       stream, p, work, (int)groups);
+  else
+    hipLaunchKernelGGL((latent_merge_kernel<T, R, C::ROWS, 1>), dim3((unsigned)groups, C::ROWS / 4), dim3(256), 0, stream,
+                       p, work, (int)groups);
   return ss_host::launch_status("latent attention (merge)");
 }
 
