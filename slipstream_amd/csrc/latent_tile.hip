@@ -472,11 +472,9 @@ __device__ __forceinline__ void latent_segment_wide(const LatentParams& p, const
     return j < tokens;
   };
 
-  Feed<C> feed(p, b, lds, kv_end, t0, tend);  // begun before anything else is waited for
-  for (int i = 0; i < 3; ++i) {
-    feed.aim(t0 + i, i, i);
-    feed.all();
-  }
+  Feed<C> feed(p, b, lds, kv_end, t0, tend);
+  feed.aim(t0, 0, 0);  // what the first scores need comes first: their keys, then the queries
+  feed.all();
 
   u32x4 qop[KS + KR];
   int lim = min(kv_end, t1 * 32);  // keys of this lane's row up to here (its part of the item's)
@@ -489,7 +487,13 @@ __device__ __forceinline__ void latent_segment_wide(const LatentParams& p, const
                        (ok ? head : head0) * p.q_sh + 8 * h;
     const uint32_t flip = p.scale_log2 < 0.f ? 0x80008000u : 0u, keep = ok ? ~0u : 0u;
 #pragma unroll
-    for (int s = 0; s < KS + KR; ++s) qop[s] = (load16(q + 16 * s) ^ u32x4{flip, flip, flip, flip}) & u32x4{keep, keep, keep, keep};
+    for (int s = 0; s < KS + KR; ++s) qop[s] = load16(q + 16 * s);
+    for (int i = 1; i < 3; ++i) {
+      feed.aim(t0 + i, i, i);
+      feed.all();
+    }
+#pragma unroll
+    for (int s = 0; s < KS + KR; ++s) qop[s] = (qop[s] ^ u32x4{flip, flip, flip, flip}) & u32x4{keep, keep, keep, keep};
   }
   const float cscale = fabsf(p.scale_log2);
   int least = lim;
@@ -648,7 +652,7 @@ __device__ __forceinline__ void latent_segment_wide(const LatentParams& p, const
         m = mn;
         // (by every lane, without a branch: behind one the compiler would gather the parts before it)
         *reinterpret_cast<float*>(lds + C::kAlpha + ((buf ^ 1) * C::ROWS + 32 * wave + (fresh() & 31)) * 4) = alpha;
-        *reinterpret_cast<int*>(lds + C::kGrew + ((buf ^ 1) * 4 + wave) * 4) = grew;
+        *reinterpret_cast<int*>(lds + C::kGrew + ((buf ^ 1) * 4 + wave) * 4) = OUT && grew;  // (before the first outputs are 0)
       } else if constexpr (i < kParts) {
         constexpr int q = i - 17;
         store16(lds + C::kP + (buf ^ 1) * C::PB + (2 * wave + q) * 1024 + fresh() * 16,
@@ -708,47 +712,54 @@ __device__ __forceinline__ void latent_segment_wide(const LatentParams& p, const
     if (h == 0) *reinterpret_cast<float2*>(lds + C::kMl + (32 * wave + n) * 8) = float2{m, sum};
   }
   __syncthreads();
-  // result r of output tile dt: value 8 chunk + 4 h + r % 4 of row n
+  // Result r of output tile dt: value 8 chunk + 4 h + r % 4 of row n. The rows go through the LDS, where the tiles
+  // were, 64 at a time, and are stored whole: a row's 16-byte pieces lie there at piece ^ (row % 16). (Stored as they
+  // are in the registers, 32 bytes of 32 rows an instruction, 128 rows in fp32 took 16 us, now 9. Scaled and
+  // rounded in the registers, whole ones took 9 as well, for the code's way into the instruction cache.)
   auto chunk = [&](int dt, int x) {
     return DT == 4 ? dt + 4 * x + 16 * wave : dt + 2 * (wave & 1) + 4 * x + 16 * (wave >> 1);
   };
-  if (whole) {
+  constexpr int B = 4 * R, L = R / 8;  // bytes of a row in the LDS, lanes of a row in the stores
+  const int rows = tokens * heads, c = lane % L;
+  T* const to = (T*)p.out + (p.cu ? 0 : b * p.o_sb) + (v.start + tok0) * p.o_st + head0 * p.o_sh + 8 * c;
+  float* const o = work.o + (int64_t)slot * C::ROWS * R + 4 * c;
 #pragma unroll
-    for (int rt = 0; rt < 4; ++rt) {
-      int tok, head;
-      const bool ok = row_of(rt, tok, head);
-      const float total = reinterpret_cast<const float2*>(lds + C::kMl + (32 * rt + n) * 8)->y;
-      const float inv = total == 0.f ? 0.f : 1.f / total;
-      T* const o = (T*)p.out + (p.cu ? 0 : b * p.o_sb) + (v.start + tok) * p.o_st + head * p.o_sh;
+  for (int half = 0; half < 2; ++half) {
+    if (half) __syncthreads();
+    const uint32_t row = lbase + n * B;
+#pragma unroll
+    for (int rt = 0; rt < 2; ++rt)
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-        for (int x = 0; x < 4; x += 2) {
-          // the halves of chunks x and x + 1 change places so that a lane holds one whole
-          uint32_t w[2][2];
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const uint32_t even = Elem<T>::pack2(acc[rt][dt][4 * x + 2 * e] * inv, acc[rt][dt][4 * x + 2 * e + 1] * inv);
-            const uint32_t odd = Elem<T>::pack2(acc[rt][dt][4 * x + 4 + 2 * e] * inv, acc[rt][dt][4 * x + 5 + 2 * e] * inv);
-            auto sw = __builtin_amdgcn_permlane32_swap(even, odd, false, false);
-            w[e][0] = sw[0], w[e][1] = sw[1];
-          }
-          if (ok) {
-            const u32x4 y = {w[0][0], w[1][0], w[0][1], w[1][1]};
-            __builtin_memcpy(o + 8 * chunk(dt, x + h), &y, 16);
-          }
+        for (int x = 0; x < 4; ++x) {
+          const f32x16& a = acc[2 * half + rt][dt];
+          *(__attribute__((address_space(3))) f32x4*)(uintptr_t)(row + 32 * rt * B + 16 * ((2 * chunk(dt, x) + h) ^ (n & 15))) =
+              f32x4{a[4 * x], a[4 * x + 1], a[4 * x + 2], a[4 * x + 3]};
         }
+    __syncthreads();
+    if (whole) {
+      const int end = min(64, rows - 64 * half);
+#pragma unroll 4
+      for (int r = (64 / L) * wave + lane / L; r < end; r += 256 / L) {
+        const float total = reinterpret_cast<const float2*>(lds + C::kMl + (64 * half + r) * 8)->y;
+        const float inv = total == 0.f ? 0.f : 1.f / total;
+        const f32x4 lo = *reinterpret_cast<const f32x4*>(lds + r * B + 16 * ((2 * c) ^ (r & 15))) * inv;
+        const f32x4 hi = *reinterpret_cast<const f32x4*>(lds + r * B + 16 * ((2 * c + 1) ^ (r & 15))) * inv;
+        const u32x4 y = {Elem<T>::pack2(lo[0], lo[1]), Elem<T>::pack2(lo[2], lo[3]), Elem<T>::pack2(hi[0], hi[1]),
+                         Elem<T>::pack2(hi[2], hi[3])};
+        const int j = (64 * half + r) / heads;
+        __builtin_memcpy(to + j * p.o_st + (64 * half + r - j * heads) * p.o_sh, &y, 16);
+      }
+    } else {
+#pragma unroll 4
+      for (int r = (64 / L) * wave + lane / L; r < 64; r += 256 / L)
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+          store16(o + (64 * half + r) * R + 4 * u * L, load16(lds + r * B + 16 * ((u * L + c) ^ (r & 15))));
     }
-  } else {
-    float* const o = work.o + (int64_t)slot * C::ROWS * R + 4 * h;
-#pragma unroll
-    for (int rt = 0; rt < 4; ++rt)
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-        for (int x = 0; x < 4; ++x)
-          *reinterpret_cast<f32x4*>(o + (32 * rt + n) * R + 8 * chunk(dt, x)) =
-              f32x4{acc[rt][dt][4 * x], acc[rt][dt][4 * x + 1], acc[rt][dt][4 * x + 2], acc[rt][dt][4 * x + 3]};
+  }
+  if (!whole) {
     float* const ml = work.ml + (int64_t)slot * C::ROWS * 2;
     ml[threadIdx.x] = *reinterpret_cast<const float*>(lds + C::kMl + 4 * threadIdx.x);
   }
