@@ -29,40 +29,46 @@ struct LatExp {
 
 template <typename T, typename C>
 __global__ __launch_bounds__(64 * C::NW) __attribute__((amdgpu_waves_per_eu(C::NW == 8 ? 2 : 1, C::NW == 8 ? 2 : 1))) void
-latent_expanded_kernel(const LatentParams p, int tiles) {
+latent_expanded_kernel(const LatentParams p) {
   extern __shared__ __attribute__((aligned(1024))) char s_exp[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 31, h = lane >> 5;
-  // workgroups go round robin over the eight XCDs: a head's tiles follow each other on one of them, whose L2
-  // then serves their keys
-  const int slot = blockIdx.x >> 3, head = 8 * (slot / tiles) + (blockIdx.x & 7);
-  if (head >= p.heads) return;
-  // the tile's sequence: the sequences' numbers of tiles summed, 64 at a time
-  int left = slot % tiles, b = -1, count = 0, start = 0;
+  // Workgroups go round robin over the eight XCDs, and a sequence's tiles of a head follow each other on one of
+  // them, whose L2 then serves their keys. The sequences of the most keys come first, so that no long tile begins
+  // when the others end (in the order of the batch: 4 chunks of 512 over up to 4096, 128 heads 540 us); of more than
+  // 64 sequences each 64 are ordered. A sequence's first tile is the number of those of the ones before it.
+  const int slot = blockIdx.x >> 3, groups = (p.heads + 7) >> 3;
+  int left = slot, b = -1, count = 0, start = 0, head = 0, tile = 0;
   for (int b0 = 0; b0 < p.batch; b0 += 64) {
-    int c = 0, s = 0;
-    if (b0 + lane < p.batch) latent_queries(p, b0 + lane, c, s);
+    int c = 0, s = 0, k = 0;
+    if (b0 + lane < p.batch) {
+      int first, length;
+      latent_queries(p, b0 + lane, c, s);
+      k = latent_keys(p, b0 + lane, first, length);
+    }
     const int mine = (c + C::ROWS - 1) / C::ROWS;
-    int sum = mine;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int below = __shfl_up(sum, o);
-      sum += lane >= o ? below : 0;
+    int before = 0, all = 0;
+    for (int i = 0; i < min(64, p.batch - b0); ++i) {
+      const int ki = __builtin_amdgcn_readlane(k, i), ti = __builtin_amdgcn_readlane(mine, i);
+      before += ki > k || (ki == k && i < lane) ? ti : 0;
+      all += ti;
     }
-    const uint64_t there = __ballot(sum > left);
-    if (there) {
-      const int i = __builtin_ctzll(there);
-      b = b0 + i;
-      count = __builtin_amdgcn_readlane(c, i);
-      start = __builtin_amdgcn_readlane(s, i);
-      left -= __builtin_amdgcn_readlane(sum - mine, i);
-      break;
+    if (left >= all * groups) {
+      left -= all * groups;
+      continue;
     }
-    left -= __builtin_amdgcn_readlane(sum, 63);
+    const int i = __builtin_ctzll(__ballot(left >= before * groups && left < (before + mine) * groups));
+    b = b0 + i;
+    count = __builtin_amdgcn_readlane(c, i);
+    start = __builtin_amdgcn_readlane(s, i);
+    const int tiles = __builtin_amdgcn_readlane(mine, i);
+    left -= __builtin_amdgcn_readlane(before, i) * groups;
+    head = 8 * (left / tiles) + (blockIdx.x & 7);
+    tile = tiles - 1 - left % tiles;  // the last ones, which see the most keys, first
+    break;
   }
-  if (b < 0) return;
-  left = __builtin_amdgcn_readfirstlane(left);
-  const int tile = (count + C::ROWS - 1) / C::ROWS - 1 - left;  // the last ones, which see the most keys, first
+  if (b < 0 || head >= p.heads) return;
+  head = __builtin_amdgcn_readfirstlane(head), tile = __builtin_amdgcn_readfirstlane(tile);
   int k0, length;
   const int keys = latent_keys(p, b, k0, length);
   const int tok0 = tile * C::ROWS;
@@ -298,7 +304,7 @@ int launch_rows(const LatentParams& p, hipStream_t stream) {
   auto kern = latent_expanded_kernel<T, C>;
   static std::atomic<uint64_t> done{0};
   if (const int st = reserve_lds((const void*)kern, C::LDS, done); st != SS_OK) return st;
-  hipLaunchKernelGGL(kern, dim3((unsigned)(tiles * slots * 8)), dim3(64 * C::NW), C::LDS, stream, p, (int)tiles);
+  hipLaunchKernelGGL(kern, dim3((unsigned)(tiles * slots * 8)), dim3(64 * C::NW), C::LDS, stream, p);
   return ss_host::launch_status("latent attention (expanded)");
 }
 
