@@ -23,7 +23,7 @@ struct LatExp {
   static constexpr int NW = NW_, D = D_, ROWS = 32 * NW, KT = 64;
   static constexpr int KP = KT * 2 * kNope, RP = KT * 2 * kRopeDim, VP = KT * 2 * kValue;  // bytes of a tile's planes
   static constexpr int kR = D * KP, kV = kR + D * RP, LDS = kV + D * VP;
-  static constexpr int NK = 16 / NW, NR = 8 / NW, PER = 2 * NK + NR;  // DMA instructions of a wave and tile
+  static constexpr int NK = 16 / NW, NR = 8 / NW;  // DMA instructions of a wave and tile: a head's keys (or values), shared keys
   static_assert(LDS <= 160 * 1024, "fits");
 };
 
@@ -100,22 +100,26 @@ latent_expanded_kernel(const LatentParams p) {
     const int row = 8 * (C::NR * wave + u);
     dma_b128(rs, (LdsBytes)(uintptr_t)(to + row * 128), (chunk8 ^ 16 * tile_swizzle(row)) + (lane8 + row * r_bytes), 0);
   };
-  // group j: the keys of tile j into slot ks and the values of tile j - 1 into slot vs; always as many
-  // instructions, so that the waits can count them
-  auto issue = [&](int j, int ks, int vs) __attribute__((always_inline)) {
-    const i32x4 rk = plane(kv0, j, kv_bytes, 2 * kNope), rr = plane(r0, j, r_bytes, 2 * kRopeDim),
-                rv = plane(kv0 + 2 * kNope, j - 1, kv_bytes, 2 * kValue);
-    asm volatile("s_nop 4" : : "s"(rk), "s"(rr), "s"(rv));  // SGPRs that a VALU wrote: five wait states before a VMEM
+  // always as many instructions, so that the waits can count them
+  auto issue_keys = [&](int j, int slot) __attribute__((always_inline)) {
+    const i32x4 rk = plane(kv0, j, kv_bytes, 2 * kNope), rr = plane(r0, j, r_bytes, 2 * kRopeDim);
+    asm volatile("s_nop 4" : : "s"(rk), "s"(rr));  // SGPRs that a VALU wrote: five wait states before a VMEM
 #pragma unroll
-    for (int u = 0; u < C::NK; ++u) dma4(rk, lds + ks * C::KP, u);
+    for (int u = 0; u < C::NK; ++u) dma4(rk, lds + slot * C::KP, u);
 #pragma unroll
-    for (int u = 0; u < C::NR; ++u) dma8(rr, lds + C::kR + ks * C::RP, u);
-#pragma unroll
-    for (int u = 0; u < C::NK; ++u) dma4(rv, lds + C::kV + vs * C::VP, u);
+    for (int u = 0; u < C::NR; ++u) dma8(rr, lds + C::kR + slot * C::RP, u);
   };
-  static_for<C::D>([&](auto j) __attribute__((always_inline)) {
+  auto issue_values = [&](int j, int slot) __attribute__((always_inline)) {
+    const i32x4 rv = plane(kv0 + 2 * kNope, j, kv_bytes, 2 * kValue);
+    asm volatile("s_nop 4" : : "s"(rv));
+#pragma unroll
+    for (int u = 0; u < C::NK; ++u) dma4(rv, lds + C::kV + slot * C::VP, u);
+  };
+  issue_keys(0, 0);
+  static_for<C::D - 1>([&](auto j) __attribute__((always_inline)) {
     constexpr int g = decltype(j)::value;
-    issue(g, g, g == 0 ? C::D - 1 : g - 1);
+    issue_keys(g + 1, g + 1);
+    issue_values(g, g);
   });
 
   // ---- the wave's rows
@@ -154,13 +158,85 @@ latent_expanded_kernel(const LatentParams p) {
   const int sl = lane & 15, vrow = 4 * h + (sl >> 2), quad = 2 * ((lane >> 4) & 1) + ((sl & 3) >> 1);
   const uint32_t vaddr = lds + C::kV + vrow * 256 + 8 * (sl & 1) + 16 * ((4 * quad) ^ lat_swizzle(vrow));
 
-  // One step of a wave: the scores of the tile in key slot ks into `next` and between their products the
-  // softmax of tile t's scores in `cur`, then (OUT) the outputs of tile t from value slot vs.
-  constexpr int AHEAD = 4, PARTS = 22;
-  auto step = [&](auto outc, int t, int ks, int vs, f32x16 (&cur)[2], f32x16 (&next)[2]) __attribute__((always_inline)) {
+  // A step of a wave in two parts: the scores of tile t + 1, then the outputs of tile t. A tile's softmax is written
+  // between the products from the outputs of the tile before to its own, a few instructions that do not wait for each
+  // other at a time: at two waves a SIMD one that waits for the instruction before it costs twice its own time.
+  constexpr int AHEAD = 4;
+  u32x4 vring[AHEAD];
+  uint32_t pk[16], va = 0;
+  float alpha = 1.f, mn = 0.f, sum = 0.f, top[4], ex[2][2], fx[2][2];
+  bool grew = false;
+  // part i of the softmax of the scores x: the maximum (0 .. 6), the exponents of pair i - 7, the probabilities of
+  // the pair before and the sum and rounding of the one before that, and the row's new state
+  constexpr int PARTS = 26, EARLY = 10;  // EARLY parts among the outputs of the tile before
+  auto part = [&](auto ic, f32x16 (&x)[2]) __attribute__((always_inline)) {
+    constexpr int i = ic;
+    if constexpr (i < 4) {
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const f32x16& v = x[u >> 1];
+        constexpr int at = i == 0 ? 0 : 2 * i + 1;  // three values, then two, two and one
+        const int e = 8 * (u & 1) + at;
+        top[u] = i == 0 ? max3(v[e], v[e + 1], v[e + 2]) : i < 3 ? max3(top[u], v[e], v[e + 1]) : max3(top[u], v[e], v[e]);
+      }
+    } else if constexpr (i == 4) {
+      top[0] = max3(top[0], top[1], top[2]);
+      top[0] = max3(top[0], top[3], top[3]);
+    } else if constexpr (i == 5) {
+      const uint32_t tb = __builtin_bit_cast(uint32_t, top[0]);
+      auto sw = __builtin_amdgcn_permlane32_swap(tb, tb, false, false);
+      top[0] = max3(__builtin_bit_cast(float, (uint32_t)sw[0]), __builtin_bit_cast(float, (uint32_t)sw[1]), kNegBig);
+      top[0] = fmaxf(m, top[0] * cscale);
+    } else if constexpr (i == 6) {
+      grew = __any(top[0] > m + kSlack);
+      mn = grew ? top[0] : m;
+      sum = 0.f;
+    } else if constexpr (i < PARTS - 1) {
+      constexpr int q = i - 7;
+      if constexpr (q >= 2) {
+        constexpr int d = q - 2;
+        pk[d] = Elem<T>::pack2(ex[d & 1][0], ex[d & 1][1]);
+        sum += ex[d & 1][0] + ex[d & 1][1];
+        asm volatile("" : "+v"(pk[d]), "+v"(sum));  // made here
+      }
+      if constexpr (q >= 1 && q <= 16) {
+        constexpr int d = q - 1;
+        ex[d & 1][0] = fast_exp2(fx[d & 1][0]), ex[d & 1][1] = fast_exp2(fx[d & 1][1]);
+        asm volatile("" : "+v"(ex[d & 1][0]), "+v"(ex[d & 1][1]));
+      }
+      if constexpr (q < 16) {
+        constexpr int e = 2 * (q & 7);
+        fx[q & 1][0] = fmaf(x[q >> 3][e], cscale, -mn), fx[q & 1][1] = fmaf(x[q >> 3][e + 1], cscale, -mn);
+        asm volatile("" : "+v"(fx[q & 1][0]), "+v"(fx[q & 1][1]));
+      }
+    } else {
+      alpha = fast_exp2(m - mn);
+      l = fmaf(l, alpha, sum);
+      m = mn;
+    }
+  };
+  auto vread = [&](auto ic) __attribute__((always_inline)) {  // output product i: 16 keys of i / 4, values of i % 4
+    constexpr int i = ic, s = i >> 2, dt = i & 3;
+    if constexpr (i < 16) {
+      const uint32_t at = va ^ (16 * dt);
+      vring[i % AHEAD] = lds_keys(at + 16 * s * 256, (at ^ 64) + (16 * s + 8) * 256);
+    }
+  };
+  auto masked = [&](int t, f32x16 (&x)[2]) __attribute__((always_inline)) {
+    if (t * C::KT + C::KT > least) {
+      asm volatile("s_nop 15\n\ts_nop 7" : "+v"(x[0]), "+v"(x[1]));  // the last products are through
+#pragma unroll
+      for (int y = 0; y < 2; ++y)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (t * C::KT + 32 * y + 8 * (e >> 2) + 4 * h + (e & 3) >= lim) x[y][e] = -__builtin_inff();
+    }
+  };
+  // the scores of the tile in key slot ks into `next`, with the later parts of `cur`'s softmax (OUT)
+  auto scores = [&](auto outc, int ks, f32x16 (&cur)[2], f32x16 (&next)[2]) __attribute__((always_inline)) {
     constexpr bool OUT = decltype(outc)::value;
-    u32x4 kring[AHEAD], vring[AHEAD];
-    const uint32_t ka = kaddr + ks * C::KP, ra = raddr + ks * C::RP, va = vaddr + vs * C::VP;
+    u32x4 kring[AHEAD];
+    const uint32_t ka = kaddr + ks * C::KP, ra = raddr + ks * C::RP;
     auto kread = [&](auto jc) __attribute__((always_inline)) {  // score product j: 32 keys x = j % 2, values of j / 2
       constexpr int j = jc, x = j & 1, s = j >> 1;
       if constexpr (s < kNope / 16)
@@ -168,97 +244,68 @@ latent_expanded_kernel(const LatentParams p) {
       else if constexpr (s < NQ)
         kring[j % AHEAD] = lds_word((ra ^ (32 * (s - kNope / 16))) + x * 4096);
     };
-    auto vread = [&](auto ic) __attribute__((always_inline)) {  // output product i: 16 keys of i / 4, values of i % 4
-      constexpr int i = ic, s = i >> 2, dt = i & 3;
-      if constexpr (i < 16) {
-        const uint32_t at = va ^ (16 * dt);
-        vring[i % AHEAD] = lds_keys(at + 16 * s * 256, (at ^ 64) + (16 * s + 8) * 256);
-      }
-    };
     static_for<AHEAD>(kread);
-    if (OUT && t * C::KT + C::KT > least) {
-#pragma unroll
-      for (int x = 0; x < 2; ++x)
-#pragma unroll
-        for (int e = 0; e < 16; ++e)
-          if (t * C::KT + 32 * x + 8 * (e >> 2) + 4 * h + (e & 3) >= lim) cur[x][e] = -__builtin_inff();
-    }
-    float top = kNegBig, mn = 0.f, sum = 0.f, alpha = 1.f;
-    bool grew = false;
-    uint32_t pk[16];
-    auto part = [&](auto ic) __attribute__((always_inline)) {
-      constexpr int i = ic;
-      if constexpr (i < 4) {
-        constexpr int x = i >> 1, e = 8 * (i & 1);
-        top = max3(max3(max3(max3(top, cur[x][e], cur[x][e + 1]), cur[x][e + 2], cur[x][e + 3]), cur[x][e + 4], cur[x][e + 5]),
-                   cur[x][e + 6], cur[x][e + 7]);
-      } else if constexpr (i == 4) {
-        const uint32_t tb = __builtin_bit_cast(uint32_t, top);
-        auto sw = __builtin_amdgcn_permlane32_swap(tb, tb, false, false);
-        top = max3(__builtin_bit_cast(float, (uint32_t)sw[0]), __builtin_bit_cast(float, (uint32_t)sw[1]), kNegBig);
-        top = fmaxf(m, top * cscale);
-        grew = __any(top > m + kSlack);
-        mn = grew ? top : m;
-      } else if constexpr (i < 21) {
-        constexpr int q = i - 5, x = q >> 3, e = 2 * (q & 7);
-        float a = fast_exp2(fmaf(cur[x][e], cscale, -mn)), c = fast_exp2(fmaf(cur[x][e + 1], cscale, -mn));
-        sum += a + c;
-        pk[q] = Elem<T>::pack2(a, c);
-        asm volatile("" : "+v"(pk[q]), "+v"(sum));  // made here
-      } else {
-        alpha = fast_exp2(m - mn);
-        l = fmaf(l, alpha, sum);
-        m = mn;
-      }
-    };
     __builtin_amdgcn_sched_barrier(0);
     static_for<2 * NQ>([&](auto jc) __attribute__((always_inline)) {
       constexpr int j = jc, x = j & 1, s = j >> 1;
       mfma32_sum<T, s == 0>(next[x], kring[j % AHEAD], qop[s]);
       kread(std::integral_constant<int, j + AHEAD>{});
       if constexpr (OUT) {
-        constexpr int from = j * PARTS / (2 * NQ), to = (j + 1) * PARTS / (2 * NQ);
-        static_for<to - from>([&](auto qc) __attribute__((always_inline)) { part(std::integral_constant<int, from + qc>{}); });
+        constexpr int from = EARLY + j * (PARTS - EARLY) / (2 * NQ), to = EARLY + (j + 1) * (PARTS - EARLY) / (2 * NQ);
+        static_for<to - from>([&](auto qc) __attribute__((always_inline)) { part(std::integral_constant<int, from + qc>{}, cur); });
         if constexpr (j >= 2 * NQ - AHEAD) vread(std::integral_constant<int, j - (2 * NQ - AHEAD)>{});
       }
       __builtin_amdgcn_sched_barrier(0);
     });
-    if constexpr (OUT) {
-      if (grew) {
+  };
+  // the outputs of tile t, with the first parts of the softmax of `next`, the scores of tile t + 1
+  auto outputs = [&](int t, f32x16 (&next)[2]) __attribute__((always_inline)) {
+    if (grew) {
 #pragma unroll
-        for (int dt = 0; dt < 4; ++dt) acc[dt] *= alpha;
-      }
-      // what a VALU wrote is read by a product two wait states later at the earliest
-      asm volatile("s_nop 1" : "+v"(acc[0]), "+v"(acc[1]), "+v"(acc[2]), "+v"(acc[3]));
-      __builtin_amdgcn_sched_barrier(0);
-      static_for<16>([&](auto ic) __attribute__((always_inline)) {
-        constexpr int i = ic, s = i >> 2, dt = i & 3;
-        mfma32_sum<T, false>(acc[dt], vring[i % AHEAD], u32x4{pk[4 * s], pk[4 * s + 1], pk[4 * s + 2], pk[4 * s + 3]});
-        vread(std::integral_constant<int, i + AHEAD>{});
-        __builtin_amdgcn_sched_barrier(0);
-      });
-    } else {
-      asm volatile("s_nop 15\n\ts_nop 7" : "+v"(next[0]), "+v"(next[1]));  // the last products are through
+      for (int dt = 0; dt < 4; ++dt) acc[dt] *= alpha;
     }
+    masked(t + 1, next);
+    // what a VALU wrote is read by a product two wait states later at the earliest
+    asm volatile("s_nop 1" : "+v"(acc[0]), "+v"(acc[1]), "+v"(acc[2]), "+v"(acc[3]));
+    __builtin_amdgcn_sched_barrier(0);
+    static_for<16>([&](auto ic) __attribute__((always_inline)) {
+      constexpr int i = ic, s = i >> 2, dt = i & 3;
+      mfma32_sum<T, false>(acc[dt], vring[i % AHEAD], u32x4{pk[4 * s], pk[4 * s + 1], pk[4 * s + 2], pk[4 * s + 3]});
+      vread(std::integral_constant<int, i + AHEAD>{});
+      if constexpr (i == 2) asm volatile("" : "+v"(next[0]), "+v"(next[1]));  // the scores are through by now
+      constexpr int from = i < 3 ? 0 : (i - 3) * EARLY / 13, to = i < 3 ? 0 : (i - 2) * EARLY / 13;
+      static_for<to - from>([&](auto qc) __attribute__((always_inline)) { part(std::integral_constant<int, from + qc>{}, next); });
+      __builtin_amdgcn_sched_barrier(0);
+    });
   };
 
+  constexpr int PER = 2 * C::NK + C::NR;  // DMA instructions of a step
   f32x16 sa[2], sb[2];
   if (tend > 0) {
-    wait_dma<(C::D - 1) * C::PER>();
+    wait_dma<(C::D - 1) * PER>();
     __syncthreads();
-    if (most > 0) step(std::false_type{}, -1, 0, 0, sb, sa);
-    int ks = 0, vs = 0;  // slots of the keys and of the values of tile t
-    // keys of t + 1 and values of t have landed; tile t's keys and tile t - 1's values are done with: tile
-    // t + D's keys and t + D - 1's values take their places. Waves whose rows see nothing of a tile do
-    // nothing else.
+    if (most > 0) {
+      scores(std::false_type{}, 0, sb, sa);
+      asm volatile("s_nop 15\n\ts_nop 7" : "+v"(sa[0]), "+v"(sa[1]));  // the last products are through
+      masked(0, sa);
+      static_for<EARLY>([&](auto qc) __attribute__((always_inline)) { part(qc, sa); });
+    }
+    int slot = 0;  // of tile t
+    // Keys of t + 1 and values of t have landed; tile t's keys and tile t - 1's values are done with: tile t + D's keys
+    // and t + D - 1's values take their places. Waves whose rows see nothing of a tile do nothing else. (With half of
+    // the waves half a step behind the others, so that a SIMD's two are not at the same part: no faster.)
     auto turn = [&](int t, f32x16 (&cur)[2], f32x16 (&next)[2]) __attribute__((always_inline)) {
-      wait_dma<(C::D - 2) * C::PER>();
+      wait_dma<(C::D - 2) * PER>();
       __syncthreads();
-      const int kn = ks + 1 == C::D ? 0 : ks + 1;
-      issue(t + C::D, ks, vs == 0 ? C::D - 1 : vs - 1);
-      if (t * C::KT < most) step(std::true_type{}, t, kn, vs, cur, next);
-      ks = kn;
-      vs = vs + 1 == C::D ? 0 : vs + 1;
+      issue_keys(t + C::D, slot);
+      issue_values(t + C::D - 1, slot == 0 ? C::D - 1 : slot - 1);
+      const int after = slot + 1 == C::D ? 0 : slot + 1;
+      va = vaddr + slot * C::VP;
+      if (t * C::KT < most) {
+        scores(std::true_type{}, after, cur, next);
+        outputs(t, next);
+      }
+      slot = after;
     };
     for (int t = 0; t < tend; t += 2) {
       turn(t, sa, sb);
