@@ -116,11 +116,6 @@ latent_expanded_kernel(const LatentParams p) {
     for (int u = 0; u < C::NK; ++u) dma4(rv, lds + C::kV + slot * C::VP, u);
   };
   issue_keys(0, 0);
-  static_for<C::D - 1>([&](auto j) __attribute__((always_inline)) {
-    constexpr int g = decltype(j)::value;
-    issue_keys(g + 1, g + 1);
-    issue_values(g, g);
-  });
 
   // ---- the wave's rows
   const int tok = tok0 + 32 * wave + n;
@@ -144,6 +139,11 @@ latent_expanded_kernel(const LatentParams p) {
     for (int s = 0; s < NQ; ++s)
       qop[s] = (load16(q + 16 * s) ^ u32x4{flip, flip, flip, flip}) & u32x4{keep, keep, keep, keep};
   }
+  static_for<C::D - 1>([&](auto j) __attribute__((always_inline)) {
+    constexpr int g = decltype(j)::value;
+    issue_keys(g + 1, g + 1);
+    issue_values(g, g);
+  });
   const float cscale = fabsf(p.scale_log2);
 
   f32x16 acc[4];

@@ -488,12 +488,12 @@ __device__ __forceinline__ void latent_segment_wide(const LatentParams& p, const
     const uint32_t flip = p.scale_log2 < 0.f ? 0x80008000u : 0u, keep = ok ? ~0u : 0u;
 #pragma unroll
     for (int s = 0; s < KS + KR; ++s) qop[s] = load16(q + 16 * s);
+#pragma unroll
+    for (int s = 0; s < KS + KR; ++s) qop[s] = (qop[s] ^ u32x4{flip, flip, flip, flip}) & u32x4{keep, keep, keep, keep};
     for (int i = 1; i < 3; ++i) {
       feed.aim(t0 + i, i, i);
       feed.all();
     }
-#pragma unroll
-    for (int s = 0; s < KS + KR; ++s) qop[s] = (qop[s] ^ u32x4{flip, flip, flip, flip}) & u32x4{keep, keep, keep, keep};
   }
   const float cscale = fabsf(p.scale_log2);
   int least = lim;
