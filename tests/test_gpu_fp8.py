@@ -244,3 +244,12 @@ def test_gemm_of_many_tokens(device, m, n, k, dtype):
     """The widest tiles, whole ones and cut ones, and keys split over workgroups."""
     q, scale, qw, ws = _operands(m, n, k, m + n + k)
     _check_gemm(fp8_gemm(q, scale, qw, ws, None, dtype), q, scale, qw, ws)
+
+
+@pytest.mark.parametrize("n,k", [(1152, 896), (4096 + 16, 2176), (700, 5120)])
+@pytest.mark.parametrize("m", [1, 2, 8, 9, 16, 17, 32, 33, 48, 65, 96, 128])
+def test_gemm_of_few_tokens(device, m, n, k):
+    """The stream kernel's tiles, its waves' shares of the keys and rows that end inside a tile."""
+    q, scale, qw, ws = _operands(m, n, k, 7 * m + n)
+    for dtype in (torch.bfloat16, torch.float16):
+        _check_gemm(fp8_gemm(q, scale, qw, ws, None, dtype), q, scale, qw, ws)
