@@ -902,18 +902,33 @@ __global__ __launch_bounds__(WPR == 1 ? 256 : 64 * WPR) void latent_merge_kernel
   if (b < 0) return;
   const RowShape shape = row_shape<ROWS>(p.heads);
   const int item = rec[1], all = rec[2] - w + 2;  // ranges w - 1 .. rec[2]
-  const SeqView v = seq_view(p, b, work.lo, work.hi);
-  const int tok0 = item / shape.hs << shape.js, head0 = item % shape.hs * ROWS;
-  const int heads = min(p.heads - head0, ROWS), tokens = min(1 << shape.js, v.n - tok0);
-  const int rr = WPR == 1 ? 4 * blockIdx.y + wave : blockIdx.y, j = rr / heads;
-  if (j >= tokens) return;
-  constexpr int PER = R / 64;  // values of a lane
+  const int rr = WPR == 1 ? 4 * blockIdx.y + wave : blockIdx.y;
+  constexpr int PER = R / 64, FIRST = 4;  // values of a lane; parts that are asked for at once
   const int each = (all + WPR - 1) / WPR, from = wave % WPR * each, parts = min(all - from, each);  // (none or less: none)
   auto row = [&](int i) { return (int64_t)(from + i == 0 ? 2 * w - 1 : 2 * (w - 1 + from + i)) * ROWS + rr; };
+  // all that the first parts need is asked for before any of it is waited for (one after the other, 256 decodes of 128
+  // heads: 29 us)
+  float2 ml = {kNegBig, 0.f};
+  f32x4 head[FIRST][PER / 4];
+  if (parts > 0) {
+    ml = *reinterpret_cast<const float2*>(work.ml + 2 * row(min(lane, parts - 1)));
+#pragma unroll
+    for (int k = 0; k < FIRST; ++k)
+#pragma unroll
+      for (int d = 0; d < PER / 4; ++d)
+        head[k][d] = *reinterpret_cast<const f32x4*>(work.o + row(min(k, parts - 1)) * R + d * 256 + 4 * lane);
+  }
+  const SeqView v = seq_view(p, b, work.lo, work.hi);
+  const int tok0 = item / shape.hs << shape.js, head0 = item % shape.hs * ROWS;
+  const int heads = min(p.heads - head0, ROWS), tokens = min(1 << shape.js, v.n - tok0), j = rr / heads;
+  if (j >= tokens) return;
+  if (lane >= parts) ml = float2{kNegBig, 0.f};
   float top = kNegBig, sum = 0.f, o[PER] = {};
   for (int i0 = 0; i0 < parts; i0 += 64) {
-    float2 ml = {kNegBig, 0.f};
-    if (i0 + lane < parts) ml = *reinterpret_cast<const float2*>(work.ml + 2 * row(i0 + lane));
+    if (i0 > 0) {
+      ml = float2{kNegBig, 0.f};
+      if (i0 + lane < parts) ml = *reinterpret_cast<const float2*>(work.ml + 2 * row(i0 + lane));
+    }
     float most = ml.x;
 #pragma unroll
     for (int x = 32; x > 0; x >>= 1) most = fmaxf(most, __shfl_xor(most, x));
@@ -943,6 +958,16 @@ __global__ __launch_bounds__(WPR == 1 ? 256 : 64 * WPR) void latent_merge_kernel
       }
     };
     int i = 0;
+    if (i0 == 0) {
+#pragma unroll
+      for (int k = 0; k < FIRST; ++k) {
+        if (k >= here) continue;
+        const float fk = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), k));
+#pragma unroll
+        for (int d = 0; d < PER; ++d) o[d] = fmaf(head[k][d >> 2][d & 3], fk, o[d]);
+      }
+      i = min(FIRST, here);
+    }
     for (; i + 8 <= here; i += 8) take(i, std::integral_constant<int, 8>{});
     if (here - i >= 4) take(i, std::integral_constant<int, 4>{}), i += 4;
     if (here - i >= 2) take(i, std::integral_constant<int, 2>{}), i += 2;
