@@ -331,8 +331,10 @@ int ss_quantize_fp8(const void* x, uint8_t* q, float* scale, int64_t rows, int64
  *   row * xs_strides[0] + block * xs_strides[1]; w_scale (block of 128 n, block of 128 k) at
  *   ws_strides[0], ws_strides[1] likewise; bias [n] of bias_dtype, or NULL; out [m, n], row stride
  *   o_stride, of out_dtype (SS_DTYPE_BF16/F16/F32). k below 2^30.
- * A block's sum is in fp32, is multiplied with fl(x_scale w_scale) and added in one fp32 rounding; the
- * result is rounded once to out_dtype.
+ * A block's sum is multiplied with fl(x_scale w_scale) and added in one fp32 rounding; the result is
+ * rounded once to out_dtype. To fp16 and fp32 a block is summed in fp32. To bf16 it is summed by the matrix
+ * instruction for e4m3, which holds fewer bits between a block's products: measured 2^-16 of the sum of 128
+ * normal products on average, 2^-15.4 of their magnitudes' sum at most, and up to 2^-10.7 of the larger of two.
  * workspace: ss_fp8_workspace_size() bytes, 16-byte aligned, any contents (x_whole, w_whole as in
  * ss_w8a8_workspace_size). With less (or NULL, 0) the call succeeds without it, more slowly. Calls that
  * share a workspace must be ordered on one stream.
@@ -468,7 +470,8 @@ int ss_latent_rope_and_cache(const void* q, void* q_out, const void* latent, con
  * sequence's n sees the keys [0, context_lens[b] - n + t]; n is tq, or of cu_seqlens, whose entries
  * are clamped into [0, total_tokens]; with it tq only tells how long sequences are likely to be, and
  * rows of no sequence are left as they are. Table entries outside [0, num_blocks) are masked, a row
- * that sees no key gives zeros. latent_dim 1..512, rope_dim 0..256, dtype SS_DTYPE_BF16/F16/F32. The
+ * that sees no key gives zeros; a new token's latent that another of the call's queries sees must be
+ * finite for those that do not. latent_dim 1..512, rope_dim 0..256, dtype SS_DTYPE_BF16/F16/F32. The
  * conventions of ss_paged_attention_varlen; no counterpart in the reference.
  * workspace: ss_latent_attention_workspace_size() bytes (total_tokens = batch * tq without cu_seqlens),
  * any contents: partial rows of keys split over workgroups. Too small a one is SS_ERR_WORKSPACE.
@@ -491,8 +494,8 @@ int ss_latent_attention(const void* q, void* out, const void* cache, const int32
  * tokens of sequence b are [cu_seqlens[b], cu_seqlens[b + 1]) of q and out, its context (these
  * tokens last) [cu_context[b], cu_context[b + 1]) of kv and k_rope; both are clamped to total_tokens and
  * total_keys, and rows of no sequence are left as they are. max_query_len only tells how long
- * sequences are likely to be. nope_dim and value_dim 1..512, rope_dim 0..256, dtype
- * SS_DTYPE_BF16/F16/F32.
+ * sequences are likely to be; a new token's values that another of the call's queries sees must be finite
+ * for those that do not. nope_dim and value_dim 1..512, rope_dim 0..256, dtype SS_DTYPE_BF16/F16/F32.
  */
 int ss_latent_attention_expanded(const void* q, void* out, const void* kv, const void* k_rope,
                                  const int32_t* cu_seqlens, const int32_t* cu_context, int64_t batch,

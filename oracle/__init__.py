@@ -12,6 +12,10 @@ Modules:
                    slipstream/kernels/triton_paged.py:65-95,133-206)
   quant            numpy restatement of the W4A16 format and GEMM
                    (slipstream/kernels/quant_ref.py:38-133)
+  fp8              numpy restatement (float64) of rows in e4m3 with a scale for every 128
+                   columns and of their product; no counterpart in the reference
+  latent           numpy restatement (float64) of the latent cache's write and of attention
+                   over latents in both forms; no counterpart in the reference
   reference_path   torch-CPU restatement of the reference's own dtype sequence
                    (bf16 GEMMs, fp32 softmax), timed as the CPU baseline
 

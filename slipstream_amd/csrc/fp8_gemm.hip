@@ -3,7 +3,8 @@
 //   out[m, n] = sum_b x_scale[m, b] w_scale[n / 128, b] (sum_{k in block b} x[m, k] w[n, k]) (+ bias[n]).
 // The matrix cores sum a block (fp8_common.h says in how many bits); its sum is multiplied with the
 // product of its scales and added to an fp32 sum in one rounding. A result is rounded once to the
-// output's type.
+// output's type. Few tokens go to the stream kernel (fp8_stream.hip), which the weights' bytes bound, more to the
+// tile kernel (fp8_tile.hip), by whose estimate is the shorter; the kernel here takes what neither may read.
 #include "fp8_common.h"
 
 namespace ss {

@@ -14,6 +14,9 @@
 //   A block whose scale would be subnormal (a < 448 * 2^-126) is zeros with scale zero. A block that
 //   holds a NaN or an infinity is zeros with scale NaN, so that every product with it is NaN.
 //   The maximum is taken over the magnitudes' bit patterns as unsigned integers.
+//
+// Bound by the memory at a step's sizes (2240 x 14336 in bf16 19 to 24 us, 4.1 to 5.1 TB/s), by the launch at a
+// decode's (197 x 4096 3.3 us).
 #include "ss_common.h"
 
 namespace {

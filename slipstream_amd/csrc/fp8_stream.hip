@@ -2,9 +2,12 @@
 //
 // A workgroup of up to eight waves multiplies 16 MT tokens with 16 NT channels; its waves share out the blocks
 // of 128 keys, one after another in turn. A wave brings its blocks' rows by DMA into a part of the LDS that is
-// its own, two in turn, and reads the matrix instruction's operands from there: no wave waits for another
-// between the first block and the last. The products of the tokens' and the channels' scales are made first,
-// for all blocks, beside the first DMAs; the waves' sums are added at the end in the order of the waves.
+// its own, two in turn, with their scales behind them, and reads the matrix instruction's operands from there: no
+// wave waits for another before the end, where the waves' sums are added in their order.
+//
+// Bound by the weights' way out of the memory: 1 x 28672 x 4096 19.3 us a call, 24.2 over three sets of weights in
+// turn (4.9 TB/s), 24 x 28672 x 4096 26.3 (4.5). With the scales of all blocks read into a table first, a wave of
+// four blocks waits for the memory twice (0.7 us).
 #include "fp8_common.h"
 #include "tile_order.h"
 

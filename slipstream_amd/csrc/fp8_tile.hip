@@ -6,6 +6,11 @@
 // instruction of 16 x 16 x 128 sums a whole block, so a product's result is multiplied with its block's scales
 // and added to the fp32 sums while the products after it run: four fused multiply-adds of 4 cycles against a
 // product's 32.
+//
+// 2240 x 28672 x 4096: 234 to 253 us, 2.1 to 2.25 PFLOP/s (the card's library product with one scale 239), the matrix
+// cores busy for half of the cycles at the 1.7 to 2 GHz that the card's power leaves; 197 x 4096 x 14336 29 us (keys
+// split over workgroups, then the sums' way out and in). To fp16 and fp32 the operands' widening is the longer part: two halves of
+// a dword in 8 cycles each, 333 x 4999 x 2064 19 us against 14.8 to bf16.
 #include "fp8_common.h"
 #include "tile_order.h"
 

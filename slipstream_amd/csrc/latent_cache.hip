@@ -10,6 +10,9 @@
 // Work layout: a workgroup a token. Its first wave normalises the latent, all four rotate the heads
 // and the key in 16-byte pieces of either half where the strides allow. The piece of the latent
 // that a lane holds after the sum (all of a latent of 512 16-bit values) is written from registers.
+//
+// Bound by the memory at a step's sizes (2240 tokens of 128 heads of 64, latents of 512: 79 MB in 14.6 to 16 us, 4.9 to
+// 5.4 TB/s), by the launch at a decode's (256 tokens of 16 heads 3.3 us).
 #include "ss_common.h"
 
 namespace {

@@ -6,10 +6,11 @@
 //   softmax         fp32; a row's keys lie in two lanes, so a maximum is one exchange
 //   O^T += V^T P^T  the scores' layout is the operand's: probabilities stay in registers
 // Keys (the heads' and the shared parts) and values come by DMA into rings in the LDS, whose 16-byte
-// chunks are swizzled as in latent_mma.h. A step runs the scores of tile t + 1 with the softmax of tile t
-// written between their products, then the outputs of tile t; two waves a SIMD.
-// Bound by the matrix cores: 2 * 320 operations a (query, key, head) against 8 + 2 KB of LDS reads for
-// 32 x 64 of them.
+// chunks are swizzled as in latent_mma.h. A step runs the scores of tile t + 1, then the outputs of tile t, with the
+// softmax of either written between their products; two waves a SIMD.
+// 4 chunks of 512 tokens over up to 4096, 128 heads: 431 to 452 us, 930 to 980 TFLOP/s; a step of 256 tokens and 64 keys
+// takes 2.2 us, its products 1.4 of them at the 1.9 GHz that the card's power leaves. A turn of 77 tokens over 512, 16
+// heads: 13.7 us, ten steps of 1 after 3.5 us of start; two groups of waves with half of the keys each take 13.2.
 #include "latent_mma.h"
 
 namespace ss {

@@ -3,9 +3,12 @@ columns of a row and for every 128 x 128 values of the weight.
 
 ``fp8_gemm(q, scale, qweight, w_scale)`` multiplies rows quantized by ``quantize_fp8`` with a weight
 quantized by ``slipstream_amd.quantized.quantize_weight_fp8`` (or stored so in a checkpoint). Each
-block of 128 is summed in fp32 by the matrix cores, times its scales, and added in fp32; the result is
-rounded once to ``out_dtype``. The reference has no counterpart; the conventions are those of
-``w8a8_gemm``. Device tensors only.
+block of 128 is summed by the matrix cores, times its scales, and added in fp32; the result is
+rounded once to ``out_dtype``. For fp16 and fp32 a block's sum is in fp32; for bf16 it is the e4m3
+instruction's, which is off by 2^-16 of itself on average over 128 normal products (2^-15.4 of their
+magnitudes' sum at most; 2^-10.7 of the larger of two alone), below the half step of the result's type where products
+do not cancel: ask for fp32 results where they do. The reference has no counterpart; the conventions are
+those of ``w8a8_gemm``. Device tensors only.
 """
 
 from __future__ import annotations

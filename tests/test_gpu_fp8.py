@@ -120,9 +120,11 @@ def _operands(m, n, k, seed, device="cuda"):
 
 
 def _check_gemm(out, q, scale, qw, ws, bias=None):
-    """A block's 128 products are exact in fp32 and their sum has at most 127 roundings of the partial sums,
-    each below 2^-23 of the terms' magnitudes (to the nearest or truncated); the scales' product and the sum
-    over blocks add two and one more a block, the bias one; and half a step of the output's type."""
+    """To fp16 and fp32 a block's 128 products are exact in fp32 and their sum has at most 127 roundings of the
+    partial sums, each below 2^-23 of the terms' magnitudes (to the nearest or truncated); the scales' product
+    and the sum over blocks add two and one more a block, the bias one; and half a step of the output's type.
+    To bf16 the e4m3 instruction sums a block, by its measured bound 2^-15.4 of the magnitudes: the 2^-15.98
+    here stands for that beside the half step, which is 2^-8."""
     want, size = ora.gemm(_f64(q).reshape(-1, q.shape[-1]), _f64(scale).reshape(-1, scale.shape[-1]), _f64(qw),
                           _f64(ws), None if bias is None else _f64(bias))
     got = _f64(out).reshape(want.shape)
