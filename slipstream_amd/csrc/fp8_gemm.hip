@@ -118,8 +118,9 @@ int check_extents(int64_t m, int64_t n, int64_t k, int out_dtype) {
 
 // Rows that the DMA kernels can read in 16-byte pieces; a tile of 256 of them stays below a descriptor's 2^30
 // bytes.
+constexpr int64_t kMostStride = 1 << 21;
 bool whole_rows(const void* base, int64_t rows, int64_t stride, int64_t k) {
-  return k % 16 == 0 && ((uintptr_t)base & 15) == 0 && (rows == 1 || stride % 16 == 0) && stride <= (1 << 21);
+  return k % 16 == 0 && ((uintptr_t)base & 15) == 0 && (rows == 1 || stride % 16 == 0) && stride <= kMostStride;
 }
 int64_t round16(int64_t n) { return (n + 15) / 16 * 16; }
 
@@ -202,7 +203,8 @@ extern "C" int ss_fp8_gemm(const uint8_t* x, const float* x_scale, const uint8_t
   const int64_t reach = (int64_t)1 << 27;
   const bool scales = p.xs_row >= 0 && p.xs_blk >= 0 && p.ws_row >= 0 && p.ws_blk >= 0 &&
                       256 * p.xs_row + blocks * p.xs_blk < reach && 2 * p.ws_row + blocks * p.ws_blk < reach;
-  if (k > 0 && scales && x_bytes + w_bytes <= left && m <= INT32_MAX && n <= INT32_MAX) {
+  // (copies of longer rows would not lie within a descriptor's reach either)
+  if (k > 0 && kp <= ss::kMostStride && scales && x_bytes + w_bytes <= left && m <= INT32_MAX && n <= INT32_MAX) {
     const bool wide = out_dtype != SS_DTYPE_BF16;
     const ss::Plan* pl = &ss::plan_for(m, n, kp, wide, true);
     if (pl->workspace() > left - x_bytes - w_bytes) pl = &ss::plan_for(m, n, kp, wide, false);

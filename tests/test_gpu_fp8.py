@@ -255,3 +255,10 @@ def test_gemm_of_few_tokens(device, m, n, k):
     q, scale, qw, ws = _operands(m, n, k, 7 * m + n)
     for dtype in (torch.bfloat16, torch.float16):
         _check_gemm(fp8_gemm(q, scale, qw, ws, None, dtype), q, scale, qw, ws)
+
+
+def test_gemm_of_very_long_rows(device):
+    """Rows longer than the DMA kernels' descriptors reach over a tile of them."""
+    q, scale, qw, ws = _operands(3, 130, (1 << 21) + 144, 17)
+    for rows in (q, q[:1]):
+        _check_gemm(fp8_gemm(rows, scale[: len(rows)], qw, ws, None, torch.float32), rows, scale[: len(rows)], qw, ws)

@@ -18,6 +18,8 @@ KERNELS = {"fp8_tile_kernel": 26, "latent_tile_kernel": 16, "latent_expanded_ker
 # after which another instruction may touch its result
 PASSES = {"16x16x16": 4, "16x16x32": 4, "16x16x128": 8, "32x32x16": 8}
 PAST = 4
+# wait states between a vector instruction and a product that reads what it wrote
+BEFORE = 2
 
 
 @pytest.fixture(scope="module")
@@ -53,9 +55,10 @@ def _registers(text: str) -> set[str]:
 
 
 def too_early(lines: list[str]) -> list[str]:
-    """Instructions that may touch a product's result before it is there: every instruction takes a wait state,
-    an s_nop n + 1, and a product waits until the matrix cores are done with the one before it. Straight through,
-    and once more from the target of each backward branch."""
+    """Instructions that may touch a product's result before it is there, and products that may read a register before
+    a vector instruction has written it: every instruction takes a wait state, an s_nop n + 1, and a product waits
+    until the matrix cores are done with the one before it. Straight through, and once more from the target of each
+    backward branch."""
     code, at = [], {}
     for line in lines:
         text, _, note = line.partition("//")
@@ -67,7 +70,7 @@ def too_early(lines: list[str]) -> list[str]:
     addresses = sorted(at)
     faults: list[str] = []
 
-    def run(i, now, free, ready, left, jump):
+    def run(i, now, free, ready, wrote, left, jump):
         while i < len(code) and left:
             text = code[i]
             op, _, args = text.partition(" ")
@@ -75,7 +78,7 @@ def too_early(lines: list[str]) -> list[str]:
                 passes = next(v for k, v in PASSES.items() if k + "_" in op)
                 dst, a, b = re.findall(r"[va]\[\d+:\d+\]", args)[:3]  # (asm products add to their own result or to 0)
                 for r in _registers(a) | _registers(b):
-                    if ready.get(r, 0) > now:
+                    if ready.get(r, 0) > now or wrote.get(r, -9) + BEFORE >= now:
                         faults.append(text)
                         break
                 now = max(now, free)
@@ -86,16 +89,20 @@ def too_early(lines: list[str]) -> list[str]:
             else:
                 if any(ready.get(r, 0) > now for r in _registers(args)):
                     faults.append(text)
+                if op.startswith("v_"):
+                    written = args if "swap" in op else args.split(",")[0]
+                    for r in _registers(written):
+                        wrote[r] = now
                 now += int(args.split()[0]) + 1 if op == "s_nop" else 1
                 if jump and (op.startswith("s_cbranch") or op == "s_branch"):
                     word = int(args.split()[0])
                     target = addresses[i] + 4 + 4 * (word - 65536 if word >= 32768 else word)
                     if target in at and target <= addresses[i]:
-                        run(at[target], now, free, dict(ready), 200, False)
+                        run(at[target], now, free, dict(ready), dict(wrote), 200, False)
             i += 1
             left -= 1
 
-    run(0, 0, 0, {}, len(code), True)
+    run(0, 0, 0, {}, {}, len(code), True)
     return faults
 
 
@@ -122,3 +129,6 @@ def test_an_early_read_is_found():
     assert not too_early(listing(first, second, third, read))
     assert too_early(listing(first, "s_nop 9", read)) == [read]
     assert not too_early(listing(first, "s_nop 11", read))
+    made = "v_mov_b32_e32 v25, 0"
+    assert too_early(listing(made, "s_nop 0", first)) == [first]
+    assert not too_early(listing(made, "s_nop 1", first))
