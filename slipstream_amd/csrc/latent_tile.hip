@@ -2,17 +2,15 @@
 // values, rotated keys of 64, pages of 8, 16, 32, ... tokens.
 //
 // All heads share a sequence's keys, so the query rows of a (sequence, few tokens) are its tokens' heads,
-// and a tile of keys that is in the LDS serves them all. A workgroup takes ROWS = 16 RT rows and walks the
+// and a tile of keys that is in the LDS serves them all. A workgroup takes 16, 32, 64 or 128 rows and walks the
 // keys in tiles of 32:
-//   S^T = K Q^T     a wave its 16 rows against the tile's 32 keys; the queries stay in registers
-//   softmax         in fp32 over the wave's rows; P^T goes to the LDS in the order in which the next
-//                   product's operand wants it (16 bytes a lane, no bank twice), with the factors by which
-//                   the rows' earlier outputs shrink
-//   O^T += C^T P^T  a wave all the workgroup's rows, but R / NW of the latents' values: so a latent is
+//   S^T = K Q^T     a wave some of the rows against some of the keys; the queries stay in registers
+//   softmax         in fp32 over the rows; P^T goes to the LDS in the order in which the next
+//                   product's operand wants it (16 bytes a lane, no bank twice)
+//   O^T += C^T P^T  a wave all the workgroup's rows, but a part of the latents' values: so a latent is
 //                   read from the LDS once by each wave for the scores and once in all for the outputs
 //                   (whole rows a wave would take twice the LDS reads, which bound the kernel then)
-// The tiles come by DMA into a ring of four (latents) and three (rotated keys); a step multiplies tile
-// t's outputs and tile t + 1's scores while tiles t + 2 and t + 3 are on their way, with one barrier.
+// The tiles come by DMA into rings in the LDS, two to four ahead (64 rows and fewer: a pair of tiles a step).
 //
 // In the LDS the 16-byte chunk c of a latent's row r lies at c ^ swizzle(r) (the four bits of r, two of
 // them swapped): a score operand's sixteen rows then lie in different banks, and so do the 8-byte pieces of
@@ -26,7 +24,7 @@
 // latent_merge_kernel adds in order: results repeat themselves to the bit.
 //
 // Measured, with the merge. 256 decodes, 1024 tokens in the middle and 8192 at most, latents of 512 (64 rotated): 16 heads
-// 138 us (3.4 TB/s), 32 155, 64 170, 128 heads 225 (488 TFLOP/s): bound by the memory, which has the partial
+// 126 us (3.7 TB/s), 32 147, 64 175, 128 heads 225 (488 TFLOP/s): bound by the memory, which has the partial
 // rows of 128 heads to take too (some 100 MB beside 525; the merge 24 us). 4 chunks of 512 over up to 4096, 16
 // heads 251 us (775 TFLOP/s; a step of 128 rows and 32 keys 1.9 us, its products 1.3). 8 decodes of 16 heads over
 // some 256 18.4 us, one over some 4096 26 us: the start (lengths, page table, keys: 8 us), then the merge (4).
@@ -41,6 +39,9 @@ namespace {
 // ns by the memory's rate, less where the caches hold it (one decode of 128 heads over some 4096 tokens, of
 // 59 ranges: 53 us with 0.5, 82 us with 0.35 of the merge's first form; 8 of them 80 and 86)
 constexpr float kStep = 1.8f, kRow = 0.5e-3f;
+// The same for 32 keys of 16 or 32 rows beside those, with its part of its items' starts (a step 1.1 to 1.25 then; taken as
+// 1.0 the step of latent_mixed_kernel's comment has 348 us, as 1.2 309, as 1.5 296, as 1.7 302)
+constexpr float kFewStep = 1.5f;
 
 template <int R_, int RT_, int NW_>
 struct LatTile {
@@ -48,14 +49,15 @@ struct LatTile {
   static constexpr int KT = 32, ROWS = 16 * RT;
   static constexpr int ROWB = 2 * R, LPLANE = KT * ROWB;  // latents of a tile in the LDS
   static constexpr int RPLANE = KT * 2 * kRopeDim;
-  static constexpr int NS = 4, NR = 3;                    // ring depths
+  static constexpr int NS = 4, NR = 4;                    // rings: two pairs of tiles
   static constexpr int DT = R / (16 * NW);                // 16-value output tiles of a wave
-  static constexpr int PB = RT * 1024;                    // bytes of a tile's P
+  static constexpr int KQ = NW / 4, RW = 4 * RT / (NW * KQ);  // sixteens of a pair's keys and row tiles whose scores a wave has
   static constexpr int RPI = 1024 / ROWB;                 // latents a DMA instruction brings
   static constexpr int NL = KT / RPI / NW;                // DMA instructions of a wave and tile, latents
-  static constexpr int kP = NS * LPLANE + NR * RPLANE, kAlpha = kP + 2 * PB, kMl = kAlpha + 2 * ROWS * 4,
-                       kGrew = kMl + ROWS * 8, kScan = kGrew + 64, LDS = kScan + 128;
+  static constexpr int kP = NS * LPLANE + NR * RPLANE, kTop = kP + 2 * RT * 1024, kSum = kTop + ROWS * 16,
+                       kScan = kSum + ROWS * 16, LDS = kScan + 128;
   static_assert(LDS <= 160 * 1024, "one workgroup a CU");
+  static_assert(KQ == 1 || (KQ == 2 && RW == 1), "scores");
 };
 
 // The same for 128 rows, four waves (one a SIMD, with all its registers) of 32 rows and R / 4 values
@@ -229,15 +231,22 @@ struct Feed {
   }
 };
 
+// 16, 32 or 64 rows: a step takes a pair of tiles, 64 keys. A wave has the scores of sixteen of them for all rows (of
+// eight waves, 32 for sixteen rows), writes their probabilities by the rows' maxima so far, and their own maxima; if one has grown by more than
+// the slack, which all waves see then, the probabilities are written once more. So the scores, whose chain of products,
+// maximum and exponents is what a step of few rows takes, are cut into four: 32 keys by one wave took 1.85 us
+// on any number of CUs, 64 take 2.1 to 2.5 (256 decodes of 16 heads 138 -> 126 us, of 32 155 -> 147; of 64, whose
+// eight waves had the scores of 32 keys and sixteen rows before too, 170 -> 175).
 template <typename T, typename C>
 __device__ __forceinline__ void latent_segment(const LatentParams& p, const LatentWork& work, char* const lds,
                                                const SeqView v, const int b, const int tok0, const int head0,
                                                const int js, const int t0, const int t1, const bool whole,
                                                const int slot) {
-  constexpr int R = C::R, RT = C::RT, NW = C::NW, DT = C::DT, KS = R / 32, KR = kRopeDim / 32;
+  constexpr int R = C::R, RT = C::RT, NW = C::NW, DT = C::DT, RW = C::RW, KQ = C::KQ, KS = R / 32, KR = kRopeDim / 32;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 15, g = lane >> 4;
-  const int heads = min(p.heads - head0, C::ROWS);  // of a token in this item
+  const int quarter = KQ == 1 ? wave : 2 * (wave >> 2), rt0 = KQ == 1 ? 0 : wave & 3;  // its first sixteen keys and row tile
+  const int heads = min(p.heads - head0, C::ROWS);       // of a token in this item
   const int tokens = min(1 << js, v.n - tok0);
   const int kv_end = max(0, min(v.keys, v.length - v.n + tok0 + tokens));
   const int tend = min(t1, (kv_end + 31) >> 5);
@@ -249,27 +258,32 @@ __device__ __forceinline__ void latent_segment(const LatentParams& p, const Late
     head = head0 + rr - j * heads;
     return j < tokens;
   };
-  const bool scores = wave < RT;
   Feed<C> feed(p, b, lds, kv_end, t0, tend);
-  for (int i = 0; i < 3; ++i) {
-    feed.aim(t0 + i, i, i);
-    feed.all();
-  }
+  auto send = [&](int t, int ring) {  // tiles t and t + 1 into ring slots ring and ring + 1
+    for (int i = 0; i < 2; ++i) {
+      feed.aim(t + i, ring + i, ring + i);
+      feed.all();
+    }
+  };
+  send(t0, 0);
   // queries: scaled inside the exponent, which needs a positive scale (a negative one is the query's sign)
-  u32x4 qop[KS + KR];
-  int lim = 0x7FFFFFFF;
-  if (scores) {
-    int tok, head;
-    const bool ok = row_of(wave, tok, head);
-    if (ok) lim = min(v.keys, v.length - v.n + tok + 1);
-    const T* const q = (const T*)p.q + (p.cu ? 0 : b * p.q_sb) + (v.start + tok) * p.q_st + head * p.q_sh + 8 * g;
-    const uint32_t flip = p.scale_log2 < 0.f ? 0x80008000u : 0u;
+  u32x4 qop[RW][KS + KR];
+  int lim[RW], least = 0x7FFFFFFF;  // keys of a lane's rows up to here; of the wave's rows, tiles before it need no mask
 #pragma unroll
-    for (int s = 0; s < KS + KR; ++s)
-      qop[s] = (ok ? load16(q + 32 * s) : u32x4{0, 0, 0, 0}) ^ u32x4{flip, flip, flip, flip};
+  for (int rw = 0; rw < RW; ++rw) {
+    int tok, head;
+    const bool ok = row_of(rt0 + rw, tok, head);
+    lim[rw] = min(kv_end, t1 * 32);
+    if (ok) lim[rw] = min(lim[rw], v.length - v.n + tok + 1);
+    least = min(least, lim[rw]);
+    const T* const q = (const T*)p.q + (p.cu ? 0 : b * p.q_sb) + (v.start + (ok ? tok : tok0)) * p.q_st +
+                       (ok ? head : head0) * p.q_sh + 8 * g;  // (a lane without a row: the item's first one, as zeros)
+    const uint32_t flip = p.scale_log2 < 0.f ? 0x80008000u : 0u, keep = ok ? ~0u : 0u;
+#pragma unroll
+    for (int s = 0; s < KS + KR; ++s) qop[rw][s] = (load16(q + 32 * s) ^ u32x4{flip, flip, flip, flip}) & u32x4{keep, keep, keep, keep};
   }
+  send(t0 + 2, 2);
   const float cscale = fabsf(p.scale_log2);
-  int least = lim;  // of the wave's rows: tiles that end before it need no mask
 #pragma unroll
   for (int o = 1; o < 16; o <<= 1) least = min(least, __shfl_xor(least, o));
   least = __builtin_amdgcn_readfirstlane(least);
@@ -280,131 +294,158 @@ __device__ __forceinline__ void latent_segment(const LatentParams& p, const Late
     bad |= (uint32_t)feed.table[i] >= (uint32_t)p.num_blocks;
   const bool holes = __syncthreads_or(bad);
 
-  auto landed = [&](auto tiles) {  // all but the youngest `tiles` tiles
-    if (wave < 4)
-      wait_dma<decltype(tiles)::value*(C::NL + 1)>();
-    else
-      wait_dma<decltype(tiles)::value * C::NL>();
-  };
-
   f32x4 acc[RT][DT];
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) acc[rt][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
-  float m = kNegBig, l = 0.f;  // of row n; l: of this lane's keys
+  float m[RT], own[RW], l[RW];  // of row n: the maxima of all row tiles and of the wave's; l: of this lane's keys
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) m[rt] = kNegBig;
+#pragma unroll
+  for (int rw = 0; rw < RW; ++rw) own[rw] = kNegBig, l[rw] = 0.f;
+  const int sw = lat_swizzle(n), vrow = 4 * g + (n >> 2), vsw = lat_swizzle(vrow);
 
-  // ---- scores and softmax of tile t in ring slots ls, rs; P and the rows' factors into buffer `buf`
-  auto score = [&](int t, int ls, int rs, int buf) {
-    const int sw = lat_swizzle(n);
-    const char* const kl = lds + ls * C::LPLANE + n * C::ROWB;
-    const char* const kr = lds + C::NS * C::LPLANE + rs * C::RPLANE + n * 2 * kRopeDim;
-    f32x4 s2[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+  for (int t = t0, ring = 0; t < tend; t += 2, ring ^= 2) {
+    if (t == t0) {  // (the second pair may be on its way)
+      if (wave < 4)
+        wait_dma<2 * (C::NL + 1)>();
+      else
+        wait_dma<2 * C::NL>();
+    } else {
+      wait_dma<0>();
+    }
+    __syncthreads();  // the pair is there, and the one before is done with
+    if (t > t0) send(t + 2, ring ^ 2);
+
+    const char* const kl = lds + (ring + (quarter >> 1)) * C::LPLANE + (16 * (quarter & 1) + n) * C::ROWB;
+    const char* const kr = lds + C::NS * C::LPLANE + (ring + (quarter >> 1)) * C::RPLANE + (16 * (quarter & 1) + n) * 2 * kRopeDim;
+    constexpr int SC = KQ == 1 ? RW : KQ, CH = KQ == 1 ? 2 : 1;  // 16 x 16 scores, and sums of each that take turns
+    f32x4 s2[SC][CH];
 #pragma unroll
-    for (int s = 0; s < KS; ++s)
+    for (int i = 0; i < SC; ++i)
 #pragma unroll
-      for (int x = 0; x < 2; ++x)
-        s2[x] = Elem<T>::mfma(load16(kl + 16 * x * C::ROWB + 16 * ((4 * s + g) ^ sw)), qop[s], s2[x]);
+      for (int h = 0; h < CH; ++h) s2[i][h] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int s = 0; s < KR; ++s)
+    for (int s = 0; s < KS + KR; ++s)
 #pragma unroll
-      for (int x = 0; x < 2; ++x)
-        s2[x] = Elem<T>::mfma(load16(kr + 16 * x * 2 * kRopeDim + 16 * ((4 * s + g) ^ tile_swizzle(n))), qop[KS + s], s2[x]);
-    float sv[8];
+      for (int x = 0; x < KQ; ++x) {
+        const u32x4 k = s < KS ? load16(kl + 16 * x * C::ROWB + 16 * ((4 * s + g) ^ sw))
+                               : load16(kr + 16 * x * 2 * kRopeDim + 16 * ((4 * (s - KS) + g) ^ tile_swizzle(n)));
 #pragma unroll
-    for (int x = 0; x < 2; ++x)
+        for (int rw = 0; rw < RW; ++rw) s2[KQ == 1 ? rw : x][s % CH] = Elem<T>::mfma(k, qop[rw][s], s2[KQ == 1 ? rw : x][s % CH]);
+      }
+    // the first tile's latents for the outputs, on their way beside the softmax
+    auto latents = [&](int tile, u32x4 (&c)[DT]) {
+      const uint32_t vp = lds_address(lds) + (ring + tile) * C::LPLANE + vrow * C::ROWB + 8 * (n & 1);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) sv[4 * x + e] = s2[x][e];
-    if (holes || t * 32 + 32 > least) {
+      for (int dt = 0; dt < DT; ++dt) {
+        const uint32_t at = vp + 16 * (out_chunk<C>(dt, (n >> 1) & 1, wave) ^ vsw);
+        c[dt] = lds_keys(at, at + 16 * C::ROWB);
+      }
+    };
+    u32x4 c[2][DT];
+    if constexpr (KQ == 1) latents(0, c[0]);  // (eight waves have no registers for it, and two a SIMD)
+    f32x4 sv[RW][KQ];
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const int key = t * 32 + 16 * x + 4 * g;  // four keys of one page
-        bool there = true;
-        if (holes && key < kv_end) {
-          there = (uint32_t)feed.table[key >> feed.shift] < (uint32_t)p.num_blocks;
+    for (int rw = 0; rw < RW; ++rw)
+#pragma unroll
+      for (int x = 0; x < KQ; ++x) sv[rw][x] = KQ == 1 ? s2[rw][0] + s2[rw][CH - 1] : s2[x][0];
+    if (holes || t * 32 + 64 > least) {
+#pragma unroll
+      for (int x = 0; x < KQ; ++x) {
+        const int key = t * 32 + 16 * (quarter + x) + 4 * g;  // four keys of one page
+        const bool there = !holes || key >= kv_end || (uint32_t)feed.table[key >> feed.shift] < (uint32_t)p.num_blocks;
+#pragma unroll
+        for (int rw = 0; rw < RW; ++rw)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (!there || key + e >= lim[rw]) sv[rw][x][e] = -__builtin_inff();
+      }
+    }
+    f32x4 pv[RW][KQ];
+    auto probabilities = [&]() {
+#pragma unroll
+      for (int rw = 0; rw < RW; ++rw)
+#pragma unroll
+        for (int x = 0; x < KQ; ++x) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) pv[rw][x][e] = fast_exp2(fmaf(sv[rw][x][e], cscale, -own[rw]));
+          *reinterpret_cast<u32x2*>(lds + C::kP + ((quarter >> 1) * RT + rt0 + rw) * 1024 + lane * 16 + 8 * ((quarter + x) & 1)) =
+              u32x2{Elem<T>::pack2(pv[rw][x][0], pv[rw][x][1]), Elem<T>::pack2(pv[rw][x][2], pv[rw][x][3])};
         }
+    };
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (!there || key + e >= min(lim, kv_end)) sv[4 * x + e] = -__builtin_inff();
-      }
+    for (int rw = 0; rw < RW; ++rw) {
+      float top = kNegBig;
+#pragma unroll
+      for (int x = 0; x < KQ; ++x) top = fmaxf(top, fmaxf(fmaxf(sv[rw][x][0], sv[rw][x][1]), fmaxf(sv[rw][x][2], sv[rw][x][3])));
+      top = max_across_rows(top);
+#pragma unroll
+      for (int x = 0; x < KQ; ++x)
+        if (g == x) *reinterpret_cast<float*>(lds + C::kTop + (16 * (rt0 + rw) + n) * 16 + 4 * (quarter + x)) = top;
     }
-    float top = fmaxf(fmaxf(fmaxf(sv[0], sv[1]), fmaxf(sv[2], sv[3])), fmaxf(fmaxf(sv[4], sv[5]), fmaxf(sv[6], sv[7])));
-    top = max_across_rows(top);
-    const float want = fmaxf(m, top * cscale);
-    const bool grew = __any(want > m + kSlack);
-    const float mn = grew ? want : m;
-    float pv[8], sum = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) pv[i] = fast_exp2(fmaf(sv[i], cscale, -mn));
-#pragma unroll
-    for (int i = 0; i < 8; ++i) sum += pv[i];
-    const float alpha = fast_exp2(m - mn);
-    l = l * alpha + sum;
-    m = mn;
-    store16(lds + C::kP + buf * C::PB + wave * 1024 + lane * 16,
-            u32x4{Elem<T>::pack2(pv[0], pv[1]), Elem<T>::pack2(pv[2], pv[3]), Elem<T>::pack2(pv[4], pv[5]),
-                  Elem<T>::pack2(pv[6], pv[7])});
-    if (g == 0) *reinterpret_cast<float*>(lds + C::kAlpha + (buf * C::ROWS + 16 * wave + n) * 4) = alpha;
-    if (lane == 0) *reinterpret_cast<int*>(lds + C::kGrew + (buf * RT + wave) * 4) = grew;
-  };
-  // ---- outputs of the tile in ring slot ls with the probabilities in buffer `buf`
-  const int vrow = 4 * g + (n >> 2);
-  auto output = [&](int ls, int buf) {
-    if (__any(*reinterpret_cast<const int*>(lds + C::kGrew + (buf * RT + (lane & (RT - 1))) * 4))) {
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt) {
-        const float alpha = *reinterpret_cast<const float*>(lds + C::kAlpha + (buf * C::ROWS + 16 * rt + n) * 4);
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt) acc[rt][dt] *= alpha;
-      }
-    }
-    const uint32_t vp = lds_address(lds) + ls * C::LPLANE + vrow * C::ROWB + 8 * (n & 1);
-    const int sw = lat_swizzle(vrow);
-    u32x4 c[DT];
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt) {
-      const uint32_t at = vp + 16 * (out_chunk<C>(dt, (n >> 1) & 1, wave) ^ sw);
-      c[dt] = lds_keys(at, at + 16 * C::ROWB);
-    }
+    probabilities();
+    __syncthreads();
+    float want[RT];
+    bool grew = false;
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-      const u32x4 pr = load16(lds + C::kP + buf * C::PB + rt * 1024 + lane * 16);
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt) acc[rt][dt] = Elem<T>::mfma(c[dt], pr, acc[rt][dt]);
+      const f32x4 top = *reinterpret_cast<const f32x4*>(lds + C::kTop + (16 * rt + n) * 16);
+      want[rt] = fmaxf(m[rt], fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * cscale);
+      grew |= want[rt] > m[rt] + kSlack;
     }
-  };
-
-  if (t0 < tend) {
-    landed(std::integral_constant<int, 2>{});
-    __syncthreads();
-    if (scores) score(t0, 0, 0, 0);
-    int ls = 0, rs = 0;  // slots of tile t
-    for (int t = t0; t < tend; ++t) {
-      landed(std::integral_constant<int, 1>{});
-      __syncthreads();  // tile t + 1 is there, P of tile t too, and tile t - 1's slots are free
-      feed.aim(t + 3, (ls + 3) & 3, rs);
-      feed.all();
-      const int rn = rs == 2 ? 0 : rs + 1;
-      if (scores && t + 1 < tend) score(t + 1, (ls + 1) & 3, rn, (t + 1 - t0) & 1);
-      output(ls, (t - t0) & 1);
-      ls = (ls + 1) & 3;
-      rs = rn;
+    if (__any(grew)) {  // the same in every wave
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        const float alpha = fast_exp2(m[rt] - want[rt]);
+        m[rt] = want[rt];
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) acc[rt][dt] *= alpha;
+#pragma unroll
+        for (int rw = 0; rw < RW; ++rw)
+          if (rt == rt0 + rw) own[rw] = want[rt], l[rw] *= alpha;
+      }
+      probabilities();
+      __syncthreads();
+    }
+#pragma unroll
+    for (int rw = 0; rw < RW; ++rw)
+#pragma unroll
+      for (int x = 0; x < KQ; ++x) l[rw] += (pv[rw][x][0] + pv[rw][x][1]) + (pv[rw][x][2] + pv[rw][x][3]);
+    if constexpr (KQ == 1) latents(1, c[1]);
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      if constexpr (KQ == 2) latents(x, c[x]);
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        const u32x4 pr = load16(lds + C::kP + (x * RT + rt) * 1024 + lane * 16);
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) acc[rt][dt] = Elem<T>::mfma(c[x][dt], pr, acc[rt][dt]);
+      }
     }
   }
   wait_dma<0>();
 
   // ---- the rows' sums, then the rows themselves
-  if (scores) {
-    const float total = sum_across_rows(l);
-    if (g == 0) *reinterpret_cast<float2*>(lds + C::kMl + (16 * wave + n) * 8) = float2{m, total};
+#pragma unroll
+  for (int rw = 0; rw < RW; ++rw) {
+    const float sum = sum_across_rows(l[rw]);
+#pragma unroll
+    for (int x = 0; x < KQ; ++x)
+      if (g == x) *reinterpret_cast<float*>(lds + C::kSum + (16 * (rt0 + rw) + n) * 16 + 4 * (quarter + x)) = x ? 0.f : sum;
   }
   __syncthreads();
+  auto total_of = [&](int rt) {
+    const f32x4 s = *reinterpret_cast<const f32x4*>(lds + C::kSum + (16 * rt + n) * 16);
+    return (s[0] + s[1]) + (s[2] + s[3]);
+  };
   if (whole) {
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
       int tok, head;
       if (!row_of(rt, tok, head)) continue;
-      const float total = reinterpret_cast<const float2*>(lds + C::kMl + (16 * rt + n) * 8)->y;
+      const float total = total_of(rt);
       const float inv = total == 0.f ? 0.f : 1.f / total;
       T* const o = (T*)p.out + (p.cu ? 0 : b * p.o_sb) + (v.start + tok) * p.o_st + head * p.o_sh + 4 * (g & 1);
 #pragma unroll
@@ -417,12 +458,13 @@ __device__ __forceinline__ void latent_segment(const LatentParams& p, const Late
   } else {
     float* const o = work.o + (int64_t)slot * C::ROWS * R + 4 * (g & 1);
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt)
+    for (int rt = 0; rt < RT; ++rt) {
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt)
         *reinterpret_cast<f32x4*>(o + (16 * rt + n) * R + 8 * out_chunk<C>(dt, g >> 1, wave)) = acc[rt][dt];
-    float* const ml = work.ml + (int64_t)slot * C::ROWS * 2;
-    for (int i = threadIdx.x; i < 2 * C::ROWS; i += 64 * NW) ml[i] = *reinterpret_cast<const float*>(lds + C::kMl + 4 * i);
+      if (wave == 0 && g == 0)
+        *reinterpret_cast<float2*>(work.ml + ((int64_t)slot * C::ROWS + 16 * rt + n) * 2) = float2{m[rt], total_of(rt)};
+    }
   }
   __syncthreads();  // the LDS is free for the next item
 }
@@ -776,16 +818,12 @@ __device__ __forceinline__ void latent_segment_wide(const LatentParams& p, const
 
 extern __shared__ __attribute__((aligned(1024))) char s_lat[];
 
+// Range w of at most `all` of the tiles of a launch's sequences
 template <typename T, typename C>
-__global__ __launch_bounds__(64 * C::NW) __attribute__((amdgpu_waves_per_eu(C::NW / 4, C::NW / 4))) void latent_tile_kernel(const LatentParams p, const LatentWork work) {
+__device__ __forceinline__ void latent_ranges(const LatentParams& p, const LatentWork& work, const int w, const int all) {
   constexpr int NT = 64 * C::NW;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const RowShape shape = row_shape<C::ROWS>(p.heads);
-  // workgroups go round robin over the eight XCDs: each XCD takes a contiguous eighth of the ranges, whose
-  // items share keys
-  const int all = gridDim.x, per_xcd = all >> 3;
-  const int w = all & 7 ? (int)blockIdx.x : (int)(blockIdx.x & 7) * per_xcd + (int)(blockIdx.x >> 3);
-
   // the sequences' lengths in tiles, summed: where this workgroup's range begins
   int64_t* const s_sum = reinterpret_cast<int64_t*>(s_lat + C::kScan);  // [NW], then what was found
   SeqView view = {0, 0, 0, 0};
@@ -878,6 +916,55 @@ __global__ __launch_bounds__(64 * C::NW) __attribute__((amdgpu_waves_per_eu(C::N
     }
     if (u >= u1) break;
     before = end;
+  }
+}
+
+template <typename T, typename C>
+__global__ __launch_bounds__(64 * C::NW) __attribute__((amdgpu_waves_per_eu(C::NW / 4, C::NW / 4))) void latent_tile_kernel(
+    const LatentParams p, const LatentWork work) {
+  // workgroups go round robin over the eight XCDs: each XCD takes a contiguous eighth of the ranges, whose
+  // items share keys
+  const int all = gridDim.x, per_xcd = all >> 3;
+  const int w = all & 7 ? (int)blockIdx.x : (int)(blockIdx.x & 7) * per_xcd + (int)(blockIdx.x >> 3);
+  latent_ranges<T, C>(p, work, w, all);
+}
+
+// A step of decodes beside chunks: sequences of few rows in F's tiles and the others in M's, in one launch. Decodes wait
+// for the memory and chunks for the matrix cores, so some workgroups of every XCD do the first while the others do
+// the second, as many as the steps' times (kFewStep, kStep) ask for: 192 decodes and 4 chunks of 512 over up to
+// 4096, 16 heads 296 us, in two launches 351.
+template <typename T, typename F, typename M>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) void latent_mixed_kernel(
+    const LatentParams p, const LatentWork few, const LatentWork many) {
+  static_assert(F::NW == 4 && M::NW == 4, "workgroups of one size");
+  float cost[2] = {0.f, 0.f};
+  for (int b = threadIdx.x; b < p.batch; b += 256) {
+    cost[0] += (float)seq_tiles(seq_view(p, b, few.lo, few.hi), row_shape<F::ROWS>(p.heads)) * kFewStep;
+    cost[1] += (float)seq_tiles(seq_view(p, b, many.lo, many.hi), row_shape<M::ROWS>(p.heads)) * kStep;
+  }
+  float* const s_cost = reinterpret_cast<float*>(s_lat);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) cost[i] += __shfl_xor(cost[i], o);
+    if ((threadIdx.x & 63) == 0) s_cost[4 * i + (threadIdx.x >> 6)] = cost[i];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 2; ++i) cost[i] = s_cost[4 * i] + s_cost[4 * i + 1] + s_cost[4 * i + 2] + s_cost[4 * i + 3];
+  __syncthreads();
+  // whole workgroups of each XCD (or of one that all are taken for), one at least for either where it has work
+  const int xcds = gridDim.x & 7 ? 1 : 8, each = gridDim.x / xcds, xcd = blockIdx.x % xcds, at = blockIdx.x / xcds;
+  int part = (int)(each * cost[0] / fmaxf(cost[0] + cost[1], 1.f) + 0.5f);
+  part = min(max(part, cost[0] > 0.f ? 1 : 0), cost[1] > 0.f ? each - 1 : each);
+  part = __builtin_amdgcn_readfirstlane(part);
+  const int rest = each - part;
+  if (at < part) {
+    if (threadIdx.x == 0) many.rec[4 * (xcds * rest + xcd * part + at)] = -1;  // of no range
+    latent_ranges<T, F>(p, few, xcd * part + at, xcds * part);
+  } else {
+    if (threadIdx.x == 0) few.rec[4 * (xcds * part + xcd * rest + at - part)] = -1;
+    latent_ranges<T, M>(p, many, xcd * rest + at - part, xcds * rest);
   }
 }
 
@@ -1024,20 +1111,21 @@ int64_t part_bytes(int rows, int r) {
   return up(groups * 2 * rows * r * 4) + up(groups * 2 * rows * 2 * 4) + up(groups * 4 * 4);
 }
 
-template <typename T, typename C>
-int launch_rows(const LatentParams& p, int lo, int hi, char* ws, hipStream_t stream) {
-  constexpr int R = C::R, NW = C::NW;
+template <typename C>
+LatentWork work_of(char* ws, int lo, int hi) {
   const int64_t groups = ss_host::device_cu_count();
   LatentWork work;
   work.o = (float*)ws;
-  work.ml = (float*)(ws + up(groups * 2 * C::ROWS * R * 4));
+  work.ml = (float*)(ws + up(groups * 2 * C::ROWS * C::R * 4));
   work.rec = (int*)((char*)work.ml + up(groups * 2 * C::ROWS * 2 * 4));
   work.lo = lo, work.hi = hi;
-  auto kern = latent_tile_kernel<T, C>;
-  static std::atomic<uint64_t> done{0};
-  if (const int st = reserve_lds((const void*)kern, C::LDS, done); st != SS_OK) return st;
-  hipLaunchKernelGGL(kern, dim3((unsigned)groups), dim3(64 * NW), C::LDS, stream, p, work);
-  if (const int st = ss_host::launch_status("latent attention"); st != SS_OK) return st;
+  return work;
+}
+
+template <typename T, typename C>
+int launch_merge(const LatentParams& p, const LatentWork& work, hipStream_t stream) {
+  constexpr int R = C::R;
+  const int64_t groups = ss_host::device_cu_count();
   // Many items are cut once or twice each: a wave a row (of 256 decodes of 128 heads). Few are cut often: sixteen
   // waves a row, and no more workgroups than there may be items.
   const RowShape shape = row_shape<C::ROWS>(p.heads);
@@ -1049,6 +1137,30 @@ int launch_rows(const LatentParams& p, int lo, int hi, char* ws, hipStream_t str
     hipLaunchKernelGGL((latent_merge_kernel<T, R, C::ROWS, 1>), dim3((unsigned)groups, C::ROWS / 4), dim3(256), 0, stream,
                        p, work, (int)groups);
   return ss_host::launch_status("latent attention (merge)");
+}
+
+template <typename T, typename C>
+int launch_rows(const LatentParams& p, int lo, int hi, char* ws, hipStream_t stream) {
+  const LatentWork work = work_of<C>(ws, lo, hi);
+  auto kern = latent_tile_kernel<T, C>;
+  static std::atomic<uint64_t> done{0};
+  if (const int st = reserve_lds((const void*)kern, C::LDS, done); st != SS_OK) return st;
+  hipLaunchKernelGGL(kern, dim3((unsigned)ss_host::device_cu_count()), dim3(64 * C::NW), C::LDS, stream, p, work);
+  if (const int st = ss_host::launch_status("latent attention"); st != SS_OK) return st;
+  return launch_merge<T, C>(p, work, stream);
+}
+
+template <typename T, typename F, typename M>
+int launch_mixed(const LatentParams& p, int lo, char* ws, hipStream_t stream) {
+  const LatentWork few = work_of<F>(ws, 0, lo), many = work_of<M>(ws + part_bytes(F::ROWS, F::R), lo, 0x7FFFFFFF);
+  constexpr int lds = F::LDS > M::LDS ? F::LDS : M::LDS;
+  auto kern = latent_mixed_kernel<T, F, M>;
+  static std::atomic<uint64_t> done{0};
+  if (const int st = reserve_lds((const void*)kern, lds, done); st != SS_OK) return st;
+  hipLaunchKernelGGL(kern, dim3((unsigned)ss_host::device_cu_count()), dim3(256), lds, stream, p, few, many);
+  if (const int st = ss_host::launch_status("latent attention (mixed)"); st != SS_OK) return st;
+  if (const int st = launch_merge<T, F>(p, few, stream); st != SS_OK) return st;
+  return launch_merge<T, M>(p, many, stream);
 }
 
 template <typename T, int R>
@@ -1097,6 +1209,8 @@ int launch_latent_tile(const LatentParams& p, int dtype, char* ws, hipStream_t s
   const int lo = few ? p.heads : 0;  // the first launch's sequences: of one token
 #define LATENT_LAUNCH(T, R)                                                                           \
   do {                                                                                                \
+    if (few == 16 && many == 128) return launch_mixed<T, LatTile<R, 1, 4>, LatWide<R>>(p, lo, ws, stream); \
+    if (few == 32 && many == 128) return launch_mixed<T, LatTile<R, 2, 4>, LatWide<R>>(p, lo, ws, stream); \
     if (few)                                                                                          \
       if (const int st = launch_for<T, R>(p, few, 0, lo, ws, stream); st != SS_OK) return st;         \
     return launch_for<T, R>(p, many, lo, kAll, ws + (few ? part_bytes(few, R) : 0), stream);          \

@@ -13,7 +13,7 @@ from pathlib import Path
 import pytest
 
 OBJDUMP = Path("/opt/rocm/llvm/bin/llvm-objdump")
-KERNELS = {"fp8_tile_kernel": 26, "latent_tile_kernel": 16, "latent_expanded_kernel": 6}
+KERNELS = {"fp8_tile_kernel": 26, "latent_tile_kernel": 16, "latent_mixed_kernel": 8, "latent_expanded_kernel": 6}
 # passes of the matrix cores (a wait state each) by a product's shape, and the states past the last of them
 # after which another instruction may touch its result
 PASSES = {"16x16x16": 4, "16x16x32": 4, "16x16x128": 8, "32x32x16": 8}
