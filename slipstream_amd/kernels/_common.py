@@ -15,6 +15,14 @@ def require_device(who: str, *tensors: torch.Tensor) -> None:
     ``slipstream/kernels/reshape_and_cache.py:19``); this package is the device
     path only and refuses CPU tensors loudly instead of computing elsewhere.
     """
+    first = tensors[0]
+    index = first.get_device() if first.is_cuda else -1
+    if index >= 0:  # the usual case, at half the cost of comparing devices
+        for t in tensors:
+            if t.get_device() != index:
+                break
+        else:
+            return
     dev = None
     for t in tensors:
         if t.device.type != "cuda":

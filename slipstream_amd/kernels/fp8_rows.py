@@ -34,7 +34,7 @@ def quantize_fp8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     cols = shape[-1]
     q = x.new_empty(shape, dtype=FP8)
     by_block = x.new_empty((blocks_of(cols), *shape[:-1]), dtype=torch.float32)
-    scale = by_block.movedim(0, -1)
+    scale = by_block.t() if x.ndim == 2 else by_block.movedim(0, -1)
     if q.numel() == 0:
         return q, scale
     require_device("quantize_fp8", x)

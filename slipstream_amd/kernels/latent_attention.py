@@ -46,6 +46,13 @@ def _workspace(device: torch.device, batch: int, tokens: int, tq: int, heads: in
     return torch.empty(nbytes, dtype=torch.uint8, device=device)
 
 
+def _ints(x: torch.Tensor) -> torch.Tensor:
+    """``x`` as a contiguous row of int32."""
+    if x.dtype == torch.int32 and x.ndim == 1 and x.is_contiguous():
+        return x
+    return _int32(x.reshape(-1))
+
+
 def _absorbed(who: str, q: torch.Tensor, out: torch.Tensor, latent_cache: torch.Tensor, block_tables: torch.Tensor,
               cu: torch.Tensor | None, ctx: torch.Tensor, layer_idx: int, scale: float, block_size: int,
               latent_dim: int, batch: int, tokens: int, tq: int, heads: int, q_strides, o_strides) -> torch.Tensor:
@@ -56,8 +63,9 @@ def _absorbed(who: str, q: torch.Tensor, out: torch.Tensor, latent_cache: torch.
         raise _ffi.KernelError(f"{who}: latent_cache must have a unit last stride")
     rope_dim = q.shape[-1] - latent_dim
     ws = _workspace(q.device, batch, tokens, tq, heads, latent_dim, rope_dim, dtype)
-    block_tables = _int32(block_tables)
-    ctx = _int32(ctx.reshape(-1))
+    if block_tables.dtype != torch.int32 or not block_tables.is_contiguous():
+        block_tables = _int32(block_tables)
+    ctx = _ints(ctx)
     cst = latent_cache.stride()
     status = launch(
         q.device, _ffi.lib().ss_latent_attention, q.data_ptr(), out.data_ptr(), layer_ptr(latent_cache, layer_idx),
@@ -147,7 +155,7 @@ def latent_attention_varlen(
         return out
     require_device("latent_attention_varlen", q, latent_cache, block_tables, cu_seqlens, context_lens)
     q = unit_last_stride(q)
-    cu = _int32(cu_seqlens.reshape(-1))
+    cu = _ints(cu_seqlens)
     if _debug():
         _check_stream(cu, total, max_query_len)
     return _absorbed("latent_attention_varlen", q, out, latent_cache, block_tables, cu, context_lens, layer_idx, scale,
@@ -206,14 +214,14 @@ def latent_attention_expanded(
     q, kv = unit_last_stride(q), unit_last_stride(kv)
     if rope_dim > 1 and k_rope.stride(1) != 1:
         k_rope = k_rope.contiguous()
-    cu, cu_ctx = _int32(cu_seqlens.reshape(-1)), _int32(cu_context.reshape(-1))
+    cu, cu_ctx = _ints(cu_seqlens), _ints(cu_context)
     if _debug():
         _check_stream(cu, total, max_query_len)
         _check_stream(cu_ctx, keys, keys)
+    qs, os, ks = q.stride(), out.stride(), kv.stride()
     status = launch(
         q.device, _ffi.lib().ss_latent_attention_expanded, q.data_ptr(), out.data_ptr(), kv.data_ptr(),
         k_rope.data_ptr(), cu.data_ptr(), cu_ctx.data_ptr(), batch, total, keys, max_query_len, heads, nope, rope_dim,
-        value_dim, _ffi.i64x2(q.stride(0), q.stride(1)), _ffi.i64x2(out.stride(0), out.stride(1)),
-        _ffi.i64x2(kv.stride(0), kv.stride(1)), k_rope.stride(0), float(scale), dtype)
+        value_dim, _ffi.i64x2(qs[0], qs[1]), _ffi.i64x2(os[0], os[1]), _ffi.i64x2(ks[0], ks[1]), k_rope.stride(0), float(scale), dtype)
     _ffi.check(status, "latent_attention_expanded")
     return out

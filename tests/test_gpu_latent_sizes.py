@@ -131,3 +131,19 @@ def test_graphs_and_streams_at_once(device):
         got += [held for _, held in graphs]
         for have, need in zip(got, (want[turn % 2], want[0], want[1])):
             assert torch.equal(have[0], need[0]) and torch.equal(have[1], need[1])
+
+
+@pytest.mark.parametrize("heads", [2, 16, 32])
+@pytest.mark.parametrize("ql,extra", [([1, 1, 1], [300, 0, 2000]), ([5, 40], [100, 7]), ([0, 1, 0, 9], [4, 90, 0, 700]),
+                                      ([0, 0, 0], [5, 0, 9])])
+def test_steps_of_one_kind(device, heads, ql, extra):
+    """Decodes alone, chunks alone or nothing at all in a call that may hold both."""
+    gen = torch.Generator().manual_seed(heads + len(ql))
+    cl = [a + b for a, b in zip(ql, extra)]
+    cache, tables = _pool(gen, cl, 16, 576, torch.bfloat16)
+    q = _randn(gen, sum(ql) + 1, heads, 576, dtype=torch.bfloat16)
+    ctx = torch.tensor(cl, dtype=torch.int32).cuda()
+    out = torch.full((sum(ql) + 1, heads, 512), 5.0, dtype=torch.bfloat16, device="cuda")
+    latent_attention_varlen(q, cache, tables.cuda(), _cu(ql), ctx, 0, 0.06, 16, 64, 512, out=out)
+    _check_absorbed(out, q, cache[0], tables, ql, cl, 0.06, 512, torch.bfloat16)
+    assert (out[sum(ql) :] == 5).all()
