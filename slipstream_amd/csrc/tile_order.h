@@ -24,7 +24,8 @@ __device__ __forceinline__ void wait_dma() {
   asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory");
 }
 
-typedef __attribute__((address_space(3))) const u32x4* LdsWords;__device__ __forceinline__ uint32_t lds_address(char* p) { return (uint32_t)(uintptr_t)(LdsBytes)p; }
+typedef __attribute__((address_space(3))) const u32x4* LdsWords;
+__device__ __forceinline__ uint32_t lds_address(char* p) { return (uint32_t)(uintptr_t)(LdsBytes)p; }
 __device__ __forceinline__ u32x4 lds_word(uint32_t at) { return *(LdsWords)(uintptr_t)at; }
 __device__ __forceinline__ float lds_float(uint32_t at) {
   return *(__attribute__((address_space(3))) const float*)(uintptr_t)at;
