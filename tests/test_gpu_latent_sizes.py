@@ -147,3 +147,42 @@ def test_steps_of_one_kind(device, heads, ql, extra):
     latent_attention_varlen(q, cache, tables.cuda(), _cu(ql), ctx, 0, 0.06, 16, 64, 512, out=out)
     _check_absorbed(out, q, cache[0], tables, ql, cl, 0.06, 512, torch.bfloat16)
     assert (out[sum(ql) :] == 5).all()
+
+
+@pytest.mark.parametrize("heads", [16, 64, 128])
+@pytest.mark.parametrize("bs", [8, 256, 2048])
+def test_page_sizes(device, heads, bs):
+    """Pages of fewer keys than a tile and of many tiles, and one that is shared by two sequences."""
+    cl = [70, 9, 2100, 8]
+    gen = torch.Generator().manual_seed(heads + bs)
+    cache, tables = _pool(gen, cl, bs, 576, torch.float16)
+    tables[1, 0] = tables[0, 0]
+    q = _randn(gen, len(cl), heads, 1, 576, dtype=torch.float16)
+    out = latent_attention_decode(q, cache, tables.cuda(), torch.tensor(cl, dtype=torch.int32).cuda(), 0, 0.06, bs, 512)
+    _check_absorbed(out[:, 0], q[:, :, 0], cache[0], tables, [1] * len(cl), cl, 0.06, 512, torch.float16)
+
+
+@pytest.mark.parametrize("heads", [16, 64, 128])
+def test_scores_that_overflow_and_hold_nan(device, heads):
+    """A latent with a NaN makes the rows that see it NaN, one with an infinity not finite, and no others; of scores far
+    apart the largest one's values are left."""
+    gen = torch.Generator().manual_seed(heads)
+    cl = [100, 300, 40, 90]
+    cache, tables = _pool(gen, cl, 16, 576, torch.bfloat16)
+    cache[0, tables[1, 7].item(), 3, 5] = float("nan")
+    cache[0, tables[2, 1].item(), 2, 9] = float("inf")
+    q = _randn(gen, 4, heads, 1, 576, dtype=torch.bfloat16)
+    ctx = torch.tensor(cl, dtype=torch.int32).cuda()
+    out = latent_attention_decode(q, cache, tables.cuda(), ctx, 0, 0.06, 16, 512)[:, 0]
+    assert torch.isnan(out[1]).all() and torch.isfinite(out[0].float()).all() and torch.isfinite(out[3].float()).all()
+    assert not torch.isfinite(out[2].float()).all()
+    good = [0, 3]
+    _check_absorbed(out[good], q[good, :, 0], cache[0], tables[good], [1, 1], [100, 90], 0.06, 512, torch.bfloat16)
+    sharp = latent_attention_decode(q[:1], cache, tables[:1].cuda(), ctx[:1], 0, 3000.0, 16, 512)[:, 0]
+    rows = cache[0][tables[0, :7].long().cuda()].reshape(-1, 576)[:100].float()
+    best = (q[0, :, 0].float() @ rows.t()).argmax(dim=1)
+    # all but the best row's probabilities are 2^-1000 and less of it. Its own is 2^(score - m) for the maximum m that was
+    # last taken (up to 2^8), rounded to bf16 for the product but not in the sum that divides: half a step (2^-8) of the
+    # value, and another when the output is rounded, 2^-7 + 2^-16 together
+    want = rows[best, :512]
+    assert ((sharp[0].float() - want).abs() <= (2.0**-7 + 2.0**-15) * want.abs()).all()
