@@ -11,7 +11,8 @@ namespace {
 constexpr int kRopeDim = 64;
 constexpr float kSlack = 8.f;  // by which (log2) a score may exceed the running maximum before it is raised
 
-typedef short tr16x4 __attribute__((ext_vector_type(4)));typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short tr16x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 // Where the 16-byte chunk c of a row r of 256 bytes and more lies in the LDS: at c ^ lat_swizzle(r). The 16
 // lanes of a pass of a 16-byte read have different rows (mod 16) and lie in different banks; of
@@ -39,6 +40,14 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
   asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
   return r;
+}
+
+// A row's sum goes over its probabilities as the product over keys takes them, rounded to the inputs' type: so the
+// weights of its values sum to one, and of a key that outweighs all others the row is its value, whatever 2^x (x up to
+// kSlack) its probability is. (Of the unrounded ones such a row is off by up to half a step.)
+template <typename T>
+__device__ __forceinline__ float pair_sum(uint32_t w) {
+  return Elem<T>::lo(w) + Elem<T>::hi(w);
 }
 
 // The operand of 16 keys of a product over keys, from rows of the LDS: the lane's four keys at `lo`, and

@@ -363,16 +363,18 @@ __device__ __forceinline__ void latent_segment(const LatentParams& p, const Late
             if (!there || key + e >= lim[rw]) sv[rw][x][e] = -__builtin_inff();
       }
     }
-    f32x4 pv[RW][KQ];
+    u32x2 pv[RW][KQ];  // as they are written
     auto probabilities = [&]() {
 #pragma unroll
       for (int rw = 0; rw < RW; ++rw)
 #pragma unroll
         for (int x = 0; x < KQ; ++x) {
+          float y[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) pv[rw][x][e] = fast_exp2(fmaf(sv[rw][x][e], cscale, -own[rw]));
+          for (int e = 0; e < 4; ++e) y[e] = fast_exp2(fmaf(sv[rw][x][e], cscale, -own[rw]));
+          pv[rw][x] = u32x2{Elem<T>::pack2(y[0], y[1]), Elem<T>::pack2(y[2], y[3])};
           *reinterpret_cast<u32x2*>(lds + C::kP + ((quarter >> 1) * RT + rt0 + rw) * 1024 + lane * 16 + 8 * ((quarter + x) & 1)) =
-              u32x2{Elem<T>::pack2(pv[rw][x][0], pv[rw][x][1]), Elem<T>::pack2(pv[rw][x][2], pv[rw][x][3])};
+              pv[rw][x];
         }
     };
 #pragma unroll
@@ -412,7 +414,7 @@ __device__ __forceinline__ void latent_segment(const LatentParams& p, const Late
 #pragma unroll
     for (int rw = 0; rw < RW; ++rw)
 #pragma unroll
-      for (int x = 0; x < KQ; ++x) l[rw] += (pv[rw][x][0] + pv[rw][x][1]) + (pv[rw][x][2] + pv[rw][x][3]);
+      for (int x = 0; x < KQ; ++x) l[rw] += pair_sum<T>(pv[rw][x][0]) + pair_sum<T>(pv[rw][x][1]);
     if constexpr (KQ == 1) latents(1, c[1]);
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
@@ -693,9 +695,9 @@ __device__ __forceinline__ void latent_segment_wide(const LatentParams& p, const
         s16[e] = a, s16[e + 1] = c;
       } else if constexpr (i < 16) {
         constexpr int e = 4 * (i - 12);
-        sum += (s16[e] + s16[e + 1]) + (s16[e + 2] + s16[e + 3]);
         pk[e / 2] = Elem<T>::pack2(s16[e], s16[e + 1]);
         pk[e / 2 + 1] = Elem<T>::pack2(s16[e + 2], s16[e + 3]);
+        sum += pair_sum<T>(pk[e / 2]) + pair_sum<T>(pk[e / 2 + 1]);
       } else if constexpr (i == 16) {
         const float alpha = fast_exp2(m - mn);
         l = fmaf(l, alpha, sum);
