@@ -189,7 +189,7 @@ latent_expanded_kernel(const LatentParams p) {
       const uint32_t tb = __builtin_bit_cast(uint32_t, top[0]);
       auto sw = __builtin_amdgcn_permlane32_swap(tb, tb, false, false);
       top[0] = max3(__builtin_bit_cast(float, (uint32_t)sw[0]), __builtin_bit_cast(float, (uint32_t)sw[1]), kNegBig);
-      top[0] = fmaxf(m, top[0] * cscale);
+      top[0] = fmaxf(m, fmaf(top[0], cscale, -kHeadroom<T>));
     } else if constexpr (i == 6) {
       grew = __any(top[0] > m + kSlack);
       mn = grew ? top[0] : m;

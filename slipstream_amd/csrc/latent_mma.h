@@ -9,7 +9,7 @@ namespace ss {
 namespace {
 
 constexpr int kRopeDim = 64;
-constexpr float kSlack = 8.f;  // by which (log2) a score may exceed the running maximum before it is raised
+constexpr float kSlack = 8.f;  // by which (log2) a score may exceed the running maximum before that is raised
 
 typedef short tr16x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -41,6 +41,12 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
   return r;
 }
+
+// Probabilities are 2^(score - m) for a row's m, raised to its maximum score less kHeadroom: in fp16 they reach 2^15 (the
+// largest value is below 2^16) and 2^-32 of the largest score's is left, where from 2^0 down to 2^8 it would be 2^-25:
+// many keys that far below one may make up a row whose largest key's value is small. bf16 has fp32's range.
+template <typename T>
+constexpr float kHeadroom = std::is_same<T, f16_t>::value ? 7.f : 0.f;
 
 // A row's sum goes over its probabilities as the product over keys takes them, rounded to the inputs' type: so the
 // weights of its values sum to one, and of a key that outweighs all others the row is its value, whatever 2^x (x up to

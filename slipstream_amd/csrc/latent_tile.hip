@@ -394,7 +394,7 @@ __device__ __forceinline__ void latent_segment(const LatentParams& p, const Late
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
       const f32x4 top = *reinterpret_cast<const f32x4*>(lds + C::kTop + (16 * rt + n) * 16);
-      want[rt] = fmaxf(m[rt], fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * cscale);
+      want[rt] = fmaxf(m[rt], fmaf(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), cscale, -kHeadroom<T>));
       grew |= want[rt] > m[rt] + kSlack;
     }
     if (__any(grew)) {  // the same in every wave
@@ -685,7 +685,7 @@ __device__ __forceinline__ void latent_segment_wide(const LatentParams& p, const
         top = max3(__builtin_bit_cast(float, (uint32_t)sw[0]), __builtin_bit_cast(float, (uint32_t)sw[1]),
                    __builtin_bit_cast(float, (uint32_t)sw[1]));
       } else if constexpr (i == 3) {
-        top = fmaxf(m, top * cscale);
+        top = fmaxf(m, fmaf(top, cscale, -kHeadroom<T>));
         grew = __any(top > m + kSlack);
         mn = grew ? top : m;
       } else if constexpr (i < 12) {

@@ -1,6 +1,9 @@
-"""What attention over latents does with probabilities in 16 bits: rows that one key outweighs."""
+"""What attention over latents does with probabilities in 16 bits: rows that one key outweighs, and rows that many keys
+far below one make up."""
 
 from __future__ import annotations
+
+import math
 
 import pytest
 import torch
@@ -108,3 +111,49 @@ def test_expanded_rows_of_one_value(device, kind, dtype, heads, ql, extra):
         at, ck = at + n, ck + c
     out = latent_attention_expanded(q, kv, kr, _cu(ql), _cu(cl), SCALE[kind], max(ql))
     assert torch.equal(out, want)
+
+
+# Many keys far below one, whose values are large: a key with score 0 and value 1, n - 1 with score -25.5 (log2) and value
+# 1024. The row is (1 + 1024 t) / (1 + t) with t = (n - 1) 2^-25.5. fp16 holds a probability of 2^-25.5 relative to the
+# largest (which is taken as 2^7) to half of 2^-24 of it, 2^-6.5 of itself, which is that part of 1024 t; bf16, which has
+# fp32's exponents, to 2^-8. The largest one's rounding is half a step of the type, fp32's are 2^-15 of the row at most, and
+# the row's own is half a step: 2^-11 in fp16, and in bf16 (7 bits behind the first one: 2^-7 from 1 to the next value) 2^-8.
+TAIL, LARGE = -25.5, 1024.0
+
+
+def _check_tail(out: torch.Tensor, n: int) -> None:
+    t = (n - 1) * 2.0**TAIL
+    want = (1 + LARGE * t) / (1 + t)
+    err = (out.double() - want).abs().max().item()
+    half = torch.finfo(out.dtype).eps / 2
+    assert err <= (2 * half + 2.0**-15) * want + 2.0**-6.5 * LARGE * t, (err, want)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads,r,batch,n", [(16, 512, 700, 700), (32, 512, 600, 300), (64, 256, 600, 300), (128, 512, 520, 300)])
+def test_many_keys_far_below_one(device, dtype, heads, r, batch, n):
+    """More sequences than workgroups, so that the far keys stand beside the near one in a row's own sum."""
+    blocks = -(-n // 16)
+    cache = torch.zeros(1, blocks, 16, r + 64, dtype=dtype, device="cuda")
+    flat = cache[0].view(-1, r + 64)
+    flat[:, :r], flat[:, r] = LARGE, TAIL
+    flat[0, :r], flat[0, r] = 1.0, 0.0
+    q = torch.zeros(batch, heads, 1, r + 64, dtype=dtype, device="cuda")
+    q[..., r] = 1.0
+    tables = torch.arange(blocks, dtype=torch.int32, device="cuda").expand(batch, blocks)
+    ctx = torch.full((batch,), n, dtype=torch.int32, device="cuda")
+    _check_tail(latent_attention_decode(q, cache, tables, ctx, 0, math.log(2), 16, r), n)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads,tq", [(128, 300), (112, 200), (3, 50)])
+def test_many_keys_far_below_one_expanded(device, dtype, heads, tq):
+    n = 700  # of which the last query sees all
+    q = torch.zeros(tq, heads, 192, dtype=dtype, device="cuda")
+    q[..., 128] = 1.0
+    kv, kr = torch.zeros(n, heads, 256, dtype=dtype, device="cuda"), torch.zeros(n, 64, dtype=dtype, device="cuda")
+    kv[..., 128:], kr[:, 0] = LARGE, TAIL
+    kv[0, :, 128:], kr[0, 0] = 1.0, 0.0
+    out = latent_attention_expanded(q, kv, kr, _cu([tq]), _cu([n]), math.log(2), tq)
+    for j in (0, tq // 2, tq - 1):
+        _check_tail(out[j], n - tq + j + 1)
