@@ -212,8 +212,8 @@ def latent_attention_expanded(
         raise _ffi.KernelError(f"unsupported dtypes q={q.dtype} kv={kv.dtype} k_rope={k_rope.dtype} (must be equal)")
     dtype = _ffi.dtype_code(q.dtype)
     q, kv = unit_last_stride(q), unit_last_stride(kv)
-    if rope_dim > 1 and k_rope.stride(1) != 1:
-        k_rope = k_rope.contiguous()
+    if rope_dim:
+        k_rope = unit_last_stride(k_rope)
     cu, cu_ctx = _ints(cu_seqlens), _ints(cu_context)
     if _debug():
         _check_stream(cu, total, max_query_len)

@@ -1,0 +1,40 @@
+"""Attention over latents from operands that do not lie on 16 bytes: the kernels that the aligned ones take, bit for bit
+the same results."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+from test_gpu_latent import _pool, _randn
+
+from slipstream_amd.kernels import latent_attention_decode, latent_attention_expanded, latent_attention_varlen
+
+pytestmark = pytest.mark.gpu
+
+
+def _cu(n):
+    return torch.tensor([0] + list(n)).cumsum(0).to(torch.int32).cuda()
+
+
+def _apart(x: torch.Tensor, before: int, behind: int) -> torch.Tensor:
+    """``x`` as a part of rows that are ``before + behind`` values longer."""
+    wide = torch.zeros((*x.shape[:-1], before + x.shape[-1] + behind), dtype=x.dtype, device=x.device)
+    part = wide[..., before : before + x.shape[-1]]
+    part.copy_(x)
+    return part
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("before,behind", [(1, 0), (0, 1), (512, 3), (3, 5)])
+def test_expanded_keys_of_any_alignment(device, dtype, before, behind):
+    """The shared keys as the last columns of a projection that has an odd number of others; queries and the heads' keys
+    likewise."""
+    gen = torch.Generator().manual_seed(before + behind)
+    heads, ql, cl = 4, [40, 3], [170, 90]
+    q, kv = _randn(gen, sum(ql), heads, 192, dtype=dtype), _randn(gen, sum(cl), heads, 256, dtype=dtype)
+    kr = _randn(gen, sum(cl), 64, dtype=dtype)
+    args = (_cu(ql), _cu(cl), 0.1, max(ql))
+    want = latent_attention_expanded(q, kv, kr, *args)
+    assert torch.equal(latent_attention_expanded(q, kv, _apart(kr, before, behind), *args), want)
+    got = latent_attention_expanded(_apart(q, before, behind), _apart(kv, before, behind), kr, *args)
+    assert torch.equal(got, want)
