@@ -67,11 +67,12 @@ def _absorbed(who: str, q: torch.Tensor, out: torch.Tensor, latent_cache: torch.
         block_tables = _int32(block_tables)
     ctx = _ints(ctx)
     cst = latent_cache.stride()
+    page = cst[1] if latent_cache.shape[1] > 1 else block_size * cst[2]  # (of one page any will do)
     status = launch(
         q.device, _ffi.lib().ss_latent_attention, q.data_ptr(), out.data_ptr(), layer_ptr(latent_cache, layer_idx),
         block_tables.data_ptr(), None if cu is None else cu.data_ptr(), ctx.data_ptr(), batch, tokens, tq, heads,
         latent_dim, rope_dim, block_tables.shape[1], block_size, latent_cache.shape[1], _ffi.i64x3(*q_strides),
-        _ffi.i64x3(*o_strides), _ffi.i64x2(cst[1], cst[2]), block_tables.stride(0), float(scale), dtype,
+        _ffi.i64x3(*o_strides), _ffi.i64x2(page, cst[2]), block_tables.stride(0), float(scale), dtype,
         ws.data_ptr(), ws.numel())
     _ffi.check(status, who)
     return out
@@ -218,10 +219,12 @@ def latent_attention_expanded(
     if _debug():
         _check_stream(cu, total, max_query_len)
         _check_stream(cu_ctx, keys, keys)
-    qs, os, ks = q.stride(), out.stride(), kv.stride()
+    # of one key any distance to the next will do: that of rows back to back, which every kernel takes
+    ks = _strides(kv, (0, 1)) if keys > 1 else [heads * kv.shape[2], *_strides(kv, (1,))]
     status = launch(
         q.device, _ffi.lib().ss_latent_attention_expanded, q.data_ptr(), out.data_ptr(), kv.data_ptr(),
         k_rope.data_ptr(), cu.data_ptr(), cu_ctx.data_ptr(), batch, total, keys, max_query_len, heads, nope, rope_dim,
-        value_dim, _ffi.i64x2(qs[0], qs[1]), _ffi.i64x2(os[0], os[1]), _ffi.i64x2(ks[0], ks[1]), k_rope.stride(0), float(scale), dtype)
+        value_dim, _ffi.i64x2(*_strides(q, (0, 1))), _ffi.i64x2(*_strides(out, (0, 1))), _ffi.i64x2(*ks),
+        k_rope.stride(0) if keys > 1 else rope_dim, float(scale), dtype)
     _ffi.check(status, "latent_attention_expanded")
     return out

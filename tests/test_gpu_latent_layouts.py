@@ -38,3 +38,28 @@ def test_expanded_keys_of_any_alignment(device, dtype, before, behind):
     assert torch.equal(latent_attention_expanded(q, kv, _apart(kr, before, behind), *args), want)
     got = latent_attention_expanded(_apart(q, before, behind), _apart(kv, before, behind), kr, *args)
     assert torch.equal(got, want)
+
+
+def _odd(x: torch.Tensor) -> torch.Tensor:
+    """Strides of the dimensions of size one that are no multiple of anything."""
+    return x.as_strided(x.shape, [s if n > 1 or i == x.ndim - 1 else 7 for i, (s, n) in enumerate(zip(x.stride(), x.shape))])
+
+
+@pytest.mark.parametrize("heads,tokens,keys", [(1, 5, 9), (4, 1, 1), (1, 1, 1), (1, 1, 40)])
+def test_expanded_of_one_head_or_token(device, heads, tokens, keys):
+    """A stride that no second head or token uses may be anything."""
+    gen = torch.Generator().manual_seed(heads + keys)
+    q, kv, kr = (_randn(gen, *s, dtype=torch.bfloat16) for s in ((tokens, heads, 192), (keys, heads, 256), (keys, 64)))
+    args = (_cu([tokens]), _cu([keys]), 0.1, tokens)
+    want = latent_attention_expanded(q, kv, kr, *args)
+
+    assert torch.equal(latent_attention_expanded(_odd(q), _odd(kv), _odd(kr), *args), want)
+
+
+@pytest.mark.parametrize("heads", [1, 16, 128])
+def test_absorbed_of_one_page_or_sequence(device, heads):
+    gen = torch.Generator().manual_seed(heads)
+    cache, tables = _randn(gen, 1, 1, 16, 576, dtype=torch.bfloat16), torch.zeros(1, 1, dtype=torch.int32, device="cuda")
+    q, ctx = _randn(gen, 1, heads, 1, 576, dtype=torch.bfloat16), torch.tensor([13], dtype=torch.int32, device="cuda")
+    want = latent_attention_decode(q, cache, tables, ctx, 0, 0.05, 16, 512)
+    assert torch.equal(latent_attention_decode(_odd(q), _odd(cache), _odd(tables), ctx, 0, 0.05, 16, 512), want)
