@@ -453,8 +453,8 @@ __device__ __forceinline__ void latent_segment(const LatentParams& p, const Late
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) {
         const f32x4 y = acc[rt][dt] * inv;
-        *reinterpret_cast<u32x2*>(o + 8 * out_chunk<C>(dt, g >> 1, wave)) =
-            u32x2{Elem<T>::pack2(y[0], y[1]), Elem<T>::pack2(y[2], y[3])};
+        const u32x2 w = {Elem<T>::pack2(y[0], y[1]), Elem<T>::pack2(y[2], y[3])};
+        __builtin_memcpy(o + 8 * out_chunk<C>(dt, g >> 1, wave), &w, 8);  // (rows may begin at any value)
       }
     }
   } else {
@@ -1093,13 +1093,15 @@ __global__ __launch_bounds__(WPR == 1 ? 256 : 64 * WPR) void latent_merge_kernel
       y.x = fmaf(x.x, f, y.x), y.y = fmaf(x.y, f, y.y);
     }
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    *reinterpret_cast<uint32_t*>(out + 2 * threadIdx.x) = Elem<T>::pack2(y.x * inv, y.y * inv);
+    const uint32_t w = Elem<T>::pack2(y.x * inv, y.y * inv);
+    __builtin_memcpy(out + 2 * threadIdx.x, &w, 4);
   } else {
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
-    for (int d = 0; d < PER; d += 4)
-      *reinterpret_cast<u32x2*>(out + d * 64 + 4 * lane) =
-          u32x2{Elem<T>::pack2(o[d] * inv, o[d + 1] * inv), Elem<T>::pack2(o[d + 2] * inv, o[d + 3] * inv)};
+    for (int d = 0; d < PER; d += 4) {
+      const u32x2 w = {Elem<T>::pack2(o[d] * inv, o[d + 1] * inv), Elem<T>::pack2(o[d + 2] * inv, o[d + 3] * inv)};
+      __builtin_memcpy(out + d * 64 + 4 * lane, &w, 8);
+    }
   }
 }
 
@@ -1191,9 +1193,7 @@ bool latent_tile_takes(const LatentParams& p, int dtype) {
   if (p.max_blocks < 1 || p.scale_log2 == 0.f) return false;  // (masked scores are -inf, times the scale)
   for (int64_t s : {p.q_sb, p.q_st, p.q_sh, p.kv_s0, p.kv_s1})
     if (s % 8) return false;
-  for (int64_t s : {p.o_sb, p.o_st, p.o_sh})
-    if (s % 4) return false;
-  return ((uintptr_t)p.q | (uintptr_t)p.kv) % 16 == 0 && (uintptr_t)p.out % 8 == 0 &&
+  return ((uintptr_t)p.q | (uintptr_t)p.kv) % 16 == 0 &&
          p.kv_s1 >= p.key_dim + p.rope_dim && p.block_size * p.kv_s1 < (1 << 29) && p.kv_s0 >= 0 &&
          p.num_blocks < (1ll << 31);
 }

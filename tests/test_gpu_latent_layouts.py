@@ -63,3 +63,26 @@ def test_absorbed_of_one_page_or_sequence(device, heads):
     q, ctx = _randn(gen, 1, heads, 1, 576, dtype=torch.bfloat16), torch.tensor([13], dtype=torch.int32, device="cuda")
     want = latent_attention_decode(q, cache, tables, ctx, 0, 0.05, 16, 512)
     assert torch.equal(latent_attention_decode(_odd(q), _odd(cache), _odd(tables), ctx, 0, 0.05, 16, 512), want)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("heads,r,ql,extra", [(16, 512, [1, 1, 1], [30, 700, 0]), (64, 256, [1, 3], [90, 400]),
+                                              (128, 512, [2, 1], [300, 2000]), (16, 512, [40, 1], [500, 30])])
+def test_absorbed_outputs_of_any_alignment(device, dtype, heads, r, ql, extra):
+    """Rows of ``out`` that begin at any value, whole items and merged ones; what lies beside them stays."""
+    gen = torch.Generator().manual_seed(heads)
+    cl = [a + b for a, b in zip(ql, extra)]
+    cache, tables = _pool(gen, cl, 16, r + 64, dtype)
+    q = _randn(gen, sum(ql), heads, r + 64, dtype=dtype)
+    ctx = torch.tensor(cl, dtype=torch.int32).cuda()
+    args = (tables.cuda(), _cu(ql), ctx, 0, 0.06, 16, max(ql), r)
+    want = latent_attention_varlen(q, cache, *args)
+    for before in (1, 2, 3):
+        wide = torch.full((sum(ql), heads, r + 4), 9.0, dtype=dtype, device="cuda")
+        got = latent_attention_varlen(q, cache, *args, out=wide[..., before : before + r])
+        assert torch.equal(got, want)
+        assert (wide[..., :before] == 9).all() and (wide[..., before + r :] == 9).all()
+        wide = torch.full((sum(ql), heads * r + 5), 9.0, dtype=dtype, device="cuda")
+        part = wide[:, before : before + heads * r].unflatten(1, (heads, r))
+        assert torch.equal(latent_attention_varlen(q, cache, *args, out=part), want)
+        assert (wide[:, :before] == 9).all() and (wide[:, before + heads * r :] == 9).all()
