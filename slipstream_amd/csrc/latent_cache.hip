@@ -74,6 +74,17 @@ struct Piece {
   }
 };
 
+// Its bits as they are: through fp32 a NaN that signals would be quieted
+template <int BYTES>
+__device__ __forceinline__ void copy_piece(char* to, const char* from) {
+  if constexpr (BYTES == 16)
+    ss::store16(to, ss::load16(from));
+  else if constexpr (BYTES == 4)
+    *reinterpret_cast<uint32_t*>(to) = *reinterpret_cast<const uint32_t*>(from);
+  else
+    *reinterpret_cast<uint16_t*>(to) = *reinterpret_cast<const uint16_t*>(from);
+}
+
 // N values a piece: 16 bytes, or one where the strides or addresses do not allow it
 template <typename T, int N>
 __global__ __launch_bounds__(256) void latent_write_kernel(const LatentWriteArgs a) {
@@ -91,17 +102,14 @@ __global__ __launch_bounds__(256) void latent_write_kernel(const LatentWriteArgs
   if (threadIdx.x < 64 && kept) {
     const char* const src = a.latent + tok * a.l_st;
     const int i0 = threadIdx.x;
-    P x, w;
-    if (i0 < pieces) {
-      x.load(src + i0 * kBytes);
-      if (a.w) w.load(a.w + i0 * kBytes);
-    }
     if (!a.w) {
-      for (int i = i0; i < pieces; i += 64) {
-        if (i != i0) x.load(src + i * kBytes);
-        x.store(row + i * kBytes);
-      }
+      for (int i = i0; i < pieces; i += 64) copy_piece<kBytes>(row + i * kBytes, src + i * kBytes);
     } else {
+      P x, w;
+      if (i0 < pieces) {
+        x.load(src + i0 * kBytes);
+        w.load(a.w + i0 * kBytes);
+      }
       float sum = 0.f;
       if (i0 < pieces) {
 #pragma unroll

@@ -1,5 +1,5 @@
-"""Attention over latents from operands that do not lie on 16 bytes: the kernels that the aligned ones take, bit for bit
-the same results."""
+"""Operands of other layouts than the usual: attention over latents from rows that do not lie on 16 bytes (the kernels that
+the aligned ones take, bit for bit the same results), latents that the cache keeps as they are."""
 
 from __future__ import annotations
 
@@ -7,7 +7,12 @@ import pytest
 import torch
 from test_gpu_latent import _pool, _randn
 
-from slipstream_amd.kernels import latent_attention_decode, latent_attention_expanded, latent_attention_varlen
+from slipstream_amd.kernels import (
+    latent_attention_decode,
+    latent_attention_expanded,
+    latent_attention_varlen,
+    latent_rope_and_cache,
+)
 
 pytestmark = pytest.mark.gpu
 
@@ -86,3 +91,17 @@ def test_absorbed_outputs_of_any_alignment(device, dtype, heads, r, ql, extra):
         part = wide[:, before : before + heads * r].unflatten(1, (heads, r))
         assert torch.equal(latent_attention_varlen(q, cache, *args, out=part), want)
         assert (wide[:, :before] == 9).all() and (wide[:, before + heads * r :] == 9).all()
+
+
+@pytest.mark.parametrize("dtype,bits", [(torch.bfloat16, torch.int16), (torch.float16, torch.int16), (torch.float32, torch.int32)])
+@pytest.mark.parametrize("before", [0, 1])
+def test_latents_without_a_norm_keep_every_bit(device, dtype, bits, before):
+    """Every 16-bit pattern, NaN that signal and subnormals among them (fp32: each with 16 other bits behind it)."""
+    n, r, d = 128, 512, 8
+    codes = torch.arange(1 << 16, dtype=torch.int32, device="cuda")
+    codes = (codes << 16 | (codes * 40503 & 0xFFFF)) if bits == torch.int32 else (codes - 32768).to(bits)
+    latent = _apart(codes.view(n, r), before, 0)  # 16 bytes a piece, or a value
+    ones = torch.ones(n, 1, d, dtype=dtype, device="cuda")
+    cache = torch.zeros(1, n // 16, 16, r + d, dtype=dtype, device="cuda")
+    latent_rope_and_cache(ones, latent.view(dtype), ones[:, 0], ones[:, 0], ones[:, 0], cache, torch.arange(n, device="cuda"), 0, 16)
+    assert torch.equal(cache.view(bits).view(n, r + d)[:, :r], codes.view(n, r))
