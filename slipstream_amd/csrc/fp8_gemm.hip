@@ -162,6 +162,7 @@ extern "C" int ss_fp8_workspace_size(int64_t m, int64_t n, int64_t k, int x_whol
   const int st = ss::check_extents(m, n, k, out_dtype);
   if (st != SS_OK || m == 0 || n == 0 || k == 0) return st;
   const int64_t kp = ss::round16(k);
+  if (kp > ss::kMostStride || m > INT32_MAX || n > INT32_MAX) return SS_OK;  // the general kernel's, without copies
   *bytes = ss::plan_for(m, n, kp, out_dtype != SS_DTYPE_BF16, true).workspace() + (x_whole && kp == k ? 0 : m * kp) +
            (w_whole && kp == k ? 0 : n * kp);
   return SS_OK;
