@@ -314,10 +314,10 @@ int ss_swiglu_int8(const void* gate, const void* up, int8_t* q, float* scale, in
 /*
  * Rows quantized to 8-bit floating point (e4m3) with an fp32 scale for every 128 columns, the inputs of
  * ss_fp8_gemm: for a block x of a row (the last one may be shorter) a = max |x|, scale = a / 448,
- * q = e4m3(x * 448 / a): the exact quotient (of fp32 x up to its own 2^-24) rounded to the nearest,
- * half to even. A block with a < 448 * 2^-126 is zeros with scale 0, one that holds a NaN or an
- * infinity zeros with scale NaN. x [rows, cols], row stride x_stride (elements, unit column stride, any
- * alignment of its elements), dtype SS_DTYPE_BF16/F16/F32; q [rows, cols] contiguous; scale (row, block)
+ * q = e4m3(x * 448 / a): the exact quotient rounded to the nearest, half to even. A block with a < 448 *
+ * 2^-126 is zeros with scale 0, one that holds a NaN or an infinity zeros with scale NaN. x [rows, cols], row
+ * stride x_stride (elements, unit column stride, any alignment of its elements), dtype
+ * SS_DTYPE_BF16/F16/F32; q [rows, cols] contiguous; scale (row, block)
  * at block * scale_stride + row, scale_stride >= rows. No counterpart in the reference.
  */
 int ss_quantize_fp8(const void* x, uint8_t* q, float* scale, int64_t rows, int64_t cols, int64_t x_stride,

@@ -3,8 +3,9 @@
 //   out[m, n] = sum_b x_scale[m, b] w_scale[n / 128, b] (sum_{k in block b} x[m, k] w[n, k]) (+ bias[n]).
 // The matrix cores sum a block (fp8_common.h says in how many bits); its sum is multiplied with the
 // product of its scales and added to an fp32 sum in one rounding. A result is rounded once to the
-// output's type. Few tokens go to the stream kernel (fp8_stream.hip), which the weights' bytes bound, more to the
-// tile kernel (fp8_tile.hip), by whose estimate is the shorter; the kernel here takes what neither may read.
+// output's type. Up to 32 tokens go to the stream kernel (fp8_stream.hip), which the weights' bytes bound, up to 128
+// to it or the tile kernel (fp8_tile.hip) by whose estimate is the shorter (plan_for), more to the tile kernel; the
+// kernel here takes what neither may read.
 #include "fp8_common.h"
 
 namespace ss {
@@ -125,6 +126,13 @@ bool whole_rows(const void* base, int64_t rows, int64_t stride, int64_t k) {
 int64_t round16(int64_t n) { return (n + 15) / 16 * 16; }
 
 // What a call runs on the current device. Kept for the last shapes of the thread.
+//
+// Over 288 calls of 1 to 2240 tokens with weights of 1152 x 896 to 28672 x 4096, to bf16 and fp16, the plan is within
+// 2.5 % of the best kernel, tile, split and waves on average (3.6 % up to 128 tokens, 1.1 % above) and 49 % off at worst
+// (128 x 14336 x 512 to fp16: 11.8 us in the stream kernel, 7.8 in the tile kernel). Up to 32 tokens the tile kernel takes
+// 1.6 times the stream kernel's time there and is never the faster, so the estimates are not asked: they agree, but
+// for outputs of 131072 and more, where they err to either side (16 x 524288 x 512 85 us by the estimates, 68 so; 8 x
+// 131072 x 128 12.4 and 14.6), and for rows of 65536 and more, which would be faster so (32 x 2048 x 65536 37.6 and 43.8).
 struct Plan {
   int64_t m = -1, n = 0, k = 0;
   bool wide = false, may_split = false;

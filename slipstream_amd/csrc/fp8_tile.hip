@@ -27,7 +27,6 @@ constexpr int ring_depth(int bm, int bn) {
   return d;
 }
 
-template <typename TI>
 __device__ __forceinline__ void mfma_block(f32x4& r, const i32x8& a, const i32x8& b) {
   asm volatile("v_mfma_f32_16x16x128_f8f6f4 %0, %1, %2, 0" : "=&v"(r) : "v"(a), "v"(b));
 }
@@ -182,7 +181,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     static_for<P>([&](auto qc) __attribute__((always_inline)) {
       constexpr int q = decltype(qc)::value, i = q / JT, j = q % JT;
       if constexpr (__is_same(TO, bf16_t)) {
-        mfma_block<TO>(part[q % 4], a[i & 1], b[j]);
+        mfma_block(part[q % 4], a[i & 1], b[j]);
       } else {
         part[q % 4] = Block<TO>::sum(a[i & 1], b[j]);
       }

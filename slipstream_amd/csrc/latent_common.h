@@ -64,7 +64,6 @@ bool latent_tile_takes(const LatentParams& p, int dtype);
 int64_t latent_tile_bytes(int64_t batch, int64_t total, int tq, int heads, int latent_dim);
 int launch_latent_tile(const LatentParams& p, int dtype, char* ws, hipStream_t stream);
 
-
 // latent_expanded.hip: the same of the expanded form (which needs no workspace)
 bool latent_expanded_takes(const LatentParams& p, int dtype);
 int launch_latent_expanded(const LatentParams& p, int dtype, hipStream_t stream);

@@ -39,8 +39,11 @@ namespace {
 // ns by the memory's rate, less where the caches hold it (one decode of 128 heads over some 4096 tokens, of
 // 59 ranges: 53 us with 0.5, 82 us with 0.35 of the merge's first form; 8 of them 80 and 86)
 constexpr float kStep = 1.8f, kRow = 0.5e-3f;
-// The same for 32 keys of 16 or 32 rows beside those, with its part of its items' starts (a step 1.1 to 1.25 then; taken as
-// 1.0 the step of latent_mixed_kernel's comment has 348 us, as 1.2 309, as 1.5 296, as 1.7 302)
+// The same for 32 keys of 16 or 32 rows beside those, with its part of its items' starts (a step 1.1 to 1.25 then). Over
+// eleven steps of 16 to 250 decodes beside 1 to 4 chunks (8, 16 and 32 heads, latents of 256 and 512) it is 5 % from the
+// best of 1.0, 1.25, 1.5 and 1.8 on average, as 1.25 is (1.0 15 %, 1.8 6 %), and 36 % at worst: 250 decodes over some 300
+// beside 2 chunks of 256, which would take 103 us with 1.0 and take 140. 32 heads would rather have 1.8 (192 decodes and 4
+// chunks of 256: 316 us, and 328), 16 rather 1.25 (192 decodes and a chunk: 134 and 139).
 constexpr float kFewStep = 1.5f;
 
 template <int R_, int RT_, int NW_>
