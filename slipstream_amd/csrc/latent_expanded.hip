@@ -8,9 +8,9 @@
 // Keys (the heads' and the shared parts) and values come by DMA into rings in the LDS, whose 16-byte
 // chunks are swizzled as in latent_mma.h. A step runs the scores of tile t + 1, then the outputs of tile t, with the
 // softmax of either written between their products; two waves a SIMD.
-// 4 chunks of 512 tokens over up to 4096, 128 heads: 431 to 452 us, 930 to 980 TFLOP/s; a step of 256 tokens and 64 keys
+// 4 chunks of 512 tokens over up to 4096, 128 heads: 445 to 472 us, 890 to 950 TFLOP/s; a step of 256 tokens and 64 keys
 // takes 2.2 us, its products 1.4 of them at the 1.9 GHz that the card's power leaves. A turn of 77 tokens over 512, 16
-// heads: 13.7 us, ten steps of 1 after 3.5 us of start; two groups of waves with half of the keys each take 13.2.
+// heads: 14.0 us, ten steps of 1 after 3.5 us of start; two groups of waves with half of the keys each took 0.5 us less.
 #include "latent_mma.h"
 
 namespace ss {
@@ -36,7 +36,7 @@ latent_expanded_kernel(const LatentParams p) {
   const int n = lane & 31, h = lane >> 5;
   // Workgroups go round robin over the eight XCDs, and a sequence's tiles of a head follow each other on one of
   // them, whose L2 then serves their keys. The sequences of the most keys come first, so that no long tile begins
-  // when the others end (in the order of the batch: 4 chunks of 512 over up to 4096, 128 heads 540 us); of more than
+  // when the others end (in the order of the batch: 4 chunks of 512 over up to 4096, 128 heads 540 us, then 464); of more than
   // 64 sequences each 64 are ordered. A sequence's first tile is the number of those of the ones before it.
   const int slot = blockIdx.x >> 3, groups = (p.heads + 7) >> 3;
   int left = slot, b = -1, count = 0, start = 0, head = 0, tile = 0;

@@ -26,7 +26,7 @@
 // Measured, with the merge. 256 decodes, 1024 tokens in the middle and 8192 at most, latents of 512 (64 rotated): 16 heads
 // 126 us (3.7 TB/s), 32 147, 64 175, 128 heads 225 (488 TFLOP/s): bound by the memory, which has the partial
 // rows of 128 heads to take too (some 100 MB beside 525; the merge 24 us). 4 chunks of 512 over up to 4096, 16
-// heads 251 us (775 TFLOP/s; a step of 128 rows and 32 keys 1.9 us, its products 1.3). 8 decodes of 16 heads over
+// heads 249 to 254 us (770 TFLOP/s; a step of 128 rows and 32 keys 1.9 us, its products 1.3). 8 decodes of 16 heads over
 // some 256 18.4 us, one over some 4096 26 us: the start (lengths, page table, keys: 8 us), then the merge (4).
 // Code that runs once counts: a workgroup's 8 KB of it took 8 us to come into the instruction cache.
 #include "latent_mma.h"
@@ -937,7 +937,7 @@ __global__ __launch_bounds__(64 * C::NW) __attribute__((amdgpu_waves_per_eu(C::N
 // A step of decodes beside chunks: sequences of few rows in F's tiles and the others in M's, in one launch. Decodes wait
 // for the memory and chunks for the matrix cores, so some workgroups of every XCD do the first while the others do
 // the second, as many as the steps' times (kFewStep, kStep) ask for: 192 decodes and 4 chunks of 512 over up to
-// 4096, 16 heads 296 us, in two launches 351.
+// 4096, 16 heads 284 to 301 us; in two launches 351, where one took 296.
 template <typename T, typename F, typename M>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) void latent_mixed_kernel(
     const LatentParams p, const LatentWork few, const LatentWork many) {

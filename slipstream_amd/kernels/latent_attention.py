@@ -15,6 +15,11 @@ masked, a row that sees no key gives zeros. The reference has no counterpart. bf
 latents (expanded: keys and values without their rotated part) up to 512 wide, rotated keys up to
 256. A latent that a query does not see must be finite where one that it sees is in the same call's
 new tokens. Device tensors only.
+
+Scores, maxima and sums are fp32. Of bf16 and fp16 inputs the probabilities are rounded to the inputs' type
+for the product with the values, and the sum that divides is of the rounded ones. Other widths than 256 or 512 and 64
+(expanded: 128, 64 and 128), pages of fewer than eight tokens or no power of two of them, fp32, a scale of 0 and a cache
+whose rows do not lie on 16 bytes run in a general kernel that is there for coverage.
 """
 
 from __future__ import annotations

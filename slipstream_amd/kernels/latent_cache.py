@@ -51,7 +51,9 @@ def latent_rope_and_cache(
 
     ``q_rope [N, H, Dr]``, ``latent [N, R]``, ``k_rope [N, Dr]``, ``cos``/``sin [N, Dr]``, all with a unit
     last stride and any other (parts of the projections' outputs are taken as they are); ``rope(x) = x *
-    cos + cat(-x2, x1) * sin``. ``slot_mapping [N]``: slots below 0 or past the pool are skipped; a slot
+    cos + cat(-x2, x1) * sin`` with ``x = [x1, x2]``, as in ``rope_and_cache``: value ``i`` turns with value ``i + Dr / 2``.
+    (Projections made for turning adjacent pairs need the rows of their rotated parts in the order ``0, 2, 4, .., 1, 3,
+    5, ..``, of the queries in each head and of the key, once at load; scores stay the same.) ``slot_mapping [N]``: slots below 0 or past the pool are skipped; a slot
     that is given twice holds parts of either row. Without ``norm_weight [R]`` the latent is copied bit
     for bit. ``out`` (``[N, H, Dr]``, unit last stride, for instance the last columns of the absorbed
     queries; ``q_rope`` itself is allowed) takes the rotated queries.
