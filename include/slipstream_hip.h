@@ -472,7 +472,9 @@ int ss_latent_rope_and_cache(const void* q, void* q_out, const void* latent, con
  * are clamped into [0, total_tokens]; with it tq only tells how long sequences are likely to be, and
  * rows of no sequence are left as they are. Table entries outside [0, num_blocks) are masked, a row
  * that sees no key gives zeros; a new token's latent that another of the call's queries sees must be
- * finite for those that do not. latent_dim 1..512, rope_dim 0..256, dtype SS_DTYPE_BF16/F16/F32. The
+ * finite for those that do not. latent_dim 1..512, rope_dim 0..256, dtype SS_DTYPE_BF16/F16/F32: scores,
+ * maxima and sums in fp32, probabilities of the 16-bit types rounded to them for the product with the latents and in
+ * the sum that divides. The
  * conventions of ss_paged_attention_varlen; no counterpart in the reference.
  * workspace: ss_latent_attention_workspace_size() bytes (total_tokens = batch * tq without cu_seqlens),
  * any contents: partial rows of keys split over workgroups. Too small a one is SS_ERR_WORKSPACE.
@@ -496,7 +498,8 @@ int ss_latent_attention(const void* q, void* out, const void* cache, const int32
  * tokens last) [cu_context[b], cu_context[b + 1]) of kv and k_rope; both are clamped to total_tokens and
  * total_keys, and rows of no sequence are left as they are. max_query_len only tells how long
  * sequences are likely to be; a new token's values that another of the call's queries sees must be finite
- * for those that do not. nope_dim and value_dim 1..512, rope_dim 0..256, dtype SS_DTYPE_BF16/F16/F32.
+ * for those that do not. nope_dim and value_dim 1..512, rope_dim 0..256, dtype SS_DTYPE_BF16/F16/F32, rounded
+ * where the absorbed form is.
  */
 int ss_latent_attention_expanded(const void* q, void* out, const void* kv, const void* k_rope,
                                  const int32_t* cu_seqlens, const int32_t* cu_context, int64_t batch,
